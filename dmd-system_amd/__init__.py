@@ -20,6 +20,8 @@ Public API:
     fused_bf16_layernorm_modulation_hidden_backward, fused_reduced_component_gradient,
     fused_tensor4d_component_gradient      its fused backward
     ModulatedLayerNormFunction, modulated_layer_norm   the same as one autograd op
+    rotary_axes, rotary_axes_qk, grid_positions, RotaryAxesFunction   rotary positions with several axes, q / k norms
+    gated_residual_norm, GatedResidualNormFunction   the joint of two sublayers: norm after, gate, residual, norm before
     load_library()                       load libmlora.so (raises if missing)
 
 The directory name is not a Python identifier; importers load it as
@@ -45,6 +47,8 @@ from .modulated_norm import (ModulatedLayerNormFunction, fused_bf16_layernorm_mo
                              fused_layernorm_modulation_hidden_backward, fused_modulated_norm_epilogue,
                              fused_modulated_norm_materialization, fused_reduced_component_gradient,
                              fused_tensor4d_component_gradient, modulated_layer_norm)
+from .rotary import RotaryAxesFunction, grid_positions, rotary_axes, rotary_axes_qk
+from .joint import GatedResidualNormFunction, gated_residual_norm
 
 
 def load_library():
@@ -65,4 +69,6 @@ __all__ = [
     "fused_layernorm_modulation", "fused_bf16_layernorm_modulation_hidden_backward",
     "fused_layernorm_modulation_hidden_backward", "fused_reduced_component_gradient",
     "fused_tensor4d_component_gradient", "ModulatedLayerNormFunction", "modulated_layer_norm",
+    "RotaryAxesFunction", "grid_positions", "rotary_axes", "rotary_axes_qk", "GatedResidualNormFunction",
+    "gated_residual_norm",
 ]

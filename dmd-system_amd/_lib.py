@@ -31,6 +31,8 @@ _pvp = ctypes.POINTER(ctypes.c_void_p)
 _pi32 = ctypes.POINTER(ctypes.c_int32)
 _pi64 = ctypes.POINTER(ctypes.c_int64)
 _pf32 = ctypes.POINTER(ctypes.c_float)
+_pf64 = ctypes.POINTER(ctypes.c_double)
+_f32 = ctypes.c_float
 
 SIGNATURES = {
     "mlora_abi_version": (_int, []),
@@ -88,6 +90,19 @@ SIGNATURES = {
     "mlora_f32_seg_outer_workspace_bytes": (_i64, [_i64, _i64, _pi32, _i32, _pi64, _pi32, _i32]),
     "mlora_f32_seg_outer_split": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _pvp, _int, _pi32, _i32,
                                          _pi64, _pi32, _i32, _vp, _i64, _vp]),
+    "mlora_rotary_turns": (_int, [_pi32, _i32, ctypes.c_double, _pf64, _pi32]),
+    "mlora_rotary_axes": (_int, [_pvp, _pvp, _pvp, _pi64, _pi32, _int, _int, _int, _int, _f32, _vp, _int, _i64, _i64,
+                                 _pf64, _pi32, _i64, _int, _i64, _i64, _i64, _vp]),
+    "mlora_rotary_axes_backward_workspace_bytes": (_i64, [_pi32, _int, _int, _i64, _i64, _i64]),
+    "mlora_rotary_axes_backward": (_int, [_pvp, _pvp, _pvp, _pvp, _pvp, _pi64, _pi64, _pi32, _int, _int, _int, _int, _f32,
+                                          _vp, _int, _i64, _i64, _pf64, _pi32, _i64, _int, _vp, _i64,
+                                          _i64, _i64, _i64, _vp]),
+    "mlora_joint": (_int, [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp, _vp, _int, _i64, _i64,
+                           _int, _vp, _int, _int, _int, _f32, _f32, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "mlora_joint_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mlora_joint_backward": (_int, [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                    _vp, _int, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _int, _int, _int, _f32, _f32,
+                                    _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _i64, _i64, _i64, _i64, _vp]),
 }
 
 _LIB = None

@@ -34,6 +34,7 @@
 //   per-token component gradient (:215-270): g·n and g at every token.
 #include "mlora_common.h"
 #include "mlora_host.h"
+#include "mlora_rows.h"
 
 #include <type_traits>
 
@@ -52,26 +53,6 @@ struct NormArgs {
   int32_t table_f32, scale_f32, shift_f32;
   float eps;
 };
-
-// Eight consecutive values at element offset e of a bf16 or float32 array.
-__device__ __forceinline__ void load8(const void *base, bool f32, int64_t e, float (&v)[8]) {
-  if (f32) {
-    const float *p = static_cast<const float *>(base) + e;
-    const f32x4 a = *(const MLORA_GLOBAL f32x4 *)p, b = *(const MLORA_GLOBAL f32x4 *)(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
-  } else {
-    const u32x4 u = *(const MLORA_GLOBAL u32x4 *)(static_cast<const uint16_t *>(base) + e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32((uint16_t)(i % 2 ? u[i / 2] >> 16 : u[i / 2] & 0xffff));
-  }
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
 
 // RN(RN(v · RN(1 + s)) + h): three roundings, no fused multiply-add.
 __device__ __forceinline__ float modulate(float v, float s, float h) {
@@ -250,17 +231,6 @@ struct NormBwdArgs {
   int32_t x_f32, g_f32, table_f32, scale_f32, dx_f32;
   float eps;
 };
-
-__device__ __forceinline__ void store8_any(void *base, bool f32, int64_t e, const float (&v)[8]) {
-  if (f32) {
-    float *p = static_cast<float *>(base) + e;
-    *(MLORA_GLOBAL f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]};
-    *(MLORA_GLOBAL f32x4 *)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  } else {
-    *(MLORA_GLOBAL u32x4 *)(static_cast<uint16_t *>(base) + e) =
-        u32x4{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7])};
-  }
-}
 
 // ((gn - gsum_w) - n · gnn_w) · rstd, each operation rounded (no fused multiply-add).
 __device__ __forceinline__ float ln_input_grad(float gn, float n, float gsum_w, float gnn_w, float rstd) {
@@ -717,11 +687,6 @@ static int fused_chunk(int64_t batches, int64_t tokens) {
   int chunk = 8;
   while (chunk < 128 && batches * ((tokens + chunk - 1) / chunk) > 512) chunk *= 2;
   return chunk;
-}
-
-// Rows of 16-byte chunks: every row start 16-byte aligned.
-static bool rows_aligned(const void *p, int64_t sb, int64_t st) {
-  return aligned16(p) && sb >= 0 && st >= 0 && sb % 8 == 0 && st % 8 == 0;
 }
 
 }  // namespace mlora

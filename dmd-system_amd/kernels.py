@@ -6,6 +6,7 @@ missing library raise.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Sequence
 
@@ -797,3 +798,188 @@ def f32_seg_outer(p: torch.Tensor, h: torch.Tensor, ranks: Sequence[int], routin
             stream))
         outs = [t if acc is None else acc + t for acc, t in zip(outs, part)]
     return outs  # type: ignore[return-value]
+
+
+# ------------------------------------------------------------------ the block between its linears
+
+_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+NORM_NONE, NORM_HEAD, NORM_ROW = 0, 1, 2  # the rotary kernels' RMSNorm
+NORM_KINDS = {"layer": 0, "rms": 1}       # the joint's norms
+
+
+class _Device:
+    """Makes t's device the current one around a launch, where it is another."""
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+@functools.lru_cache(maxsize=64)
+def rotary_turns(axis_dims: tuple, theta: float):
+    """(turns, axis): each pair's frequency / 2π and axis, as the host arrays of the rotary entry points."""
+    n = sum(axis_dims) // 2
+    turns, axis = (ctypes.c_double * max(n, 1))(), (ctypes.c_int32 * max(n, 1))()
+    _lib.check("mlora_rotary_turns", _lib.load().mlora_rotary_turns(_lib.i32_array(axis_dims), len(axis_dims), theta,
+                                                                     turns, axis))
+    return turns, axis
+
+
+def _check_heads(name: str, t: torch.Tensor, dtype, lead) -> None:
+    _require(t.is_cuda and t.dtype == dtype, f"{name} must be a {dtype} device tensor")
+    _require(t.dim() == 4 and tuple(t.shape[:2]) == tuple(lead), f"{name} must be [{lead[0]}, {lead[1]}, heads, head_dim]")
+    _require(rows_layout(t), f"{name} needs unit stride in the head and 16-byte aligned heads (strides multiples of 8)")
+
+
+def rows_layout(t: torch.Tensor) -> bool:
+    """Whether the row kernels take t as it lies: unit last stride, the others non-negative multiples of 8
+    elements, 16-byte aligned."""
+    if t.numel() == 0:
+        return True
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return False
+    return t.data_ptr() % 16 == 0 and all(s >= 0 and s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+
+
+def _strides(t: torch.Tensor, n: int) -> list:
+    """The first n element strides, 0 in a dimension of one (its stride is never used)."""
+    return [s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape[:n])]
+
+
+def _pos_args(positions: torch.Tensor, B: int, L: int):
+    _require(positions.is_cuda and positions.dtype in _POS_TYPES, "positions must be an int32, int64 or float32 device tensor")
+    _require(positions.dim() == 3 and positions.shape[0] in (1, B) and positions.shape[1] == L
+             and positions.shape[2] >= 1 and (positions.stride(2) == 1 or positions.shape[2] == 1),
+             f"positions must be [{B} or 1, {L}, axes] with unit axis stride")
+    sb, st = _strides(positions, 2)
+    return positions.data_ptr(), _POS_TYPES[positions.dtype], sb, st
+
+
+def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: Sequence[int], *, theta: float,
+                halves: bool, norm: int, weights: Sequence[torch.Tensor | None], eps: float) -> list[torch.Tensor]:
+    """The normed and rotated tensors (one or two [B, L, H_i, D] of one dtype), contiguous."""
+    B, L, _, D = xs[0].shape
+    for i, x in enumerate(xs):
+        _check_heads(f"tensor {i}", x, xs[0].dtype, (B, L))
+        _require(x.shape[3] == D, "the tensors share one head_dim")
+    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    if B * L == 0 or any(x.shape[2] == 0 for x in xs):
+        _require(B * L == 0, "a tensor without heads")
+        return ys
+    turns, axis = rotary_turns(tuple(axis_dims), float(theta))
+    w_dt = weights[0].dtype if norm != NORM_NONE else torch.float32
+    with _Device(xs[0]):
+        _lib.check("mlora_rotary_axes", _lib.load().mlora_rotary_axes(
+            _lib.ptr_array([x.data_ptr() for x in xs]), _lib.ptr_array([y.data_ptr() for y in ys]),
+            _lib.ptr_array([_ptr(w) for w in weights]), _lib.i64_array([s for x in xs for s in _strides(x, 3)]),
+            _lib.i32_array([x.shape[2] for x in xs]), len(xs), _DT[xs[0].dtype], _DT[w_dt], norm, eps,
+            *_pos_args(positions, B, L), turns, axis, positions.shape[2], int(halves), B, L, D, _stream(xs[0])))
+    return ys
+
+
+def rotary_axes_backward(xs: Sequence[torch.Tensor] | None, gs: Sequence[torch.Tensor], positions: torch.Tensor,
+                         axis_dims: Sequence[int], *, theta: float, halves: bool, norm: int,
+                         weights: Sequence[torch.Tensor | None], eps: float, want_dx: Sequence[bool],
+                         want_dw: Sequence[bool]) -> tuple[list, list]:
+    """(dx, dw) lists of rotary_axes; None where not wanted."""
+    B, L, _, D = gs[0].shape
+    for i, g in enumerate(gs):
+        _check_heads(f"gradient {i}", g, gs[0].dtype, (B, L))
+        if norm != NORM_NONE:
+            _check_heads(f"tensor {i}", xs[i], gs[0].dtype, (B, L))
+            _require(xs[i].shape == g.shape, "a gradient has its tensor's shape")
+    dev = gs[0].device
+    dxs = [torch.empty(g.shape, dtype=g.dtype, device=dev) if w else None for g, w in zip(gs, want_dx)]
+    dws = [torch.empty(w.shape, dtype=w.dtype, device=dev) if k else None for w, k in zip(weights, want_dw)]
+    turns, axis = rotary_turns(tuple(axis_dims), float(theta))
+    heads = _lib.i32_array([g.shape[2] for g in gs])
+    lib = _lib.load()
+    nbytes = lib.mlora_rotary_axes_backward_workspace_bytes(heads, len(gs), norm, B, L, D) if any(want_dw) else 0
+    _lib.check("mlora_rotary_axes_backward_workspace_bytes", min(nbytes, 0))
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    w_dt = weights[0].dtype if norm != NORM_NONE else torch.float32
+    pos = _pos_args(positions, B, L)
+    with _Device(gs[0]):
+        _lib.check("mlora_rotary_axes_backward", lib.mlora_rotary_axes_backward(
+            _lib.ptr_array([x.data_ptr() for x in xs]) if norm != NORM_NONE else None,
+            _lib.ptr_array([g.data_ptr() for g in gs]), _lib.ptr_array([_ptr(d) for d in dxs]),
+            _lib.ptr_array([_ptr(w) for w in weights]), _lib.ptr_array([_ptr(d) for d in dws]),
+            _lib.i64_array([s for x in xs for s in _strides(x, 3)]) if norm != NORM_NONE else None,
+            _lib.i64_array([s for g in gs for s in _strides(g, 3)]), heads, len(gs), _DT[gs[0].dtype], _DT[w_dt], norm,
+            eps, *pos, turns, axis, positions.shape[2], int(halves), _ptr(ws), nbytes, B, L, D, _stream(gs[0])))
+    return dxs, dws
+
+
+def _vec(name: str, v: torch.Tensor | None, B: int, W: int) -> tuple:
+    """(pointer, dtype code, element stride per sample) of a [B or 1, W] vector, None allowed."""
+    if v is None:
+        return None, _lib.F32, 0
+    _require(v.is_cuda and v.dtype in _DT and v.dim() == 2 and v.shape[0] in (1, B) and v.shape[1] == W,
+             f"{name} must be a bfloat16 or float32 device tensor [{B} or 1, {W}]")
+    _require(rows_layout(v), f"{name} needs unit stride and 16-byte aligned rows")
+    return v.data_ptr(), _DT[v.dtype], _strides(v, 1)[0]
+
+
+def _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps):
+    B, T, W = x.shape
+    for name, t in (("x", x), ("y", y)):
+        _require(t.is_cuda and t.dtype in _DT and tuple(t.shape) == (B, T, W) and rows_layout(t),
+                 f"{name} must be a bfloat16 or float32 [{B}, {T}, {W}] device tensor with 16-byte aligned rows")
+    g_ptr, g_dt, g_sb = _vec("gate", gate, B, W)
+    s_ptr, s_dt, s_sb = _vec("scale", scale, B, W)
+    h_ptr, h_dt, h_sb = _vec("shift", shift, B, W)
+    _require(scale is None or shift is None or s_dt == h_dt, "scale and shift share a dtype")
+    p_ptr, p_dt, _ = _vec("post weight", post_w, 1, W)
+    post_kind = -1 if post is None else NORM_KINDS[post]
+    head = (x.data_ptr(), _DT[x.dtype], *_strides(x, 2), y.data_ptr(), _DT[y.dtype], *_strides(y, 2))
+    tail = (g_ptr, g_dt, g_sb, s_ptr, h_ptr, s_dt, s_sb, h_sb, int(unit_offset), p_ptr, p_dt, NORM_KINDS[norm],
+            post_kind, alpha, eps)
+    return head, tail
+
+
+def joint(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None, scale: torch.Tensor | None,
+          shift: torch.Tensor | None, post_w: torch.Tensor | None, *, norm: str, post: str | None, unit_offset: bool,
+          alpha: float, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """(x1, out) of the sublayer joint; vectors are [B or 1, W], post_w [1, W]."""
+    head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
+    x1 = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty(x.shape, dtype=y.dtype, device=x.device)
+    if x.numel():
+        with _Device(x):
+            _lib.check("mlora_joint", _lib.load().mlora_joint(*head, *tail, x1.data_ptr(), out.data_ptr(), *x.shape,
+                                                              _stream(x)))
+    return x1, out
+
+
+def joint_backward(x: torch.Tensor, y: torch.Tensor, gx: torch.Tensor | None, go: torch.Tensor | None,
+                   gate: torch.Tensor | None, scale: torch.Tensor | None, shift: torch.Tensor | None,
+                   post_w: torch.Tensor | None, *, norm: str, post: str | None, unit_offset: bool, alpha: float,
+                   eps: float, want: Sequence[bool]) -> list:
+    """[dx, dy, dgate, dscale, dshift, dpost] (None where not wanted); a [1, W] vector's gradient is summed
+    over the samples."""
+    B, T, W = x.shape
+    head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
+    for name, t, like in (("gx", gx, x), ("go", go, y)):
+        _require(t is None or (t.is_cuda and t.dtype == like.dtype and t.shape == x.shape and rows_layout(t)),
+                 f"{name} must have its output's shape and dtype, with 16-byte aligned rows")
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if w else None
+            for t, w in zip((x, y, gate, scale, shift, post_w), want)]
+    if W == 0:
+        return outs
+    lib = _lib.load()
+    nbytes = lib.mlora_joint_backward_workspace_bytes(B, T, W) if any(want[2:]) else 0
+    _lib.check("mlora_joint_backward_workspace_bytes", min(nbytes, 0))
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device) if nbytes else None
+    grads = [v for t in (gx, go) for v in ((None, 0, 0) if t is None else (t.data_ptr(), *_strides(t, 2)))]
+    shared = [int(v is not None and v.shape[0] == 1) for v in (gate, scale, shift)]
+    with _Device(x):
+        _lib.check("mlora_joint_backward", lib.mlora_joint_backward(
+            *head, *grads, *tail, *(_ptr(o) for o in outs), *shared, _ptr(ws), nbytes, B, T, W, _stream(x)))
+    return outs

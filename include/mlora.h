@@ -492,6 +492,78 @@ int mlora_f32_seg_outer_split(const void *p, int64_t ldp, int64_t M, int64_t C,
                               void *workspace, int64_t workspace_bytes,
                               void *stream);
 
+/* ------------------------------------------------------------------ rotary positions with several axes
+ *
+ * For n (1 or 2: q, or q and k) tensors x_i [batches, tokens, heads_i, head_dim] (bf16 or float32, unit
+ * stride in the head, element strides x_strides[3 i] (batch), [3 i + 1] (token), [3 i + 2] (head), each a
+ * multiple of 8, 16-byte aligned): an optional RMSNorm, then the rotation of every pair of a head by
+ * position · frequency, rounded once into y_i (contiguous, x's type).
+ *   norm     0 none; 1 over each head, weight w_i [head_dim]; 2 over the row, w_i [heads_i · head_dim]
+ *   halves   0: pair p is elements 2p, 2p + 1; 1: elements p, p + head_dim / 2
+ *   pos      [batches, tokens, n_axes] with unit axis stride (pos_stride_b 0: shared), pos_type 0 int32,
+ *            1 int64, 2 float32
+ *   turns    host array [head_dim / 2]: pair p's frequency / 2 pi; axis: host array [head_dim / 2], its axis.
+ *            mlora_rotary_turns fills both for theta^(-2 i / d) frequencies and axes of d = axis_dims[c]
+ *            channels each, in order (angles are formed and reduced in 64 bits)
+ * head_dim is a multiple of 16 up to 256, heads_i · head_dim at most 8192.
+ * Reference: rope_apply over a (frames, height, width) grid (wan/modules/model.py), and the q / k norms
+ * in front of it. */
+int mlora_rotary_turns(const int32_t *axis_dims, int32_t n_axes, double theta, double *turns, int32_t *axis);
+int mlora_rotary_axes(const void *const *xs, void *const *ys, const void *const *ws, const int64_t *x_strides,
+                      const int32_t *heads, int n, int dtype, int w_dtype, int norm, float eps,
+                      const void *pos, int pos_type, int64_t pos_stride_b, int64_t pos_stride_t,
+                      const double *turns, const int32_t *axis, int64_t n_axes, int halves,
+                      int64_t batches, int64_t tokens, int64_t head_dim, void *stream);
+
+/* Its gradients: dx_i (contiguous, x's type; NULL: not wanted) from the upstream g_i and, with a norm, x_i
+ * (without one xs may be NULL), and dw_i (w's shape and type; NULL: not wanted), summed in a fixed order
+ * through `workspace` (16-byte aligned, at least the queried bytes when some dw_i is wanted). */
+int64_t mlora_rotary_axes_backward_workspace_bytes(const int32_t *heads, int n, int norm, int64_t batches,
+                                                   int64_t tokens, int64_t head_dim);
+int mlora_rotary_axes_backward(const void *const *xs, const void *const *gs, void *const *dxs,
+                               const void *const *ws, void *const *dws, const int64_t *x_strides,
+                               const int64_t *g_strides, const int32_t *heads, int n, int dtype, int w_dtype,
+                               int norm, float eps, const void *pos, int pos_type, int64_t pos_stride_b,
+                               int64_t pos_stride_t, const double *turns, const int32_t *axis, int64_t n_axes,
+                               int halves, void *workspace, int64_t workspace_bytes,
+                               int64_t batches, int64_t tokens, int64_t head_dim, void *stream);
+
+/* ------------------------------------------------------------------ the joint of two sublayers
+ *
+ *   p = N_post(y) · post_w (or y);  u = alpha · x + gate · p;  x1 = u;  out = N(u) · m + shift
+ * with m = 1 + scale (unit_offset) or scale. x and x1 are bf16 or float32, y and out bf16 or float32 (a
+ * bf16 x needs a bf16 y); rows [batches, tokens, width] with 16-byte aligned row starts (element strides
+ * multiples of 8), x1 and out contiguous. Each output is rounded once from float32 arithmetic.
+ *   norm   0 LayerNorm, 1 RMSNorm;  post  -1 none, else as norm
+ *   gate, scale, shift: [batches, width] with an element stride per sample (0: shared), bf16 or float32,
+ *          scale and shift of one type; post_w [width]. NULL: 1, 1, 0, 1 (a shift needs a scale).
+ * width is a multiple of 8 up to 8192.
+ * Reference: x + y · e[2], then the modulated norm that opens the next sublayer (wan/modules/model.py:298-313). */
+int mlora_joint(const void *x, int x_dtype, int64_t x_stride_b, int64_t x_stride_t,
+                const void *y, int y_dtype, int64_t y_stride_b, int64_t y_stride_t,
+                const void *gate, int gate_dtype, int64_t gate_stride_b,
+                const void *scale, const void *shift, int affine_dtype, int64_t scale_stride_b, int64_t shift_stride_b,
+                int unit_offset, const void *post_w, int post_dtype, int norm, int post, float alpha, float eps,
+                void *x1, void *out, int64_t batches, int64_t tokens, int64_t width, void *stream);
+
+/* Its gradients from gx (of x1, x's type) and go (of out, y's type), either NULL for zero: dx, dy (contiguous;
+ * NULL: not wanted), and dgate / dscale / dshift ([batches, width], or [width] summed over the samples where
+ * the *_shared flag is set) and dpost [width] in their vectors' types (NULL: not wanted), summed in a fixed
+ * order through `workspace` (16-byte aligned, the queried bytes, needed when some vector's gradient is wanted). */
+int64_t mlora_joint_backward_workspace_bytes(int64_t batches, int64_t tokens, int64_t width);
+int mlora_joint_backward(const void *x, int x_dtype, int64_t x_stride_b, int64_t x_stride_t,
+                         const void *y, int y_dtype, int64_t y_stride_b, int64_t y_stride_t,
+                         const void *gx, int64_t gx_stride_b, int64_t gx_stride_t,
+                         const void *go, int64_t go_stride_b, int64_t go_stride_t,
+                         const void *gate, int gate_dtype, int64_t gate_stride_b,
+                         const void *scale, const void *shift, int affine_dtype,
+                         int64_t scale_stride_b, int64_t shift_stride_b, int unit_offset,
+                         const void *post_w, int post_dtype, int norm, int post, float alpha, float eps,
+                         void *dx, void *dy, void *dgate, void *dscale, void *dshift, void *dpost,
+                         int gate_shared, int scale_shared, int shift_shared,
+                         void *workspace, int64_t workspace_bytes,
+                         int64_t batches, int64_t tokens, int64_t width, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
