@@ -21,6 +21,7 @@ Public API:
     fused_tensor4d_component_gradient      its fused backward
     ModulatedLayerNormFunction, modulated_layer_norm   the same as one autograd op
     rotary_axes, rotary_axes_qk, grid_positions, RotaryAxesFunction   rotary positions with several axes, q / k norms
+    cross_attention, CrossAttentionFunction   attention to an encoder's states of another length
     gated_residual_norm, GatedResidualNormFunction   the joint of two sublayers: norm after, gate, residual, norm before
     load_library()                       load libmlora.so (raises if missing)
 
@@ -48,6 +49,7 @@ from .modulated_norm import (ModulatedLayerNormFunction, fused_bf16_layernorm_mo
                              fused_modulated_norm_materialization, fused_reduced_component_gradient,
                              fused_tensor4d_component_gradient, modulated_layer_norm)
 from .rotary import RotaryAxesFunction, grid_positions, rotary_axes, rotary_axes_qk
+from .attention import CrossAttentionFunction, cross_attention
 from .joint import GatedResidualNormFunction, gated_residual_norm
 
 
@@ -70,5 +72,5 @@ __all__ = [
     "fused_layernorm_modulation_hidden_backward", "fused_reduced_component_gradient",
     "fused_tensor4d_component_gradient", "ModulatedLayerNormFunction", "modulated_layer_norm",
     "RotaryAxesFunction", "grid_positions", "rotary_axes", "rotary_axes_qk", "GatedResidualNormFunction",
-    "gated_residual_norm",
+    "gated_residual_norm", "CrossAttentionFunction", "cross_attention",
 ]

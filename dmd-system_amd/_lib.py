@@ -103,6 +103,13 @@ SIGNATURES = {
     "mlora_joint_backward": (_int, [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
                                     _vp, _int, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _int, _int, _int, _f32, _f32,
                                     _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "mlora_cross_attention_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "mlora_cross_attention": (_int, [_vp, _pi64, _vp, _pi64, _vp, _pi64, _int, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _i64,
+                                     _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "mlora_cross_attention_backward_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "mlora_cross_attention_backward": (_int, [_vp, _pi64, _vp, _pi64, _vp, _pi64, _int, _vp, _vp, _i64, _f32, _vp, _vp,
+                                              _vp, _pi64, _vp, _vp, _vp, _vp, _i64,
+                                              _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
 }
 
 _LIB = None

@@ -983,3 +983,72 @@ def joint_backward(x: torch.Tensor, y: torch.Tensor, gx: torch.Tensor | None, go
         _lib.check("mlora_joint_backward", lib.mlora_joint_backward(
             *head, *grads, *tail, *(_ptr(o) for o in outs), *shared, _ptr(ws), nbytes, B, T, W, _stream(x)))
     return outs
+
+
+ATTENTION_MAX_STRIDE = 1 << 22  # token strides of q, k, v stay below this (elements)
+
+
+def attention_layout(t: torch.Tensor) -> bool:
+    """Whether the attention kernels take a [B, L, heads, D] operand as it lies."""
+    return rows_layout(t) and (t.numel() == 0 or t.shape[1] < 2 or t.stride(1) < ATTENTION_MAX_STRIDE)
+
+
+def _attention_args(q, k, v, key_lengths, key_mask, scale):
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    for name, t, shape in (("q", q, (B, Lq, H, D)), ("k", k, (B, Lk, Hk, D)), ("v", v, (B, Lk, Hk, D))):
+        _require(t.is_cuda and t.dtype == q.dtype and t.dtype in _DT and tuple(t.shape) == shape and attention_layout(t),
+                 f"{name} must be a [batch, tokens, heads, head_dim] device tensor of q's dtype with 16-byte aligned heads "
+                 f"and a token stride below {ATTENTION_MAX_STRIDE}")
+    _require(key_lengths is None or (key_lengths.is_cuda and key_lengths.dtype == torch.int32
+                                     and tuple(key_lengths.shape) == (B,) and key_lengths.is_contiguous()),
+             f"key_lengths must be a contiguous int32 device vector of {B}")
+    _require(key_mask is None or (key_mask.is_cuda and key_mask.dtype == torch.bool and key_mask.dim() == 2
+                                  and key_mask.shape[0] in (1, B) and key_mask.shape[1] == Lk
+                                  and (key_mask.stride(1) == 1 or Lk < 2)),
+             f"key_mask must be a bool device tensor [{B} or 1, {Lk}] with unit stride")
+    operands = [a for t in (q, k, v) for a in (t.data_ptr(), _lib.i64_array(_strides(t, 3)))]
+    mask = (None, 0) if key_mask is None else (key_mask.data_ptr(), _strides(key_mask, 1)[0])
+    return (*operands, _DT[q.dtype], _ptr(key_lengths), *mask, scale), (B, Lq, Lk, H, Hk, D)
+
+
+@functools.lru_cache(maxsize=512)
+def _attention_workspace(name: str, dtype: int, sizes: tuple) -> int:
+    nbytes = getattr(_lib.load(), name)(dtype, *sizes)
+    _lib.check(name, min(nbytes, 0))
+    return nbytes
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_lengths: torch.Tensor | None,
+                    key_mask: torch.Tensor | None, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse) of softmax(scale q kᵀ) v over the keys that count; lse [B, H, Lq] float32, base 2."""
+    args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
+    B, Lq, _, H, _, _ = sizes
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
+    nbytes = _attention_workspace("mlora_cross_attention_workspace_bytes", _DT[q.dtype], sizes)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
+    with _Device(q):
+        _lib.check("mlora_cross_attention", _lib.load().mlora_cross_attention(
+            *args, out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, *sizes, _stream(q)))
+    return out, lse
+
+
+def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+                             g: torch.Tensor, *, key_lengths: torch.Tensor | None, key_mask: torch.Tensor | None,
+                             scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv), contiguous, from the forward's out and lse and the upstream gradient g of out."""
+    args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
+    for name, t in (("out", out), ("g", g)):
+        _require(t.is_cuda and t.dtype == q.dtype and t.shape == q.shape, f"{name} must have q's shape and dtype")
+    _require(out.is_contiguous() and attention_layout(g), "out is contiguous, g's heads are 16-byte aligned")
+    _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == q.shape[0] * q.shape[1] * q.shape[2],
+             "lse is the forward's [batch, heads, tokens]")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    nbytes = _attention_workspace("mlora_cross_attention_backward_workspace_bytes", _DT[q.dtype], sizes)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
+    with _Device(q):
+        _lib.check("mlora_cross_attention_backward", _lib.load().mlora_cross_attention_backward(
+            *args, out.data_ptr(), lse.data_ptr(), g.data_ptr(), _lib.i64_array(_strides(g, 3)),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes, *sizes, _stream(q)))
+    return dq, dk, dv

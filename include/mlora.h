@@ -564,6 +564,38 @@ int mlora_joint_backward(const void *x, int x_dtype, int64_t x_stride_b, int64_t
                          void *workspace, int64_t workspace_bytes,
                          int64_t batches, int64_t tokens, int64_t width, void *stream);
 
+/* ------------------------------------------------------------------ attention to an encoder's states
+ *
+ * out = softmax(scale · q kᵀ) v per head, q [B, Lq, H, D], k and v [B, Lk, Hk, D] (bf16 or float32, one type;
+ * unit stride in the head, element strides {batch, token, head}, multiples of 8, token strides below 2^22,
+ * 16-byte aligned); query head h reads key head h / (H / Hk). D is a multiple of 8 up to 128, scale > 0.
+ *   key_lengths  device int32 [B] or NULL: sample b has its first key_lengths[b] keys (clamped to [0, Lk])
+ *   key_mask     device bytes [B, Lk] (batch stride in bytes, 0: shared; unit key stride) or NULL: keys
+ *                with a zero byte do not count
+ * Whatever k and v hold at keys that do not count is not used. A query without keys gets zeros. out
+ * [B, Lq, H, D] contiguous; lse [B, H, Lq] float32: base-2 logarithm of the sum of 2^(score · log2 e), +inf for
+ * a query without keys (the backward reads it). workspace (16-byte aligned, the queried bytes, 0: may be
+ * NULL) holds partial sums where few rows meet many keys.
+ * Reference: flash_attention(q, k, v, k_lens=context_lens) of WanT2VCrossAttention (wan/modules/model.py). */
+int64_t mlora_cross_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk,
+                                              int64_t D);
+int mlora_cross_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                          const void *v, const int64_t *v_strides, int dtype, const int32_t *key_lengths,
+                          const uint8_t *key_mask, int64_t key_mask_stride_b, float scale, void *out, float *lse,
+                          void *workspace, int64_t workspace_bytes,
+                          int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, void *stream);
+
+/* Its gradients for the upstream g ([B, Lq, H, D], strided like q): dq, dk, dv contiguous, zeros at keys that do
+ * not count. out and lse are the forward's. Sums have a fixed order. */
+int64_t mlora_cross_attention_backward_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                                                       int64_t Hk, int64_t D);
+int mlora_cross_attention_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                                   const void *v, const int64_t *v_strides, int dtype, const int32_t *key_lengths,
+                                   const uint8_t *key_mask, int64_t key_mask_stride_b, float scale,
+                                   const void *out, const float *lse, const void *g, const int64_t *g_strides,
+                                   void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes,
+                                   int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
