@@ -80,15 +80,19 @@ struct HeadTile {
 template <class T, int DP>
 struct FragReader;
 
+// rows<OFF, R0>: rows R0 + lane % 32 (R0 a multiple of 32) of the tile OFF bytes past the reader's base, contraction
+// elements 16s + 8h .. + 7 of the row. cols<OFF, R0>: columns 32d + lane % 32, contraction over rows R0 + perm(h, j) (R0 a
+// multiple of 16).
 template <int DP>
 struct FragReader<uint16_t, DP> {
   using Tile = HeadTile<uint16_t, DP>;
-  int32_t row[DP / 16];     // row lane % 32, chunk of step s
+  int32_t row[DP / 16];     // LDS address of row lane % 32, chunk of step s
   int32_t col[DP / 32][2];  // transposed: d block, first and second group of four rows
-  __device__ __forceinline__ void init(int lane) {
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
+    const int32_t at = (int32_t)(uintptr_t)base;
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) row[s] = r * Tile::RB + (((2 * s + h) ^ Tile::swz(r)) << 4);
+    for (int s = 0; s < DP / 16; ++s) row[s] = at + r * Tile::RB + (((2 * s + h) ^ Tile::swz(r)) << 4);
     // group g of 16 lanes: columns 16·(g & 1) .. + 15 of the block, rows 4·(g >> 1) + e; lane m = 4e + c of
     // the group addresses row e, columns 4c .. 4c + 3, and receives column m of the four rows
     const int g = lane >> 4, m = lane & 15, e = m >> 2, c = m & 3;
@@ -97,19 +101,27 @@ struct FragReader<uint16_t, DP> {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int key = 8 * w + 4 * (g >> 1) + e, chunk = 4 * d + 2 * (g & 1) + (c >> 1);
-        col[d][w] = key * Tile::RB + ((chunk ^ Tile::swz(key)) << 4) + 8 * (c & 1);
+        col[d][w] = at + key * Tile::RB + ((chunk ^ Tile::swz(key)) << 4) + 8 * (c & 1);
       }
   }
-  // rows r0 + lane % 32 (r0 a multiple of 32), contraction elements 16s + 8h .. + 7 of the row
-  __device__ __forceinline__ void rows(const MLORA_LDS char *t, int r0, int s, Frag<uint16_t> &f) const {
-    f.v = *(const lds_u4 *)(t + row[s] + r0 * Tile::RB);
+  // the other buffer: every address ^ by (the base and the tiles of a buffer within an aligned block of `by` bytes)
+  __device__ __forceinline__ void flip(int by) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) row[s] ^= by;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) col[d][0] ^= by, col[d][1] ^= by;
   }
-  // columns 32d + lane % 32, contraction over rows r0 + perm(h, j) (r0 a multiple of 16)
-  __device__ __forceinline__ void cols(const MLORA_LDS char *t, int r0, int d, Frag<uint16_t> &f) const {
+  template <int OFF, int R0>
+  __device__ __forceinline__ void rows(int s, Frag<uint16_t> &f) const {
+    f.v = *(const lds_u4 *)((const MLORA_LDS char *)(uintptr_t)(uint32_t)row[s] + OFF + R0 * Tile::RB);
+  }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void cols(int d, Frag<uint16_t> &f) const {
     typedef MLORA_LDS bf16x4 lds_b4;
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)(t + col[d][0] + r0 * Tile::RB));
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)(t + col[d][1] + r0 * Tile::RB));
-    const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+    const MLORA_LDS char *p = (const MLORA_LDS char *)(uintptr_t)(uint32_t)col[d][0] + OFF + R0 * Tile::RB;
+    const MLORA_LDS char *r = (const MLORA_LDS char *)(uintptr_t)(uint32_t)col[d][1] + OFF + R0 * Tile::RB;
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)p));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)r));
     f.v = u32x4{x[0], x[1], y[0], y[1]};
   }
 };
@@ -117,22 +129,26 @@ struct FragReader<uint16_t, DP> {
 template <int DP>
 struct FragReader<float, DP> {
   using Tile = HeadTile<float, DP>;
-  int32_t base, sw, h, lane32;
-  __device__ __forceinline__ void init(int lane) {
-    lane32 = lane & 31, h = lane >> 5, base = lane32 * Tile::RB, sw = Tile::swz(lane32);
+  int32_t row, col, sw, h, lane32;
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
+    lane32 = lane & 31, h = lane >> 5, sw = Tile::swz(lane32);
+    col = (int32_t)(uintptr_t)base, row = col + lane32 * Tile::RB;
   }
-  __device__ __forceinline__ void rows(const MLORA_LDS char *t, int r0, int s, Frag<float> &f) const {
-    const f32x4 a = *(const lds_f4 *)(t + base + r0 * Tile::RB + (((4 * s + 2 * h) ^ sw) << 4));
-    const f32x4 b = *(const lds_f4 *)(t + base + r0 * Tile::RB + (((4 * s + 2 * h + 1) ^ sw) << 4));
+  __device__ __forceinline__ void flip(int by) { row ^= by, col ^= by; }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void rows(int s, Frag<float> &f) const {
+    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)row + OFF + R0 * Tile::RB;
+    const f32x4 a = *(const lds_f4 *)(t + (((4 * s + 2 * h) ^ sw) << 4)), b = *(const lds_f4 *)(t + (((4 * s + 2 * h + 1) ^ sw) << 4));
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.v[j] = a[j], f.v[j + 4] = b[j];
   }
-  __device__ __forceinline__ void cols(const MLORA_LDS char *t, int r0, int d, Frag<float> &f) const {
-    const int chunk = 8 * d + (lane32 >> 2);
+  template <int OFF, int R0>
+  __device__ __forceinline__ void cols(int d, Frag<float> &f) const {
+    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)col + OFF;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int r = 8 * (j / 4) + 4 * h + j % 4;  // r0 is a multiple of 16: swz(r0 + r) = swz(r)
-      f.v[j] = *(const MLORA_LDS float *)(t + (r0 + r) * Tile::RB + ((chunk ^ Tile::swz(r)) << 4) + 4 * (lane32 & 3));
+      const int r = 8 * (j / 4) + 4 * h + j % 4, chunk = 8 * d + (lane32 >> 2);  // swz(R0 + r) = swz(r)
+      f.v[j] = *(const MLORA_LDS float *)(t + (R0 + r) * Tile::RB + ((chunk ^ Tile::swz(r)) << 4) + 4 * (lane32 & 3));
     }
   }
 };

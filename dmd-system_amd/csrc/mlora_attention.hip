@@ -24,7 +24,7 @@ struct AttnArgs {
   const uint8_t *mask;
   float *part_o, *part_ml;  // splits: [splits][B·Hk·rows][D] sums and [splits][B·Hk·rows][2] (m, l)
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, mask_sb;
-  int32_t batches, Lq, Lk, H, Hk, G, D, rows, row_tiles, splits, split_tiles;
+  int32_t batches, Lq, Lk, H, Hk, G, D, rows, row_tiles, turns, splits, split_tiles;
   float c;            // scale · log2 e
 };
 
@@ -32,14 +32,17 @@ struct AttnArgs {
 template <int KT>
 struct KeyMask {
   const uint8_t *mask;  // null: no mask
-  int len;
+  int len;              // keys from here on do not count (the sample's length, or the split's end before it)
   __device__ __forceinline__ int byte(int tile, int lane) const {  // of key tile·KT + lane
-    const int key = tile * KT + lane;
-    return mask != nullptr && lane < KT && key < len ? mask[key] : 1;
+    if (mask == nullptr) return 1;
+    return mask[max(min(tile * KT + (lane & (KT - 1)), len - 1), 0)];
   }
   __device__ __forceinline__ uint64_t bits(int tile, int lane_byte) const {
     uint64_t b = low_bits(min(len - tile * KT, KT));
-    if (mask != nullptr) b &= __ballot(lane_byte != 0);
+    if (mask != nullptr) {
+      asm volatile("" : "+v"(lane_byte));  // looked at here and not where it was loaded
+      b &= __ballot(lane_byte != 0);
+    }
     return b;
   }
 };
@@ -48,15 +51,21 @@ __device__ __forceinline__ int sample_keys(const AttnArgs &a, int b) {
   return a.lengths == nullptr ? a.Lk : min(max(a.lengths[b], 0), a.Lk);
 }
 
-__device__ __forceinline__ void load_frag(const uint16_t *p, bool on, Frag<uint16_t> &f) {
-  f.v = on ? *(const MLORA_GLOBAL u32x4 *)p : u32x4{0, 0, 0, 0};
-}
-__device__ __forceinline__ void load_frag(const float *p, bool on, Frag<float> &f) {
-  const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-  const f32x4 a = on ? *(const MLORA_GLOBAL f32x4 *)p : z, b = on ? *(const MLORA_GLOBAL f32x4 *)(p + 4) : z;
+// 8 elements at base + off, or zeros (base itself is always readable: no branch around the load).
+__device__ __forceinline__ void load_frag(const uint16_t *base, int64_t off, bool on, Frag<uint16_t> &f) {
+  const u32x4 v = *(const MLORA_GLOBAL u32x4 *)(base + (on ? off : 0));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) f.v[j] = a[j], f.v[j + 4] = b[j];
+  for (int j = 0; j < 4; ++j) f.v[j] = on ? v[j] : 0;
 }
+__device__ __forceinline__ void load_frag(const float *base, int64_t off, bool on, Frag<float> &f) {
+  const float *p = base + (on ? off : 0);
+  const f32x4 a = *(const MLORA_GLOBAL f32x4 *)p, b = *(const MLORA_GLOBAL f32x4 *)(p + 4);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f.v[j] = on ? a[j] : 0.f, f.v[j + 4] = on ? b[j] : 0.f;
+}
+
+// The running maximum before any key: finite, so that 2^(−inf − m) is 0 and not NaN where a block has no live key.
+constexpr float kNoMax = -1e30f;
 
 // The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step.
 template <class T, int DP, int NQ, int KT>
@@ -68,7 +77,7 @@ struct Softmax {
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      m[n] = -INFINITY, l[n] = 0.f;
+      m[n] = kNoMax, l[n] = 0.f;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -76,25 +85,26 @@ struct Softmax {
     }
   }
 
-  // One tile of keys in LDS with at least one live bit.
-  __device__ __forceinline__ void step(const FragReader<T, DP> &fr, const MLORA_LDS char *kt, const MLORA_LDS char *vt,
-                                       uint64_t bits, float c, int lane) {
+  // One tile of keys KOFF bytes from the reader's base, V at VOFF.
+  template <int KOFF, int VOFF>
+  __device__ __forceinline__ void step(const FragReader<T, DP> &fr, uint64_t bits, float c, int lane) {
     constexpr int NB = KT / 32;
     f32x16 s[NQ][NB];
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][kb][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
+    for (int ks = 0; ks < DP / 16; ++ks)  // the blocks' sums in turn: a sum waits for its last product
+      static_for<NB>([&](auto kb) __attribute__((always_inline)) {
         Frag<T> kf;
-        fr.rows(kt, 32 * kb, ks, kf);
+        fr.template rows<KOFF, 32 * decltype(kb)::value>(ks, kf);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s[n][kb] = mma16(kf, q[n][ks], s[n][kb]);
-      }
-    }
+        return true;
+      });
     if (bits != low_bits(KT)) {
       const uint64_t mine = bits >> (4 * (lane >> 5));
 #pragma unroll
@@ -133,28 +143,28 @@ struct Softmax {
       }
       l[n] += frag_sum(p[n]);
     }
-#pragma unroll
-    for (int ks = 0; ks < KT / 16; ++ks)
+    static_for<KT / 16>([&](auto ks) __attribute__((always_inline)) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         Frag<T> vf;
-        fr.cols(vt, 16 * ks, d, vf);
+        fr.template cols<VOFF, 16 * decltype(ks)::value>(d, vf);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][d] = mma16(vf, p[n][ks], o[n][d]);
       }
+      return true;
+    });
   }
 
-  // The sum of the weights as the product with V sees them.
+  // The sum of the weights as the product with V sees them (bf16: two per v_dot2_f32_bf16 with ones).
   static __device__ __forceinline__ float frag_sum(const Frag<T> (&p)[KT / 16]) {
     float t = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
       if constexpr (sizeof(T) == 2) {
+        const auto ones = __builtin_bit_cast(bf16x2, 0x3f803f80u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          t += __uint_as_float(p[ks].v[j] << 16);
-          t += __uint_as_float(p[ks].v[j] & 0xffff0000u);
-        }
+        for (int j = 0; j < 4; ++j)
+          t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)p[ks].v[j]), ones, t, false);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) t += p[ks].v[j];
@@ -170,25 +180,44 @@ __device__ __forceinline__ int64_t row_at(int r, int Lq, int64_t sl, int64_t sh)
   return g * sh + i * sl;
 }
 
-// Writes NQ x 32 rows of the O^T registers (times f[n]) to out, 8 or 16 bytes per lane and store.
+// Writes NQ x 32 rows of the O^T registers (times f[n]) to out. The halves of a column hold alternating groups of
+// four channels; they swap groups, so that a lane has eight neighbouring channels: one 16-byte store of bf16.
 template <class T, int DP, int NQ>
 __device__ __forceinline__ void store_rows(T *base, const f32x16 (&o)[NQ][DP / 32], const float (&f)[NQ], int row0, int rows,
                                            int Lq, int64_t sl, int64_t sh, int D, int lane) {
+  auto swap = [](uint32_t &x, uint32_t &y) __attribute__((always_inline)) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0], y = r[1];
+  };
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int r = row0 + 32 * n + (lane & 31);
-    if (r >= rows) continue;
-    T *p = base + row_at(r, Lq, sl, sh) + 4 * (lane >> 5);
+    T *p = base + row_at(min(r, rows - 1), Lq, sl, sh) + 8 * (lane >> 5);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = 32 * d + 8 * i;
-        if (at >= D) continue;  // the head dimension is a multiple of 8
-        const float x0 = o[n][d][4 * i] * f[n], x1 = o[n][d][4 * i + 1] * f[n], x2 = o[n][d][4 * i + 2] * f[n],
-                    x3 = o[n][d][4 * i + 3] * f[n];
-        if constexpr (sizeof(T) == 2) *(MLORA_GLOBAL u32x2 *)(p + at) = u32x2{pack2_bf16(x0, x1), pack2_bf16(x2, x3)};
-        else *(MLORA_GLOBAL f32x4 *)(p + at) = f32x4{x0, x1, x2, x3};
+      for (int i = 0; i < 4; i += 2) {
+        const int at = 32 * d + 8 * i + 8 * (lane >> 5);  // the head dimension is a multiple of 8
+        uint32_t x[4], y[4];
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[j] = pack2_bf16(o[n][d][4 * i + 2 * j] * f[n], o[n][d][4 * i + 2 * j + 1] * f[n]);
+            y[j] = pack2_bf16(o[n][d][4 * i + 4 + 2 * j] * f[n], o[n][d][4 * i + 5 + 2 * j] * f[n]);
+            swap(x[j], y[j]);
+          }
+          if (r < rows && at < D) *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i) = u32x4{x[0], x[1], y[0], y[1]};
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = __float_as_uint(o[n][d][4 * i + j] * f[n]), y[j] = __float_as_uint(o[n][d][4 * i + 4 + j] * f[n]);
+            swap(x[j], y[j]);
+          }
+          if (r < rows && at < D) {
+            *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i) = u32x4{x[0], x[1], x[2], x[3]};
+            *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i + 4) = u32x4{y[0], y[1], y[2], y[3]};
+          }
+        }
       }
   }
 }
@@ -198,24 +227,28 @@ struct AttnTile {
   static constexpr int KT = sizeof(T) == 2 ? 64 : 32;  // keys per tile: 16 KB of K and of V at 128 channels
 };
 
-// Four waves of NQ x 32 rows each against the same key tiles, two buffers of K and V in LDS: tile t + 1 loads
-// while tile t is multiplied; one barrier per tile.
-template <class T, int DP, int NQ>
-__global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attn_fwd_kernel(const AttnArgs a) {
+// Four waves of 32 rows each against the same key tiles, two buffers of K and V in LDS: tile t + 1 loads while tile
+// t is multiplied; one barrier per tile. A workgroup takes `turns` row tiles of one head in a row: the key tiles
+// go on loading from one to the next, and the next rows' q arrives under the present ones' products (with one row
+// tile per workgroup and 512 keys, every workgroup waits for q and its first keys, in step with all others).
+template <class T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(const AttnArgs a) {
   constexpr int KT = AttnTile<T>::KT;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024 / 4;
   __shared__ u32x4 smem[4 * TB / 16];  // K, V of buffer 0, K, V of buffer 1
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
-  int id = xcd_contiguous(blockIdx.x, gridDim.x);  // one key head's row tiles stay on one XCD's L2
-  const int rt = id % a.row_tiles;
-  id /= a.row_tiles;
-  const int sp = id % a.splits;
-  id /= a.splits;
-  const int hk = id % a.Hk, b = id / a.Hk;
-  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, sample_keys(a, b)};
-  const int t0 = sp * a.split_tiles, t1 = min(t0 + a.split_tiles, (km.len + KT - 1) / KT);
+  int id = blockIdx.x;  // heads first: rows of all heads are read together, whole token rows of memory
+  const int hk = id % a.Hk;
+  id /= a.Hk;
+  const int groups = (a.row_tiles + a.turns - 1) / a.turns;
+  const int rt0 = id % groups * a.turns, rt1 = min(rt0 + a.turns, a.row_tiles);
+  id /= groups;
+  const int sp = id % a.splits, b = id / a.splits;
+  const int t0 = sp * a.split_tiles;
+  const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)sample_keys(a, b)), t1 = (end + KT - 1) / KT;
+  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, end};
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
   TileLoader<T, DP, N> kl, vl;
@@ -224,68 +257,71 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attn_fwd_kernel(const At
     kl.load(kp + (int64_t)t * KT * a.k_sl, bits, lds + buf * 2 * TB);
     vl.load(vp + (int64_t)t * KT * a.v_sl, bits, lds + buf * 2 * TB + TB);
   };
+  auto after = [&](int t) __attribute__((always_inline)) { return t + 1 < t1 ? t + 1 : t0; };  // the tiles go round
   uint64_t bits = 0, next = 0;
   if (t0 < t1) {
     bits = km.bits(t0, km.byte(t0, lane));
     stage(t0, 0, bits);
-    next = km.bits(t0 + 1, km.byte(t0 + 1, lane));
+    next = km.bits(after(t0), km.byte(after(t0), lane));
   }
   FragReader<T, DP> fr;
-  fr.init(lane);
-  Softmax<T, DP, NQ, KT> sm;
-  sm.init();
-  const int row0 = (rt * 4 + wave) * 32 * NQ;
+  fr.init(lane, lds);
+  Softmax<T, DP, 1, KT> sm;
   const T *qp = static_cast<const T *>(a.q) + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const T *p = qp + row_at(min(row0 + 32 * n + (lane & 31), a.rows - 1), a.Lq, a.q_sl, a.q_sh);
+  Frag<T> qn[DP / 16];
+  auto load_q = [&](int rt) __attribute__((always_inline)) {
+    const T *p = qp + row_at(min((rt * 4 + wave) * 32 + (lane & 31), a.rows - 1), a.Lq, a.q_sl, a.q_sh);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
-      load_frag(p + d, d < a.D, sm.q[n][s]);
+      load_frag(p, d, d < a.D, qn[s]);
     }
-  }
-  auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
-    wait_vmcnt<0>();
-    lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    int byte = 1;
-    if (t + 1 < t1) {
-      stage(t + 1, B ^ 1, next);
-      byte = km.byte(t + 2, lane);
-    }
-    if (bits != 0) sm.step(fr, lds + B * 2 * TB, lds + B * 2 * TB + TB, bits, a.c, lane);
-    bits = next;
-    next = km.bits(t + 2, byte);
   };
-  for (int t = t0; t < t1; t += 2) {
-    turn(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t1) turn(std::integral_constant<int, 1>{}, t + 1);
-  }
-  const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
-  if (a.splits > 1) {
-    const int64_t all = (int64_t)a.batches * a.Hk * a.rows, first = sp * all + head_rows;
-    float one[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      one[n] = 1.f;
-      const float l = half_sum(sm.l[n]);
-      const int r = row0 + 32 * n + lane;
-      if (lane < 32 && r < a.rows) *(float2 *)(a.part_ml + 2 * (first + r)) = float2{sm.m[n], l};
-    }
-    store_rows<float, DP, NQ>(a.part_o + first * a.D, sm.o, one, row0, a.rows, a.rows, a.D, 0, a.D, lane);
-    return;
-  }
-  float inv[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const float l = half_sum(sm.l[n]);
-    inv[n] = l > 0.f || l != l ? 1.0f / l : 0.f;
-    const int r = row0 + 32 * n + lane;
-    if (lane < 32 && r < a.rows) a.lse[head_rows + r] = l > 0.f ? sm.m[n] + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
-  }
+  load_q(rt0);
+  const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows, all = (int64_t)a.batches * a.Hk * a.rows;
   T *op = static_cast<T *>(a.out) + ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
-  store_rows<T, DP, NQ>(op, sm.o, inv, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
+  constexpr int kLoadsQ = DP / 16 * sizeof(T) / 2;
+  int buf = 0;
+  for (int rt = rt0; rt < rt1; ++rt) {
+    sm.init();
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) sm.q[0][s] = qn[s];
+    for (int t = t0; t < t1; ++t) {
+      // the tile's loads: the next rows' q, asked for behind them, need not be there yet; at the first tile of later
+      // rows they were waited for before the stores, which nothing waits for
+      if (t == t0 + 1) wait_vmcnt<kLoadsQ>();
+      else if (t > t0 || rt == rt0) wait_vmcnt<0>();
+      lds_pipeline_barrier();  // tile t is in LDS, and every wave has read the tile before it
+      buf ^= 1;
+      stage(after(t), buf, rt + 1 < rt1 || t + 1 < t1 ? next : 0);  // behind the last one nothing is read
+      const int byte = km.byte(after(after(t)), lane);
+      if (t == t0) {  // kept between the tile's loads and the next wait, which counts them
+        asm volatile("" ::: "memory");
+        load_q(min(rt + 1, rt1 - 1));
+        asm volatile("" ::: "memory");
+      }
+      if (bits != 0) sm.template step<0, TB>(fr, bits, a.c, lane);
+      fr.flip(2 * TB);
+      bits = next;
+      next = km.bits(after(after(t)), byte);
+    }
+    const int row0 = (rt * 4 + wave) * 32, r = row0 + (lane & 31);
+    const float l = half_sum(sm.l[0]);
+    if (t1 - t0 == 1) wait_vmcnt<kLoadsQ>();  // the next rows' first tile
+    else wait_vmcnt<0>();
+    if (a.splits > 1) {
+      const int64_t first = sp * all + head_rows;
+      const float one[1] = {1.f};
+      if (lane < 32 && r < a.rows) *(float2 *)(a.part_ml + 2 * (first + r)) = float2{sm.m[0], l};
+      store_rows<float, DP, 1>(a.part_o + first * a.D, sm.o, one, row0, a.rows, a.rows, a.D, 0, a.D, lane);
+    } else {
+      const float inv[1] = {l > 0.f || l != l ? 1.0f / l : 0.f};
+      const float lse = l > 0.f ? sm.m[0] + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+      if (lane < 32 && r < a.rows) a.lse[head_rows + r] = lse;
+      store_rows<T, DP, 1>(op, sm.o, inv, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
+    }
+  }
+  wait_vmcnt<0>();
 }
 
 // Few rows (at most 32 NQ per key head): the NW waves take different key tiles, each with its own buffers (no
@@ -301,16 +337,18 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024;
   static_assert(NW * NQ * ND * 4 * 64 * 16 <= 4 * TB * NW, "the waves' sums fit the buffers");
-  __shared__ u32x4 smem[4 * TB * NW / 16];
-  __shared__ float2 ml[NW][NQ][32];
+  // one array, so that the readers' buffers start at multiples of 4 TB; (m, l) of [wave][n][query] behind them
+  __shared__ u32x4 smem[4 * TB * NW / 16 + NW * NQ * 16];
+  float2 (&ml)[NW][NQ][32] = *(float2 (*)[NW][NQ][32])(smem + 4 * TB * NW / 16);
   const int wave = wave_id(), lane = threadIdx.x & 63;
   MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 4 * TB;
   int id = blockIdx.x;
   const int sp = id % a.splits;
   id /= a.splits;
   const int hk = id % a.Hk, b = id / a.Hk;
-  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, sample_keys(a, b)};
-  const int t0 = sp * a.split_tiles + wave, t1 = min((sp + 1) * a.split_tiles, (km.len + KT - 1) / KT);
+  const int t0 = sp * a.split_tiles + wave;
+  const int end = (int)min((int64_t)(sp + 1) * a.split_tiles * KT, (int64_t)sample_keys(a, b)), t1 = (end + KT - 1) / KT;
+  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, end};
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
   TileLoader<T, DP, N> kl, vl;
@@ -326,7 +364,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
     next = km.bits(t0 + NW, km.byte(t0 + NW, lane));
   }
   FragReader<T, DP> fr;
-  fr.init(lane);
+  fr.init(lane, lds);
   Softmax<T, DP, NQ, KT> sm;
   sm.init();
   const T *qp = static_cast<const T *>(a.q) + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
@@ -336,19 +374,16 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
-      load_frag(p + d, d < a.D, sm.q[n][s]);
+      load_frag(p, d, d < a.D, sm.q[n][s]);
     }
   }
   auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
     constexpr int B = decltype(buf)::value;
     wait_vmcnt<0>();  // tile t is in this wave's buffer
     asm volatile("" ::: "memory");
-    int byte = 1;
-    if (t + NW < t1) {
-      stage(t + NW, B ^ 1, next);
-      byte = km.byte(t + 2 * NW, lane);
-    }
-    if (bits != 0) sm.step(fr, lds + B * 2 * TB, lds + B * 2 * TB + TB, bits, a.c, lane);
+    stage(t + NW, 1 - B, next);  // past the last tile: no live row, nothing is read
+    const int byte = km.byte(t + 2 * NW, lane);
+    if (bits != 0) sm.template step<2 * B * TB, 2 * B * TB + TB>(fr, bits, a.c, lane);
     bits = next;
     next = km.bits(t + 2 * NW, byte);
   };
@@ -356,6 +391,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
     turn(std::integral_constant<int, 0>{}, t);
     if (t + NW < t1) turn(std::integral_constant<int, 1>{}, t + NW);
   }
+  wait_vmcnt<0>();
   // join the waves: every wave leaves its sums, then sums its share of the 32 x 32 tiles over the waves
   float l[NQ];
 #pragma unroll
@@ -385,7 +421,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
       const float2 v = ml[q][n][lane & 31];
-      w[q] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - m);
+      w[q] = __builtin_amdgcn_exp2f(v.x - m);
       lsum += w[q] * v.y;
     }
     const float inv = a.splits > 1 ? 1.f : lsum > 0.f || lsum != lsum ? 1.0f / lsum : 0.f;
@@ -408,24 +444,33 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
   }
 }
 
-// Joins the splits of a row: weights 2^(m_s − max m).
+// Joins the splits of a row, one workgroup per row: weights 2^(m_s − max m). Eight groups of 32 lanes (4 channels
+// each) take every eighth split, and their sums are added in order through LDS.
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
-  const int64_t all = (int64_t)a.batches * a.Hk * a.rows;
-  const int per = 256 / 32;
-  const int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / 32;
-  if (row >= all) return;
-  const int at = threadIdx.x % 32;
+  __shared__ f32x4 sums[8][32];
+  __shared__ float ls[8];
+  const int64_t all = (int64_t)a.batches * a.Hk * a.rows, row = blockIdx.x;
+  const int at = threadIdx.x % 32, g = threadIdx.x / 32;
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
+  for (int s = at; s < a.splits; s += 32) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
+#pragma unroll
+  for (int i = 16; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+  for (int s = g; s < a.splits; s += 8) {
     const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * all + row));
-    const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+    const float w = __builtin_amdgcn_exp2f(ml.x - m);
     l += w * ml.y;
     if (4 * at < a.D) o += w * *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + 4 * at);
   }
+  sums[g][at] = o;
+  if (at == 0) ls[g] = l;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) o += sums[i][at], l += ls[i];
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   if (at == 0) a.lse[row] = l > 0.f ? m + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
   if (4 * at >= a.D) return;
@@ -465,10 +510,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   __shared__ u32x4 smem[4 * TB / 16];
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
-  int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int rt = id % a.row_tiles;
-  id /= a.row_tiles;
-  const int hk = id % a.Hk, b = id / a.Hk;
+  int id = blockIdx.x;  // heads first: rows of all heads are read together, whole token rows of memory
+  const int hk = id % a.Hk;
+  id /= a.Hk;
+  const int rt = id % a.row_tiles, b = id / a.row_tiles;
   const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, sample_keys(a, b)};
   const int t1 = (km.len + KT - 1) / KT;
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
@@ -486,7 +531,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     next = km.bits(1, km.byte(1, lane));
   }
   FragReader<T, DP> fr;
-  fr.init(lane);
+  fr.init(lane, lds);
   const int row0 = (rt * 4 + wave) * 32, r = row0 + (lane & 31), rc = min(r, a.rows - 1);
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
   const int64_t oat = ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
@@ -500,9 +545,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     for (int s = 0; s < DP / 16; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
       Frag<T> of;
-      load_frag(qp + d, d < a.D, q[s]);
-      load_frag(gp_ + d, d < a.D, g[s]);
-      load_frag(op + d, d < a.D, of);
+      load_frag(qp, d, d < a.D, q[s]);
+      load_frag(gp_, d, d < a.D, g[s]);
+      load_frag(op, d, d < a.D, of);
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -523,18 +568,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-  auto step = [&](const MLORA_LDS char *kt, const MLORA_LDS char *vt, uint64_t bits) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kb = 0; kb < KT / 32; ++kb) {
+  auto step = [&](uint64_t bits) __attribute__((always_inline)) {
+    static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
+      constexpr int kb = decltype(block)::value;
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         Frag<T> kf, vf;
-        fr.rows(kt, 32 * kb, ks, kf);
+        fr.template rows<0, 32 * kb>(ks, kf);
         s = mma16(kf, q[ks], s);
-        fr.rows(vt, 32 * kb, ks, vf);
+        fr.template rows<TB, 32 * kb>(ks, vf);
         dp = mma16(vf, g[ks], dp);
       }
       if (bits != low_bits(KT)) {
@@ -542,38 +587,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
       }
-      Frag<T> ds[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.c - lse) * (dp[i] - delta);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        to_frag(s, ks, ds[ks]);
+      static_for<2>([&](auto ks) __attribute__((always_inline)) {
+        Frag<T> ds;
+        to_frag(s, ks, ds);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> kf;
-          fr.cols(kt, 32 * kb + 16 * ks, d, kf);
-          dq[d] = mma16(kf, ds[ks], dq[d]);
+          fr.template cols<0, 32 * kb + 16 * decltype(ks)::value>(d, kf);
+          dq[d] = mma16(kf, ds, dq[d]);
         }
-      }
-    }
+        return true;
+      });
+      return true;
+    });
   };
-  auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
+  for (int t = 0; t < t1; ++t) {
     wait_vmcnt<0>();
     lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    int byte = 1;
-    if (t + 1 < t1) {
-      stage(t + 1, B ^ 1, next);
-      byte = km.byte(t + 2, lane);
-    }
-    if (bits != 0) step(lds + B * 2 * TB, lds + B * 2 * TB + TB, bits);
+    stage(t + 1, (t + 1) & 1, next);  // past the last tile: no live row, nothing is read
+    const int byte = km.byte(t + 2, lane);
+    if (bits != 0) step(bits);
+    fr.flip(2 * TB);
     bits = next;
     next = km.bits(t + 2, byte);
-  };
-  for (int t = 0; t < t1; t += 2) {
-    turn(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t1) turn(std::integral_constant<int, 1>{}, t + 1);
   }
+  wait_vmcnt<0>();
   const float f[1] = {ba.scale};
   f32x16 o[1][ND];
 #pragma unroll
@@ -581,192 +621,182 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   store_rows<T, DP, 1>(static_cast<T *>(ba.dq) + oat, o, f, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
 }
 
-// Four waves own 32 NK keys each (K and V fragments in registers) and share tiles of QT query rows of one head
-// in LDS, double-buffered: q, the output's gradient, lse and delta.
-template <class T, int DP, int NK>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const AttnBwdArgs ba) {
+// NW waves own 32 keys each (K fragments in registers; V in LDS for bf16, whose two waves per SIMD leave no room
+// for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient, lse and
+// delta.
+template <class T, int DP, int NW>
+struct DkvTile {  // query rows per tile: half as many where four waves' V would leave room for one workgroup only
+  static constexpr int QT = sizeof(T) == 2 && !(DP == 128 && NW == 4) ? 64 : 32;
+};
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
-  constexpr int QT = AttnTile<T>::KT, ND = DP / 32;
+  constexpr int QT = DkvTile<T, DP, NW>::QT, ND = DP / 32, NS = DP / 16;
+  constexpr bool VLDS = sizeof(T) == 2;
   using Tile = HeadTile<T, DP>;
-  constexpr int TB = QT * Tile::RB, N = TB / 1024 / 4;
-  __shared__ u32x4 smem[4 * TB / 16];
-  __shared__ f32x4 stats[2][2][QT / 4];  // buffer; lse, delta
+  constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = VLDS ? 32 * Tile::RB : 0;
+  // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then lse and delta per buffer
+  __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + QT];
+  f32x4 (&stats)[2][2][QT / 4] = *(f32x4 (*)[2][2][QT / 4])(smem + (4 * TB + NW * VB) / 16);
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
-  int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  int id = blockIdx.x;  // heads first, as above
+  const int hk = id % a.Hk;
+  id /= a.Hk;
   const int kb = id % ba.key_blocks;
   id /= ba.key_blocks;
-  const int sp = id % ba.q_splits;
-  id /= ba.q_splits;
-  const int hk = id % a.Hk, b = id / a.Hk;
+  const int sp = id % ba.q_splits, b = id / ba.q_splits;
   const int len = sample_keys(a, b);
-  const int key0 = (kb * 4 + wave) * 32 * NK;
+  const int key0 = (kb * NW + wave) * 32, key = key0 + (lane & 31);
   const uint8_t *mask = a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb;
-  Frag<T> k[NK][DP / 16], v[NK][DP / 16];
-  bool live[NK];
+  const bool live = key < len && (mask == nullptr || mask[key] != 0);
+  const uint64_t live_bits = __ballot(live) & 0xffffffffull;
+  const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
+  const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
+  Frag<T> k[NS], v[VLDS ? 1 : NS];
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int key = key0 + 32 * n + (lane & 31);
-    live[n] = key < len && (mask == nullptr || mask[key] != 0);
-    const int64_t at = live[n] ? key : 0;
-    const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh + at * a.k_sl;
-    const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh + at * a.v_sl;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      const int d = 16 * s + 8 * (lane >> 5);
-      load_frag(kp + d, live[n] && d < a.D, k[n][s]);
-      load_frag(vp + d, live[n] && d < a.D, v[n][s]);
-    }
+  for (int s = 0; s < NS; ++s) {
+    const int d = 16 * s + 8 * (lane >> 5);
+    load_frag(kp, key * a.k_sl + d, live && d < a.D, k[s]);
+    if constexpr (!VLDS) load_frag(vp, key * a.v_sl + d, live && d < a.D, v[s]);
   }
-  f32x16 dk[NK][ND], dv[NK][ND];
+  MLORA_LDS char *vt = lds + 4 * TB + wave * VB;
+  if constexpr (VLDS) {
+    TileLoader<T, DP, VB / 1024> vl;
+    vl.init(lane, 0, 1, a.v_sl, a.D);
+    vl.load(vp + (int64_t)key0 * a.v_sl, live_bits, vt);
+  }
+  f32x16 dk[1][ND], dv[1][ND];
 #pragma unroll
-  for (int n = 0; n < NK; ++n)
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dk[n][d][i] = 0.f, dv[n][d][i] = 0.f;
+    for (int i = 0; i < 16; ++i) dk[0][d][i] = 0.f, dv[0][d][i] = 0.f;
   const int t0 = sp * ba.q_split_tiles;
-  const int t1 = kb * 128 * NK >= len ? 0 : min(t0 + ba.q_split_tiles, ba.q_tiles);  // no key at all: zeros
+  const int t1 = kb * 32 * NW >= len ? 0 : min(t0 + ba.q_split_tiles, ba.q_tiles);  // no key at all: zeros
   TileLoader<T, DP, N> ql, gl;
-  ql.init(lane, wave, 4, a.q_sl, a.D), gl.init(lane, wave, 4, ba.g_sl, a.D);
+  ql.init(lane, wave, NW, a.q_sl, a.D), gl.init(lane, wave, NW, ba.g_sl, a.D);
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
-  FragReader<T, DP> fr;
-  fr.init(lane);
+  FragReader<T, DP> fr, vr;
+  fr.init(lane, lds), vr.init(lane, vt);
   // a tile's rows into LDS; returns lse (threads 0 .. QT - 1) or delta (QT .. 2 QT - 1) of the thread's row
   auto stage = [&](int t, int buf) __attribute__((always_inline)) -> float {
     const int g = t / ba.head_q_tiles, i0 = (t - g * ba.head_q_tiles) * QT, h = hk * a.G + g;
-    const uint64_t rows = low_bits(min(a.Lq - i0, QT));
+    const uint64_t rows = t < t1 ? low_bits(min(a.Lq - i0, QT)) : 0;  // past the last tile: nothing is read
     ql.load(static_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh + i0 * a.q_sl, rows, lds + buf * 2 * TB);
     gl.load(static_cast<const T *>(ba.g) + b * ba.g_sb + h * ba.g_sh + i0 * ba.g_sl, rows, lds + buf * 2 * TB + TB);
     const int i = threadIdx.x % QT;
     const float *src = threadIdx.x < QT ? a.lse : ba.delta;
     float x = threadIdx.x < QT ? INFINITY : 0.f;  // rows behind the last: P = 0
-    if (threadIdx.x < 2 * QT && i0 + i < a.Lq) x = src[head_rows + (int64_t)g * a.Lq + i0 + i];
+    if (threadIdx.x < 2 * QT && t < t1 && i0 + i < a.Lq) x = src[head_rows + (int64_t)g * a.Lq + i0 + i];
     return x;
   };
   auto keep = [&](int buf, float x) __attribute__((always_inline)) {
     if (threadIdx.x < 2 * QT) ((float *)stats[buf][threadIdx.x / QT])[threadIdx.x % QT] = x;
   };
-  auto step = [&](const MLORA_LDS char *qt, const MLORA_LDS char *gt, int buf) __attribute__((always_inline)) {
+  auto step = [&](int buf) __attribute__((always_inline)) {
+    static_for<QT / 32>([&](auto block) __attribute__((always_inline)) {
+      constexpr int qb = decltype(block)::value;
+      __builtin_amdgcn_sched_barrier(0);  // between the phases too: interleaved, they spill
+      f32x16 s, dp;
 #pragma unroll
-    for (int qb = 0; qb < QT / 32; ++qb) {
-      f32x16 s[NK], dp[NK];
+      for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = 0.f, dp[n][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        Frag<T> f;
-        fr.rows(qt, 32 * qb, ks, f);
-#pragma unroll
-        for (int n = 0; n < NK; ++n) s[n] = mma16(f, k[n][ks], s[n]);
+      for (int ks = 0; ks < NS; ++ks) {  // the two sums in turn: a sum waits for its last product
+        Frag<T> qf, gf, vf;
+        fr.template rows<0, 32 * qb>(ks, qf);
+        s = mma16(qf, k[ks], s);
+        fr.template rows<TB, 32 * qb>(ks, gf);
+        if constexpr (VLDS) vr.template rows<0, 0>(ks, vf);
+        else vf = v[ks];
+        dp = mma16(gf, vf, dp);
       }
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        Frag<T> f;
-        fr.rows(gt, 32 * qb, ks, f);
-#pragma unroll
-        for (int n = 0; n < NK; ++n) dp[n] = mma16(f, v[n][ks], dp[n]);
-      }
-      Frag<T> pf[NK][2], df[NK][2];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const f32x4 lse = stats[buf][0][8 * qb + 2 * i4 + (lane >> 5)], delta = stats[buf][1][8 * qb + 2 * i4 + (lane >> 5)];
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = __builtin_amdgcn_exp2f(s[n][4 * i4 + j] * a.c - lse[j]);
-            s[n][4 * i4 + j] = p;
-            dp[n][4 * i4 + j] = p * (dp[n][4 * i4 + j] - delta[j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float p = __builtin_amdgcn_exp2f(s[4 * i4 + j] * a.c - lse[j]);
+          s[4 * i4 + j] = p;
+          dp[4 * i4 + j] = p * (dp[4 * i4 + j] - delta[j]);
+        }
       }
-#pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) to_frag(s[n], ks, pf[n][ks]), to_frag(dp[n], ks, df[n][ks]);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<2>([&](auto ks) __attribute__((always_inline)) {
+        Frag<T> pf;
+        to_frag(s, ks, pf);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> f;
-          fr.cols(gt, 32 * qb + 16 * ks, d, f);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) dv[n][d] = mma16(f, pf[n][ks], dv[n][d]);
+          fr.template cols<TB, 32 * qb + 16 * decltype(ks)::value>(d, f);
+          dv[0][d] = mma16(f, pf, dv[0][d]);
         }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        return true;
+      });
+      static_for<2>([&](auto ks) __attribute__((always_inline)) {
+        Frag<T> df;
+        to_frag(dp, ks, df);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> f;
-          fr.cols(qt, 32 * qb + 16 * ks, d, f);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) dk[n][d] = mma16(f, df[n][ks], dk[n][d]);
+          fr.template cols<0, 32 * qb + 16 * decltype(ks)::value>(d, f);
+          dk[0][d] = mma16(f, df, dk[0][d]);
         }
-    }
+        return true;
+      });
+      return true;
+    });
   };
   if (t0 < t1) keep(0, stage(t0, 0));
-  auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
     wait_vmcnt<0>();
     lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    float x = 0.f;
-    if (t + 1 < t1) x = stage(t + 1, B ^ 1);
-    step(lds + B * 2 * TB, lds + B * 2 * TB + TB, B);
-    if (t + 1 < t1) keep(B ^ 1, x);
-  };
-  for (int t = t0; t < t1; t += 2) {
-    turn(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t1) turn(std::integral_constant<int, 1>{}, t + 1);
+    const float x = stage(t + 1, buf ^ 1);
+    if (live_bits != 0) step(buf);
+    keep(buf ^ 1, x);
+    fr.flip(2 * TB);
   }
-  float fk[NK], fv[NK];
+  wait_vmcnt<0>();
+  if (!live) {  // a masked key's column holds whatever its zeroed fragments gave
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {  // a masked key's column holds whatever its zeroed fragments gave
-    fk[n] = ba.scale, fv[n] = 1.f;
-    if (!live[n]) {
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dk[n][d][i] = 0.f, dv[n][d][i] = 0.f;
-    }
+      for (int i = 0; i < 16; ++i) dk[0][d][i] = 0.f, dv[0][d][i] = 0.f;
   }
   if (ba.q_splits > 1) {
-    f32x4 *p = ba.part + (((((int64_t)sp * a.batches + b) * a.Hk + hk) * ba.key_blocks + kb) * 4 + wave) * (2 * NK * ND * 4 * 64) + lane;
+    f32x4 *p = ba.part + (((((int64_t)sp * a.batches + b) * a.Hk + hk) * ba.key_blocks + kb) * NW + wave) * (2 * ND * 4 * 64) + lane;
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          *(MLORA_GLOBAL f32x4 *)(p + ((n * ND + d) * 4 + i) * 64) =
-              f32x4{dk[n][d][4 * i], dk[n][d][4 * i + 1], dk[n][d][4 * i + 2], dk[n][d][4 * i + 3]};
-          *(MLORA_GLOBAL f32x4 *)(p + (((NK + n) * ND + d) * 4 + i) * 64) =
-              f32x4{dv[n][d][4 * i], dv[n][d][4 * i + 1], dv[n][d][4 * i + 2], dv[n][d][4 * i + 3]};
-        }
+      for (int i = 0; i < 4; ++i) {
+        *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dk[0][d][4 * i], dk[0][d][4 * i + 1], dk[0][d][4 * i + 2], dk[0][d][4 * i + 3]};
+        *(MLORA_GLOBAL f32x4 *)(p + ((ND + d) * 4 + i) * 64) = f32x4{dv[0][d][4 * i], dv[0][d][4 * i + 1], dv[0][d][4 * i + 2], dv[0][d][4 * i + 3]};
+      }
     return;
   }
   const int64_t at = ((int64_t)b * a.Lk * a.Hk + hk) * a.D;
-  store_rows<T, DP, NK>(static_cast<T *>(ba.dk) + at, dk, fk, key0, a.Lk, a.Lk, (int64_t)a.Hk * a.D, 0, a.D, lane);
-  store_rows<T, DP, NK>(static_cast<T *>(ba.dv) + at, dv, fv, key0, a.Lk, a.Lk, (int64_t)a.Hk * a.D, 0, a.D, lane);
+  const float fk[1] = {ba.scale}, fv[1] = {1.f};
+  store_rows<T, DP, 1>(static_cast<T *>(ba.dk) + at, dk, fk, key0, a.Lk, a.Lk, (int64_t)a.Hk * a.D, 0, a.D, lane);
+  store_rows<T, DP, 1>(static_cast<T *>(ba.dv) + at, dv, fv, key0, a.Lk, a.Lk, (int64_t)a.Hk * a.D, 0, a.D, lane);
 }
 
 // Adds the splits of dk and dv in split order and writes them out.
-template <class T, int DP, int NK>
+template <class T, int DP, int NW>
 __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
   constexpr int ND = DP / 32;
-  const int64_t per = (int64_t)a.batches * a.Hk * ba.key_blocks * 4 * 2 * NK * ND * 4 * 64;
+  const int64_t per = (int64_t)a.batches * a.Hk * ba.key_blocks * NW * 2 * ND * 4 * 64;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= per) return;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < ba.q_splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(ba.part + s * per + e);
   int64_t u = e / 64;
-  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), n = (int)(u / 4 / ND % NK), which = (int)(u / 4 / ND / NK % 2);
-  u /= 4 * ND * NK * 2;  // (b, hk, key block, wave)
-  const int64_t wave_block = u % (4 * ba.key_blocks), bh = u / (4 * ba.key_blocks);
-  const int64_t key = wave_block * 32 * NK + 32 * n + (lane & 31);
+  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), which = (int)(u / 4 / ND % 2);
+  u /= 4 * ND * 2;  // (b, hk, key block, wave)
+  const int64_t key = u % (NW * ba.key_blocks) * 32 + (lane & 31), bh = u / (NW * ba.key_blocks);
   const int ch = 32 * d + 8 * i + 4 * (lane >> 5);
   if (key >= a.Lk || ch >= a.D) return;
   T *p = static_cast<T *>(which ? ba.dv : ba.dk) + ((bh / a.Hk * a.Lk + key) * a.Hk + bh % a.Hk) * a.D + ch;
@@ -777,38 +807,49 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const AttnBwdArgs ba
 
 // The kernels are named here because hipcc's host pass does not instantiate a kernel that holds generic lambdas
 // from a launch inside one.
-#define MLORA_ATTN(T, DP)                                        \
-  template __global__ void attn_fwd_kernel<T, DP, 1>(const AttnArgs); \
+#define MLORA_ATTN(T, DP)                                             \
+  template __global__ void attn_fwd_kernel<T, DP>(const AttnArgs);    \
   template __global__ void attn_few_kernel<T, DP, 1>(const AttnArgs); \
-  template __global__ void attn_few_kernel<T, DP, 2>(const AttnArgs); \
   template __global__ void attn_dq_kernel<T, DP>(const AttnBwdArgs);  \
-  template __global__ void attn_dkv_kernel<T, DP, 1>(const AttnBwdArgs);
+  template __global__ void attn_dkv_kernel<T, DP, 4>(const AttnBwdArgs);
 MLORA_ATTN(uint16_t, 64)
 MLORA_ATTN(uint16_t, 128)
 MLORA_ATTN(float, 64)
 MLORA_ATTN(float, 128)
 #undef MLORA_ATTN
-template __global__ void attn_dkv_kernel<uint16_t, 64, 2>(const AttnBwdArgs);
+template __global__ void attn_few_kernel<uint16_t, 64, 2>(const AttnArgs);
+template __global__ void attn_few_kernel<uint16_t, 128, 2>(const AttnArgs);
+template __global__ void attn_few_kernel<float, 64, 2>(const AttnArgs);
+template __global__ void attn_dkv_kernel<uint16_t, 128, 8>(const AttnBwdArgs);
 
 // ------------------------------------------------------------------ host
 
-constexpr int kAttnMaxHeadDim = 128, kFewRows = 64;
+constexpr int kAttnMaxHeadDim = 128;
 
 struct AttnPlan {
   bool few;
   int nq;  // 32-row blocks per wave
-  int64_t row_tiles, splits, split_tiles;
+  int64_t row_tiles, turns, splits, split_tiles;
 };
+
+// Row tiles per workgroup: up to 4 where few key tiles leave a workgroup mostly waiting for its first loads and
+// at least 1024 workgroups (two for every place) remain. 2 x 32760 rows of 12 heads of 128: 512 keys 285 us with
+// one, 263 with four; 64 keys 141 and 120; 1024 keys 494 and 451; at 4096 keys one row's tile is best (819, 909).
+static int64_t row_turns(int64_t tiles, int64_t key_tiles) {
+  const int64_t most = key_tiles <= 16 ? 4 : 1, turns = tiles / 1024;
+  return turns < 1 ? 1 : turns > most ? most : turns;
+}
 
 // How a forward is cut: few rows per key head run waves over different keys, more rows 128 per workgroup;
 // the keys are split where that leaves less than a workgroup for every compute unit and there are enough of them.
 static AttnPlan attn_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, int64_t D, bool f32) {
   AttnPlan p{};
-  p.few = rows <= kFewRows;
+  p.few = rows <= (f32 && D > 64 ? 32 : 64);
   const int64_t waves = p.few && f32 && D > 64 ? 2 : 4;
   const int64_t kt = p.few || f32 ? 32 : 64, tiles = (Lk + kt - 1) / kt;
   p.nq = p.few && rows > 32 ? 2 : 1;
   p.row_tiles = p.few ? 1 : (rows + 127) / 128;
+  p.turns = p.few ? 1 : row_turns(batches * Hk * p.row_tiles, tiles);
   const int64_t groups = batches * Hk * p.row_tiles;
   const int64_t least = p.few ? 4 * waves : 8;  // tiles that a split is worth its join for
   int64_t splits = groups > 0 && groups < 256 ? 256 / groups : 1;
@@ -825,20 +866,20 @@ static int64_t attn_part_floats(const AttnPlan &p, int64_t batches, int64_t Hk, 
 }
 
 struct DkvPlan {
-  int nk;
+  int nw;  // waves per workgroup, 32 keys each
   int64_t key_blocks, q_tiles, head_q_tiles, splits, split_tiles;
 };
 
-// dk / dv: 128 nk keys per workgroup; the query rows are split where the keys alone leave compute units idle.
+// dk / dv: 32 nw keys per workgroup; the query rows are split where the keys alone leave compute units idle.
 static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t D, bool f32) {
   DkvPlan p{};
-  const int64_t qt = f32 ? 32 : 64;
-  p.nk = !f32 && D <= 64 && Lk > 128 ? 2 : 1;
-  p.key_blocks = (Lk + 128 * p.nk - 1) / (128 * p.nk);
+  p.nw = !f32 && D > 64 && Lk > 128 ? 8 : 4;
+  const int64_t qt = f32 || (D > 64 && p.nw == 4) ? 32 : 64;
+  p.key_blocks = (Lk + 32 * p.nw - 1) / (32 * p.nw);
   p.head_q_tiles = (Lq + qt - 1) / qt;
   p.q_tiles = G * p.head_q_tiles;
-  const int64_t groups = batches * Hk * p.key_blocks;
-  int64_t splits = groups > 0 && groups < 256 ? 256 / groups : 1;
+  const int64_t groups = batches * Hk * p.key_blocks, most = !f32 && p.nw == 4 ? 512 : 256;  // workgroups that run at once
+  int64_t splits = groups > 0 && groups < most ? most / groups : 1;
   if (splits > p.q_tiles / 4) splits = p.q_tiles / 4;
   if (splits < 1) splits = 1;
   p.split_tiles = (p.q_tiles + splits - 1) / splits;
@@ -847,9 +888,13 @@ static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int
   return p;
 }
 
+// 16-byte vectors of one split of dk and dv, in register order.
+static int64_t dkv_vectors(const DkvPlan &p, int64_t batches, int64_t Hk, int64_t D) {
+  return batches * Hk * p.key_blocks * p.nw * 2 * (D > 64 ? 4 : 2) * 4 * 64;
+}
+
 static int64_t dkv_part_bytes(const DkvPlan &p, int64_t batches, int64_t Hk, int64_t D) {
-  const int64_t nd = D > 64 ? 4 : 2;
-  return p.splits > 1 ? p.splits * batches * Hk * p.key_blocks * 4 * 2 * p.nk * nd * 4 * 64 * 16 : 0;
+  return p.splits > 1 ? p.splits * dkv_vectors(p, batches, Hk, D) * 16 : 0;
 }
 
 // Sizes and types shared by every entry. MLORA_OK, or the status.
@@ -937,21 +982,22 @@ extern "C" int mlora_cross_attention(const void *q, const int64_t *q_strides, co
     if (workspace == nullptr || workspace_bytes < floats * (int64_t)sizeof(float)) return MLORA_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
   }
-  a.out = out, a.row_tiles = (int32_t)p.row_tiles, a.splits = (int32_t)p.splits, a.split_tiles = (int32_t)p.split_tiles;
+  a.out = out, a.row_tiles = (int32_t)p.row_tiles, a.turns = (int32_t)p.turns, a.splits = (int32_t)p.splits, a.split_tiles = (int32_t)p.split_tiles;
   a.part_o = static_cast<float *>(workspace);
   a.part_ml = a.part_o + p.splits * B * Hk * a.rows * D;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(B * Hk * p.row_tiles * p.splits));
+  const dim3 grid((unsigned)(B * Hk * ((p.row_tiles + p.turns - 1) / p.turns) * p.splits));
   with_head(f32, D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     if (p.few && p.nq == 1) hipLaunchKernelGGL((attn_few_kernel<T, DP, 1>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
-    else if (p.few) hipLaunchKernelGGL((attn_few_kernel<T, DP, 2>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, 1>), grid, dim3(256), 0, s, a);
+    else if (!p.few) hipLaunchKernelGGL((attn_fwd_kernel<T, DP>), grid, dim3(256), 0, s, a);
+    else if constexpr (sizeof(T) * DP < 512)
+      hipLaunchKernelGGL((attn_few_kernel<T, DP, 2>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
   });
   st = launch_status();
   if (st || p.splits == 1) return st;
-  const dim3 joins((unsigned)((B * Hk * a.rows + 7) / 8));
+  const dim3 joins((unsigned)(B * Hk * a.rows));
   if (f32) hipLaunchKernelGGL(attn_join_kernel<float>, joins, dim3(256), 0, s, a);
   else hipLaunchKernelGGL(attn_join_kernel<uint16_t>, joins, dim3(256), 0, s, a);
   return launch_status();
@@ -1006,20 +1052,19 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   }
   if (Lk == 0) return MLORA_OK;
   const dim3 grid((unsigned)(B * Hk * p.key_blocks * p.splits));
-  const int64_t vectors = B * Hk * p.key_blocks * 4 * 2 * p.nk * (D > 64 ? 4 : 2) * 4 * 64;
+  const dim3 joins((unsigned)((dkv_vectors(p, B, Hk, D) + 255) / 256));
   with_head(f32, D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
-    auto run = [&](auto nk) {
-      constexpr int NK = decltype(nk)::value;
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NK>), grid, dim3(256), 0, s, ba);
-      if (p.splits > 1)
-        hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, NK>), dim3((unsigned)((vectors + 255) / 256)), dim3(256), 0, s, ba);
-    };
-    if constexpr (sizeof(T) == 2 && DP == 64) {
-      if (p.nk == 2) return run(std::integral_constant<int, 2>{});
+    if constexpr (sizeof(T) == 2 && DP == 128) {
+      if (p.nw == 8) {
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 8>), grid, dim3(512), 0, s, ba);
+        if (p.splits > 1) hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, 8>), joins, dim3(256), 0, s, ba);
+        return;
+      }
     }
-    run(std::integral_constant<int, 1>{});
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4>), grid, dim3(256), 0, s, ba);
+    if (p.splits > 1) hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, 4>), joins, dim3(256), 0, s, ba);
   });
   return launch_status();
 }

@@ -16,8 +16,8 @@
 // stored x1 costs nothing and keeps û exact.
 //
 // Both passes are HBM-bound. A row is held in registers by WPR waves (8 values per lane and chunk); the
-// vectors of the workgroup's sample sit in LDS, since in registers they would halve the waves that hide
-// the loads' latency. A workgroup takes `chunk` rows of one sample; the backward's column sums stay in
+// vectors of the workgroup's sample do not: in registers they would halve the waves that hide the loads'
+// latency. A workgroup takes `chunk` rows of one sample; the backward's column sums stay in
 // registers over those rows, are added over the workgroup's rows in flight through LDS, and leave as one
 // partial row per workgroup (fixed order, no atomics).
 #include "mlora_common.h"
@@ -55,7 +55,7 @@ struct RowSum {
   float (*red)[2][NW];  // four slots: a slot is written again only after two more barriers
   int wave, first, slot = 0;
   __device__ __forceinline__ void operator()(float &a, float &b) {
-    a = wave_sum(a), b = wave_sum(b);
+    a = lanes_sum<64>(a), b = lanes_sum<64>(b);
     if constexpr (WPR > 1) {
       if ((threadIdx.x & 63) == 0) red[slot][0][wave] = a, red[slot][1][wave] = b;
       __syncthreads();
@@ -66,7 +66,7 @@ struct RowSum {
     }
   }
   __device__ __forceinline__ float operator()(float a) {
-    a = wave_sum(a);
+    a = lanes_sum<64>(a);
     if constexpr (WPR > 1) {
       if ((threadIdx.x & 63) == 0) red[slot][0][wave] = a;
       __syncthreads();
@@ -79,40 +79,56 @@ struct RowSum {
   }
 };
 
-// The sample's vectors in LDS: values 8c .. 8c + 3 of vector v at [v][0][c], 8c + 4 .. 8c + 7 at [v][1][c]
-// (two conflict-free 16-byte reads per chunk).
-struct VecLds {
+// The sample's vectors: gate, m, shift, w_post, formed from their sources (ones or zeros where there is none).
+// LDS: copied once per workgroup, values 8c .. 8c + 3 of vector v at [v][0][c], 8c + 4 .. 8c + 7 at [v][1][c]
+// (two conflict-free 16-byte reads per chunk). Else read again for every row, out of the L1 and L2 caches: rows of
+// several waves are wide, their vectors would fill the LDS and leave one workgroup per compute unit, whose rows
+// move in step (11040 x 2 rows of 5120 normed on both sides, bf16: forward 315 us against 206, backward 740 against
+// 411).
+template <bool LDS>
+struct Vectors {
+  const JointArgs &a;
+  int64_t b;
   f32x4 *base;
   int nchunks;
   __device__ __forceinline__ f32x4 *at(int v) const { return base + (int64_t)v * 2 * nchunks; }
-  __device__ __forceinline__ void read(int v, int c, float (&o)[8]) const {
-    const f32x4 a = at(v)[c], b = at(v)[nchunks + c];
+  __device__ __forceinline__ void source(int v, int c, float (&o)[8]) const {
+    const void *p = v == kVecGate ? a.gate : v == kVecMult ? a.scale : v == kVecShift ? a.shift : a.post_w;
+    const bool f32 = v == kVecGate ? a.gate_f32 : v == kVecMult ? a.scale_f32 : v == kVecShift ? a.shift_f32 : a.post_f32;
+    const int64_t off = v == kVecGate ? a.gate_sb : v == kVecMult ? a.scale_sb : v == kVecShift ? a.shift_sb : 0;
+    if (p == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = a[i], o[i + 4] = b[i];
+      for (int i = 0; i < 8; ++i) o[i] = v == kVecShift ? 0.f : 1.f;
+      return;
+    }
+    load8(p, f32, b * off + 8 * c, o);
+    if (v == kVecMult && a.unit_offset) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] += 1.f;
+    }
   }
-  __device__ __forceinline__ void fill(int v, const void *src, bool f32, int64_t off, float add, float missing) const {
-    for (int c = threadIdx.x; c < nchunks; c += blockDim.x) {
-      float t[8];
-      if (src != nullptr) {
-        load8(src, f32, off + 8 * c, t);
+  __device__ __forceinline__ void read(int v, int c, float (&o)[8]) const {
+    if constexpr (LDS) {
+      const f32x4 x = at(v)[c], y = at(v)[nchunks + c];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] += add;
-      } else {
+      for (int i = 0; i < 4; ++i) o[i] = x[i], o[i + 4] = y[i];
+    } else {
+      source(v, c, o);
+    }
+  }
+  __device__ __forceinline__ void fill() const {
+    if constexpr (LDS) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = missing;
-      }
-      at(v)[c] = f32x4{t[0], t[1], t[2], t[3]};
-      at(v)[nchunks + c] = f32x4{t[4], t[5], t[6], t[7]};
+      for (int v = 0; v < kVecs; ++v)
+        for (int c = threadIdx.x; c < nchunks; c += blockDim.x) {
+          float t[8];
+          source(v, c, t);
+          at(v)[c] = f32x4{t[0], t[1], t[2], t[3]};
+          at(v)[nchunks + c] = f32x4{t[4], t[5], t[6], t[7]};
+        }
     }
   }
 };
-
-__device__ __forceinline__ void fill_vectors(const VecLds &vec, const JointArgs &a, int64_t b) {
-  vec.fill(kVecGate, a.gate, a.gate_f32, b * a.gate_sb, 0.f, 1.f);
-  vec.fill(kVecMult, a.scale, a.scale_f32, b * a.scale_sb, a.unit_offset ? 1.f : 0.f, 1.f);
-  vec.fill(kVecShift, a.shift, a.shift_f32, b * a.shift_sb, 0.f, 0.f);
-  vec.fill(kVecPost, a.post_w, a.post_f32, 0, 0.f, 1.f);
-}
 
 // v <- N(v) for the row's values (zeros past the width); returns 1 / σ.
 template <int NCH, int WPR, class Sum>
@@ -145,22 +161,39 @@ __device__ __forceinline__ float norm_row(float (&v)[NCH][8], int c0, int nchunk
   return r;
 }
 
+// A row's chunks as they lie in memory, to be asked for a row ahead.
 template <int NCH, int WPR, bool F32>
-__device__ __forceinline__ void load_chunks(const void *p, int64_t o, int c0, int nchunks, bool live, float (&v)[NCH][8]) {
+struct RawRow {
+  u32x4 r[NCH][F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *p, int64_t o, int c0, int nchunks, bool live) {
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) {
-    const int c = c0 + 64 * WPR * k;
-    if (live && c < nchunks) load8(p, F32, o + 8 * c, v[k]);
-    else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+    for (int k = 0; k < NCH; ++k) {
+      const int c = c0 + 64 * WPR * k;
+      const bool on = live && c < nchunks;
+      if constexpr (F32) {
+        const float *q = static_cast<const float *>(p) + o + 8 * c;
+        r[k][0] = on ? *(const MLORA_GLOBAL u32x4 *)q : u32x4{0, 0, 0, 0};
+        r[k][1] = on ? *(const MLORA_GLOBAL u32x4 *)(q + 4) : u32x4{0, 0, 0, 0};
+      } else {
+        r[k][0] = on ? *(const MLORA_GLOBAL u32x4 *)(static_cast<const uint16_t *>(p) + o + 8 * c) : u32x4{0, 0, 0, 0};
+      }
     }
   }
-}
+  __device__ __forceinline__ void unpack(float (&v)[NCH][8]) const {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (F32) v[k][i] = __uint_as_float(r[k][i / 4][i % 4]);
+        else v[k][i] = __uint_as_float(i % 2 ? r[k][0][i / 2] & 0xffff0000u : r[k][0][i / 2] << 16);
+      }
+  }
+};
 
 template <int NCH, int WPR, int NW, bool XF32, bool YF32>
 __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
   constexpr int STREAMS = NW / WPR;
+  constexpr bool kAhead = WPR > 1;
   __shared__ float red[4][2][NW];
   extern __shared__ f32x4 dyn[];
   const int wave = wave_id(), lane = threadIdx.x & 63, stream = wave / WPR;
@@ -168,16 +201,24 @@ __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
   const int64_t b = blockIdx.x / a.n_chunks;
   const int t0 = (blockIdx.x % a.n_chunks) * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
   const float inv_w = 1.0f / (float)a.width;
-  const VecLds vec{dyn, nchunks};
-  fill_vectors(vec, a, b);
+  const Vectors<WPR == 1> vec{a, b, dyn, nchunks};
+  vec.fill();
   RowSum<WPR, NW> sum{red, wave, stream * WPR};
   __syncthreads();
+  RawRow<NCH, WPR, XF32> rx;
+  RawRow<NCH, WPR, YF32> ry;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    rx.load(a.x, b * a.x_sb + t * a.x_st, c0, nchunks, t < t1);
+    ry.load(a.y, b * a.y_sb + t * a.y_st, c0, nchunks, t < t1);
+  };
+  if constexpr (kAhead) load(t0 + stream);
   // every stream runs the same number of rows, so that every wave meets the same barriers
   for (int t = t0 + stream; t - stream < t1; t += STREAMS) {
     const bool live = t < t1;
     float u[NCH][8], p[NCH][8];
-    load_chunks<NCH, WPR, XF32>(a.x, b * a.x_sb + t * a.x_st, c0, nchunks, live, u);
-    load_chunks<NCH, WPR, YF32>(a.y, b * a.y_sb + t * a.y_st, c0, nchunks, live, p);
+    if constexpr (!kAhead) load(t);
+    rx.unpack(u), ry.unpack(p);
+    if constexpr (kAhead) load(t + STREAMS);
     if (a.post >= 0) {
       norm_row<NCH, WPR>(p, c0, nchunks, a.post, inv_w, a.eps, sum);
 #pragma unroll
@@ -222,6 +263,7 @@ template <int NCH, int WPR, int NW, bool XF32, bool YF32, bool SUMS, bool POST>
 __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdArgs ba) {
   const JointArgs &a = ba.f;
   constexpr int STREAMS = NW / WPR, NV = SUMS ? (POST ? 4 : 3) : 1;
+  constexpr bool kAhead = WPR > 1;  // the next row's loads under this row's sums and barriers
   __shared__ float red[4][2][NW];
   extern __shared__ f32x4 dyn[];  // the vectors; after the rows, one partial row of each sum
   const int wave = wave_id(), lane = threadIdx.x & 63, stream = wave / WPR;
@@ -229,8 +271,8 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
   const int64_t b = blockIdx.x / a.n_chunks;
   const int t0 = (blockIdx.x % a.n_chunks) * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
   const float inv_w = 1.0f / (float)a.width;
-  const VecLds vec{dyn, nchunks};
-  fill_vectors(vec, a, b);
+  const Vectors<WPR == 1> vec{a, b, dyn, nchunks};
+  vec.fill();
   RowSum<WPR, NW> sum{red, wave, stream * WPR};
   float acc[NV][NCH][8];  // dgate, dscale, dshift, dw_post
 #pragma unroll
@@ -240,13 +282,21 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[v][k][i] = 0.f;
   __syncthreads();
+  RawRow<NCH, WPR, XF32> rx, rgx;
+  RawRow<NCH, WPR, YF32> ry, rgo;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    rx.load(a.x, b * a.x_sb + t * a.x_st, c0, nchunks, t < t1);
+    ry.load(a.y, b * a.y_sb + t * a.y_st, c0, nchunks, t < t1);
+    rgo.load(ba.go, b * ba.go_sb + t * ba.go_st, c0, nchunks, t < t1 && ba.go != nullptr);
+    rgx.load(ba.gx, b * ba.gx_sb + t * ba.gx_st, c0, nchunks, t < t1 && ba.gx != nullptr);
+  };
+  if constexpr (kAhead) load(t0 + stream);
   for (int t = t0 + stream; t - stream < t1; t += STREAMS) {
     const bool live = t < t1;
     float u[NCH][8], p[NCH][8], go[NCH][8], d[NCH][8];
-    load_chunks<NCH, WPR, XF32>(a.x, b * a.x_sb + t * a.x_st, c0, nchunks, live, u);
-    load_chunks<NCH, WPR, YF32>(a.y, b * a.y_sb + t * a.y_st, c0, nchunks, live, p);
-    load_chunks<NCH, WPR, YF32>(ba.go, b * ba.go_sb + t * ba.go_st, c0, nchunks, live && ba.go != nullptr, go);
-    load_chunks<NCH, WPR, XF32>(ba.gx, b * ba.gx_sb + t * ba.gx_st, c0, nchunks, live && ba.gx != nullptr, d);
+    if constexpr (!kAhead) load(t);
+    rx.unpack(u), ry.unpack(p), rgo.unpack(go), rgx.unpack(d);
+    if constexpr (kAhead) load(t + STREAMS);
     float rp = 1.f;
     if constexpr (POST) rp = norm_row<NCH, WPR>(p, c0, nchunks, a.post, inv_w, a.eps, sum);  // p holds p̂
 #pragma unroll
@@ -331,52 +381,63 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
     }
   }
   if constexpr (SUMS) {
-    // the streams' sums, added in stream order in the vectors' place
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < STREAMS; ++w) {
-      if (stream == w) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-          for (int k = 0; k < NCH; ++k) {
-            const int c = c0 + 64 * WPR * k;
-            if (c >= nchunks) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f32x4 s = f32x4{acc[v][k][4 * h], acc[v][k][4 * h + 1], acc[v][k][4 * h + 2], acc[v][k][4 * h + 3]};
-              f32x4 &dst = vec.at(v)[h * nchunks + c];
-              if (w > 0) s += dst;
-              dst = s;
-            }
-          }
-      }
-      __syncthreads();
-    }
     float *out = ba.partial + (int64_t)blockIdx.x * kVecs * a.width;
-    for (int e = threadIdx.x; e < NV * 2 * nchunks; e += 64 * NW) {
-      const int v = e / (2 * nchunks), h = e % 2, c = e / 2 % nchunks;
-      *(MLORA_GLOBAL f32x4 *)(out + v * a.width + 8 * c + 4 * h) = vec.at(v)[h * nchunks + c];
+    if constexpr (STREAMS > 1) {  // the streams' sums, added in stream order in the vectors' place
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < STREAMS; ++w) {
+        if (stream == w) {
+#pragma unroll
+          for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < NCH; ++k) {
+              const int c = c0 + 64 * WPR * k;
+              if (c >= nchunks) break;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                f32x4 s = f32x4{acc[v][k][4 * h], acc[v][k][4 * h + 1], acc[v][k][4 * h + 2], acc[v][k][4 * h + 3]};
+                f32x4 &dst = vec.at(v)[h * nchunks + c];
+                if (w > 0) s += dst;
+                dst = s;
+              }
+            }
+        }
+        __syncthreads();
+      }
+      for (int e = threadIdx.x; e < NV * 2 * nchunks; e += 64 * NW) {
+        const int v = e / (2 * nchunks), h = e % 2, c = e / 2 % nchunks;
+        *(MLORA_GLOBAL f32x4 *)(out + v * a.width + 8 * c + 4 * h) = vec.at(v)[h * nchunks + c];
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+          const int c = c0 + 64 * WPR * k;
+          if (c < nchunks) store8_any(out, true, v * a.width + 8 * c, acc[v][k]);
+        }
     }
   }
 }
 
-// Rows per workgroup: the fewest (a multiple of the rows in flight) that leave at most `most` workgroups.
+// Rows per workgroup (a multiple of the rows in flight): what leaves about `most` workgroups.
 static int joint_chunk(int64_t batches, int64_t tokens, int streams, int64_t most) {
-  int64_t chunk = streams;
-  while (chunk < 4096 && batches * ((tokens + chunk - 1) / chunk) > most) chunk *= 2;
-  return (int)chunk;
+  const int64_t per_sample = batches < most ? most / batches : 1;
+  const int64_t rows = (tokens + per_sample - 1) / per_sample;
+  return (int)((rows + streams - 1) / streams * streams);
 }
-constexpr int64_t kJointMostFwd = 4096, kJointMostBwd = 512;
+constexpr int64_t kJointMostFwd = 4096, kJointWavesBwd = 2048;
 
+// A row's waves and chunks per lane. Rows of more than one wave have a workgroup each.
 struct JointTile {
   int nch, wpr, nw;
 };
-static JointTile joint_tile(int64_t width) {
+static JointTile joint_tile(int64_t width, bool heavy) {
   const int n = (int)((width / 8 + 63) / 64);  // chunks of 8 values per lane of one wave
-  if (n <= 3) return {n, 1, 4};
-  if (n <= 6) return {n <= 4 ? 2 : 3, 2, 4};
-  if (n <= 12) return {n <= 8 ? 2 : 3, 4, 8};
+  if (n <= (heavy ? 2 : 3)) return {n, 1, 4};
+  if (heavy) return {2, n <= 4 ? 2 : n <= 8 ? 4 : 8, n <= 4 ? 2 : n <= 8 ? 4 : 8};
+  if (n <= 6) return {n <= 4 ? 2 : 3, 2, 2};
+  if (n <= 12) return {n <= 8 ? 2 : 3, 4, 4};
   return {2, 8, 8};
 }
 
@@ -384,30 +445,29 @@ static JointTile joint_tile(int64_t width) {
 template <class F>
 static void with_tile(const JointTile &t, F &&f) {
   using std::integral_constant;
+  auto one = integral_constant<int, 1>{};
+  auto two = integral_constant<int, 2>{};
+  auto three = integral_constant<int, 3>{};
+  auto four = integral_constant<int, 4>{};
+  auto eight = integral_constant<int, 8>{};
   if (t.wpr == 1) {
-    auto one = integral_constant<int, 1>{};
-    auto four = integral_constant<int, 4>{};
-    if (t.nch == 1) f(integral_constant<int, 1>{}, one, four);
-    else if (t.nch == 2) f(integral_constant<int, 2>{}, one, four);
-    else f(integral_constant<int, 3>{}, one, four);
+    if (t.nch == 1) f(one, one, four);
+    else if (t.nch == 2) f(two, one, four);
+    else f(three, one, four);
   } else if (t.wpr == 2) {
-    auto two = integral_constant<int, 2>{};
-    auto four = integral_constant<int, 4>{};
-    if (t.nch == 2) f(integral_constant<int, 2>{}, two, four);
-    else f(integral_constant<int, 3>{}, two, four);
+    if (t.nch == 2) f(two, two, two);
+    else f(three, two, two);
+  } else if (t.wpr == 4) {
+    if (t.nch == 2) f(two, four, four);
+    else f(three, four, four);
   } else {
-    auto four = integral_constant<int, 4>{};
-    auto eight = integral_constant<int, 8>{};
-    if (t.wpr == 8) f(integral_constant<int, 2>{}, eight, eight);
-    else if (t.nch == 2) f(integral_constant<int, 2>{}, four, eight);
-    else f(integral_constant<int, 3>{}, four, eight);
+    f(two, eight, eight);
   }
 }
 
-static int64_t joint_bwd_chunks(int64_t batches, int64_t tokens, int64_t width) {
-  const JointTile t = joint_tile(width);
-  const int64_t chunk = joint_chunk(batches, tokens, t.nw / t.wpr, kJointMostBwd);
-  return (tokens + chunk - 1) / chunk;
+// Workgroups of the backward that run at once: eight waves per compute unit.
+static int joint_bwd_chunk(const JointTile &t, int64_t batches, int64_t tokens) {
+  return joint_chunk(batches, tokens, t.nw / t.wpr, kJointWavesBwd / t.nw);
 }
 
 // Checks shared by both directions; fills everything but the outputs and the split of the rows.
@@ -465,11 +525,11 @@ extern "C" int mlora_joint(const void *x, int x_dtype, int64_t x_sb, int64_t x_s
   if (st || batches == 0 || tokens == 0 || width == 0) return st;
   if (x1 == nullptr || out == nullptr) return MLORA_ERR_INVALID;
   if (!aligned16(x1) || !aligned16(out)) return MLORA_ERR_UNSUPPORTED;
-  const JointTile tile = joint_tile(width);
+  const JointTile tile = joint_tile(width, false);
   a.x1 = x1, a.out = out;
   a.chunk = joint_chunk(batches, tokens, tile.nw / tile.wpr, kJointMostFwd);
   a.n_chunks = (int32_t)((tokens + a.chunk - 1) / a.chunk);
-  const unsigned lds = (unsigned)(kVecs * width * sizeof(float));
+  const unsigned lds = tile.wpr == 1 ? (unsigned)(kVecs * width * sizeof(float)) : 0;
   with_tile(tile, [&](auto nch, auto wpr, auto nw) {
     with_types(x_dtype == MLORA_F32, y_dtype == MLORA_F32, [&](auto xf, auto yf) {
       auto kernel = joint_kernel<decltype(nch)::value, decltype(wpr)::value, decltype(nw)::value, decltype(xf)::value,
@@ -486,7 +546,12 @@ extern "C" int64_t mlora_joint_backward_workspace_bytes(int64_t batches, int64_t
   if (batches == 0 || tokens == 0 || width == 0) return 0;
   if (width > kJointMaxWidth) return MLORA_ERR_UNSUPPORTED;
   if (tokens > (INT32_MAX - 8192) / batches) return MLORA_ERR_LIMIT;
-  return batches * joint_bwd_chunks(batches, tokens, width) * kVecs * width * (int64_t)sizeof(float);
+  int64_t most = 0;  // of the two tiles that a call of this size may take
+  for (bool heavy : {false, true}) {
+    const int64_t chunk = joint_bwd_chunk(joint_tile(width, heavy), batches, tokens), n = (tokens + chunk - 1) / chunk;
+    most = n > most ? n : most;
+  }
+  return batches * most * kVecs * width * (int64_t)sizeof(float);
 }
 
 extern "C" int mlora_joint_backward(const void *x, int x_dtype, int64_t x_sb, int64_t x_st, const void *y, int y_dtype,
@@ -520,20 +585,26 @@ extern "C" int mlora_joint_backward(const void *x, int x_dtype, int64_t x_sb, in
         return MLORA_ERR_WORKSPACE;
       if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
     }
-    const JointTile tile = joint_tile(width);
-    a.chunk = joint_chunk(batches, tokens, tile.nw / tile.wpr, kJointMostBwd);
+    // normed after and with sums wanted: two chunks per lane at most, three would leave one wave per SIMD
+    const JointTile tile = joint_tile(width, sums && post >= 0);
+    a.chunk = joint_bwd_chunk(tile, batches, tokens);
     a.n_chunks = (int32_t)((tokens + a.chunk - 1) / a.chunk);
     n_chunks = a.n_chunks;
     ba.gx = gx, ba.go = go, ba.gx_sb = gx_sb, ba.gx_st = gx_st, ba.go_sb = go_sb, ba.go_st = go_st;
     ba.dx = dx, ba.dy = dy, ba.partial = static_cast<float *>(workspace);
-    const unsigned lds = (unsigned)(kVecs * width * sizeof(float));
+    const unsigned lds = tile.wpr == 1 ? (unsigned)(kVecs * width * sizeof(float)) : 0;
     with_tile(tile, [&](auto nch, auto wpr, auto nw) {
       with_types(x_dtype == MLORA_F32, y_dtype == MLORA_F32, [&](auto xf, auto yf) {
         constexpr int NCH = decltype(nch)::value, WPR = decltype(wpr)::value, NW = decltype(nw)::value;
         constexpr bool XF = decltype(xf)::value, YF = decltype(yf)::value;
         const dim3 grid((unsigned)(batches * a.n_chunks)), block(64 * NW);
-        if (sums && post >= 0) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, true>), grid, block, lds, s, ba);
-        else if (sums) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, false>), grid, block, lds, s, ba);
+        if constexpr (NCH < 3) {
+          if (sums && post >= 0) {
+            hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, true>), grid, block, lds, s, ba);
+            return;
+          }
+        }
+        if (sums) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, false>), grid, block, lds, s, ba);
         else if (post >= 0) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, false, true>), grid, block, lds, s, ba);
         else hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, false, false>), grid, block, lds, s, ba);
       });

@@ -53,11 +53,41 @@ struct RotArgs {
   uint8_t axis[kRotMaxPairs];
 };
 
-__device__ __forceinline__ double load_pos(const RotArgs &a, int64_t o) {
-  if (a.pos_type == kPosI32) return (double)static_cast<const int32_t *>(a.pos)[o];
-  if (a.pos_type == kPosI64) return (double)static_cast<const int64_t *>(a.pos)[o];
-  return (double)static_cast<const float *>(a.pos)[o];
+// A position as it lies in memory, and its value.
+__device__ __forceinline__ uint64_t load_pos(const RotArgs &a, int64_t o) {
+  if (a.pos_type == kPosI64) return static_cast<const uint64_t *>(a.pos)[o];
+  return static_cast<const uint32_t *>(a.pos)[o];
 }
+__device__ __forceinline__ double pos_value(const RotArgs &a, uint64_t p) {
+  if (a.pos_type == kPosI64) return (double)(int64_t)p;
+  return a.pos_type == kPosI32 ? (double)(int32_t)p : (double)__uint_as_float((uint32_t)p);
+}
+
+// A unit's two chunks as they lie in memory, to be asked for a row ahead.
+template <bool F32>
+struct RawUnit {
+  u32x4 r[2][F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *p, int64_t e0, int64_t e1, bool on) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t e = h ? e1 : e0;
+      if constexpr (F32) {
+        const float *q = static_cast<const float *>(p) + e;
+        r[h][0] = on ? *(const MLORA_GLOBAL u32x4 *)q : u32x4{0, 0, 0, 0};
+        r[h][1] = on ? *(const MLORA_GLOBAL u32x4 *)(q + 4) : u32x4{0, 0, 0, 0};
+      } else {
+        r[h][0] = on ? *(const MLORA_GLOBAL u32x4 *)(static_cast<const uint16_t *>(p) + e) : u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (F32) v[i] = __uint_as_float(r[i / 8][i % 8 / 4][i % 4]);
+      else v[i] = __uint_as_float(i % 2 ? r[i / 8][0][i % 8 / 2] & 0xffff0000u : r[i / 8][0][i % 8 / 2] << 16);
+    }
+  }
+};
 
 // BWD: g is turned back and, with a norm, taken through it; else x is normed and turned.
 template <int NU, int WPR, bool F32, bool HALVES, bool NORM, bool BWD>
@@ -108,7 +138,7 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(const RotArgs a)
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < NU; ++k) s += v[k];
-      s = wave_sum(s);
+      s = lanes_sum<64>(s);
       if constexpr (WPR > 1) {
         if (lane == 0) red[slot][wave] = s;
         __syncthreads();
@@ -121,8 +151,12 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(const RotArgs a)
       for (int k = 0; k < NU; ++k) v[k] = s;
     } else if (64 % uph == 0) {  // a head's units are neighbouring lanes
 #pragma unroll
-      for (int k = 0; k < NU; ++k)
-        for (int m = 1; m < uph; m *= 2) v[k] += __shfl_xor(v[k], m);
+      for (int k = 0; k < NU; ++k) {
+        if (uph >= 2) v[k] = lanes_add<1>(v[k]);
+        if (uph >= 4) v[k] = lanes_add<2>(v[k]);
+        if (uph >= 8) v[k] = lanes_add<4>(v[k]);
+        if (uph >= 16) v[k] = lanes_add<8>(v[k]);
+      }
     } else {  // heads run across lanes, units and waves
       float *part = unit_part[slot] + stream * UNITS;
 #pragma unroll
@@ -138,32 +172,49 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(const RotArgs a)
       slot ^= 1;
     }
   };
+  // the next row's loads under this row's work (float32 rows are twice the registers: their waves do more)
+  constexpr bool kAhead = !F32;
+  RawUnit<F32> rv[!BWD || NORM ? NU : 1], rg[BWD ? NU : 1];
+  uint64_t pos[2];
+  auto load = [&](int r) __attribute__((always_inline)) {
+    const bool live = r < r1;
+    const int rc = min(r, a.rows - 1);
+    const int64_t b = rc / a.tokens, t = rc % a.tokens;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pos[i] = load_pos(a, b * a.pos_sb + t * a.pos_st + ax[i]);
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+      const bool on = live && lane + 64 * (k * WPR + sub) < units;
+      if constexpr (!BWD || NORM) {
+        const int64_t e = b * x.x_sb + t * x.x_st + head[k] * x.x_sh;
+        rv[k].load(x.x, e + e0[k], e + e1[k], on);
+      }
+      if constexpr (BWD) {
+        const int64_t e = b * x.g_sb + t * x.g_st + head[k] * x.g_sh;
+        rg[k].load(x.g, e + e0[k], e + e1[k], on);
+      }
+    }
+  };
+  if constexpr (kAhead) load(r0 + stream);
   // every stream runs the same number of rows, so that every wave meets the same barriers
   for (int r = r0 + stream; r - stream < r1; r += STREAMS) {
     const bool live = r < r1;
-    const int64_t b = min(r, a.rows - 1) / a.tokens, t = min(r, a.rows - 1) % a.tokens;
+    if constexpr (!kAhead) load(r);
     float v[NU][16], g[BWD ? NU : 1][16];
-    auto load = [&](const void *src, int64_t sb, int64_t st, int64_t sh, float (&o)[16], int k)
-        __attribute__((always_inline)) {
-      float lo[8] = {}, hi[8] = {};
-      if (live && lane + 64 * (k * WPR + sub) < units) {
-        const int64_t e = b * sb + t * st + head[k] * sh;
-        load8(src, F32, e + e0[k], lo), load8(src, F32, e + e1[k], hi);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = lo[i], o[i + 8] = hi[i];
-    };
 #pragma unroll
     for (int k = 0; k < NU; ++k) {
-      if constexpr (!BWD || NORM) load(x.x, x.x_sb, x.x_st, x.x_sh, v[k], k);
-      if constexpr (BWD) load(x.g, x.g_sb, x.g_st, x.g_sh, g[k], k);
+      if constexpr (!BWD || NORM) rv[k].unpack(v[k]);
+      if constexpr (BWD) rg[k].unpack(g[k]);
     }
+    double phi[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) phi[i] = pos_value(a, pos[i]) * turn[i];
+    if constexpr (kAhead) load(r + STREAMS);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (lane + 64 * i >= pairs) break;
-      const double phi = load_pos(a, b * a.pos_sb + t * a.pos_st + ax[i]) * turn[i];
       float s, c;
-      sincospif(2.0f * (float)(phi - __builtin_rint(phi)), &s, &c);
+      sincospif(2.0f * (float)(phi[i] - __builtin_rint(phi[i])), &s, &c);
       angles[wave][lane + 64 * i] = float2{c, BWD ? -s : s};
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -272,11 +323,10 @@ static RotTile rot_tile(int64_t width) {
   return {2, n <= 4 ? 2 : 4};
 }
 
-// Tokens per workgroup: the fewest (a multiple of the rows in flight) that leave at most `most` workgroups.
+// Tokens per workgroup (a multiple of the rows in flight): what leaves about `most` workgroups.
 static int64_t rot_chunk(int64_t rows, int64_t width, int64_t most) {
-  int64_t chunk = kRotWaves / rot_tile(width).wpr;
-  while (chunk < 65536 && (rows + chunk - 1) / chunk > most) chunk *= 2;
-  return chunk;
+  const int64_t streams = kRotWaves / rot_tile(width).wpr, n = (rows + most - 1) / most;
+  return (n + streams - 1) / streams * streams;
 }
 constexpr int64_t kRotMostFwd = 4096, kRotMostBwd = 512;
 

@@ -28,6 +28,36 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// v plus its value M lanes across (M = 1, 2, 4, ...: groups of M lanes already hold one value each, so that a
+// mirrored half row is as good as an exchange), in the VALU's own lane moves: a shuffle through the LDS unit costs
+// some hundred cycles, six of them per sum and several sums per row in a row's critical path.
+template <int M>
+__device__ __forceinline__ float lanes_add(float v) {
+  const uint32_t u = __float_as_uint(v);
+  if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else if constexpr (M == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else {
+    constexpr int kMove = M == 1 ? 0xB1 : M == 2 ? 0x4E : M == 4 ? 0x141 : 0x140;  // quad pairs, quad halves, mirrors
+    return v + __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)u, kMove, 0xf, 0xf, false));
+  }
+}
+
+// The sum of N neighbouring lanes (a power of two), in each of them.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (N >= 2) v = lanes_add<1>(v);
+  if constexpr (N >= 4) v = lanes_add<2>(v);
+  if constexpr (N >= 8) v = lanes_add<4>(v);
+  if constexpr (N >= 16) v = lanes_add<8>(v);
+  if constexpr (N >= 32) v = lanes_add<16>(v);
+  if constexpr (N >= 64) v = lanes_add<32>(v);
+  return v;
+}
+
 __device__ __forceinline__ void store8_any(void *base, bool f32, int64_t e, const float (&v)[8]) {
   if (f32) {
     float *p = static_cast<float *>(base) + e;
