@@ -12,6 +12,7 @@ the backward. float32: float32 throughout, on the fp32 matrix core.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -39,7 +40,7 @@ class CrossAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, key_mask, scale: float):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        out, lse = kernels.cross_attention(q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
+        out, lse = kernels.cross_attention(q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale, checked=True)
         ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask)
         ctx.scale = scale
         return out
@@ -48,9 +49,47 @@ class CrossAttentionFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         q, k, v, out, lse, key_lengths, key_mask = ctx.saved_tensors
-        grads = kernels.cross_attention_backward(q, k, v, out, lse, _aligned(g.to(q.dtype)), key_lengths=key_lengths,
-                                                 key_mask=key_mask, scale=ctx.scale)
-        return (*(d if want else None for d, want in zip(grads, ctx.needs_input_grad)), None, None, None)
+        grads = kernels.cross_attention_backward(q, k, v, out, lse, _aligned(g if g.dtype is q.dtype else g.to(q.dtype)),
+                                                 key_lengths=key_lengths, key_mask=key_mask, scale=ctx.scale, checked=True)
+        return (*[d if want else None for d, want in zip(grads, ctx.needs_input_grad)], None, None, None)
+
+
+def _meta(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+# What a call's shapes, types and options allow, checked once per combination of them.
+@functools.lru_cache(maxsize=256)
+def _plan(q, k, v, key_lengths, key_mask, scale) -> float:
+    for name, (shape, dtype, device) in (("q", q), ("k", k), ("v", v)):
+        if len(shape) != 4:
+            _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(shape)}")
+        if dtype not in _DTYPES:
+            _fail(f"{name} must be bfloat16 or float32, got {dtype}")
+        if dtype != q[1] or device != q[2]:
+            _fail("q, k and v share one dtype and device")
+    B, _, H, D = q[0]
+    Lk, Hk = k[0][1:3]
+    if k[0] != v[0] or k[0][0] != B or k[0][3] != D:
+        _fail(f"k and v must be [{B}, tokens, heads, {D}], got {tuple(k[0])} and {tuple(v[0])}")
+    if Hk < 1 or H < 1 or H % Hk:
+        _fail(f"{H} query heads do not share {Hk} key heads evenly")
+    if D % 8 or not 8 <= D <= 128:
+        _fail(f"head_dim must be a multiple of 8 up to 128, got {D}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        _fail("scale must be positive")
+    if key_lengths is not None:
+        shape, dtype, device = key_lengths
+        if device != q[2] or dtype not in (torch.int32, torch.int64) or tuple(shape) != (B,):
+            _fail(f"key_lengths must be int32 or int64 [{B}] on q's device")
+    if key_mask is not None:
+        shape, dtype, device = key_mask
+        if device != q[2] or dtype is not torch.bool or tuple(shape) not in ((Lk,), (1, Lk), (B, Lk)):
+            _fail(f"key_mask must be bool [{B}, {Lk}] on q's device")
+    if q[2].type != "cuda":
+        _fail("the tensors must be ROCm device tensors")
+    return scale
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_lengths: torch.Tensor | None = None,
@@ -60,38 +99,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     q [B, Lq, H, D], k and v [B, Lk, Hk, D], bfloat16 or float32, D a multiple of 8 up to 128. key_lengths:
     int32 or int64 [B] on q's device, the number of leading keys that count (clamped to [0, Lk]). key_mask:
     bool [B, Lk] (or [1, Lk], [Lk] for every sample), True where a key counts. scale > 0, 1 / sqrt(D) if not given."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(t.shape)}")
-        if t.dtype not in _DTYPES:
-            _fail(f"{name} must be bfloat16 or float32, got {t.dtype}")
-        if t.dtype != q.dtype or t.device != q.device:
-            _fail("q, k and v share one dtype and device")
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1:3]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        _fail(f"k and v must be [{B}, tokens, heads, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if Hk < 1 or H < 1 or H % Hk:
-        _fail(f"{H} query heads do not share {Hk} key heads evenly")
-    if D % 8 or not 8 <= D <= 128:
-        _fail(f"head_dim must be a multiple of 8 up to 128, got {D}")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        _fail("scale must be positive")
+    scale = _plan(_meta(q), _meta(k), _meta(v), _meta(key_lengths), _meta(key_mask), scale)
     if key_lengths is not None:
-        if key_lengths.device != q.device or key_lengths.dtype not in (torch.int32, torch.int64) or tuple(key_lengths.shape) != (B,):
-            _fail(f"key_lengths must be int32 or int64 [{B}] on q's device")
         if key_lengths.dtype is torch.int64:
-            key_lengths = key_lengths.clamp(0, Lk).to(torch.int32)
+            key_lengths = key_lengths.clamp(0, k.shape[1]).to(torch.int32)
         key_lengths = key_lengths.contiguous()
     if key_mask is not None:
         if key_mask.dim() == 1:
             key_mask = key_mask.unsqueeze(0)
-        if key_mask.device != q.device or key_mask.dtype is not torch.bool or key_mask.dim() != 2 \
-                or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Lk:
-            _fail(f"key_mask must be bool [{B}, {Lk}] on q's device")
-        if key_mask.stride(1) != 1 and Lk > 1:
+        if not key_mask.is_contiguous() and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    if not q.is_cuda:
-        _fail("the tensors must be ROCm device tensors")
     return CrossAttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)

@@ -807,19 +807,41 @@ NORM_NONE, NORM_HEAD, NORM_ROW = 0, 1, 2  # the rotary kernels' RMSNorm
 NORM_KINDS = {"layer": 0, "rms": 1}       # the joint's norms
 
 
-class _Device:
-    """Makes t's device the current one around a launch, where it is another."""
+def _call(name: str, t: torch.Tensor, *args) -> None:
+    """The C entry `name` on t's device and its current stream (the entry's last argument)."""
+    fn = getattr(_lib.load(), name)
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(name, status)
 
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+@functools.lru_cache(maxsize=512)
+def _bytes(name: str, *args) -> int:
+    """What a workspace query answers, by value."""
+    fn = getattr(_lib.load(), name)
+    nbytes = fn(*(_lib.i32_array(a) if isinstance(a, tuple) else a for a in args))
+    _lib.check(name, min(nbytes, 0))
+    return nbytes
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _i64s(values: tuple):
+    """Sizes and strides as a host array, by value (the entries only read it)."""
+    return _lib.i64_array(values)
+
+
+@functools.lru_cache(maxsize=256)
+def _i32s(values: tuple):
+    return _lib.i32_array(values)
 
 
 @functools.lru_cache(maxsize=64)
@@ -841,16 +863,27 @@ def _check_heads(name: str, t: torch.Tensor, dtype, lead) -> None:
 def rows_layout(t: torch.Tensor) -> bool:
     """Whether the row kernels take t as it lies: unit last stride, the others non-negative multiples of 8
     elements, 16-byte aligned."""
+    shape = t.shape
+    if t.is_contiguous():
+        return t.data_ptr() % 16 == 0 and (shape[-1] % 8 == 0 or t.dim() == 1)
     if t.numel() == 0:
         return True
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    if t.stride(-1) != 1 and shape[-1] != 1:
         return False
-    return t.data_ptr() % 16 == 0 and all(s >= 0 and s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+    return t.data_ptr() % 16 == 0 and all(s >= 0 and s % 8 == 0 for s, n in zip(t.stride()[:-1], shape[:-1]) if n > 1)
 
 
-def _strides(t: torch.Tensor, n: int) -> list:
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy that the row kernels take."""
+    if rows_layout(t):
+        return t
+    t = t.contiguous()
+    return t if rows_layout(t) else t.clone()
+
+
+def _strides(t: torch.Tensor, n: int) -> tuple:
     """The first n element strides, 0 in a dimension of one (its stride is never used)."""
-    return [s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape[:n])]
+    return tuple([s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape)])
 
 
 def _pos_args(positions: torch.Tensor, B: int, L: int):
@@ -862,126 +895,157 @@ def _pos_args(positions: torch.Tensor, B: int, L: int):
     return positions.data_ptr(), _POS_TYPES[positions.dtype], sb, st
 
 
-def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: Sequence[int], *, theta: float,
-                halves: bool, norm: int, weights: Sequence[torch.Tensor | None], eps: float) -> list[torch.Tensor]:
-    """The normed and rotated tensors (one or two [B, L, H_i, D] of one dtype), contiguous."""
-    B, L, _, D = xs[0].shape
-    for i, x in enumerate(xs):
-        _check_heads(f"tensor {i}", x, xs[0].dtype, (B, L))
-        _require(x.shape[3] == D, "the tensors share one head_dim")
+def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: tuple, *, theta: float,
+                halves: bool, norm: int, weights: Sequence[torch.Tensor | None], eps: float,
+                checked: bool = False) -> list[torch.Tensor]:
+    """The normed and rotated tensors (one or two [B, L, H_i, D] of one dtype), contiguous. checked: the caller
+    has made the checks of layout and type."""
+    first = xs[0]
+    B, L, _, D = first.shape
+    if not checked:
+        for i, x in enumerate(xs):
+            _check_heads(f"tensor {i}", x, first.dtype, (B, L))
+            _require(x.shape[3] == D and x.shape[2] >= 1, "the tensors have heads of one head_dim")
+        _check_weights(weights, norm, first)
+        _check_positions(positions, B, L)
     ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-    if B * L == 0 or any(x.shape[2] == 0 for x in xs):
-        _require(B * L == 0, "a tensor without heads")
+    if B * L == 0:
         return ys
-    turns, axis = rotary_turns(tuple(axis_dims), float(theta))
-    w_dt = weights[0].dtype if norm != NORM_NONE else torch.float32
-    with _Device(xs[0]):
-        _lib.check("mlora_rotary_axes", _lib.load().mlora_rotary_axes(
-            _lib.ptr_array([x.data_ptr() for x in xs]), _lib.ptr_array([y.data_ptr() for y in ys]),
-            _lib.ptr_array([_ptr(w) for w in weights]), _lib.i64_array([s for x in xs for s in _strides(x, 3)]),
-            _lib.i32_array([x.shape[2] for x in xs]), len(xs), _DT[xs[0].dtype], _DT[w_dt], norm, eps,
-            *_pos_args(positions, B, L), turns, axis, positions.shape[2], int(halves), B, L, D, _stream(xs[0])))
+    turns, axis = rotary_turns(axis_dims, theta)
+    _call("mlora_rotary_axes", first,
+          _lib.ptr_array([x.data_ptr() for x in xs]), _lib.ptr_array([y.data_ptr() for y in ys]),
+          _lib.ptr_array([w.data_ptr() for w in weights]) if norm else None,
+          _i64s(tuple([s for x in xs for s in _strides(x, 3)])), _i32s(tuple([x.shape[2] for x in xs])), len(xs),
+          _DT[first.dtype], _DT[weights[0].dtype] if norm else _lib.F32, norm, eps, positions.data_ptr(),
+          _POS_TYPES[positions.dtype], *_strides(positions, 2), turns, axis, positions.shape[2], halves, B, L, D)
     return ys
 
 
+def _check_weights(weights, norm: int, x: torch.Tensor) -> None:
+    _require(norm in (NORM_NONE, NORM_HEAD, NORM_ROW), "norm is NORM_NONE, NORM_HEAD or NORM_ROW")
+    for w in weights if norm else ():
+        _require(w is not None and w.is_cuda and w.dtype in _DT and w.dtype == weights[0].dtype and w.dim() == 1
+                 and rows_layout(w), "norm weights must be 16-byte aligned contiguous device vectors of one dtype")
+
+
+def _check_positions(positions: torch.Tensor, B: int, L: int) -> None:
+    _require(positions.is_cuda and positions.dtype in _POS_TYPES, "positions must be an int32, int64 or float32 device tensor")
+    _require(positions.dim() == 3 and positions.shape[0] in (1, B) and positions.shape[1] == L
+             and positions.shape[2] >= 1 and (positions.stride(2) == 1 or positions.shape[2] == 1),
+             f"positions must be [{B} or 1, {L}, axes] with unit axis stride")
+
+
 def rotary_axes_backward(xs: Sequence[torch.Tensor] | None, gs: Sequence[torch.Tensor], positions: torch.Tensor,
-                         axis_dims: Sequence[int], *, theta: float, halves: bool, norm: int,
+                         axis_dims: tuple, *, theta: float, halves: bool, norm: int,
                          weights: Sequence[torch.Tensor | None], eps: float, want_dx: Sequence[bool],
-                         want_dw: Sequence[bool]) -> tuple[list, list]:
+                         want_dw: Sequence[bool], checked: bool = False) -> tuple[list, list]:
     """(dx, dw) lists of rotary_axes; None where not wanted."""
-    B, L, _, D = gs[0].shape
-    for i, g in enumerate(gs):
-        _check_heads(f"gradient {i}", g, gs[0].dtype, (B, L))
-        if norm != NORM_NONE:
-            _check_heads(f"tensor {i}", xs[i], gs[0].dtype, (B, L))
-            _require(xs[i].shape == g.shape, "a gradient has its tensor's shape")
-    dev = gs[0].device
+    first = gs[0]
+    B, L, _, D = first.shape
+    if not checked:
+        for i, g in enumerate(gs):
+            _check_heads(f"gradient {i}", g, first.dtype, (B, L))
+            if norm:
+                _check_heads(f"tensor {i}", xs[i], first.dtype, (B, L))
+                _require(xs[i].shape == g.shape, "a gradient has its tensor's shape")
+        _check_weights(weights, norm, first)
+        _check_positions(positions, B, L)
+    dev = first.device
     dxs = [torch.empty(g.shape, dtype=g.dtype, device=dev) if w else None for g, w in zip(gs, want_dx)]
     dws = [torch.empty(w.shape, dtype=w.dtype, device=dev) if k else None for w, k in zip(weights, want_dw)]
-    turns, axis = rotary_turns(tuple(axis_dims), float(theta))
-    heads = _lib.i32_array([g.shape[2] for g in gs])
-    lib = _lib.load()
-    nbytes = lib.mlora_rotary_axes_backward_workspace_bytes(heads, len(gs), norm, B, L, D) if any(want_dw) else 0
-    _lib.check("mlora_rotary_axes_backward_workspace_bytes", min(nbytes, 0))
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    w_dt = weights[0].dtype if norm != NORM_NONE else torch.float32
-    pos = _pos_args(positions, B, L)
-    with _Device(gs[0]):
-        _lib.check("mlora_rotary_axes_backward", lib.mlora_rotary_axes_backward(
-            _lib.ptr_array([x.data_ptr() for x in xs]) if norm != NORM_NONE else None,
-            _lib.ptr_array([g.data_ptr() for g in gs]), _lib.ptr_array([_ptr(d) for d in dxs]),
-            _lib.ptr_array([_ptr(w) for w in weights]), _lib.ptr_array([_ptr(d) for d in dws]),
-            _lib.i64_array([s for x in xs for s in _strides(x, 3)]) if norm != NORM_NONE else None,
-            _lib.i64_array([s for g in gs for s in _strides(g, 3)]), heads, len(gs), _DT[gs[0].dtype], _DT[w_dt], norm,
-            eps, *pos, turns, axis, positions.shape[2], int(halves), _ptr(ws), nbytes, B, L, D, _stream(gs[0])))
+    turns, axis = rotary_turns(axis_dims, theta)
+    heads = tuple([g.shape[2] for g in gs])
+    nbytes = _bytes("mlora_rotary_axes_backward_workspace_bytes", heads, len(gs), norm, B, L, D) if any(want_dw) else 0
+    ws = _workspace(nbytes, dev)
+    _call("mlora_rotary_axes_backward", first,
+          _lib.ptr_array([x.data_ptr() for x in xs]) if norm else None,
+          _lib.ptr_array([g.data_ptr() for g in gs]), _lib.ptr_array([_ptr(d) for d in dxs]),
+          _lib.ptr_array([w.data_ptr() for w in weights]) if norm else None,
+          _lib.ptr_array([_ptr(d) for d in dws]) if nbytes or any(want_dw) else None,
+          _i64s(tuple([s for x in xs for s in _strides(x, 3)])) if norm else None,
+          _i64s(tuple([s for g in gs for s in _strides(g, 3)])), _i32s(heads), len(gs), _DT[first.dtype],
+          _DT[weights[0].dtype] if norm else _lib.F32, norm, eps, positions.data_ptr(), _POS_TYPES[positions.dtype],
+          *_strides(positions, 2), turns, axis, positions.shape[2], halves, _ptr(ws), nbytes, B, L, D)
     return dxs, dws
 
 
-def _vec(name: str, v: torch.Tensor | None, B: int, W: int) -> tuple:
-    """(pointer, dtype code, element stride per sample) of a [B or 1, W] vector, None allowed."""
+def vector_layout(v: torch.Tensor, B: int, W: int) -> bool:
+    """Whether v is a vector of the joint: [W], [B or 1, W] or [B or 1, 1, W]."""
+    shape = tuple(v.shape)
+    return shape in ((W,), (1, W), (B, W), (1, 1, W), (B, 1, W))
+
+
+def _vec(v: torch.Tensor | None) -> tuple:
+    """(pointer, dtype code, element stride per sample) of a vector, None allowed."""
     if v is None:
         return None, _lib.F32, 0
-    _require(v.is_cuda and v.dtype in _DT and v.dim() == 2 and v.shape[0] in (1, B) and v.shape[1] == W,
-             f"{name} must be a bfloat16 or float32 device tensor [{B} or 1, {W}]")
-    _require(rows_layout(v), f"{name} needs unit stride and 16-byte aligned rows")
-    return v.data_ptr(), _DT[v.dtype], _strides(v, 1)[0]
+    return v.data_ptr(), _DT[v.dtype], v.stride(0) if v.dim() > 1 and v.shape[0] > 1 else 0
 
 
-def _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps):
+def _check_joint(x, y, gate, scale, shift, post_w, norm, post) -> None:
     B, T, W = x.shape
     for name, t in (("x", x), ("y", y)):
         _require(t.is_cuda and t.dtype in _DT and tuple(t.shape) == (B, T, W) and rows_layout(t),
                  f"{name} must be a bfloat16 or float32 [{B}, {T}, {W}] device tensor with 16-byte aligned rows")
-    g_ptr, g_dt, g_sb = _vec("gate", gate, B, W)
-    s_ptr, s_dt, s_sb = _vec("scale", scale, B, W)
-    h_ptr, h_dt, h_sb = _vec("shift", shift, B, W)
-    _require(scale is None or shift is None or s_dt == h_dt, "scale and shift share a dtype")
-    p_ptr, p_dt, _ = _vec("post weight", post_w, 1, W)
-    post_kind = -1 if post is None else NORM_KINDS[post]
+    for name, v in (("gate", gate), ("scale", scale), ("shift", shift), ("post weight", post_w)):
+        _require(v is None or (v.is_cuda and v.dtype in _DT and vector_layout(v, B, W) and rows_layout(v)),
+                 f"{name} must be a bfloat16 or float32 device vector [{W}], [{B}, {W}] or [{B}, 1, {W}], 16-byte aligned")
+    _require(post_w is None or post_w.numel() == W, "the post weight is shared by the samples")
+    _require(scale is None or shift is None or scale.dtype == shift.dtype, "scale and shift share a dtype")
+    _require(norm in NORM_KINDS and (post is None or post in NORM_KINDS), "norm and post are 'layer' or 'rms'")
+
+
+def _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps):
+    g_ptr, g_dt, g_sb = _vec(gate)
+    s_ptr, s_dt, s_sb = _vec(scale)
+    h_ptr, _, h_sb = _vec(shift)
+    p_ptr, p_dt, _ = _vec(post_w)
     head = (x.data_ptr(), _DT[x.dtype], *_strides(x, 2), y.data_ptr(), _DT[y.dtype], *_strides(y, 2))
-    tail = (g_ptr, g_dt, g_sb, s_ptr, h_ptr, s_dt, s_sb, h_sb, int(unit_offset), p_ptr, p_dt, NORM_KINDS[norm],
-            post_kind, alpha, eps)
+    tail = (g_ptr, g_dt, g_sb, s_ptr, h_ptr, s_dt, s_sb, h_sb, unit_offset, p_ptr, p_dt, NORM_KINDS[norm],
+            -1 if post is None else NORM_KINDS[post], alpha, eps)
     return head, tail
 
 
 def joint(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None, scale: torch.Tensor | None,
           shift: torch.Tensor | None, post_w: torch.Tensor | None, *, norm: str, post: str | None, unit_offset: bool,
-          alpha: float, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
-    """(x1, out) of the sublayer joint; vectors are [B or 1, W], post_w [1, W]."""
+          alpha: float, eps: float, checked: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(x1, out) of the sublayer joint; vectors as vector_layout says. checked: the caller has made the checks."""
+    if not checked:
+        _check_joint(x, y, gate, scale, shift, post_w, norm, post)
     head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
-    x1 = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out = torch.empty(x.shape, dtype=y.dtype, device=x.device)
+    shape, dev = x.shape, x.device
+    x1 = torch.empty(shape, dtype=x.dtype, device=dev)
+    out = torch.empty(shape, dtype=y.dtype, device=dev)
     if x.numel():
-        with _Device(x):
-            _lib.check("mlora_joint", _lib.load().mlora_joint(*head, *tail, x1.data_ptr(), out.data_ptr(), *x.shape,
-                                                              _stream(x)))
+        _call("mlora_joint", x, *head, *tail, x1.data_ptr(), out.data_ptr(), *shape)
     return x1, out
 
 
 def joint_backward(x: torch.Tensor, y: torch.Tensor, gx: torch.Tensor | None, go: torch.Tensor | None,
                    gate: torch.Tensor | None, scale: torch.Tensor | None, shift: torch.Tensor | None,
                    post_w: torch.Tensor | None, *, norm: str, post: str | None, unit_offset: bool, alpha: float,
-                   eps: float, want: Sequence[bool]) -> list:
-    """[dx, dy, dgate, dscale, dshift, dpost] (None where not wanted); a [1, W] vector's gradient is summed
-    over the samples."""
+                   eps: float, want: Sequence[bool], checked: bool = False) -> list:
+    """[dx, dy, dgate, dscale, dshift, dpost] (None where not wanted), in their operands' shapes: the gradient of a
+    vector of all samples is summed over them."""
+    if not checked:
+        _check_joint(x, y, gate, scale, shift, post_w, norm, post)
+        for name, t, like in (("gx", gx, x), ("go", go, y)):
+            _require(t is None or (t.is_cuda and t.dtype == like.dtype and t.shape == x.shape and rows_layout(t)),
+                     f"{name} must have its output's shape and dtype, with 16-byte aligned rows")
     B, T, W = x.shape
     head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
-    for name, t, like in (("gx", gx, x), ("go", go, y)):
-        _require(t is None or (t.is_cuda and t.dtype == like.dtype and t.shape == x.shape and rows_layout(t)),
-                 f"{name} must have its output's shape and dtype, with 16-byte aligned rows")
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if w else None
+    dev = x.device
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
             for t, w in zip((x, y, gate, scale, shift, post_w), want)]
     if W == 0:
         return outs
-    lib = _lib.load()
-    nbytes = lib.mlora_joint_backward_workspace_bytes(B, T, W) if any(want[2:]) else 0
-    _lib.check("mlora_joint_backward_workspace_bytes", min(nbytes, 0))
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device) if nbytes else None
-    grads = [v for t in (gx, go) for v in ((None, 0, 0) if t is None else (t.data_ptr(), *_strides(t, 2)))]
-    shared = [int(v is not None and v.shape[0] == 1) for v in (gate, scale, shift)]
-    with _Device(x):
-        _lib.check("mlora_joint_backward", lib.mlora_joint_backward(
-            *head, *grads, *tail, *(_ptr(o) for o in outs), *shared, _ptr(ws), nbytes, B, T, W, _stream(x)))
+    nbytes = _bytes("mlora_joint_backward_workspace_bytes", B, T, W) if any(want[2:]) else 0
+    ws = _workspace(nbytes, dev)
+    gx_args = (None, 0, 0) if gx is None else (gx.data_ptr(), *_strides(gx, 2))
+    go_args = (None, 0, 0) if go is None else (go.data_ptr(), *_strides(go, 2))
+    shared = [v is not None and v.numel() == W for v in (gate, scale, shift)]
+    _call("mlora_joint_backward", x, *head, *gx_args, *go_args, *tail, *[_ptr(o) for o in outs], *shared, _ptr(ws), nbytes,
+          B, T, W)
     return outs
 
 
@@ -993,7 +1057,7 @@ def attention_layout(t: torch.Tensor) -> bool:
     return rows_layout(t) and (t.numel() == 0 or t.shape[1] < 2 or t.stride(1) < ATTENTION_MAX_STRIDE)
 
 
-def _attention_args(q, k, v, key_lengths, key_mask, scale):
+def _check_attention(q, k, v, key_lengths, key_mask) -> None:
     B, Lq, H, D = q.shape
     Lk, Hk = k.shape[1:3]
     for name, t, shape in (("q", q, (B, Lq, H, D)), ("k", k, (B, Lk, Hk, D)), ("v", v, (B, Lk, Hk, D))):
@@ -1007,48 +1071,50 @@ def _attention_args(q, k, v, key_lengths, key_mask, scale):
                                   and key_mask.shape[0] in (1, B) and key_mask.shape[1] == Lk
                                   and (key_mask.stride(1) == 1 or Lk < 2)),
              f"key_mask must be a bool device tensor [{B} or 1, {Lk}] with unit stride")
-    operands = [a for t in (q, k, v) for a in (t.data_ptr(), _lib.i64_array(_strides(t, 3)))]
-    mask = (None, 0) if key_mask is None else (key_mask.data_ptr(), _strides(key_mask, 1)[0])
-    return (*operands, _DT[q.dtype], _ptr(key_lengths), *mask, scale), (B, Lq, Lk, H, Hk, D)
 
 
-@functools.lru_cache(maxsize=512)
-def _attention_workspace(name: str, dtype: int, sizes: tuple) -> int:
-    nbytes = getattr(_lib.load(), name)(dtype, *sizes)
-    _lib.check(name, min(nbytes, 0))
-    return nbytes
+def _attention_args(q, k, v, key_lengths, key_mask, scale):
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    mask = (None, 0) if key_mask is None else (key_mask.data_ptr(), *_strides(key_mask, 1))
+    return (q.data_ptr(), _i64s(_strides(q, 3)), k.data_ptr(), _i64s(_strides(k, 3)), v.data_ptr(), _i64s(_strides(v, 3)),
+            _DT[q.dtype], _ptr(key_lengths), *mask, scale), (B, Lq, Lk, H, Hk, D)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_lengths: torch.Tensor | None,
-                    key_mask: torch.Tensor | None, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
-    """(out, lse) of softmax(scale q kᵀ) v over the keys that count; lse [B, H, Lq] float32, base 2."""
+                    key_mask: torch.Tensor | None, scale: float,
+                    checked: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse) of softmax(scale q kᵀ) v over the keys that count; lse [B, H, Lq] float32, base 2. checked: the
+    caller has made the checks."""
+    if not checked:
+        _check_attention(q, k, v, key_lengths, key_mask)
     args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
     B, Lq, _, H, _, _ = sizes
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
-    nbytes = _attention_workspace("mlora_cross_attention_workspace_bytes", _DT[q.dtype], sizes)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-    with _Device(q):
-        _lib.check("mlora_cross_attention", _lib.load().mlora_cross_attention(
-            *args, out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, *sizes, _stream(q)))
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev)
+    nbytes = _bytes("mlora_cross_attention_workspace_bytes", _DT[q.dtype], *sizes)
+    ws = _workspace(nbytes, dev)
+    _call("mlora_cross_attention", q, *args, out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, *sizes)
     return out, lse
 
 
 def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
                              g: torch.Tensor, *, key_lengths: torch.Tensor | None, key_mask: torch.Tensor | None,
-                             scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                             scale: float, checked: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv), contiguous, from the forward's out and lse and the upstream gradient g of out."""
+    if not checked:
+        _check_attention(q, k, v, key_lengths, key_mask)
+        for name, t in (("out", out), ("g", g)):
+            _require(t.is_cuda and t.dtype == q.dtype and t.shape == q.shape, f"{name} must have q's shape and dtype")
+        _require(out.is_contiguous() and attention_layout(g), "out is contiguous, g's heads are 16-byte aligned")
+        _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == q.shape[0] * q.shape[1] * q.shape[2],
+                 "lse is the forward's [batch, heads, tokens]")
     args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
-    for name, t in (("out", out), ("g", g)):
-        _require(t.is_cuda and t.dtype == q.dtype and t.shape == q.shape, f"{name} must have q's shape and dtype")
-    _require(out.is_contiguous() and attention_layout(g), "out is contiguous, g's heads are 16-byte aligned")
-    _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == q.shape[0] * q.shape[1] * q.shape[2],
-             "lse is the forward's [batch, heads, tokens]")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    nbytes = _attention_workspace("mlora_cross_attention_backward_workspace_bytes", _DT[q.dtype], sizes)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-    with _Device(q):
-        _lib.check("mlora_cross_attention_backward", _lib.load().mlora_cross_attention_backward(
-            *args, out.data_ptr(), lse.data_ptr(), g.data_ptr(), _lib.i64_array(_strides(g, 3)),
-            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes, *sizes, _stream(q)))
+    dev = q.device
+    dq, dk, dv = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+    nbytes = _bytes("mlora_cross_attention_backward_workspace_bytes", _DT[q.dtype], *sizes)
+    ws = _workspace(nbytes, dev)
+    _call("mlora_cross_attention_backward", q, *args, out.data_ptr(), lse.data_ptr(), g.data_ptr(), _i64s(_strides(g, 3)),
+          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes, *sizes)
     return dq, dk, dv

@@ -12,6 +12,7 @@ q, k and the norm weights. Outputs are rounded once from float32 arithmetic; ang
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Sequence
 
@@ -52,73 +53,59 @@ def grid_positions(grid_sizes, tokens: int, device=None, start=0) -> torch.Tenso
     return out.to(device) if device is not None else out
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    if kernels.rows_layout(t):
-        return t
-    t = t.contiguous()
-    return t if kernels.rows_layout(t) else t.clone()
-
-
-def _norm_kinds(name: str, x: torch.Tensor, w: torch.Tensor | None) -> set:
-    if w is None:
-        return {kernels.NORM_NONE}
-    H, D = x.shape[2:]
-    if w.device != x.device or w.dtype not in _DTYPES or w.dim() != 1 or w.shape[0] not in (D, H * D):
-        _fail(f"{name} must be a bfloat16 or float32 vector of {D} (per head) or {H * D} (the row) on q's device")
-    return {kind for kind, n in ((kernels.NORM_ROW, H * D), (kernels.NORM_HEAD, D)) if n == w.shape[0]}
-
-
 class RotaryAxesFunction(torch.autograd.Function):
-    """``apply(positions, axis_dims, theta, halves, norm, eps, n, *tensors, *weights)`` -> n tensors."""
+    """``apply(positions, cfg, n, *tensors, *weights)`` -> n tensors; cfg as _plan gives it, no weights without a
+    norm."""
 
     @staticmethod
-    def forward(ctx, positions, axis_dims, theta, halves, norm, eps, n, *args):
+    def forward(ctx, positions, cfg, n, *args):
+        args = [t if kernels.rows_layout(t) else kernels.aligned(t) for t in args]
         xs, ws = args[:n], args[n:]
-        xs = [_aligned(x) for x in xs]
-        ws = [_aligned(w) for w in ws] if norm else list(ws)
-        ys = kernels.rotary_axes(xs, positions, axis_dims, theta=theta, halves=halves, norm=norm, weights=ws, eps=eps)
-        ctx.save_for_backward(positions, *(xs if norm else ()), *(ws if norm else ()))
-        ctx.cfg = (axis_dims, theta, halves, norm, eps, n)
+        ctx.save_for_backward(positions, *(args if ws else ()))
+        ctx.cfg, ctx.n = cfg, n
         ctx.like = [(x.shape, x.dtype, x.device) for x in xs]
         ctx.set_materialize_grads(False)
-        return tuple(ys)
+        return tuple(kernels.rotary_axes(xs, positions, weights=ws, checked=True, **cfg))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        axis_dims, theta, halves, norm, eps, n = ctx.cfg
-        none = (None,) * (7 + 2 * n)
+        n, needs = ctx.n, ctx.needs_input_grad
         if all(g is None for g in grads):
-            return none
+            return (None,) * len(needs)
         positions, *saved = ctx.saved_tensors
-        xs, ws = (saved[:n], saved[n:]) if norm else (None, [None] * n)
         gs = []
         for g, (shape, dtype, device) in zip(grads, ctx.like):
-            g = torch.zeros(shape, dtype=dtype, device=device) if g is None else g.to(dtype)
-            gs.append(_aligned(g))
-        want_dx, want_dw = ctx.needs_input_grad[7:7 + n], ctx.needs_input_grad[7 + n:]
-        dxs, dws = kernels.rotary_axes_backward(xs, gs, positions, axis_dims, theta=theta, halves=halves, norm=norm,
-                                                weights=ws, eps=eps, want_dx=want_dx, want_dw=want_dw)
-        return (*none[:7], *dxs, *dws)
+            if g is None:
+                g = torch.zeros(shape, dtype=dtype, device=device)
+            gs.append(kernels.aligned(g if g.dtype is dtype else g.to(dtype)))
+        dxs, dws = kernels.rotary_axes_backward(saved[:n] if saved else None, gs, positions, weights=saved[n:],
+                                                want_dx=needs[3:3 + n], want_dw=needs[3 + n:], checked=True, **ctx.cfg)
+        return (None, None, None, *dxs, *dws)
 
 
-def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
-    first = xs[0]
-    for name, x in zip(names, xs):
-        if x.dim() != 4:
-            _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(x.shape)}")
-        if x.dtype not in _DTYPES:
-            _fail(f"{name} must be bfloat16 or float32, got {x.dtype}")
-        if x.dtype != first.dtype or x.device != first.device:
+def _meta(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+# What a call's shapes, types and options allow, checked once per combination of them.
+@functools.lru_cache(maxsize=256)
+def _plan(names, xs, ws, positions, axis_dims, theta, pairing, eps) -> dict:
+    first, dtype, device = xs[0]
+    for name, (shape, dt, dev) in zip(names, xs):
+        if len(shape) != 4:
+            _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(shape)}")
+        if dt not in _DTYPES:
+            _fail(f"{name} must be bfloat16 or float32, got {dt}")
+        if dt != dtype or dev != device:
             _fail("q and k share one dtype and device")
-        if x.shape[:2] != first.shape[:2] or x.shape[3] != first.shape[3]:
-            _fail(f"q and k share batch, tokens and head_dim, got {tuple(first.shape)} and {tuple(x.shape)}")
-    B, L, _, D = first.shape
+        if shape[:2] != first[:2] or shape[3] != first[3]:
+            _fail(f"q and k share batch, tokens and head_dim, got {tuple(first)} and {tuple(shape)}")
+    B, L, _, D = first
     if D % 16 or not 16 <= D <= 256:
         _fail(f"head_dim must be a multiple of 16 up to 256, got {D}")
-    if any(not 1 <= x.shape[2] <= 8192 // D for x in xs):
+    if any(not 1 <= shape[2] <= 8192 // D for shape, _, _ in xs):
         _fail(f"heads * head_dim must be between {D} and 8192")
-    axis_dims = tuple(int(d) for d in axis_dims)
     if not axis_dims or any(d < 0 or d % 2 for d in axis_dims) or sum(axis_dims) != D:
         _fail(f"axis_dims must be even channel counts that add up to head_dim {D}, got {axis_dims}")
     if pairing not in _PAIRINGS:
@@ -127,27 +114,40 @@ def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
         _fail("theta must be positive")
     if not (math.isfinite(eps) and eps > 0):
         _fail("eps must be positive")
-    if positions.device != first.device or positions.dtype not in (torch.int32, torch.int64, torch.float32):
+    shape, dt, dev = positions
+    if dev != device or dt not in (torch.int32, torch.int64, torch.float32):
         _fail("positions must be int32, int64 or float32 on q's device")
-    if positions.requires_grad:
-        _fail("positions take no gradient")
-    if positions.dim() == 2:
-        positions = positions.unsqueeze(0)
-    if positions.dim() != 3 or positions.shape[0] not in (1, B) or tuple(positions.shape[1:]) != (L, len(axis_dims)):
-        _fail(f"positions must be [{L}, {len(axis_dims)}] or [{B}, {L}, {len(axis_dims)}], got {tuple(positions.shape)}")
-    if positions.shape[2] > 1 and positions.stride(2) != 1 or any(s < 0 for s in positions.stride()):
-        positions = positions.contiguous()
+    if tuple(shape) not in ((L, len(axis_dims)), (1, L, len(axis_dims)), (B, L, len(axis_dims))):
+        _fail(f"positions must be [{L}, {len(axis_dims)}] or [{B}, {L}, {len(axis_dims)}], got {tuple(shape)}")
     if len({w is None for w in ws}) > 1:
         _fail("q_weight and k_weight come together")
-    kinds = set.intersection(*(_norm_kinds(f"{name}_weight", x, w) for name, x, w in zip(names, xs, ws)))
+    kinds = {kernels.NORM_NONE} if ws[0] is None else {kernels.NORM_ROW, kernels.NORM_HEAD}
+    for name, (shape, _, _), w in zip(names, xs, ws):
+        if w is None:
+            continue
+        H = shape[2]
+        if w[2] != device or w[1] not in _DTYPES or tuple(w[0]) not in ((D,), (H * D,)):
+            _fail(f"{name}_weight must be a bfloat16 or float32 vector of {D} (per head) or {H * D} (the row) on q's device")
+        kinds &= {kind for kind, n in ((kernels.NORM_ROW, H * D), (kernels.NORM_HEAD, D)) if n == w[0][0]}
     if not kinds:
         _fail("q and k are normed alike: both over the row or both per head")
-    if ws[0] is not None and any(w.dtype != ws[0].dtype for w in ws):
+    if ws[0] is not None and any(w[1] != ws[0][1] for w in ws):
         _fail("q_weight and k_weight share a dtype")
-    if not first.is_cuda:
+    if device.type != "cuda":
         _fail("the tensors must be ROCm device tensors")
-    return RotaryAxesFunction.apply(positions, axis_dims, float(theta), pairing == "halves", max(kinds), float(eps),
-                                    len(xs), *xs, *ws)
+    return dict(axis_dims=axis_dims, theta=float(theta), halves=pairing == "halves", norm=max(kinds), eps=float(eps))
+
+
+def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
+    if positions.requires_grad:
+        _fail("positions take no gradient")
+    cfg = _plan(names, tuple([_meta(x) for x in xs]), tuple([_meta(w) for w in ws]), _meta(positions),
+                tuple([int(d) for d in axis_dims]), theta, pairing, eps)
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(0)
+    if not positions.is_contiguous() and (positions.stride(2) != 1 or any(s < 0 for s in positions.stride())):
+        positions = positions.contiguous()
+    return RotaryAxesFunction.apply(positions, cfg, len(xs), *xs, *(ws if cfg["norm"] else ()))
 
 
 def rotary_axes(x: torch.Tensor, positions: torch.Tensor, axis_dims: Sequence[int], *, theta: float = 10000.0,
@@ -158,11 +158,11 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, axis_dims: Sequence[in
     axis_dims: channels of each axis (even, adding up to D), in the order of the positions. pairing:
     "adjacent" turns channels 2i and 2i + 1, "halves" channels i and i + D / 2. weight: RMSNorm first, over the
     token's whole row for [H * D], over each head for [D]."""
-    return _apply([x], [weight], ["x"], positions, axis_dims, theta, pairing, eps)[0]
+    return _apply((x,), (weight,), ("x",), positions, axis_dims, theta, pairing, eps)[0]
 
 
 def rotary_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axis_dims: Sequence[int], *,
                    theta: float = 10000.0, pairing: str = "adjacent", q_weight: torch.Tensor | None = None,
                    k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """rotary_axes of q and k (their head counts may differ) in one launch."""
-    return _apply([q, k], [q_weight, k_weight], ["q", "k"], positions, axis_dims, theta, pairing, eps)
+    return _apply((q, k), (q_weight, k_weight), ("q", "k"), positions, axis_dims, theta, pairing, eps)

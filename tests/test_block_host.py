@@ -162,3 +162,70 @@ def test_joint_entries_validate_before_launch(pkg):
     assert bwd(nbytes=ws - 1) == L.ERR_WORKSPACE and bwd(work=0) == L.ERR_WORKSPACE and bwd(work=0xc004) == L.ERR_UNSUPPORTED
     assert bwd(gate=0) == L.ERR_INVALID and bwd(dpost=0xf000) == L.ERR_INVALID
     assert bwd(gx=0x8004) == L.ERR_UNSUPPORTED and bwd(dx=0x9008) == L.ERR_UNSUPPORTED
+
+
+def test_attention_refusals(pkg):
+    q, k = torch.zeros(2, 5, 4, 64), torch.zeros(2, 7, 2, 64)
+
+    def bad(match, q=q, k=k, v=None, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            pkg.cross_attention(q, k, k if v is None else v, **kw)
+
+    bad("batch, tokens", q=q[0])
+    bad("bfloat16 or float32", q=q.half())
+    bad("one dtype", k=k.to(BF))
+    bad("k and v must be", v=k[:, :6])
+    bad("k and v must be", k=k[:1])
+    bad("k and v must be", k=torch.zeros(2, 7, 2, 32))
+    bad("share", k=torch.zeros(2, 7, 3, 64))
+    bad("share", k=torch.zeros(2, 7, 0, 64))
+    bad("multiple of 8", q=torch.zeros(2, 5, 4, 60), k=torch.zeros(2, 7, 2, 60))
+    bad("multiple of 8", q=torch.zeros(2, 5, 4, 136), k=torch.zeros(2, 7, 2, 136))
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        bad("scale", scale=scale)
+    bad("key_lengths", key_lengths=torch.zeros(2))
+    bad("key_lengths", key_lengths=torch.zeros(3, dtype=torch.int32))
+    bad("key_mask", key_mask=torch.zeros(2, 7, dtype=torch.uint8))
+    bad("key_mask", key_mask=torch.zeros(2, 6, dtype=torch.bool))
+    bad("ROCm device", key_lengths=torch.zeros(2, dtype=torch.int64), key_mask=torch.zeros(7, dtype=torch.bool))
+
+
+def test_attention_entries_validate_before_launch(pkg):
+    L, lib = pkg._lib, pkg._lib.load()
+    st = (1280, 256, 64)
+
+    def fwd(q=0x1000, k=0x2000, v=0x3000, qs=st, ks=st, dt=L.BF16, mask=None, mask_sb=0, scale=0.125, out=0x4000, lse=0x5000,
+            work=0x6000, nbytes=1 << 30, B=2, Lq=5, Lk=7, H=4, Hk=4, D=64):
+        return lib.mlora_cross_attention(q, L.i64_array(qs), k, L.i64_array(ks), v, L.i64_array(st), dt, None, mask, mask_sb,
+                                         scale, out, lse, work, nbytes, B, Lq, Lk, H, Hk, D, None)
+
+    assert fwd(B=0) == L.OK and fwd(Lq=0, q=0, out=0, lse=0) == L.OK
+    for kw, code in ((dict(q=0), L.ERR_INVALID), (dict(q=0x1008), L.ERR_UNSUPPORTED), (dict(k=0), L.ERR_INVALID),
+                     (dict(qs=(1280, 252, 64)), L.ERR_UNSUPPORTED), (dict(qs=(1280, -256, 64)), L.ERR_UNSUPPORTED),
+                     (dict(ks=(1280, 1 << 22, 64)), L.ERR_LIMIT), (dict(dt=L.FP8_E4M3), L.ERR_UNSUPPORTED),
+                     (dict(mask=0x7000, mask_sb=-1), L.ERR_INVALID), (dict(scale=0.0), L.ERR_INVALID),
+                     (dict(scale=float("inf")), L.ERR_INVALID), (dict(out=0), L.ERR_INVALID), (dict(out=0x4004), L.ERR_UNSUPPORTED),
+                     (dict(lse=0), L.ERR_INVALID), (dict(lse=0x5002), L.ERR_UNSUPPORTED), (dict(Hk=3), L.ERR_INVALID),
+                     (dict(H=0), L.ERR_INVALID), (dict(D=60), L.ERR_UNSUPPORTED), (dict(D=136), L.ERR_UNSUPPORTED),
+                     (dict(Lk=1 << 31), L.ERR_LIMIT), (dict(Lq=1 << 30, H=8, Hk=1), L.ERR_LIMIT), (dict(Lq=-1), L.ERR_INVALID),
+                     (dict(B=1 << 20, Lq=1 << 24), L.ERR_LIMIT)):
+        assert fwd(**kw) == code, kw
+    # few rows against many keys: partial sums need a workspace
+    size = lambda *a: lib.mlora_cross_attention_workspace_bytes(L.BF16, *a)  # noqa: E731
+    need = size(1, 1, 4096, 4, 4, 64)
+    assert need > 0 and need % ((64 + 2) * 4 * 4) == 0 and size(1, 4096, 64, 4, 4, 64) == 0 and size(1, 1, 0, 4, 4, 64) == 0
+    assert size(1, 1, 4096, 4, 3, 64) == L.ERR_INVALID
+    assert fwd(B=1, Lq=1, Lk=4096, nbytes=need - 1) == L.ERR_WORKSPACE and fwd(B=1, Lq=1, Lk=4096, work=0) == L.ERR_WORKSPACE
+    assert fwd(B=1, Lq=1, Lk=4096, work=0x6004) == L.ERR_UNSUPPORTED
+    back = lib.mlora_cross_attention_backward_workspace_bytes(L.BF16, 2, 5, 7, 4, 4, 64)
+    assert back >= 2 * 4 * 5 * 4
+
+    def bwd(g=0x7000, gs=st, dq=0x8000, dk=0x9000, out=0x4000, work=0x6000, nbytes=back, lse=0x5000):
+        return lib.mlora_cross_attention_backward(0x1000, L.i64_array(st), 0x2000, L.i64_array(st), 0x3000, L.i64_array(st),
+                                                  L.BF16, None, None, 0, 0.125, out, lse, g, L.i64_array(gs), dq, dk, 0xa000,
+                                                  work, nbytes, 2, 5, 7, 4, 4, 64, None)
+
+    assert bwd(g=0) == L.ERR_INVALID and bwd(gs=(1280, 252, 64)) == L.ERR_UNSUPPORTED and bwd(dq=0) == L.ERR_INVALID
+    assert bwd(dk=0) == L.ERR_INVALID and bwd(dk=0x9004) == L.ERR_UNSUPPORTED and bwd(out=0) == L.ERR_INVALID
+    assert bwd(lse=0) == L.ERR_INVALID and bwd(nbytes=back - 1) == L.ERR_WORKSPACE and bwd(work=0) == L.ERR_WORKSPACE
+    assert bwd(work=0x6008) == L.ERR_UNSUPPORTED
