@@ -495,10 +495,10 @@ struct AttnBwdArgs {
   const void *o, *g;  // the output [B, Lq, H, D] contiguous, and its gradient
   void *dq, *dk, *dv;  // contiguous
   float *delta;        // [B, H, Lq]
-  f32x4 *part;         // dk / dv splits, in register order
+  f32x4 *part;         // splits of dq, then of dk and dv, in register order
   int64_t g_sb, g_sl, g_sh;
   float scale;
-  int32_t key_blocks, q_tiles, head_q_tiles, q_splits, q_split_tiles;
+  int32_t key_blocks, q_tiles, head_q_tiles, q_splits, q_split_tiles;  // dk / dv; dq's splits are f's
 };
 
 template <class T, int DP>
@@ -513,9 +513,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   int id = blockIdx.x;  // heads first: rows of all heads are read together, whole token rows of memory
   const int hk = id % a.Hk;
   id /= a.Hk;
-  const int rt = id % a.row_tiles, b = id / a.row_tiles;
-  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, sample_keys(a, b)};
-  const int t1 = (km.len + KT - 1) / KT;
+  const int rt = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int b = id % a.batches, sp = id / a.batches;
+  const int t0 = sp * a.split_tiles;
+  const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)sample_keys(a, b)), t1 = (end + KT - 1) / KT;
+  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, end};
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
   TileLoader<T, DP, N> kl, vl;
@@ -525,10 +528,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     vl.load(vp + (int64_t)t * KT * a.v_sl, bits, lds + buf * 2 * TB + TB);
   };
   uint64_t bits = 0, next = 0;
-  if (t1 > 0) {
-    bits = km.bits(0, km.byte(0, lane));
-    stage(0, 0, bits);
-    next = km.bits(1, km.byte(1, lane));
+  if (t0 < t1) {
+    bits = km.bits(t0, km.byte(t0, lane));
+    stage(t0, 0, bits);
+    next = km.bits(t0 + 1, km.byte(t0 + 1, lane));
   }
   FragReader<T, DP> fr;
   fr.init(lane, lds);
@@ -561,7 +564,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     }
   }
   delta = half_sum(delta);
-  if (lane < 32 && r < a.rows) ba.delta[head_rows + r] = delta;
+  if (lane < 32 && r < a.rows && sp == 0) ba.delta[head_rows + r] = delta;
   const float lse = a.lse[head_rows + rc];
   f32x16 dq[ND];
 #pragma unroll
@@ -603,10 +606,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
       return true;
     });
   };
-  for (int t = 0; t < t1; ++t) {
+  for (int t = t0; t < t1; ++t) {
     wait_vmcnt<0>();
     lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    stage(t + 1, (t + 1) & 1, next);  // past the last tile: no live row, nothing is read
+    stage(t + 1, (t + 1 - t0) & 1, next);  // past the last tile: no live row, nothing is read
     const int byte = km.byte(t + 2, lane);
     if (bits != 0) step(bits);
     fr.flip(2 * TB);
@@ -614,11 +617,43 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     next = km.bits(t + 2, byte);
   }
   wait_vmcnt<0>();
+  if (a.splits > 1) {
+    f32x4 *p = ba.part + ((((int64_t)sp * a.batches + b) * a.row_tiles + rt) * a.Hk + hk) * (4 * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dq[d][4 * i], dq[d][4 * i + 1], dq[d][4 * i + 2], dq[d][4 * i + 3]};
+    return;
+  }
   const float f[1] = {ba.scale};
   f32x16 o[1][ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[0][d] = dq[d];
   store_rows<T, DP, 1>(static_cast<T *>(ba.dq) + oat, o, f, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
+}
+
+// Adds the splits of dq in split order and writes them out.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_dq_join_kernel(const AttnBwdArgs ba) {
+  const AttnArgs &a = ba.f;
+  constexpr int ND = DP / 32;
+  const int64_t per = (int64_t)a.batches * a.row_tiles * a.Hk * 4 * ND * 4 * 64;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
+  int64_t u = e / 64;
+  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % 4);
+  u /= 4 * ND * 4;  // (b, row tile, hk)
+  const int hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * 128 + wave * 32 + (lane & 31);
+  const int64_t b = u / a.Hk / a.row_tiles;
+  const int ch = 32 * d + 8 * i + 4 * (lane >> 5);
+  if (r >= a.rows || ch >= a.D) return;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(ba.part + s * per + e);
+  x *= ba.scale;
+  T *p = static_cast<T *>(ba.dq) + (b * a.Lq * a.H + (int64_t)hk * a.G) * a.D + row_at(r, a.Lq, (int64_t)a.H * a.D, a.D) + ch;
+  if constexpr (sizeof(T) == 2) *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
+  else *(MLORA_GLOBAL f32x4 *)p = x;
 }
 
 // NW waves own 32 keys each (K fragments in registers; V in LDS for bf16, whose two waves per SIMD leave no room
@@ -865,6 +900,30 @@ static int64_t attn_part_floats(const AttnPlan &p, int64_t batches, int64_t Hk, 
   return p.splits > 1 ? p.splits * batches * Hk * rows * (D + 2) : 0;
 }
 
+struct DqPlan {
+  int64_t row_tiles, splits, split_tiles;
+};
+
+// dq: 128 rows per workgroup; the keys are split where the rows alone leave places for workgroups free.
+static DqPlan dq_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, bool f32) {
+  DqPlan p{};
+  p.row_tiles = (rows + 127) / 128;
+  const int64_t kt = f32 ? AttnTile<float>::KT : AttnTile<uint16_t>::KT, tiles = (Lk + kt - 1) / kt;
+  const int64_t groups = batches * Hk * p.row_tiles, most = f32 ? 256 : 512;
+  int64_t splits = groups > 0 && groups < most ? most / groups : 1;
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits < 1) splits = 1;
+  p.split_tiles = (tiles + splits - 1) / splits;
+  if (p.split_tiles < 1) p.split_tiles = 1;
+  p.splits = tiles > 0 ? (tiles + p.split_tiles - 1) / p.split_tiles : 1;
+  return p;
+}
+
+// 16-byte vectors of one split of dq, in register order.
+static int64_t dq_vectors(const DqPlan &p, int64_t batches, int64_t Hk, int64_t D) {
+  return batches * p.row_tiles * Hk * 4 * (D > 64 ? 4 : 2) * 4 * 64;
+}
+
 struct DkvPlan {
   int nw;  // waves per workgroup, 32 keys each
   int64_t key_blocks, q_tiles, head_q_tiles, splits, split_tiles;
@@ -893,8 +952,11 @@ static int64_t dkv_vectors(const DkvPlan &p, int64_t batches, int64_t Hk, int64_
   return batches * Hk * p.key_blocks * p.nw * 2 * (D > 64 ? 4 : 2) * 4 * 64;
 }
 
-static int64_t dkv_part_bytes(const DkvPlan &p, int64_t batches, int64_t Hk, int64_t D) {
-  return p.splits > 1 ? p.splits * dkv_vectors(p, batches, Hk, D) * 16 : 0;
+// The splits of dq, and after they are joined those of dk and dv in the same place.
+static int64_t bwd_part_bytes(const DqPlan &q, const DkvPlan &p, int64_t batches, int64_t Hk, int64_t D) {
+  const int64_t dq = q.splits > 1 ? q.splits * dq_vectors(q, batches, Hk, D) * 16 : 0;
+  const int64_t dkv = p.splits > 1 ? p.splits * dkv_vectors(p, batches, Hk, D) * 16 : 0;
+  return dq > dkv ? dq : dkv;
 }
 
 // Sizes and types shared by every entry. MLORA_OK, or the status.
@@ -1007,8 +1069,10 @@ extern "C" int64_t mlora_cross_attention_backward_workspace_bytes(int dtype, int
                                                                   int64_t Hk, int64_t D) {
   const int st = attn_sizes(dtype, B, Lq, Lk, H, Hk, D);
   if (st) return st;
-  // delta, rounded up to whole 16-byte vectors, then the splits of dk and dv
-  return (B * H * Lq + 3) / 4 * 16 + dkv_part_bytes(dkv_plan(B, Lq, Lk, Hk, H / Hk, D, dtype == MLORA_F32), B, Hk, D);
+  // delta, rounded up to whole 16-byte vectors, then the splits
+  const bool f32 = dtype == MLORA_F32;
+  return (B * H * Lq + 3) / 4 * 16 +
+         bwd_part_bytes(dq_plan(B, H / Hk * Lq, Lk, Hk, f32), dkv_plan(B, Lq, Lk, Hk, H / Hk, D, f32), B, Hk, D);
 }
 
 extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_strides, const void *k,
@@ -1040,12 +1104,16 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   ba.part = static_cast<f32x4 *>(workspace) + (B * H * Lq + 3) / 4;
   ba.key_blocks = (int32_t)p.key_blocks, ba.q_tiles = (int32_t)p.q_tiles, ba.head_q_tiles = (int32_t)p.head_q_tiles;
   ba.q_splits = (int32_t)p.splits, ba.q_split_tiles = (int32_t)p.split_tiles;
-  a.row_tiles = (int32_t)((a.rows + 127) / 128);
+  const DqPlan qp = dq_plan(B, a.rows, Lk, Hk, f32);
+  a.row_tiles = (int32_t)qp.row_tiles, a.splits = (int32_t)qp.splits, a.split_tiles = (int32_t)qp.split_tiles;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (Lq > 0) {
     with_head(f32, D, [&](auto t, auto dp) {
-      hipLaunchKernelGGL((attn_dq_kernel<decltype(t), decltype(dp)::value>), dim3((unsigned)(B * Hk * a.row_tiles)),
-                         dim3(256), 0, s, ba);
+      using T = decltype(t);
+      constexpr int DP = decltype(dp)::value;
+      hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3((unsigned)(B * Hk * a.row_tiles * qp.splits)), dim3(256), 0, s, ba);
+      if (qp.splits > 1)
+        hipLaunchKernelGGL((attn_dq_join_kernel<T, DP>), dim3((unsigned)(dq_vectors(qp, B, Hk, D) / 256)), dim3(256), 0, s, ba);
     });
     st = launch_status();
     if (st) return st;
