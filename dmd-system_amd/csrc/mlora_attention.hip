@@ -876,7 +876,9 @@ static int64_t row_turns(int64_t tiles, int64_t key_tiles) {
 }
 
 // How a forward is cut: few rows per key head run waves over different keys, more rows 128 per workgroup;
-// the keys are split where that leaves less than a workgroup for every compute unit and there are enough of them.
+// the keys are split where that leaves less than a workgroup for every compute unit and there are enough of them:
+// a float32 tile takes about as long as a join, a bf16 tile a sixth of it (2 x 64 rows x 512 keys, 12 heads of 128,
+// float32: 47 us where a split takes 8 tiles at least, 31 with 4, 23 with 2; bf16 14.7, 16.3 and 15.6).
 static AttnPlan attn_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, int64_t D, bool f32) {
   AttnPlan p{};
   p.few = rows <= (f32 && D > 64 ? 32 : 64);
@@ -886,7 +888,7 @@ static AttnPlan attn_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk,
   p.row_tiles = p.few ? 1 : (rows + 127) / 128;
   p.turns = p.few ? 1 : row_turns(batches * Hk * p.row_tiles, tiles);
   const int64_t groups = batches * Hk * p.row_tiles;
-  const int64_t least = p.few ? 4 * waves : 8;  // tiles that a split is worth its join for
+  const int64_t least = p.few ? (f32 ? waves : 4 * waves) : f32 ? 2 : 8;  // tiles that a split is worth its join for
   int64_t splits = groups > 0 && groups < 256 ? 256 / groups : 1;
   if (splits > tiles / least) splits = tiles / least;
   if (splits < 1) splits = 1;
@@ -904,14 +906,17 @@ struct DqPlan {
   int64_t row_tiles, splits, split_tiles;
 };
 
-// dq: 128 rows per workgroup; the keys are split where the rows alone leave places for workgroups free.
+// dq: 128 rows per workgroup; the keys are split where the rows alone leave places for workgroups free (bf16, 300
+// rows x 8192 keys, 8 heads of 128: the backward takes 72 us, unsplit 226), four tiles at least to a split for bf16,
+// one for float32 (200 rows x 300 keys, 16 heads of 64: bf16 20 us, with one tile 24; float32 41, with four 66).
 static DqPlan dq_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, bool f32) {
   DqPlan p{};
   p.row_tiles = (rows + 127) / 128;
   const int64_t kt = f32 ? AttnTile<float>::KT : AttnTile<uint16_t>::KT, tiles = (Lk + kt - 1) / kt;
   const int64_t groups = batches * Hk * p.row_tiles, most = f32 ? 256 : 512;
   int64_t splits = groups > 0 && groups < most ? most / groups : 1;
-  if (splits > tiles / 4) splits = tiles / 4;
+  const int64_t least = f32 ? 1 : 4;
+  if (splits > tiles / least) splits = tiles / least;
   if (splits < 1) splits = 1;
   p.split_tiles = (tiles + splits - 1) / splits;
   if (p.split_tiles < 1) p.split_tiles = 1;
@@ -929,7 +934,8 @@ struct DkvPlan {
   int64_t key_blocks, q_tiles, head_q_tiles, splits, split_tiles;
 };
 
-// dk / dv: 32 nw keys per workgroup; the query rows are split where the keys alone leave compute units idle.
+// dk / dv: 32 nw keys per workgroup; the query rows are split where the keys alone leave compute units idle, with
+// dq's least numbers of tiles.
 static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t D, bool f32) {
   DkvPlan p{};
   p.nw = !f32 && D > 64 && Lk > 128 ? 8 : 4;
@@ -939,7 +945,8 @@ static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int
   p.q_tiles = G * p.head_q_tiles;
   const int64_t groups = batches * Hk * p.key_blocks, most = !f32 && p.nw == 4 ? 512 : 256;  // workgroups that run at once
   int64_t splits = groups > 0 && groups < most ? most / groups : 1;
-  if (splits > p.q_tiles / 4) splits = p.q_tiles / 4;
+  const int64_t least = f32 ? 1 : 4;
+  if (splits > p.q_tiles / least) splits = p.q_tiles / least;
   if (splits < 1) splits = 1;
   p.split_tiles = (p.q_tiles + splits - 1) / splits;
   if (p.split_tiles < 1) p.split_tiles = 1;
