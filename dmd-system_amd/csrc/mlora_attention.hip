@@ -518,6 +518,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   const int b = id % a.batches, sp = id / a.batches;
   const int t0 = sp * a.split_tiles;
   const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)sample_keys(a, b)), t1 = (end + KT - 1) / KT;
+  // Few keys, and out's rounding to bf16 tells in delta (5 keys: 1.4e-3 of dq, as much as dS's): it is summed from P and
+  // dP, formed once more, where all the keys are in one tile. From 65 keys on it is below a third of dS's.
+  const bool one = sample_keys(a, b) <= KT;
   const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, end};
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
@@ -564,34 +567,39 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     }
   }
   delta = half_sum(delta);
-  if (lane < 32 && r < a.rows && sp == 0) ba.delta[head_rows + r] = delta;
   const float lse = a.lse[head_rows + rc];
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
+  auto weights = [&](auto block, uint64_t bits, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {  // P and dP
+    constexpr int kb = decltype(block)::value;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      Frag<T> kf, vf;
+      fr.template rows<0, 32 * kb>(ks, kf);
+      s = mma16(kf, q[ks], s);
+      fr.template rows<TB, 32 * kb>(ks, vf);
+      dp = mma16(vf, g[ks], dp);
+    }
+    if (bits != low_bits(KT)) {
+      const uint64_t mine = bits >> (4 * (lane >> 5));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.c - lse);
+  };
   auto step = [&](uint64_t bits) __attribute__((always_inline)) {
     static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
       constexpr int kb = decltype(block)::value;
       f32x16 s, dp;
+      weights(block, bits, s, dp);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        Frag<T> kf, vf;
-        fr.template rows<0, 32 * kb>(ks, kf);
-        s = mma16(kf, q[ks], s);
-        fr.template rows<TB, 32 * kb>(ks, vf);
-        dp = mma16(vf, g[ks], dp);
-      }
-      if (bits != low_bits(KT)) {
-        const uint64_t mine = bits >> (4 * (lane >> 5));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.c - lse) * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
       static_for<2>([&](auto ks) __attribute__((always_inline)) {
         Frag<T> ds;
         to_frag(s, ks, ds);
@@ -611,12 +619,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
     stage(t + 1, (t + 1 - t0) & 1, next);  // past the last tile: no live row, nothing is read
     const int byte = km.byte(t + 2, lane);
+    if (sizeof(T) == 2 && one && bits != 0) {
+      float sum = 0.f;
+      static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
+        f32x16 s, dp;
+        weights(block, bits, s, dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += s[i] * dp[i];
+        return true;
+      });
+      delta = half_sum(sum);
+    }
     if (bits != 0) step(bits);
     fr.flip(2 * TB);
     bits = next;
     next = km.bits(t + 2, byte);
   }
   wait_vmcnt<0>();
+  if (lane < 32 && r < a.rows && sp == 0) ba.delta[head_rows + r] = delta;
   if (a.splits > 1) {
     f32x4 *p = ba.part + ((((int64_t)sp * a.batches + b) * a.row_tiles + rt) * a.Hk + hk) * (4 * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
 #pragma unroll
