@@ -109,4 +109,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
             key_mask = key_mask.unsqueeze(0)
         if not key_mask.is_contiguous() and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    return CrossAttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
+    if kernels.wants_grad((q, k, v)):
+        return CrossAttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
+    return kernels.cross_attention(_aligned(q), _aligned(k), _aligned(v), key_lengths=key_lengths, key_mask=key_mask,
+                                   scale=scale, checked=True)[0]

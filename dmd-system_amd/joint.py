@@ -27,13 +27,16 @@ def _fail(message: str) -> None:
     raise RuntimeError("gated residual norm: " + message)
 
 
+def _laid_out(*tensors):
+    return [t if t is None or kernels.rows_layout(t) else kernels.aligned(t) for t in tensors]
+
+
 class GatedResidualNormFunction(torch.autograd.Function):
     """``apply(x, y, gate, scale, shift, post_weight, cfg)`` -> (x1, out); cfg as _plan gives it."""
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, post_weight, cfg):
-        args = [t if t is None or kernels.rows_layout(t) else kernels.aligned(t)
-                for t in (x, y, gate, scale, shift, post_weight)]
+        args = _laid_out(x, y, gate, scale, shift, post_weight)
         ctx.save_for_backward(*args)
         ctx.cfg = cfg
         ctx.set_materialize_grads(False)
@@ -108,4 +111,7 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | N
     else by scale (a norm's weight, with shift its bias)."""
     cfg = _plan(_meta(x), _meta(y), _meta(gate), _meta(scale), _meta(shift), _meta(post_weight), norm, unit_offset,
                 post_norm, residual_scale, eps)
-    return GatedResidualNormFunction.apply(x, y, gate, scale, shift, post_weight, cfg)
+    args = (x, y, gate, scale, shift, post_weight)
+    if kernels.wants_grad(args):
+        return GatedResidualNormFunction.apply(*args, cfg)
+    return kernels.joint(*_laid_out(*args), **cfg, checked=True)

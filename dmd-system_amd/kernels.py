@@ -829,6 +829,16 @@ def _bytes(name: str, *args) -> int:
     return nbytes
 
 
+def wants_grad(tensors) -> bool:
+    """Whether autograd has to record an operator on these (None allowed); if not, its forward is called as it is,
+    without the 4 us of a Function's apply."""
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
@@ -886,15 +896,6 @@ def _strides(t: torch.Tensor, n: int) -> tuple:
     return tuple([s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape)])
 
 
-def _pos_args(positions: torch.Tensor, B: int, L: int):
-    _require(positions.is_cuda and positions.dtype in _POS_TYPES, "positions must be an int32, int64 or float32 device tensor")
-    _require(positions.dim() == 3 and positions.shape[0] in (1, B) and positions.shape[1] == L
-             and positions.shape[2] >= 1 and (positions.stride(2) == 1 or positions.shape[2] == 1),
-             f"positions must be [{B} or 1, {L}, axes] with unit axis stride")
-    sb, st = _strides(positions, 2)
-    return positions.data_ptr(), _POS_TYPES[positions.dtype], sb, st
-
-
 def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: tuple, *, theta: float,
                 halves: bool, norm: int, weights: Sequence[torch.Tensor | None], eps: float,
                 checked: bool = False) -> list[torch.Tensor]:
@@ -908,7 +909,7 @@ def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: 
             _require(x.shape[3] == D and x.shape[2] >= 1, "the tensors have heads of one head_dim")
         _check_weights(weights, norm, first)
         _check_positions(positions, B, L)
-    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    ys = [_new(x) for x in xs]
     if B * L == 0:
         return ys
     turns, axis = rotary_turns(axis_dims, theta)
@@ -951,8 +952,8 @@ def rotary_axes_backward(xs: Sequence[torch.Tensor] | None, gs: Sequence[torch.T
         _check_weights(weights, norm, first)
         _check_positions(positions, B, L)
     dev = first.device
-    dxs = [torch.empty(g.shape, dtype=g.dtype, device=dev) if w else None for g, w in zip(gs, want_dx)]
-    dws = [torch.empty(w.shape, dtype=w.dtype, device=dev) if k else None for w, k in zip(weights, want_dw)]
+    dxs = [_new(g) if w else None for g, w in zip(gs, want_dx)]
+    dws = [_new(w) if k else None for w, k in zip(weights, want_dw)]
     turns, axis = rotary_turns(axis_dims, theta)
     heads = tuple([g.shape[2] for g in gs])
     nbytes = _bytes("mlora_rotary_axes_backward_workspace_bytes", heads, len(gs), norm, B, L, D) if any(want_dw) else 0
@@ -1013,11 +1014,9 @@ def joint(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None, scale: to
     if not checked:
         _check_joint(x, y, gate, scale, shift, post_w, norm, post)
     head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
-    shape, dev = x.shape, x.device
-    x1 = torch.empty(shape, dtype=x.dtype, device=dev)
-    out = torch.empty(shape, dtype=y.dtype, device=dev)
+    x1, out = _new(x), _new(y)
     if x.numel():
-        _call("mlora_joint", x, *head, *tail, x1.data_ptr(), out.data_ptr(), *shape)
+        _call("mlora_joint", x, *head, *tail, x1.data_ptr(), out.data_ptr(), *x.shape)
     return x1, out
 
 
@@ -1034,13 +1033,11 @@ def joint_backward(x: torch.Tensor, y: torch.Tensor, gx: torch.Tensor | None, go
                      f"{name} must have its output's shape and dtype, with 16-byte aligned rows")
     B, T, W = x.shape
     head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
-    dev = x.device
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
-            for t, w in zip((x, y, gate, scale, shift, post_w), want)]
+    outs = [_new(t) if w else None for t, w in zip((x, y, gate, scale, shift, post_w), want)]
     if W == 0:
         return outs
     nbytes = _bytes("mlora_joint_backward_workspace_bytes", B, T, W) if any(want[2:]) else 0
-    ws = _workspace(nbytes, dev)
+    ws = _workspace(nbytes, x.device)
     gx_args = (None, 0, 0) if gx is None else (gx.data_ptr(), *_strides(gx, 2))
     go_args = (None, 0, 0) if go is None else (go.data_ptr(), *_strides(go, 2))
     shared = [v is not None and v.numel() == W for v in (gate, scale, shift)]
@@ -1091,7 +1088,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
     B, Lq, _, H, _, _ = sizes
     dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = _new(q)
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev)
     nbytes = _bytes("mlora_cross_attention_workspace_bytes", _DT[q.dtype], *sizes)
     ws = _workspace(nbytes, dev)
@@ -1111,10 +1108,9 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == q.shape[0] * q.shape[1] * q.shape[2],
                  "lse is the forward's [batch, heads, tokens]")
     args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
-    dev = q.device
-    dq, dk, dv = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+    dq, dk, dv = _new(q), _new(k), _new(v)
     nbytes = _bytes("mlora_cross_attention_backward_workspace_bytes", _DT[q.dtype], *sizes)
-    ws = _workspace(nbytes, dev)
+    ws = _workspace(nbytes, q.device)
     _call("mlora_cross_attention_backward", q, *args, out.data_ptr(), lse.data_ptr(), g.data_ptr(), _i64s(_strides(g, 3)),
           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes, *sizes)
     return dq, dk, dv

@@ -59,7 +59,7 @@ class RotaryAxesFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, positions, cfg, n, *args):
-        args = [t if kernels.rows_layout(t) else kernels.aligned(t) for t in args]
+        args = [kernels.aligned(t) for t in args]
         xs, ws = args[:n], args[n:]
         ctx.save_for_backward(positions, *(args if ws else ()))
         ctx.cfg, ctx.n = cfg, n
@@ -147,7 +147,11 @@ def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
         positions = positions.unsqueeze(0)
     if not positions.is_contiguous() and (positions.stride(2) != 1 or any(s < 0 for s in positions.stride())):
         positions = positions.contiguous()
-    return RotaryAxesFunction.apply(positions, cfg, len(xs), *xs, *(ws if cfg["norm"] else ()))
+    args = (*xs, *ws) if cfg["norm"] else xs
+    if kernels.wants_grad(args):
+        return RotaryAxesFunction.apply(positions, cfg, len(xs), *args)
+    args = [kernels.aligned(t) for t in args]
+    return tuple(kernels.rotary_axes(args[:len(xs)], positions, weights=args[len(xs):], checked=True, **cfg))
 
 
 def rotary_axes(x: torch.Tensor, positions: torch.Tensor, axis_dims: Sequence[int], *, theta: float = 10000.0,
