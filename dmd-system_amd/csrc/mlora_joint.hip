@@ -15,11 +15,15 @@
 // u and its statistics are formed again from x and y: dgate needs y anyway, so reading x in place of a
 // stored x1 costs nothing and keeps û exact.
 //
-// Both passes are HBM-bound. A row is held in registers by WPR waves (8 values per lane and chunk); the
-// vectors of the workgroup's sample do not: in registers they would halve the waves that hide the loads'
-// latency. A workgroup takes `chunk` rows of one sample; the backward's column sums stay in
-// registers over those rows, are added over the workgroup's rows in flight through LDS, and leave as one
-// partial row per workgroup (fixed order, no atomics).
+// dgate and dw_post are one sum, S = Σ du·p̂ per channel: dgate = w_post·S, dw_post = gate·S (gate is the
+// workgroup's sample's), multiplied behind the rows.
+//
+// Both passes are HBM-bound and run at what a large copy reaches (4.9 TB/s): 2 x 32760 rows of 1536, float32 stream,
+// bf16 y, every vector's gradient: 229 us forward (604 MB in, 604 MB out), 376 backward; 2 x 11040 rows of
+// 5120, bf16, normed on both sides: 175 and 291. A row is held in registers by WPR waves (8 values per lane and
+// chunk). A workgroup takes `chunk` rows of one sample; the backward's column sums stay in registers over
+// those rows, are added over the workgroup's rows in flight through LDS, and leave as one partial row
+// per workgroup (fixed order, no atomics).
 #include "mlora_common.h"
 #include "mlora_host.h"
 #include "mlora_rows.h"
@@ -81,10 +85,10 @@ struct RowSum {
 
 // The sample's vectors: gate, m, shift, w_post, formed from their sources (ones or zeros where there is none).
 // LDS: copied once per workgroup, values 8c .. 8c + 3 of vector v at [v][0][c], 8c + 4 .. 8c + 7 at [v][1][c]
-// (two conflict-free 16-byte reads per chunk). Else read again for every row, out of the L1 and L2 caches: rows of
-// several waves are wide, their vectors would fill the LDS and leave one workgroup per compute unit, whose rows
-// move in step (11040 x 2 rows of 5120 normed on both sides, bf16: forward 315 us against 206, backward 740 against
-// 411).
+// (two conflict-free 16-byte reads per chunk): for rows of one wave, four of which share them. Rows of several
+// waves are wide and have a workgroup each: its lanes read what they need into registers once (2 x 11040 rows
+// of 5120 normed on both sides, bf16: backward 291 us; 418 with the vectors read from the caches for every row, 740
+// from LDS, which they would fill).
 template <bool LDS>
 struct Vectors {
   const JointArgs &a;
@@ -193,7 +197,7 @@ struct RawRow {
 template <int NCH, int WPR, int NW, bool XF32, bool YF32>
 __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
   constexpr int STREAMS = NW / WPR;
-  constexpr bool kAhead = WPR > 1;
+  constexpr bool kAhead = WPR > 1, kHeld = WPR > 1;
   __shared__ float red[4][2][NW];
   extern __shared__ f32x4 dyn[];
   const int wave = wave_id(), lane = threadIdx.x & 63, stream = wave / WPR;
@@ -205,6 +209,24 @@ __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
   vec.fill();
   RowSum<WPR, NW> sum{red, wave, stream * WPR};
   __syncthreads();
+  float gw[kHeld ? NCH : 1][8], mult[kHeld ? NCH : 1][8], shift[kHeld ? NCH : 1][8];
+  auto read_gw = [&](int c, float (&g)[8]) __attribute__((always_inline)) {  // gate · w_post
+    vec.read(kVecGate, c, g);
+    if (a.post < 0) return;
+    float w[8];
+    vec.read(kVecPost, c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] *= w[i];
+  };
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = min(c0 + 64 * WPR * k, nchunks - 1);
+      read_gw(c, gw[k]);
+      vec.read(kVecMult, c, mult[k]);
+      vec.read(kVecShift, c, shift[k]);
+    }
+  }
   RawRow<NCH, WPR, XF32> rx;
   RawRow<NCH, WPR, YF32> ry;
   auto load = [&](int t) __attribute__((always_inline)) {
@@ -219,27 +241,16 @@ __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
     if constexpr (!kAhead) load(t);
     rx.unpack(u), ry.unpack(p);
     if constexpr (kAhead) load(t + STREAMS);
-    if (a.post >= 0) {
-      norm_row<NCH, WPR>(p, c0, nchunks, a.post, inv_w, a.eps, sum);
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + 64 * WPR * k;
-        if (c >= nchunks) break;
-        float w[8];
-        vec.read(kVecPost, c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[k][i] *= w[i];
-      }
-    }
+    if (a.post >= 0) norm_row<NCH, WPR>(p, c0, nchunks, a.post, inv_w, a.eps, sum);
     const int64_t row = (b * a.tokens + t) * a.width;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = c0 + 64 * WPR * k;
       if (c >= nchunks) break;
       float g[8];
-      vec.read(kVecGate, c, g);
+      if constexpr (!kHeld) read_gw(c, g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[k][i] = a.alpha * u[k][i] + g[i] * p[k][i];
+      for (int i = 0; i < 8; ++i) u[k][i] = a.alpha * u[k][i] + (kHeld ? gw[kHeld ? k : 0][i] : g[i]) * p[k][i];
       if (live) store8_any(a.x1, XF32, row + 8 * c, u[k]);
     }
     norm_row<NCH, WPR>(u, c0, nchunks, a.norm, inv_w, a.eps, sum);
@@ -247,12 +258,12 @@ __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
     for (int k = 0; k < NCH; ++k) {
       const int c = c0 + 64 * WPR * k;
       if (!live || c >= nchunks) break;
-      float m[8], h[8];
-      vec.read(kVecMult, c, m);
-      vec.read(kVecShift, c, h);
+      float m[8], h[8], o[8];
+      if constexpr (!kHeld) vec.read(kVecMult, c, m), vec.read(kVecShift, c, h);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] += u[k][i] * m[i];
-      store8_any(a.out, YF32, row + 8 * c, h);
+      for (int i = 0; i < 8; ++i)
+        o[i] = (kHeld ? shift[kHeld ? k : 0][i] : h[i]) + u[k][i] * (kHeld ? mult[kHeld ? k : 0][i] : m[i]);
+      store8_any(a.out, YF32, row + 8 * c, o);
     }
   }
 }
@@ -262,8 +273,9 @@ __global__ __launch_bounds__(64 * NW) void joint_kernel(const JointArgs a) {
 template <int NCH, int WPR, int NW, bool XF32, bool YF32, bool SUMS, bool POST>
 __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdArgs ba) {
   const JointArgs &a = ba.f;
-  constexpr int STREAMS = NW / WPR, NV = SUMS ? (POST ? 4 : 3) : 1;
+  constexpr int STREAMS = NW / WPR, NV = POST ? 4 : 3;
   constexpr bool kAhead = WPR > 1;  // the next row's loads under this row's sums and barriers
+  constexpr bool kHeld = WPR > 1;
   __shared__ float red[4][2][NW];
   extern __shared__ f32x4 dyn[];  // the vectors; after the rows, one partial row of each sum
   const int wave = wave_id(), lane = threadIdx.x & 63, stream = wave / WPR;
@@ -274,14 +286,32 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
   const Vectors<WPR == 1> vec{a, b, dyn, nchunks};
   vec.fill();
   RowSum<WPR, NW> sum{red, wave, stream * WPR};
-  float acc[NV][NCH][8];  // dgate, dscale, dshift, dw_post
+  float acc[SUMS ? 3 : 1][NCH][8];  // Σ du·p̂ (dgate = w_post times it, dw_post = gate times it), dscale, dshift
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < (SUMS ? 3 : 1); ++v)
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[v][k][i] = 0.f;
   __syncthreads();
+  auto read_gw = [&](int c, float (&g)[8]) __attribute__((always_inline)) {  // gate · w_post
+    vec.read(kVecGate, c, g);
+    if constexpr (POST) {
+      float w[8];
+      vec.read(kVecPost, c, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] *= w[i];
+    }
+  };
+  float gw[kHeld ? NCH : 1][8], mult[kHeld ? NCH : 1][8];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = min(c0 + 64 * WPR * k, nchunks - 1);
+      read_gw(c, gw[k]);
+      vec.read(kVecMult, c, mult[k]);
+    }
+  }
   RawRow<NCH, WPR, XF32> rx, rgx;
   RawRow<NCH, WPR, YF32> ry, rgo;
   auto load = [&](int t) __attribute__((always_inline)) {
@@ -304,15 +334,9 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
       const int c = c0 + 64 * WPR * k;
       if (c >= nchunks) break;
       float g[8];
-      vec.read(kVecGate, c, g);
-      if constexpr (POST) {
-        float w[8];
-        vec.read(kVecPost, c, w);
+      if constexpr (!kHeld) read_gw(c, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= w[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[k][i] = a.alpha * u[k][i] + g[i] * p[k][i];
+      for (int i = 0; i < 8; ++i) u[k][i] = a.alpha * u[k][i] + (kHeld ? gw[kHeld ? k : 0][i] : g[i]) * p[k][i];
     }
     const float r = norm_row<NCH, WPR>(u, c0, nchunks, a.norm, inv_w, a.eps, sum);  // u holds û
     float s1 = 0.f, s2 = 0.f;
@@ -321,11 +345,11 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
       const int c = c0 + 64 * WPR * k;
       if (c >= nchunks) break;
       float m[8];
-      vec.read(kVecMult, c, m);
+      if constexpr (!kHeld) vec.read(kVecMult, c, m);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (SUMS) acc[1][k][i] += go[k][i] * u[k][i], acc[2][k][i] += go[k][i];
-        go[k][i] *= m[i];  // h
+        go[k][i] *= kHeld ? mult[kHeld ? k : 0][i] : m[i];  // h
         s1 += go[k][i];
         s2 += go[k][i] * u[k][i];
       }
@@ -339,23 +363,15 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
     for (int k = 0; k < NCH; ++k) {
       const int c = c0 + 64 * WPR * k;
       if (c >= nchunks) break;
-      float g[8], w[8];
-      vec.read(kVecGate, c, g);
-      if constexpr (POST) vec.read(kVecPost, c, w);
+      float g[8];
+      if constexpr (!kHeld) read_gw(c, g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float du = d[k][i] + r * (go[k][i] - s1 - u[k][i] * s2);
         d[k][i] = du;
-        const float dp = g[i] * du;
-        if constexpr (POST) {
-          if constexpr (SUMS) acc[0][k][i] += du * (p[k][i] * w[i]), acc[NV - 1][k][i] += dp * p[k][i];
-          go[k][i] = dp * w[i];  // q
-          q1 += go[k][i];
-          q2 += go[k][i] * p[k][i];
-        } else {
-          if constexpr (SUMS) acc[0][k][i] += du * p[k][i];
-          go[k][i] = dp;
-        }
+        if constexpr (SUMS) acc[0][k][i] += du * p[k][i];
+        go[k][i] = (kHeld ? gw[kHeld ? k : 0][i] : g[i]) * du;  // dp, or q
+        if constexpr (POST) q1 += go[k][i], q2 += go[k][i] * p[k][i];
       }
       if (live && ba.dx != nullptr) {
         float o[8];
@@ -381,6 +397,19 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
     }
   }
   if constexpr (SUMS) {
+    float post[POST ? NCH : 1][8];  // dw_post
+    if constexpr (POST) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        const int c = min(c0 + 64 * WPR * k, nchunks - 1);
+        float g[8], w[8];
+        vec.read(kVecGate, c, g);
+        vec.read(kVecPost, c, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) post[k][i] = acc[0][k][i] * g[i], acc[0][k][i] *= w[i];
+      }
+    }
+    auto total = [&](int v, int k, int i) __attribute__((always_inline)) { return v == kVecPost ? post[POST ? k : 0][i] : acc[v < 3 ? v : 0][k][i]; };
     float *out = ba.partial + (int64_t)blockIdx.x * kVecs * a.width;
     if constexpr (STREAMS > 1) {  // the streams' sums, added in stream order in the vectors' place
       __syncthreads();
@@ -395,7 +424,7 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
               if (c >= nchunks) break;
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                f32x4 s = f32x4{acc[v][k][4 * h], acc[v][k][4 * h + 1], acc[v][k][4 * h + 2], acc[v][k][4 * h + 3]};
+                f32x4 s = f32x4{total(v, k, 4 * h), total(v, k, 4 * h + 1), total(v, k, 4 * h + 2), total(v, k, 4 * h + 3)};
                 f32x4 &dst = vec.at(v)[h * nchunks + c];
                 if (w > 0) s += dst;
                 dst = s;
@@ -414,7 +443,10 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           const int c = c0 + 64 * WPR * k;
-          if (c < nchunks) store8_any(out, true, v * a.width + 8 * c, acc[v][k]);
+          float t[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) t[i] = total(v, k, i);
+          if (c < nchunks) store8_any(out, true, v * a.width + 8 * c, t);
         }
     }
   }
@@ -428,17 +460,17 @@ static int joint_chunk(int64_t batches, int64_t tokens, int streams, int64_t mos
 }
 constexpr int64_t kJointMostFwd = 4096, kJointWavesBwd = 2048;
 
-// A row's waves and chunks per lane. Rows of more than one wave have a workgroup each.
+// A row's waves and chunks per lane. Rows of more than one wave have a workgroup each; with three chunks per lane
+// there, the backward's sums would leave one wave per SIMD (2 x 11040 rows of 5120, bf16: 342 us with three chunks
+// on four waves, 291 with two on eight; the forward 179 and 175).
 struct JointTile {
   int nch, wpr, nw;
 };
-static JointTile joint_tile(int64_t width, bool heavy) {
+static JointTile joint_tile(int64_t width) {
   const int n = (int)((width / 8 + 63) / 64);  // chunks of 8 values per lane of one wave
-  if (n <= (heavy ? 2 : 3)) return {n, 1, 4};
-  if (heavy) return {2, n <= 4 ? 2 : n <= 8 ? 4 : 8, n <= 4 ? 2 : n <= 8 ? 4 : 8};
-  if (n <= 6) return {n <= 4 ? 2 : 3, 2, 2};
-  if (n <= 12) return {n <= 8 ? 2 : 3, 4, 4};
-  return {2, 8, 8};
+  if (n <= 3) return {n, 1, 4};
+  const int waves = n <= 4 ? 2 : n <= 8 ? 4 : 8;
+  return {2, waves, waves};
 }
 
 // f(nch, wpr, nw) with the tile's values as integral constants.
@@ -455,11 +487,9 @@ static void with_tile(const JointTile &t, F &&f) {
     else if (t.nch == 2) f(two, one, four);
     else f(three, one, four);
   } else if (t.wpr == 2) {
-    if (t.nch == 2) f(two, two, two);
-    else f(three, two, two);
+    f(two, two, two);
   } else if (t.wpr == 4) {
-    if (t.nch == 2) f(two, four, four);
-    else f(three, four, four);
+    f(two, four, four);
   } else {
     f(two, eight, eight);
   }
@@ -525,7 +555,7 @@ extern "C" int mlora_joint(const void *x, int x_dtype, int64_t x_sb, int64_t x_s
   if (st || batches == 0 || tokens == 0 || width == 0) return st;
   if (x1 == nullptr || out == nullptr) return MLORA_ERR_INVALID;
   if (!aligned16(x1) || !aligned16(out)) return MLORA_ERR_UNSUPPORTED;
-  const JointTile tile = joint_tile(width, false);
+  const JointTile tile = joint_tile(width);
   a.x1 = x1, a.out = out;
   a.chunk = joint_chunk(batches, tokens, tile.nw / tile.wpr, kJointMostFwd);
   a.n_chunks = (int32_t)((tokens + a.chunk - 1) / a.chunk);
@@ -546,12 +576,8 @@ extern "C" int64_t mlora_joint_backward_workspace_bytes(int64_t batches, int64_t
   if (batches == 0 || tokens == 0 || width == 0) return 0;
   if (width > kJointMaxWidth) return MLORA_ERR_UNSUPPORTED;
   if (tokens > (INT32_MAX - 8192) / batches) return MLORA_ERR_LIMIT;
-  int64_t most = 0;  // of the two tiles that a call of this size may take
-  for (bool heavy : {false, true}) {
-    const int64_t chunk = joint_bwd_chunk(joint_tile(width, heavy), batches, tokens), n = (tokens + chunk - 1) / chunk;
-    most = n > most ? n : most;
-  }
-  return batches * most * kVecs * width * (int64_t)sizeof(float);
+  const int64_t chunk = joint_bwd_chunk(joint_tile(width), batches, tokens);
+  return batches * ((tokens + chunk - 1) / chunk) * kVecs * width * (int64_t)sizeof(float);
 }
 
 extern "C" int mlora_joint_backward(const void *x, int x_dtype, int64_t x_sb, int64_t x_st, const void *y, int y_dtype,
@@ -585,8 +611,7 @@ extern "C" int mlora_joint_backward(const void *x, int x_dtype, int64_t x_sb, in
         return MLORA_ERR_WORKSPACE;
       if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
     }
-    // normed after and with sums wanted: two chunks per lane at most, three would leave one wave per SIMD
-    const JointTile tile = joint_tile(width, sums && post >= 0);
+    const JointTile tile = joint_tile(width);
     a.chunk = joint_bwd_chunk(tile, batches, tokens);
     a.n_chunks = (int32_t)((tokens + a.chunk - 1) / a.chunk);
     n_chunks = a.n_chunks;
@@ -598,13 +623,8 @@ extern "C" int mlora_joint_backward(const void *x, int x_dtype, int64_t x_sb, in
         constexpr int NCH = decltype(nch)::value, WPR = decltype(wpr)::value, NW = decltype(nw)::value;
         constexpr bool XF = decltype(xf)::value, YF = decltype(yf)::value;
         const dim3 grid((unsigned)(batches * a.n_chunks)), block(64 * NW);
-        if constexpr (NCH < 3) {
-          if (sums && post >= 0) {
-            hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, true>), grid, block, lds, s, ba);
-            return;
-          }
-        }
-        if (sums) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, false>), grid, block, lds, s, ba);
+        if (sums && post >= 0) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, true>), grid, block, lds, s, ba);
+        else if (sums) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, true, false>), grid, block, lds, s, ba);
         else if (post >= 0) hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, false, true>), grid, block, lds, s, ba);
         else hipLaunchKernelGGL((joint_backward_kernel<NCH, WPR, NW, XF, YF, false, false>), grid, block, lds, s, ba);
       });
