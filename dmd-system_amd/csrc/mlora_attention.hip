@@ -955,18 +955,33 @@ struct DkvPlan {
 };
 
 // dk / dv: 32 nw keys per workgroup; the query rows are split where the keys alone leave compute units idle, with
-// dq's least numbers of tiles.
+// dq's least numbers of tiles. Where a compute unit holds one workgroup, also beyond 256 of them: a last round that
+// is nearly empty costs as much as a full one. The number of splits is the one with the least estimated time, of
+// the rounds at 4 TFLOP/s (float32: 0.45) per compute unit and of writing and reading the splits at 5 TB/s
+// (32760 rows x 4096 keys, 12 heads of 128, bf16, 192 workgroups unsplit: the backward 2911 us, with 4 splits 2699;
+// 8192 x 8192, 10 heads, 320 workgroups: 1415 and 1263; float32, 2 x 32760 x 512, 12 heads: 8465 and 7085).
 static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t D, bool f32) {
   DkvPlan p{};
   p.nw = !f32 && D > 64 && Lk > 128 ? 8 : 4;
-  const int64_t qt = f32 || (D > 64 && p.nw == 4) ? 32 : 64;
+  const int64_t qt = f32 || (D > 64 && p.nw == 4) ? 32 : 64, dp = D > 64 ? 128 : 64;
   p.key_blocks = (Lk + 32 * p.nw - 1) / (32 * p.nw);
   p.head_q_tiles = (Lq + qt - 1) / qt;
   p.q_tiles = G * p.head_q_tiles;
-  const int64_t groups = batches * Hk * p.key_blocks, most = !f32 && p.nw == 4 ? 512 : 256;  // workgroups that run at once
-  int64_t splits = groups > 0 && groups < most ? most / groups : 1;
-  const int64_t least = f32 ? 1 : 4;
-  if (splits > p.q_tiles / least) splits = p.q_tiles / least;
+  const int64_t groups = batches * Hk * p.key_blocks;
+  const int64_t most_splits = p.q_tiles / (f32 ? 1 : 4);
+  int64_t splits = 1;
+  if (!f32 && p.nw == 4) {
+    if (groups > 0 && groups < 512) splits = 512 / groups;  // two workgroups per compute unit
+    if (splits > most_splits) splits = most_splits;
+  } else if (groups > 0) {
+    const double tile_us = 8e-6 * (double)(qt * 32 * p.nw * dp) / (f32 ? 0.45 : 4.0);
+    const double split_us = (double)(groups * p.nw * 64 * dp) * 4.0 * 2.0 / 5e6;  // dk and dv, out and in
+    double best = 0.0;
+    for (int64_t n = 1; n <= most_splits && n * groups <= 2048; ++n) {  // 512 MB of splits at most
+      const double us = (double)((groups * n + 255) / 256 * ((p.q_tiles + n - 1) / n)) * tile_us + (n > 1 ? (double)n * split_us : 0.0);
+      if (n == 1 || us < 0.97 * best) best = us, splits = n;
+    }
+  }
   if (splits < 1) splits = 1;
   p.split_tiles = (p.q_tiles + splits - 1) / splits;
   if (p.split_tiles < 1) p.split_tiles = 1;
@@ -993,8 +1008,8 @@ static int attn_sizes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, i
   if (D < 8 || D % 8 != 0 || D > kAttnMaxHeadDim) return MLORA_ERR_UNSUPPORTED;
   const int64_t most = INT32_MAX - 65536;
   if (H > most || Lk > most || (Lq > 0 && H > most / Lq)) return MLORA_ERR_LIMIT;  // rows per key head
-  // workgroups: one per (sample, key head, 128 rows or keys), splits only below 256 of them
-  const int64_t blocks = (H / Hk * Lq + 127) / 128 + (Lk + 127) / 128 + 256;
+  // workgroups: one per (sample, key head, 128 rows or keys), splits up to 2048 of them
+  const int64_t blocks = (H / Hk * Lq + 127) / 128 + (Lk + 127) / 128 + 2048;
   if (B > 0 && (Hk > most / B || blocks > most / (B * Hk))) return MLORA_ERR_LIMIT;
   return MLORA_OK;
 }
