@@ -274,3 +274,28 @@ def test_wan_shape(pkg, dev):
     for b, h in ((0, 0), (1, 11)):
         sub = [t[b:b + 1, :, h:h + 1] for t in (q, k, v)]
         check(*sub, out[b:b + 1, :, h:h + 1].contiguous(), g[b:b + 1, :, h:h + 1], [d[b:b + 1, :, h:h + 1] for d in grads])
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("shape", [
+    (1, 700, 2100, 16, 16, 72),  # rows of dk and dv split although the keys alone are many workgroups
+    (1, 300, 1500, 6, 2, 96),    # keys of dq split, several row tiles per key head
+])
+def test_backward_split_with_many_workgroups(pkg, dev, shape, dtype):
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, g = make(*shape, dtype, dev, 19)
+    mask = torch.rand(B, Lk, generator=torch.Generator().manual_seed(4)) < 0.9
+    out, grads = run(pkg, q, k, v, g, key_mask=mask.to(dev))
+    check(q, k, v, out, g, grads, live=live_keys(B, Lk, None, mask))
+
+
+def test_one_tensor_as_q_k_and_v(pkg, dev):
+    """The gradients of its three uses add up: each rounded once, so is each sum (two additions)."""
+    x = make(2, 90, 90, 3, 3, 64, BF, dev, 23)[0]
+    g = make(2, 90, 90, 3, 3, 64, BF, dev, 24)[3]
+    _, (dq, dk, dv) = run(pkg, x, x, x, g)
+    leaf = x.detach().requires_grad_(True)
+    got, = torch.autograd.grad(pkg.cross_attention(leaf, leaf, leaf), [leaf], [g])
+    parts = [ref.f64(t) for t in (dq, dk, dv)]
+    room = 2 * ref.half_step(BF) * sum(p.abs() for p in parts)
+    assert ((ref.f64(got) - sum(parts)).abs() <= room * (1 + ref.half_step(BF))).all()

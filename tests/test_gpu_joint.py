@@ -186,3 +186,12 @@ def test_captured_and_replayed(pkg, dev):
         got = [o.clone() for o in outs]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("types", [(BF, BF), (F, BF), (F, F)])
+@pytest.mark.parametrize("W", [1032, 1544, 2048, 4104, 7168])
+def test_widths_between_the_tiles(pkg, dev, W, types):
+    """Rows whose last wave or last chunk is partly or wholly empty, all gradients, several workgroups per sample."""
+    d = make(2, 300, W, *types, dev, W, post=True)
+    outs, grads = run(pkg, d, norm="layer", post_norm="layer")
+    check(d, outs, grads, norm="layer", post_norm="layer")
