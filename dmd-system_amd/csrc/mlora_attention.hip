@@ -1,4 +1,4 @@
-// Attention of q to an encoder's keys and values of another length, forward:
+// Attention of q to an encoder's keys and values of another length. Forward:
 //
 //   s_j = scale · q·k_j over the sample's live keys (its first key_lengths[b], those with key_mask set);
 //   out = Σ_j p_j v_j with p = softmax(s);  a query without a live key gets zeros.
@@ -12,6 +12,16 @@
 //
 // Rows: the G = heads / kv_heads query heads that share a key head are packed, row r = g·Lq + i, so that shared
 // keys are read once for all of them.
+//
+// Products are of transposed tiles (Sᵀ = K·Qᵀ, Oᵀ = Vᵀ·Pᵀ): a column of a 32 x 32 result is a query, its softmax
+// needs one exchange between two lanes, and the result's registers are the next product's operand as they lie.
+//
+// What bounds it, bf16 with 128 channels: a 32 x 32 block of scores costs the SIMD's matrix core 16 products of
+// 32 cycles and its vector unit about as many cycles (16 exp2 at a quarter of the rate, the maximum, fma, packing);
+// the two waves of a SIMD overlap the two only in part. Counters at 2 x 32760 rows x 512 keys, 12 heads: matrix
+// cores busy 34 % of the cycles, no LDS bank conflict. Measured there: forward 273 us (755 TFLOP/s), dq 382 (810),
+// dk / dv 420 (980); forward at 4096 keys 990 TFLOP/s, dq 1140. Few rows are bound by reading K and V: 48 rows per
+// key head x 65520 keys, 8 key heads, 268 MB: 50 us, 5.4 TB/s, and 5 us for the join of its 32 splits.
 #include "mlora_attention.h"
 
 namespace mlora {
@@ -487,8 +497,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 //   P = 2^(s' − lse),  delta = Σ_d do·out,  dP = do·Vᵀ,  dS = P·(dP − delta)
 //   dq = scale · dS·K,   dk = scale · dSᵀ·q,   dv = Pᵀ·do
 // Two kernels form P again: one owns query rows (dq, and delta on the way), one owns keys (dk, dv). That
-// is 7 products instead of 5, and no atomics: every sum has a fixed order. bf16: P and dS are rounded to bf16
-// as operands of the products that follow.
+// is 7 products instead of 5, and no atomics: every sum has a fixed order. One kernel for all three would write and
+// add up float32 parts of dq per 256 keys (402 MB each at 2 x 32760 rows of 12 x 128: more time than its
+// two products). bf16: P and dS are rounded to bf16 as operands of the products that follow: half a step each,
+// 1.7e-3 of dq and dk in the mean square, as much as their own rounding.
 
 struct AttnBwdArgs {
   AttnArgs f;

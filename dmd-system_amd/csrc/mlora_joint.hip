@@ -19,8 +19,8 @@
 // workgroup's sample's), multiplied behind the rows.
 //
 // Both passes are HBM-bound and run at what a large copy reaches (4.9 TB/s): 2 x 32760 rows of 1536, float32 stream,
-// bf16 y, every vector's gradient: 229 us forward (604 MB in, 604 MB out), 376 backward; 2 x 11040 rows of
-// 5120, bf16, normed on both sides: 175 and 291. A row is held in registers by WPR waves (8 values per lane and
+// bf16 y, every vector's gradient: 219 us forward (604 MB in, 604 MB out), 378 backward; 2 x 11040 rows of
+// 5120, bf16, normed on both sides: 159 and 291. A row is held in registers by WPR waves (8 values per lane and
 // chunk). A workgroup takes `chunk` rows of one sample; the backward's column sums stay in registers over
 // those rows, are added over the workgroup's rows in flight through LDS, and leave as one partial row
 // per workgroup (fixed order, no atomics).
@@ -452,17 +452,20 @@ __global__ __launch_bounds__(64 * NW) void joint_backward_kernel(const JointBwdA
   }
 }
 
-// Rows per workgroup (a multiple of the rows in flight): what leaves about `most` workgroups.
+// Rows per workgroup (a multiple of the rows in flight): what leaves about `most` workgroups. Forward: many, so that
+// the last ones end together, but each copies or reads the vectors (2 x 32760 rows of 1536 / 2 x 11040 of 5120:
+// 2048 workgroups 234 / 169 us, 4096 228 / 164, 8192 219 / 159, 16384 212 / 174). Backward: those that run at
+// once, since each leaves a partial row of every sum (half or twice as many: 315 and 322 us against 321).
 static int joint_chunk(int64_t batches, int64_t tokens, int streams, int64_t most) {
   const int64_t per_sample = batches < most ? most / batches : 1;
   const int64_t rows = (tokens + per_sample - 1) / per_sample;
   return (int)((rows + streams - 1) / streams * streams);
 }
-constexpr int64_t kJointMostFwd = 4096, kJointWavesBwd = 2048;
+constexpr int64_t kJointMostFwd = 8192, kJointWavesBwd = 2048;
 
 // A row's waves and chunks per lane. Rows of more than one wave have a workgroup each; with three chunks per lane
 // there, the backward's sums would leave one wave per SIMD (2 x 11040 rows of 5120, bf16: 342 us with three chunks
-// on four waves, 291 with two on eight; the forward 179 and 175).
+// on four waves, 291 with two on eight).
 struct JointTile {
   int nch, wpr, nw;
 };
