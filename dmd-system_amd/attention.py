@@ -7,8 +7,8 @@ image's k / v linears, of any two lengths (Lq = Lk is the block's self-attention
 length or masked out do not count, whatever they hold; a query without keys gets zeros, and so do its gradients.
 Query heads may share key heads (H a multiple of Hk). Gradients of q, k and v, summed in a fixed order.
 
-bf16: scores, softmax and sums in float32; the weights are rounded to bf16 for their product with v, as is dS in
-the backward. float32: float32 throughout, on the fp32 matrix core.
+bf16: scores, softmax and sums in float32; the weights are rounded to bf16 for their product with v, as they and dS
+are in a backward of more than 2^30 products (below, both enter in two parts, to 16 bits). float32: float32 throughout, on the fp32 matrix core.
 """
 from __future__ import annotations
 

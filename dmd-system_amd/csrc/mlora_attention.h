@@ -51,6 +51,14 @@ __device__ __forceinline__ void to_frag(const f32x16 &x, int s, Frag<float> &f) 
   for (int j = 0; j < 8; ++j) f.v[j] = x[8 * s + j];
 }
 
+// What that rounding left, as a second operand.
+__device__ __forceinline__ void rest_frag(const f32x16 &x, int s, const Frag<uint16_t> &f, Frag<uint16_t> &r) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r.v[j] = pack2_bf16(x[8 * s + 2 * j] - __uint_as_float(f.v[j] << 16),
+                        x[8 * s + 2 * j + 1] - __uint_as_float(f.v[j] & 0xffff0000u));
+}
+
 // The other half's value (lane ^ 32): max and sum over the two halves of a column.
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

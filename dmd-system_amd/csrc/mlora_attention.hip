@@ -500,7 +500,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // is 7 products instead of 5, and no atomics: every sum has a fixed order. One kernel for all three would write and
 // add up float32 parts of dq per 256 keys (402 MB each at 2 x 32760 rows of 12 x 128: more time than its
 // two products). bf16: P and dS are rounded to bf16 as operands of the products that follow: half a step each,
-// 1.7e-3 of dq and dk in the mean square, as much as their own rounding.
+// 1.7e-3 of dq, dk and dv in the mean square where few rows add up, as much as their own rounding. FINE: what the
+// rounding left is a second operand, and only the gradients' own rounding remains (dq's error at 512 keys 2.4e-3 ->
+// 1.7e-3). At 2 x 32760 rows x 512 keys, 12 heads of 128, that costs dq 414 -> 456 us and dk alone 460 -> 617:
+// it is done up to 2^30 products of scores and channels, where the backward's kernels take less than the call's host
+// side (500 x 512, 12 heads of 128: 49 -> 59 us, 1000 x 1000, 8 of 64: 41 -> 44).
 
 struct AttnBwdArgs {
   AttnArgs f;
@@ -513,7 +517,7 @@ struct AttnBwdArgs {
   int32_t key_blocks, q_tiles, head_q_tiles, q_splits, q_split_tiles;  // dk / dv; dq's splits are f's
 };
 
-template <class T, int DP>
+template <class T, int DP, bool FINE>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
   constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
@@ -613,13 +617,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
       static_for<2>([&](auto ks) __attribute__((always_inline)) {
-        Frag<T> ds;
+        Frag<T> ds, rest;
         to_frag(s, ks, ds);
+        if constexpr (FINE) rest_frag(s, ks, ds, rest);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> kf;
           fr.template cols<0, 32 * kb + 16 * decltype(ks)::value>(d, kf);
           dq[d] = mma16(kf, ds, dq[d]);
+          if constexpr (FINE) dq[d] = mma16(kf, rest, dq[d]);
         }
         return true;
       });
@@ -692,11 +698,11 @@ __global__ __launch_bounds__(256) void attn_dq_join_kernel(const AttnBwdArgs ba)
 // for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient, lse and
 // delta.
 template <class T, int DP, int NW>
-struct DkvTile {  // query rows per tile: half as many where four waves' V would leave room for one workgroup only
+struct DkvTile {  // query rows per tile: half as many where that leaves room for another workgroup
   static constexpr int QT = sizeof(T) == 2 && !(DP == 128 && NW == 4) ? 64 : 32;
 };
 
-template <class T, int DP, int NW>
+template <class T, int DP, int NW, bool FINE>
 __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
   constexpr int QT = DkvTile<T, DP, NW>::QT, ND = DP / 32, NS = DP / 16;
@@ -791,24 +797,28 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_
       }
       __builtin_amdgcn_sched_barrier(0);
       static_for<2>([&](auto ks) __attribute__((always_inline)) {
-        Frag<T> pf;
+        Frag<T> pf, rest;
         to_frag(s, ks, pf);
+        if constexpr (FINE) rest_frag(s, ks, pf, rest);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> f;
           fr.template cols<TB, 32 * qb + 16 * decltype(ks)::value>(d, f);
           dv[0][d] = mma16(f, pf, dv[0][d]);
+          if constexpr (FINE) dv[0][d] = mma16(f, rest, dv[0][d]);
         }
         return true;
       });
       static_for<2>([&](auto ks) __attribute__((always_inline)) {
-        Frag<T> df;
+        Frag<T> df, rest;
         to_frag(dp, ks, df);
+        if constexpr (FINE) rest_frag(dp, ks, df, rest);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           Frag<T> f;
           fr.template cols<0, 32 * qb + 16 * decltype(ks)::value>(d, f);
           dk[0][d] = mma16(f, df, dk[0][d]);
+          if constexpr (FINE) dk[0][d] = mma16(f, rest, dk[0][d]);
         }
         return true;
       });
@@ -877,8 +887,8 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const AttnBwdArgs ba
 #define MLORA_ATTN(T, DP)                                             \
   template __global__ void attn_fwd_kernel<T, DP>(const AttnArgs);    \
   template __global__ void attn_few_kernel<T, DP, 1>(const AttnArgs); \
-  template __global__ void attn_dq_kernel<T, DP>(const AttnBwdArgs);  \
-  template __global__ void attn_dkv_kernel<T, DP, 4>(const AttnBwdArgs);
+  template __global__ void attn_dq_kernel<T, DP, false>(const AttnBwdArgs);  \
+  template __global__ void attn_dkv_kernel<T, DP, 4, false>(const AttnBwdArgs);
 MLORA_ATTN(uint16_t, 64)
 MLORA_ATTN(uint16_t, 128)
 MLORA_ATTN(float, 64)
@@ -887,7 +897,14 @@ MLORA_ATTN(float, 128)
 template __global__ void attn_few_kernel<uint16_t, 64, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<uint16_t, 128, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<float, 64, 2>(const AttnArgs);
-template __global__ void attn_dkv_kernel<uint16_t, 128, 8>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<uint16_t, 128, 8, false>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<uint16_t, 64, true>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<uint16_t, 128, true>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<float, 64, 2, false>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<float, 128, 2, false>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<uint16_t, 64, 4, true>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<uint16_t, 128, 4, true>(const AttnBwdArgs);
+template __global__ void attn_dkv_kernel<uint16_t, 128, 8, true>(const AttnBwdArgs);
 
 // ------------------------------------------------------------------ host
 
@@ -966,15 +983,18 @@ struct DkvPlan {
   int64_t key_blocks, q_tiles, head_q_tiles, splits, split_tiles;
 };
 
-// dk / dv: 32 nw keys per workgroup; the query rows are split where the keys alone leave compute units idle, with
-// dq's least numbers of tiles. Where a compute unit holds one workgroup, also beyond 256 of them: a last round that
-// is nearly empty costs as much as a full one. The number of splits is the one with the least estimated time, of
-// the rounds at 4 TFLOP/s (float32: 0.45) per compute unit and of writing and reading the splits at 5 TB/s
-// (32760 rows x 4096 keys, 12 heads of 128, bf16, 192 workgroups unsplit: the backward 2911 us, with 4 splits 2699;
-// 8192 x 8192, 10 heads, 320 workgroups: 1415 and 1263; float32, 2 x 32760 x 512, 12 heads: 8465 and 7085).
+// dk / dv: 32 nw keys per workgroup. float32 takes 2 waves where they hold all keys: a wave without keys holds
+// its SIMD's one place until its workgroup ends (3 x 3074 rows x 12 keys, 40 heads of 80: 527 us with 4 waves,
+// 322 with 2; bf16, with two waves per SIMD, gains nothing: the backward of 2 x 8000 x 64, 16 heads of 64, 65
+// and 75). The query rows are split where the keys alone leave compute units idle, with dq's least numbers of
+// tiles. Where a compute unit holds one workgroup, also beyond 256 of them: a last round that is nearly empty
+// costs as much as a full one. The number of splits is the one with the least estimated time, of the rounds at
+// 4 TFLOP/s (float32: 0.45) per compute unit and of writing and reading the splits at 5 TB/s (32760 rows x 4096
+// keys, 12 heads of 128, bf16, 192 workgroups unsplit: the backward 2911 us, with 4 splits 2699; 8192 x 8192,
+// 10 heads, 320 workgroups: 1415 and 1263; float32, 2 x 32760 x 512, 12 heads: 8465 and 7085).
 static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t D, bool f32) {
   DkvPlan p{};
-  p.nw = !f32 && D > 64 && Lk > 128 ? 8 : 4;
+  p.nw = f32 ? (Lk <= 64 ? 2 : 4) : D > 64 && Lk > 128 ? 8 : 4;
   const int64_t qt = f32 || (D > 64 && p.nw == 4) ? 32 : 64, dp = D > 64 ? 128 : 64;
   p.key_blocks = (Lk + 32 * p.nw - 1) / (32 * p.nw);
   p.head_q_tiles = (Lq + qt - 1) / qt;
@@ -986,11 +1006,12 @@ static DkvPlan dkv_plan(int64_t batches, int64_t Lq, int64_t Lk, int64_t Hk, int
     if (groups > 0 && groups < 512) splits = 512 / groups;  // two workgroups per compute unit
     if (splits > most_splits) splits = most_splits;
   } else if (groups > 0) {
-    const double tile_us = 8e-6 * (double)(qt * 32 * p.nw * dp) / (f32 ? 0.45 : 4.0);
+    const int64_t places = p.nw == 2 ? 512 : 256;
+    const double tile_us = 8e-6 * (double)(qt * 32 * p.nw * dp) / (f32 ? 0.45 : 4.0) * (double)places / 256.0;
     const double split_us = (double)(groups * p.nw * 64 * dp) * 4.0 * 2.0 / 5e6;  // dk and dv, out and in
     double best = 0.0;
     for (int64_t n = 1; n <= most_splits && n * groups <= 2048; ++n) {  // 512 MB of splits at most
-      const double us = (double)((groups * n + 255) / 256 * ((p.q_tiles + n - 1) / n)) * tile_us + (n > 1 ? (double)n * split_us : 0.0);
+      const double us = (double)((groups * n + places - 1) / places * ((p.q_tiles + n - 1) / n)) * tile_us + (n > 1 ? (double)n * split_us : 0.0);
       if (n == 1 || us < 0.97 * best) best = us, splits = n;
     }
   }
@@ -1160,12 +1181,19 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   ba.q_splits = (int32_t)p.splits, ba.q_split_tiles = (int32_t)p.split_tiles;
   const DqPlan qp = dq_plan(B, a.rows, Lk, Hk, f32);
   a.row_tiles = (int32_t)qp.row_tiles, a.splits = (int32_t)qp.splits, a.split_tiles = (int32_t)qp.split_tiles;
+  const bool fine = (double)B * (double)H * (double)Lq * (double)Lk * (double)D <= 1073741824.0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (Lq > 0) {
     with_head(f32, D, [&](auto t, auto dp) {
       using T = decltype(t);
       constexpr int DP = decltype(dp)::value;
-      hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3((unsigned)(B * Hk * a.row_tiles * qp.splits)), dim3(256), 0, s, ba);
+      const dim3 grid((unsigned)(B * Hk * a.row_tiles * qp.splits));
+      if constexpr (sizeof(T) == 2) {
+        if (fine) hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), 0, s, ba);
+        else hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), 0, s, ba);
+      } else {
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), 0, s, ba);
+      }
       if (qp.splits > 1)
         hipLaunchKernelGGL((attn_dq_join_kernel<T, DP>), dim3((unsigned)(dq_vectors(qp, B, Hk, D) / 256)), dim3(256), 0, s, ba);
     });
@@ -1180,13 +1208,26 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
     constexpr int DP = decltype(dp)::value;
     if constexpr (sizeof(T) == 2 && DP == 128) {
       if (p.nw == 8) {
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 8>), grid, dim3(512), 0, s, ba);
+        if (fine) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 8, true>), grid, dim3(512), 0, s, ba);
+        else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 8, false>), grid, dim3(512), 0, s, ba);
         if (p.splits > 1) hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, 8>), joins, dim3(256), 0, s, ba);
         return;
       }
     }
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4>), grid, dim3(256), 0, s, ba);
-    if (p.splits > 1) hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, 4>), joins, dim3(256), 0, s, ba);
+    auto go = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      if constexpr (sizeof(T) == 2) {
+        if (fine) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NW, true>), grid, dim3(64 * NW), 0, s, ba);
+        else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NW, false>), grid, dim3(64 * NW), 0, s, ba);
+      } else {
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NW, false>), grid, dim3(64 * NW), 0, s, ba);
+      }
+      if (p.splits > 1) hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP, NW>), joins, dim3(256), 0, s, ba);
+    };
+    if constexpr (sizeof(T) == 4) {
+      if (p.nw == 2) return go(std::integral_constant<int, 2>{});
+    }
+    go(std::integral_constant<int, 4>{});
   });
   return launch_status();
 }

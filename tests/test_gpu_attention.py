@@ -299,3 +299,17 @@ def test_one_tensor_as_q_k_and_v(pkg, dev):
     parts = [ref.f64(t) for t in (dq, dk, dv)]
     room = 2 * ref.half_step(BF) * sum(p.abs() for p in parts)
     assert ((ref.f64(got) - sum(parts)).abs() <= room * (1 + ref.half_step(BF))).all()
+
+
+def test_finer_operands_of_small_backwards(pkg, dev):
+    """Up to 2^30 products the weights and dS enter their products in two parts: beside float32 sums (2^-18 in all
+    here) only the gradients' own rounding is left, and delta's from the rounded out: its half step u relative to
+    every |do| |out|. Root mean squares: u / sqrt(3) at most for the rounding, the same for out's."""
+    q, k, v, g = make(2, 40, 180, 6, 2, 64, BF, dev, 31)
+    _, grads = run(pkg, q, k, v, g)
+    o, dq, dk, dv, parts = ref.attention(q, k, v, do=g)
+    u = ref.half_step(BF)
+    for name, got, want in (("dq", grads[0], dq), ("dk", grads[1], dk), ("dv", grads[2], dv)):
+        err = float((ref.f64(got) - want).norm() / want.norm())
+        slack = 0 if name == "dv" else 0.5  # delta: a fraction of dP's spread, out being a mean over the keys
+        assert err <= u / math.sqrt(3) * (1 + slack), (name, err)
