@@ -74,8 +74,9 @@ __device__ __forceinline__ void load_frag(const float *base, int64_t off, bool o
   for (int j = 0; j < 4; ++j) f.v[j] = on ? a[j] : 0.f, f.v[j + 4] = on ? b[j] : 0.f;
 }
 
-// The running maximum before any key: finite, so that 2^(−inf − m) is 0 and not NaN where a block has no live key.
-constexpr float kNoMax = -1e30f;
+// The running maximum before any key: below every other score, but finite, so that 2^(−inf − m) is 0 and not NaN where
+// a block has no live key.
+constexpr float kNoMax = -3.4028234664e38f;
 
 // The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step.
 template <class T, int DP, int NQ, int KT>
@@ -504,7 +505,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // rounding left is a second operand, and only the gradients' own rounding remains (dq's error at 512 keys 2.4e-3 ->
 // 1.7e-3). At 2 x 32760 rows x 512 keys, 12 heads of 128, that costs dq 414 -> 456 us and dk alone 460 -> 617:
 // it is done up to 2^30 products of scores and channels, where the backward's kernels take less than the call's host
-// side (500 x 512, 12 heads of 128: 49 -> 59 us, 1000 x 1000, 8 of 64: 41 -> 44).
+// side (500 x 512, 12 heads of 128: 49 -> 59 us, 1000 x 1000, 8 of 64: 41 -> 44). Single rows of a long cache pay
+// too (4 x 1 x 58981 keys, 40 heads on 4 of 64: 407 -> 513 us): it is there that dv, a sum of few rows, has the most to
+// lose.
 
 struct AttnBwdArgs {
   AttnArgs f;

@@ -313,3 +313,34 @@ def test_finer_operands_of_small_backwards(pkg, dev):
         err = float((ref.f64(got) - want).norm() / want.norm())
         slack = 0 if name == "dv" else 0.5  # delta: a fraction of dP's spread, out being a mean over the keys
         assert err <= u / math.sqrt(3) * (1 + slack), (name, err)
+
+
+@pytest.mark.parametrize("shape, keys", [
+    ((1, 2500, 700, 8, 4, 96), "mask"),
+    ((2, 17000, 70, 8, 8, 64), "lengths"),
+    ((1, 10001, 100, 9, 3, 120), "mask"),
+    ((1, 4100, 600, 9, 9, 64), "lengths"),
+])
+def test_large_backwards(pkg, dev, shape, keys):
+    """Beyond 2^30 products, where the weights and dS enter their products rounded to bf16."""
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, g = make(*shape, BF, dev, 41)
+    gen = torch.Generator().manual_seed(8)
+    lengths = torch.tensor([Lk - 3, Lk // 2][:B], dtype=torch.int32) if keys == "lengths" else None
+    mask = torch.rand(B, Lk, generator=gen) < 0.7 if keys == "mask" else None
+    kw = dict(key_lengths=None if lengths is None else lengths.to(dev), key_mask=None if mask is None else mask.to(dev))
+    out, grads = run(pkg, q, k, v, g, **kw)
+    check(q, k, v, out, g, grads, live=live_keys(B, Lk, lengths, mask))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq, Lk", [(3, 50), (3, 3000), (200, 50)])
+def test_very_low_scores_are_scores(pkg, dev, Lq, Lk, dtype):
+    """Every score -2^103 (exact in bf16 and float32): all keys weigh the same, and none of them is a masked one.
+    The weights are 1 and their sum Lk exact: v's sum is off by Lk additions, the output by its own half step."""
+    q, k, v, _ = make(1, Lq, Lk, 2, 2, 32, dtype, dev, 5)
+    q, k = torch.full_like(q, 2.0 ** 49), torch.full_like(k, -(2.0 ** 49))
+    out = pkg.cross_attention(q, k, v, scale=1.0)
+    want = ref.f64(v).mean(1, keepdim=True).expand(out.shape)
+    room = ref.half_step(dtype) * want.abs() + (Lk + 4) * 2 ** -24 * ref.f64(v).abs().mean(1, keepdim=True)
+    assert ((ref.f64(out) - want).abs() <= room * (1 + 2 ** -7)).all()
