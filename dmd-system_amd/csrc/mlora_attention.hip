@@ -520,12 +520,12 @@ struct AttnBwdArgs {
   int32_t key_blocks, q_tiles, head_q_tiles, q_splits, q_split_tiles;  // dk / dv; dq's splits are f's
 };
 
-template <class T, int DP, bool FINE>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const AttnBwdArgs ba) {
+template <class T, int DP, int NW, bool FINE>
+__global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
   constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
   using Tile = HeadTile<T, DP>;
-  constexpr int TB = KT * Tile::RB, N = TB / 1024 / 4;
+  constexpr int TB = KT * Tile::RB, N = TB / 1024 / NW;
   __shared__ u32x4 smem[4 * TB / 16];
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
   TileLoader<T, DP, N> kl, vl;
-  kl.init(lane, wave, 4, a.k_sl, a.D), vl.init(lane, wave, 4, a.v_sl, a.D);
+  kl.init(lane, wave, NW, a.k_sl, a.D), vl.init(lane, wave, NW, a.v_sl, a.D);
   auto stage = [&](int t, int buf, uint64_t bits) __attribute__((always_inline)) {
     kl.load(kp + (int64_t)t * KT * a.k_sl, bits, lds + buf * 2 * TB);
     vl.load(vp + (int64_t)t * KT * a.v_sl, bits, lds + buf * 2 * TB + TB);
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   }
   FragReader<T, DP> fr;
   fr.init(lane, lds);
-  const int row0 = (rt * 4 + wave) * 32, r = row0 + (lane & 31), rc = min(r, a.rows - 1);
+  const int row0 = (rt * NW + wave) * 32, r = row0 + (lane & 31), rc = min(r, a.rows - 1);
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
   const int64_t oat = ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
   Frag<T> q[DP / 16], g[DP / 16];
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   wait_vmcnt<0>();
   if (lane < 32 && r < a.rows && sp == 0) ba.delta[head_rows + r] = delta;
   if (a.splits > 1) {
-    f32x4 *p = ba.part + ((((int64_t)sp * a.batches + b) * a.row_tiles + rt) * a.Hk + hk) * (4 * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
+    f32x4 *p = ba.part + ((((int64_t)sp * a.batches + b) * a.row_tiles + rt) * a.Hk + hk) * (NW * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -675,16 +675,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 }
 
 // Adds the splits of dq in split order and writes them out.
-template <class T, int DP>
+template <class T, int DP, int NW>
 __global__ __launch_bounds__(256) void attn_dq_join_kernel(const AttnBwdArgs ba) {
   const AttnArgs &a = ba.f;
   constexpr int ND = DP / 32;
-  const int64_t per = (int64_t)a.batches * a.row_tiles * a.Hk * 4 * ND * 4 * 64;
+  const int64_t per = (int64_t)a.batches * a.row_tiles * a.Hk * NW * ND * 4 * 64;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
   int64_t u = e / 64;
-  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % 4);
-  u /= 4 * ND * 4;  // (b, row tile, hk)
-  const int hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * 128 + wave * 32 + (lane & 31);
+  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % NW);
+  u /= 4 * ND * NW;  // (b, row tile, hk)
+  const int hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * (32 * NW) + wave * 32 + (lane & 31);
   const int64_t b = u / a.Hk / a.row_tiles;
   const int ch = 32 * d + 8 * i + 4 * (lane >> 5);
   if (r >= a.rows || ch >= a.D) return;
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const AttnBwdArgs ba
 #define MLORA_ATTN(T, DP)                                             \
   template __global__ void attn_fwd_kernel<T, DP>(const AttnArgs);    \
   template __global__ void attn_few_kernel<T, DP, 1>(const AttnArgs); \
-  template __global__ void attn_dq_kernel<T, DP, false>(const AttnBwdArgs);  \
+  template __global__ void attn_dq_kernel<T, DP, 4, false>(const AttnBwdArgs);  \
   template __global__ void attn_dkv_kernel<T, DP, 4, false>(const AttnBwdArgs);
 MLORA_ATTN(uint16_t, 64)
 MLORA_ATTN(uint16_t, 128)
@@ -901,8 +901,10 @@ template __global__ void attn_few_kernel<uint16_t, 64, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<uint16_t, 128, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<float, 64, 2>(const AttnArgs);
 template __global__ void attn_dkv_kernel<uint16_t, 128, 8, false>(const AttnBwdArgs);
-template __global__ void attn_dq_kernel<uint16_t, 64, true>(const AttnBwdArgs);
-template __global__ void attn_dq_kernel<uint16_t, 128, true>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<uint16_t, 64, 4, true>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<uint16_t, 128, 4, true>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<float, 64, 2, false>(const AttnBwdArgs);
+template __global__ void attn_dq_kernel<float, 128, 2, false>(const AttnBwdArgs);
 template __global__ void attn_dkv_kernel<float, 64, 2, false>(const AttnBwdArgs);
 template __global__ void attn_dkv_kernel<float, 128, 2, false>(const AttnBwdArgs);
 template __global__ void attn_dkv_kernel<uint16_t, 64, 4, true>(const AttnBwdArgs);
@@ -955,17 +957,21 @@ static int64_t attn_part_floats(const AttnPlan &p, int64_t batches, int64_t Hk, 
 }
 
 struct DqPlan {
+  int nw;  // waves per workgroup, 32 rows each
   int64_t row_tiles, splits, split_tiles;
 };
 
-// dq: 128 rows per workgroup; the keys are split where the rows alone leave places for workgroups free (bf16, 300
-// rows x 8192 keys, 8 heads of 128: the backward takes 72 us, unsplit 226), four tiles at least to a split for bf16,
-// one for float32 (200 rows x 300 keys, 16 heads of 64: bf16 20 us, with one tile 24; float32 41, with four 66).
+// dq: 32 nw rows per workgroup, two waves for up to 64 float32 rows (a wave without rows holds its SIMD's one
+// place: 4 x 2 rows x 4779 keys, 12 heads of 128: the backward 433 us with four, 335 with two). The keys are
+// split where the rows alone leave places for workgroups free (bf16, 300 rows x 8192 keys, 8 heads of 128: the
+// backward takes 72 us, unsplit 226), four tiles at least to a split for bf16, one for float32 (200 rows x 300
+// keys, 16 heads of 64: bf16 20 us, with one tile 24; float32 41, with four 66).
 static DqPlan dq_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, bool f32) {
   DqPlan p{};
-  p.row_tiles = (rows + 127) / 128;
+  p.nw = f32 && rows <= 64 ? 2 : 4;
+  p.row_tiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
   const int64_t kt = f32 ? AttnTile<float>::KT : AttnTile<uint16_t>::KT, tiles = (Lk + kt - 1) / kt;
-  const int64_t groups = batches * Hk * p.row_tiles, most = f32 ? 256 : 512;
+  const int64_t groups = batches * Hk * p.row_tiles, most = f32 && p.nw == 4 ? 256 : 512;
   int64_t splits = groups > 0 && groups < most ? most / groups : 1;
   const int64_t least = f32 ? 1 : 4;
   if (splits > tiles / least) splits = tiles / least;
@@ -978,7 +984,7 @@ static DqPlan dq_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, boo
 
 // 16-byte vectors of one split of dq, in register order.
 static int64_t dq_vectors(const DqPlan &p, int64_t batches, int64_t Hk, int64_t D) {
-  return batches * p.row_tiles * Hk * 4 * (D > 64 ? 4 : 2) * 4 * 64;
+  return batches * p.row_tiles * Hk * p.nw * (D > 64 ? 4 : 2) * 4 * 64;
 }
 
 struct DkvPlan {
@@ -1190,15 +1196,18 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
     with_head(f32, D, [&](auto t, auto dp) {
       using T = decltype(t);
       constexpr int DP = decltype(dp)::value;
-      const dim3 grid((unsigned)(B * Hk * a.row_tiles * qp.splits));
-      if constexpr (sizeof(T) == 2) {
-        if (fine) hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), 0, s, ba);
-        else hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), 0, s, ba);
-      } else {
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), 0, s, ba);
+      const dim3 grid((unsigned)(B * Hk * a.row_tiles * qp.splits)), joins((unsigned)(dq_vectors(qp, B, Hk, D) / 256));
+      if constexpr (sizeof(T) == 4) {
+        if (qp.nw == 2) {
+          hipLaunchKernelGGL((attn_dq_kernel<T, DP, 2, false>), grid, dim3(128), 0, s, ba);
+          if (qp.splits > 1) hipLaunchKernelGGL((attn_dq_join_kernel<T, DP, 2>), joins, dim3(256), 0, s, ba);
+          return;
+        }
+      } else if (fine) {
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4, true>), grid, dim3(256), 0, s, ba);
       }
-      if (qp.splits > 1)
-        hipLaunchKernelGGL((attn_dq_join_kernel<T, DP>), dim3((unsigned)(dq_vectors(qp, B, Hk, D) / 256)), dim3(256), 0, s, ba);
+      if (sizeof(T) == 4 || !fine) hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4, false>), grid, dim3(256), 0, s, ba);
+      if (qp.splits > 1) hipLaunchKernelGGL((attn_dq_join_kernel<T, DP, 4>), joins, dim3(256), 0, s, ba);
     });
     st = launch_status();
     if (st) return st;
