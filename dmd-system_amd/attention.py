@@ -16,7 +16,6 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -46,7 +45,7 @@ class CrossAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @kernels.first_order
     def backward(ctx, g):
         q, k, v, out, lse, key_lengths, key_mask = ctx.saved_tensors
         grads = kernels.cross_attention_backward(q, k, v, out, lse, _aligned(g if g.dtype is q.dtype else g.to(q.dtype)),

@@ -16,7 +16,6 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -43,7 +42,7 @@ class GatedResidualNormFunction(torch.autograd.Function):
         return kernels.joint(*args, **cfg, checked=True)
 
     @staticmethod
-    @once_differentiable
+    @kernels.first_order
     def backward(ctx, gx, go):
         if gx is None and go is None:
             return (None,) * 7

@@ -17,7 +17,6 @@ import math
 from typing import Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -68,7 +67,7 @@ class RotaryAxesFunction(torch.autograd.Function):
         return tuple(kernels.rotary_axes(xs, positions, weights=ws, checked=True, **cfg))
 
     @staticmethod
-    @once_differentiable
+    @kernels.first_order
     def backward(ctx, *grads):
         n, needs = ctx.n, ctx.needs_input_grad
         if all(g is None for g in grads):

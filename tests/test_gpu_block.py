@@ -204,3 +204,15 @@ def test_offsets_past_32_bits(pkg, dev):
             out += [o.detach(), *torch.autograd.grad(o, leaves, [g])]
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_no_second_derivatives(pkg, dev):
+    """A gradient that is differentiated again is refused, not wrong."""
+    q = torch.randn(1, 4, 2, 32, device=dev, requires_grad=True)
+    x = torch.randn(1, 4, 64, device=dev, requires_grad=True)
+    pos = torch.arange(4, device=dev, dtype=torch.int32).view(4, 1)
+    for leaf, out in ((q, pkg.cross_attention(q, q, q)), (q, pkg.rotary_axes(q, pos, (32,), weight=torch.ones(32, device=dev))),
+                      (x, pkg.gated_residual_norm(x, x)[1])):
+        d, = torch.autograd.grad(out.square().sum(), [leaf], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            d.sum().backward()
