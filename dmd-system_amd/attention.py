@@ -75,7 +75,7 @@ def _plan(q, k, v, key_lengths, key_mask, scale) -> float:
         _fail(f"{H} query heads do not share {Hk} key heads evenly")
     if D % 8 or not 8 <= D <= 128:
         _fail(f"head_dim must be a multiple of 8 up to 128, got {D}")
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else scale
     if not (math.isfinite(scale) and scale > 0):
         _fail("scale must be positive")
     if key_lengths is not None:
@@ -98,6 +98,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     q [B, Lq, H, D], k and v [B, Lk, Hk, D], bfloat16 or float32, D a multiple of 8 up to 128. key_lengths:
     int32 or int64 [B] on q's device, the number of leading keys that count (clamped to [0, Lk]). key_mask:
     bool [B, Lk] (or [1, Lk], [Lk] for every sample), True where a key counts. scale > 0, 1 / sqrt(D) if not given."""
+    if scale is not None:
+        scale = kernels.number("scale", scale, _fail)
     scale = _plan(_meta(q), _meta(k), _meta(v), _meta(key_lengths), _meta(key_mask), scale)
     if key_lengths is not None:
         if key_lengths.dtype is torch.int64:

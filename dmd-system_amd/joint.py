@@ -94,7 +94,7 @@ def _plan(x, y, gate, scale, shift, post_weight, norm, unit_offset, post_norm, r
         _fail("scale and shift share a dtype")
     if x[2].type != "cuda":
         _fail("the tensors must be ROCm device tensors")
-    return dict(norm=norm, post=post_norm, unit_offset=bool(unit_offset), alpha=float(residual_scale), eps=float(eps))
+    return dict(norm=norm, post=post_norm, unit_offset=unit_offset, alpha=residual_scale, eps=eps)
 
 
 def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = None,
@@ -108,8 +108,8 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | N
     and shift are per sample ([B, W] or [B, 1, W]) or shared ([W]). norm / post_norm: "layer" or "rms" (both
     with `eps`); without post_norm y joins as it is. unit_offset: out is scaled by 1 + scale (a modulation),
     else by scale (a norm's weight, with shift its bias)."""
-    cfg = _plan(_meta(x), _meta(y), _meta(gate), _meta(scale), _meta(shift), _meta(post_weight), norm, unit_offset,
-                post_norm, residual_scale, eps)
+    cfg = _plan(_meta(x), _meta(y), _meta(gate), _meta(scale), _meta(shift), _meta(post_weight), norm, bool(unit_offset),
+                post_norm, kernels.number("residual_scale", residual_scale, _fail), kernels.number("eps", eps, _fail))
     args = (x, y, gate, scale, shift, post_weight)
     if kernels.wants_grad(args):
         return GatedResidualNormFunction.apply(*args, cfg)

@@ -847,6 +847,21 @@ def wants_grad(tensors) -> bool:
     return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
 
 
+def number(name: str, value, fail) -> float:
+    """An option as a Python float, read at every call: the cached checks never see the object it came in. One that
+    wants a gradient is refused, since there is none."""
+    if type(value) is float:
+        return value
+    if isinstance(value, torch.Tensor):
+        if wants_grad((value,)):
+            fail(f"{name} takes no gradient")
+        value = value.detach()
+    try:
+        return float(value)
+    except (TypeError, ValueError, RuntimeError):
+        fail(f"{name} must be a number, got a {type(value).__name__}")
+
+
 def _new(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 

@@ -134,14 +134,15 @@ def _plan(names, xs, ws, positions, axis_dims, theta, pairing, eps) -> dict:
         _fail("q_weight and k_weight share a dtype")
     if device.type != "cuda":
         _fail("the tensors must be ROCm device tensors")
-    return dict(axis_dims=axis_dims, theta=float(theta), halves=pairing == "halves", norm=max(kinds), eps=float(eps))
+    return dict(axis_dims=axis_dims, theta=theta, halves=pairing == "halves", norm=max(kinds), eps=eps)
 
 
 def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
     if positions.requires_grad:
         _fail("positions take no gradient")
     cfg = _plan(names, tuple([_meta(x) for x in xs]), tuple([_meta(w) for w in ws]), _meta(positions),
-                tuple([int(d) for d in axis_dims]), theta, pairing, eps)
+                tuple([int(d) for d in axis_dims]), kernels.number("theta", theta, _fail), pairing,
+                kernels.number("eps", eps, _fail))
     if positions.dim() == 2:
         positions = positions.unsqueeze(0)
     if not positions.is_contiguous() and (positions.stride(2) != 1 or any(s < 0 for s in positions.stride())):
