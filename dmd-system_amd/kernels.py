@@ -11,6 +11,7 @@ import functools
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -832,18 +833,28 @@ def _bytes(name: str, *args) -> int:
 
 def first_order(backward):
     """once_differentiable, entered only where autograd records the backward (create_graph): elsewhere its context alone
-    costs a small backward 3 us."""
+    costs a small backward 3 us. A tangent of an upstream gradient would be dropped, and is refused."""
     guarded = once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        refuse_tangents(grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
 
+def refuse_tangents(tensors) -> None:
+    """Raises where one of these (None allowed) carries a tangent of torch.autograd.forward_ad: the kernels see values
+    only, and the result would be without one."""
+    if forward_ad._current_level >= 0 and any([t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                               for t in tensors]):
+        raise RuntimeError("the block operators have no forward-mode derivative")
+
+
 def wants_grad(tensors) -> bool:
     """Whether autograd has to record an operator on these (None allowed); if not, its forward is called as it is,
-    without the 4 us of a Function's apply."""
+    without the 4 us of a Function's apply. Forward mode is refused, also under torch.no_grad."""
+    refuse_tangents(tensors)
     return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
 
 

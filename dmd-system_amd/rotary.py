@@ -140,6 +140,7 @@ def _plan(names, xs, ws, positions, axis_dims, theta, pairing, eps) -> dict:
 def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
     if positions.requires_grad:
         _fail("positions take no gradient")
+    kernels.refuse_tangents((positions,))
     cfg = _plan(names, tuple([_meta(x) for x in xs]), tuple([_meta(w) for w in ws]), _meta(positions),
                 tuple([int(d) for d in axis_dims]), kernels.number("theta", theta, _fail), pairing,
                 kernels.number("eps", eps, _fail))

@@ -77,3 +77,50 @@ def test_unit_offset_is_read_at_every_call(pkg, recorded):
         flag.fill_(now)
         pkg.gated_residual_norm(x, x, scale=w, unit_offset=flag)
         assert recorded[-1]["unit_offset"] is now
+
+
+def calls(pkg):
+    """(tensors, the operator on them) for every tensor operand that can carry a tangent."""
+    pos, rows, w = torch.zeros(3, 1), torch.randn(1, 3, 16), torch.ones(16)
+    q, k, v = heads(), heads(), heads()
+    one = torch.ones(32)
+    out = [([q, k, v], lambda *t: pkg.cross_attention(*t)),
+           ([rows, rows + 1, w, w + 1, w + 2, w + 3], lambda *t: pkg.gated_residual_norm(*t[:5], post_norm="rms", post_weight=t[5])),
+           ([q, k, one, one + 1, pos], lambda *t: pkg.rotary_axes_qk(t[0], t[1], t[4], (16,), q_weight=t[2], k_weight=t[3]))]
+    return [(tensors, i, f) for tensors, f in out for i in range(len(tensors))]
+
+
+@pytest.mark.parametrize("which", range(14))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(pkg, recorded, which, grad):
+    """No operator has a forward-mode derivative: a tangent is never dropped without a word, with or without
+    torch.no_grad (which does not switch forward mode off)."""
+    from torch.autograd import forward_ad
+
+    tensors, at, f = calls(pkg)[which]
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        f(*tensors)  # a level without tangents changes nothing
+        recorded.clear()
+        tensors = [forward_ad.make_dual(t, torch.ones_like(t)) if i == at else t for i, t in enumerate(tensors)]
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(*tensors)
+
+
+def test_forward_mode_over_a_backward_is_refused(pkg, recorded):
+    from torch.autograd import forward_ad
+
+    q = heads().requires_grad_()
+    out = pkg.cross_attention(q, heads(), heads())
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, [q], [g])
+
+
+def test_forward_mode_numbers_are_refused(pkg, recorded):
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        value = forward_ad.make_dual(torch.tensor(0.5), torch.tensor(1.0))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pkg.cross_attention(heads(), heads(), heads(), scale=value)
