@@ -3,11 +3,13 @@
 //   s_j = scale · q·k_j over the sample's live keys (its first key_lengths[b], those with key_mask set);
 //   out = Σ_j p_j v_j with p = softmax(s);  a query without a live key gets zeros.
 //
-// One pass over the keys with a running maximum m and sum l per query (base 2: s' = s·scale·log2 e):
-//   P = 2^(s' − m),  l = Σ P,  O = Σ P·V;  out = O / l,  lse = m + log2 l (what the backward needs; +inf
-// for a query without keys, so that every 2^(s' − lse) is 0). The running maximum is raised only when a tile's
-// exceeds it by more than 2^8 (P then stays below 2^8, far from any limit, and rounding is relative), so the
-// rescaling of O is a rare branch. bf16: P is rounded to bf16 for the product with V, and l sums the rounded
+// One pass over the keys with a running maximum m (of the products themselves) and sum l per query, c = scale·log2 e:
+//   P = 2^(s·c − m·c),  l = Σ P,  O = Σ P·V;  out = O / l,  lse = m·c + log2 l (+inf for a query without keys, so
+// that every 2^(s·c − lse) is 0). The running maximum is raised only when a tile's exceeds it by a factor of more
+// than 2^8 (P then stays below 2^8, far from any limit, and rounding is relative), so the rescaling of O is a rare
+// branch. Scores of any finite size count by their differences (RowRef): where |m·c| is small, the exponent is one fma
+// whose constant's rounding all weights of the row share; from 2^10 on s − m is formed first, which is exact where
+// it matters, and the backward, whose lse would have lost log2 l, measures m and l once more. bf16: P is rounded to bf16 for the product with V, and l sums the rounded
 // values, so that the weights that multiply V add up to one. Everything else is float32.
 //
 // Rows: the G = heads / kv_heads query heads that share a key head are packed, row r = g·Lq + i, so that shared
@@ -78,12 +80,34 @@ __device__ __forceinline__ void load_frag(const float *base, int64_t off, bool o
 // a block has no live key.
 constexpr float kNoMax = -3.4028234664e38f;
 
+// What a row's exponents are relative to: P = 2^((s − a)·c − r), a function of the row's largest product m alone. Near
+// zero a = 0 and r = m·c rounded, off by 2^-15 at most, the same for the whole row; far from zero a = m and r = 0, since
+// the rounding of m·c would grow with it and end in 2^128 or 0 (at |m·c| of 3e9).
+struct RowRef {
+  float a, r;
+};
+constexpr float kFar = 1024.f;
+__device__ __forceinline__ RowRef row_ref(float m, float c) {
+  const float mc = m * c;
+  const bool far = !(fabsf(mc) < kFar);
+  return {far ? m : 0.f, far ? 0.f : mc};
+}
+// 2^(x − y): what sums relative to x become relative to y.
+__device__ __forceinline__ float ref_factor(const RowRef &x, const RowRef &y, float c) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x.a - y.a, c, x.r - y.r));
+}
+// The logarithm of a row's sum l relative to row_ref(m): +inf without keys, finite for finite scores.
+__device__ __forceinline__ float row_lse(float m, float l, float c) {
+  const float mc = fminf(fmaxf(m * c, kNoMax), -kNoMax);
+  return l > 0.f ? mc + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+}
+
 // The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step.
 template <class T, int DP, int NQ, int KT>
 struct Softmax {
   f32x16 o[NQ][DP / 32];
   Frag<T> q[NQ][DP / 16];
-  float m[NQ], l[NQ];
+  float m[NQ], l[NQ];  // the largest product so far, the sum relative to row_ref(m)
 
   __device__ __forceinline__ void init() {
 #pragma unroll
@@ -135,20 +159,29 @@ struct Softmax {
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][kb][i]);
-      mx = half_max(mx) * c;
-      if (__any(mx > m[n] + 8.f)) {
-        const float to = fmaxf(m[n], mx), f = __builtin_amdgcn_exp2f(m[n] - to);
-        m[n] = to;
+      mx = half_max(mx);
+      RowRef ref = row_ref(m[n], c);
+      if (__any(__builtin_fmaf(mx - ref.a, c, -ref.r) > 8.f)) {
+        m[n] = fmaxf(m[n], mx);
+        const RowRef up = row_ref(m[n], c);
+        const float f = ref_factor(ref, up, c);
+        ref = up;
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[n][d][i] *= f;
       }
+      if (__any(ref.a != 0.f)) {
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[n][kb][i] -= ref.a;
+      }
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][kb][i] = __builtin_amdgcn_exp2f(s[n][kb][i] * c - m[n]);
+        for (int i = 0; i < 16; ++i) s[n][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][i], c, -ref.r));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) to_frag(s[n][kb], ks, p[n][2 * kb + ks]);
       }
@@ -327,8 +360,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(c
       store_rows<float, DP, 1>(a.part_o + first * a.D, sm.o, one, row0, a.rows, a.rows, a.D, 0, a.D, lane);
     } else {
       const float inv[1] = {l > 0.f || l != l ? 1.0f / l : 0.f};
-      const float lse = l > 0.f ? sm.m[0] + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
-      if (lane < 32 && r < a.rows) a.lse[head_rows + r] = lse;
+      if (lane < 32 && r < a.rows) a.lse[head_rows + r] = row_lse(sm.m[0], l, a.c);
       store_rows<T, DP, 1>(op, sm.o, inv, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
     }
   }
@@ -426,19 +458,20 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int r = 32 * n + (lane & 31);
-    float m = -INFINITY, lsum = 0.f, w[NW];
+    float m = kNoMax, lsum = 0.f, w[NW];
 #pragma unroll
     for (int q = 0; q < NW; ++q) m = fmaxf(m, ml[q][n][lane & 31].x);
+    const RowRef top = row_ref(m, a.c);
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
       const float2 v = ml[q][n][lane & 31];
-      w[q] = __builtin_amdgcn_exp2f(v.x - m);
+      w[q] = ref_factor(row_ref(v.x, a.c), top, a.c);
       lsum += w[q] * v.y;
     }
     const float inv = a.splits > 1 ? 1.f : lsum > 0.f || lsum != lsum ? 1.0f / lsum : 0.f;
     if (wave == 0 && lane < 32 && r < a.rows) {
       if (a.splits > 1) *(float2 *)(a.part_ml + 2 * (sp * all + head_rows + r)) = float2{m, lsum};
-      else a.lse[head_rows + r] = lsum > 0.f ? m + __builtin_amdgcn_logf(lsum) : lsum != lsum ? lsum : INFINITY;
+      else a.lse[head_rows + r] = row_lse(m, lsum, a.c);
     }
     const int64_t at = row_at(min(r, a.rows - 1), a.Lq, (int64_t)a.H * a.D, a.D);
     for (int u = wave; u < 4 * ND; u += NW) {  // 4 consecutive channels per lane
@@ -455,7 +488,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
   }
 }
 
-// Joins the splits of a row, one workgroup per row: weights 2^(m_s − max m). Eight groups of 32 lanes (4 channels
+// Joins the splits of a row, one workgroup per row: weights 2^((m_s − max m)·c). Eight groups of 32 lanes (4 channels
 // each) take every eighth split, and their sums are added in order through LDS.
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
@@ -463,16 +496,17 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   __shared__ float ls[8];
   const int64_t all = (int64_t)a.batches * a.Hk * a.rows, row = blockIdx.x;
   const int at = threadIdx.x % 32, g = threadIdx.x / 32;
-  float m = -INFINITY;
+  float m = kNoMax;
   for (int s = at; s < a.splits; s += 32) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
 #pragma unroll
   for (int i = 16; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+  const RowRef top = row_ref(m, a.c);
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = g; s < a.splits; s += 8) {
     const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * all + row));
-    const float w = __builtin_amdgcn_exp2f(ml.x - m);
+    const float w = ref_factor(row_ref(ml.x, a.c), top, a.c);
     l += w * ml.y;
     if (4 * at < a.D) o += w * *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + 4 * at);
   }
@@ -483,7 +517,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 #pragma unroll
   for (int i = 1; i < 8; ++i) o += sums[i][at], l += ls[i];
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-  if (at == 0) a.lse[row] = l > 0.f ? m + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+  if (at == 0) a.lse[row] = row_lse(m, l, a.c);
   if (4 * at >= a.D) return;
   const int r = (int)(row % a.rows), hk = (int)(row / a.rows % a.Hk), b = (int)(row / a.rows / a.Hk);
   T *p = static_cast<T *>(a.out) + ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D +
@@ -495,7 +529,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 
 // ------------------------------------------------------------------ backward
 //
-//   P = 2^(s' − lse),  delta = Σ_d do·out,  dP = do·Vᵀ,  dS = P·(dP − delta)
+//   P = 2^(s·c − lse),  delta = Σ_d do·out,  dP = do·Vᵀ,  dS = P·(dP − delta)
 //   dq = scale · dS·K,   dk = scale · dSᵀ·q,   dv = Pᵀ·do
 // Two kernels form P again: one owns query rows (dq, and delta on the way), one owns keys (dk, dv). That
 // is 7 products instead of 5, and no atomics: every sum has a fixed order. One kernel for all three would write and
@@ -513,7 +547,8 @@ struct AttnBwdArgs {
   AttnArgs f;
   const void *o, *g;  // the output [B, Lq, H, D] contiguous, and its gradient
   void *dq, *dk, *dv;  // contiguous
-  float *delta;        // [B, H, Lq]
+  float *stats;        // [3][B·H·Lq]: x, delta and a of every row, P = 2^((s − a)·c − x): a = 0 and x = lse, but far from
+                       // zero a = m and x = log2 l
   f32x4 *part;         // splits of dq, then of dk and dv, in register order
   int64_t g_sb, g_sl, g_sh;
   float scale;
@@ -526,7 +561,8 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
   constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024 / NW;
-  __shared__ u32x4 smem[4 * TB / 16];
+  __shared__ u32x4 smem[4 * TB / 16 + 1];  // K, V of buffer 0, K, V of buffer 1; a flag of every wave
+  int *wave_far = (int *)(smem + 4 * TB / 16);
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
   int id = blockIdx.x;  // heads first: rows of all heads are read together, whole token rows of memory
@@ -535,12 +571,12 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
   const int rt = id % a.row_tiles;
   id /= a.row_tiles;
   const int b = id % a.batches, sp = id / a.batches;
-  const int t0 = sp * a.split_tiles;
-  const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)sample_keys(a, b)), t1 = (end + KT - 1) / KT;
+  const int t0 = sp * a.split_tiles, keys = sample_keys(a, b);
+  const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)keys), t1 = (end + KT - 1) / KT;
   // Few keys, and out's rounding to bf16 tells in delta (5 keys: 1.4e-3 of dq, as much as dS's): it is summed from P and
   // dP, formed once more, where all the keys are in one tile. From 65 keys on it is below a third of dS's.
-  const bool one = sample_keys(a, b) <= KT;
-  const KeyMask<KT> km{a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb, end};
+  const bool one = keys <= KT;
+  const uint8_t *mask = a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb;
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
   TileLoader<T, DP, N> kl, vl;
@@ -550,13 +586,28 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
     vl.load(vp + (int64_t)t * KT * a.v_sl, bits, lds + buf * 2 * TB + TB);
   };
   uint64_t bits = 0, next = 0;
-  if (t0 < t1) {
-    bits = km.bits(t0, km.byte(t0, lane));
-    stage(t0, 0, bits);
-    next = km.bits(t0 + 1, km.byte(t0 + 1, lane));
-  }
+  auto start = [&](const KeyMask<KT> &km, int first) __attribute__((always_inline)) {
+    bits = km.bits(first, km.byte(first, lane));
+    stage(first, 0, bits);
+    next = km.bits(first + 1, km.byte(first + 1, lane));
+  };
   FragReader<T, DP> fr;
   fr.init(lane, lds);
+  // body(live bits) for the tiles first .. last - 1 after start(first); tile `last` is asked for too: without live keys
+  auto sweep = [&](const KeyMask<KT> &km, int first, int last, auto body) __attribute__((always_inline)) {
+    for (int t = first; t < last; ++t) {
+      wait_vmcnt<0>();
+      lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
+      stage(t + 1, (t + 1 - first) & 1, next);  // past the last tile: no live row, nothing is read
+      const int byte = km.byte(t + 2, lane);
+      if (bits != 0) body(bits);
+      fr.flip(2 * TB);
+      bits = next;
+      next = km.bits(t + 2, byte);
+    }
+    wait_vmcnt<0>();
+  };
+  if (t0 < t1) start(KeyMask<KT>{mask, end}, t0);
   const int row0 = (rt * NW + wave) * 32, r = row0 + (lane & 31), rc = min(r, a.rows - 1);
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
   const int64_t oat = ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
@@ -586,13 +637,8 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
     }
   }
   delta = half_sum(delta);
-  const float lse = a.lse[head_rows + rc];
-  f32x16 dq[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-  auto weights = [&](auto block, uint64_t bits, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {  // P and dP
+  float x = a.lse[head_rows + rc], shift = 0.f;  // P = 2^((s − shift)·c − x)
+  auto scores = [&](auto block, uint64_t bits, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {  // S and dP
     constexpr int kb = decltype(block)::value;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
@@ -609,8 +655,66 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
     }
+  };
+  // Rows far from zero, whose lse says nothing of log2 l: their maximum, sum and delta are measured over all keys of
+  // the sample. The workgroup's waves share the tiles, so that they all do.
+  const bool wave_is_far = __any(fabsf(x) >= kFar && fabsf(x) < INFINITY);
+  if (lane == 0) wave_far[wave] = wave_is_far;
+  lds_pipeline_barrier();
+  int any_far = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.c - lse);
+  for (int w = 0; w < NW; ++w) any_far |= wave_far[w];
+  if (__builtin_amdgcn_readfirstlane(any_far)) {
+    float m = kNoMax, l = 0.f, pd = 0.f;
+    const KeyMask<KT> km{mask, keys};
+    const int last = (keys + KT - 1) / KT;
+    wait_vmcnt<0>();
+    lds_pipeline_barrier();  // what is on its way into the buffers has arrived
+    start(km, 0);
+    sweep(km, 0, last, [&](uint64_t bits) __attribute__((always_inline)) {
+      static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
+        f32x16 s, dp;
+        scores(block, bits, s, dp);
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(m, half_max(mx));
+        const float f = __builtin_amdgcn_exp2f((m - mx) * a.c);
+        m = mx, l *= f, pd *= f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f((s[i] - m) * a.c);
+          l += p, pd += p * dp[i];
+        }
+        return true;
+      });
+    });
+    if (last & 1) fr.flip(2 * TB);
+    lds_pipeline_barrier();  // every wave has read the last tile
+    if (t0 < t1) start(KeyMask<KT>{mask, end}, t0);
+    l = half_sum(l), pd = half_sum(pd);
+    if (l > 0.f) {
+      const RowRef ref = row_ref(m, a.c);
+      const float ll = __builtin_amdgcn_logf(l);
+      shift = ref.a, x = ref.a != 0.f ? ll : __builtin_fmaf(m, a.c, ll), delta = pd / l;
+    } else {
+      x = l != l ? l : INFINITY;
+    }
+  }
+  const bool shifted = __any(shift != 0.f);
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
+  auto weights = [&](auto block, uint64_t bits, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {  // P and dP
+    scores(block, bits, s, dp);
+    if (shifted) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] -= shift;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -x));
   };
   auto step = [&](uint64_t bits) __attribute__((always_inline)) {
     static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
@@ -635,12 +739,8 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
       return true;
     });
   };
-  for (int t = t0; t < t1; ++t) {
-    wait_vmcnt<0>();
-    lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    stage(t + 1, (t + 1 - t0) & 1, next);  // past the last tile: no live row, nothing is read
-    const int byte = km.byte(t + 2, lane);
-    if (sizeof(T) == 2 && one && bits != 0) {
+  sweep(KeyMask<KT>{mask, end}, t0, t1, [&](uint64_t bits) __attribute__((always_inline)) {
+    if (sizeof(T) == 2 && one) {
       float sum = 0.f;
       static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
         f32x16 s, dp;
@@ -651,13 +751,13 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
       });
       delta = half_sum(sum);
     }
-    if (bits != 0) step(bits);
-    fr.flip(2 * TB);
-    bits = next;
-    next = km.bits(t + 2, byte);
+    step(bits);
+  });
+  if (lane < 32 && r < a.rows && sp == 0) {
+    const int64_t all = (int64_t)a.batches * a.Hk * a.rows;
+    float *p = ba.stats + head_rows + r;
+    p[0] = x, p[all] = delta, p[2 * all] = shift;
   }
-  wait_vmcnt<0>();
-  if (lane < 32 && r < a.rows && sp == 0) ba.delta[head_rows + r] = delta;
   if (a.splits > 1) {
     f32x4 *p = ba.part + ((((int64_t)sp * a.batches + b) * a.row_tiles + rt) * a.Hk + hk) * (NW * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
 #pragma unroll
@@ -698,8 +798,8 @@ __global__ __launch_bounds__(256) void attn_dq_join_kernel(const AttnBwdArgs ba)
 }
 
 // NW waves own 32 keys each (K fragments in registers; V in LDS for bf16, whose two waves per SIMD leave no room
-// for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient, lse and
-// delta.
+// for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient and the rows'
+// x, delta and a (the last read only in a tile that has one: a flag per buffer says so).
 template <class T, int DP, int NW>
 struct DkvTile {  // query rows per tile: half as many where that leaves room for another workgroup
   static constexpr int QT = sizeof(T) == 2 && !(DP == 128 && NW == 4) ? 64 : 32;
@@ -712,9 +812,12 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_
   constexpr bool VLDS = sizeof(T) == 2;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = VLDS ? 32 * Tile::RB : 0;
-  // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then lse and delta per buffer
-  __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + QT];
-  f32x4 (&stats)[2][2][QT / 4] = *(f32x4 (*)[2][2][QT / 4])(smem + (4 * TB + NW * VB) / 16);
+  // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then x, delta and a per buffer and a flag
+  // for each
+  static_assert(64 * NW >= 3 * QT, "a thread loads one of a row's three values");
+  __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + 3 * QT / 2 + 1];
+  f32x4 (&stats)[2][3][QT / 4] = *(f32x4 (*)[2][3][QT / 4])(smem + (4 * TB + NW * VB) / 16);
+  int *tile_far = (int *)(smem + (4 * TB + NW * VB) / 16 + 3 * QT / 2);
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
   int id = blockIdx.x;  // heads first, as above
@@ -752,25 +855,27 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_
   const int t1 = kb * 32 * NW >= len ? 0 : min(t0 + ba.q_split_tiles, ba.q_tiles);  // no key at all: zeros
   TileLoader<T, DP, N> ql, gl;
   ql.init(lane, wave, NW, a.q_sl, a.D), gl.init(lane, wave, NW, ba.g_sl, a.D);
-  const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
+  const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows, all = (int64_t)a.batches * a.Hk * a.rows;
   FragReader<T, DP> fr, vr;
   fr.init(lane, lds), vr.init(lane, vt);
-  // a tile's rows into LDS; returns lse (threads 0 .. QT - 1) or delta (QT .. 2 QT - 1) of the thread's row
+  // a tile's rows into LDS; returns x (threads 0 .. QT - 1), delta (QT .. 2 QT - 1) or a (.. 3 QT - 1) of the thread's row
   auto stage = [&](int t, int buf) __attribute__((always_inline)) -> float {
     const int g = t / ba.head_q_tiles, i0 = (t - g * ba.head_q_tiles) * QT, h = hk * a.G + g;
     const uint64_t rows = t < t1 ? low_bits(min(a.Lq - i0, QT)) : 0;  // past the last tile: nothing is read
     ql.load(static_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh + i0 * a.q_sl, rows, lds + buf * 2 * TB);
     gl.load(static_cast<const T *>(ba.g) + b * ba.g_sb + h * ba.g_sh + i0 * ba.g_sl, rows, lds + buf * 2 * TB + TB);
-    const int i = threadIdx.x % QT;
-    const float *src = threadIdx.x < QT ? a.lse : ba.delta;
-    float x = threadIdx.x < QT ? INFINITY : 0.f;  // rows behind the last: P = 0
-    if (threadIdx.x < 2 * QT && t < t1 && i0 + i < a.Lq) x = src[head_rows + (int64_t)g * a.Lq + i0 + i];
+    const int i = threadIdx.x % QT, which = threadIdx.x / QT;
+    float x = which == 0 ? INFINITY : 0.f;  // rows behind the last: P = 0
+    if (which < 3 && t < t1 && i0 + i < a.Lq) x = ba.stats[which * all + head_rows + (int64_t)g * a.Lq + i0 + i];
     return x;
   };
   auto keep = [&](int buf, float x) __attribute__((always_inline)) {
-    if (threadIdx.x < 2 * QT) ((float *)stats[buf][threadIdx.x / QT])[threadIdx.x % QT] = x;
+    if (threadIdx.x < 3 * QT) ((float *)stats[buf][threadIdx.x / QT])[threadIdx.x % QT] = x;
+    const bool far = __any(threadIdx.x / QT == 2 && x != 0.f);  // the threads with a's are lanes of one wave
+    if (threadIdx.x == 2 * QT) tile_far[buf] = far;
   };
   auto step = [&](int buf) __attribute__((always_inline)) {
+    const int far = __builtin_amdgcn_readfirstlane(tile_far[buf]);  // a scalar: kept in a vector register it spills (+10 %)
     static_for<QT / 32>([&](auto block) __attribute__((always_inline)) {
       constexpr int qb = decltype(block)::value;
       __builtin_amdgcn_sched_barrier(0);  // between the phases too: interleaved, they spill
@@ -788,12 +893,20 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dkv_
         dp = mma16(gf, vf, dp);
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (far) {
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const f32x4 shift = stats[buf][2][8 * qb + 2 * i4 + (lane >> 5)];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * i4 + j] -= shift[j];
+        }
+      }
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 lse = stats[buf][0][8 * qb + 2 * i4 + (lane >> 5)], delta = stats[buf][1][8 * qb + 2 * i4 + (lane >> 5)];
+        const f32x4 x = stats[buf][0][8 * qb + 2 * i4 + (lane >> 5)], delta = stats[buf][1][8 * qb + 2 * i4 + (lane >> 5)];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = __builtin_amdgcn_exp2f(s[4 * i4 + j] * a.c - lse[j]);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + j], a.c, -x[j]));
           s[4 * i4 + j] = p;
           dp[4 * i4 + j] = p * (dp[4 * i4 + j] - delta[j]);
         }
@@ -1070,7 +1183,7 @@ static int attn_args(AttnArgs &a, const void *q, const int64_t *qs, const void *
                      float scale, const float *lse, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D) {
   int st = attn_sizes(dtype, B, Lq, Lk, H, Hk, D);
   if (st) return st;
-  if (!(scale > 0.f && scale < INFINITY) || qs == nullptr || ks == nullptr || vs == nullptr || mask_sb < 0)
+  if (!(scale > 0.f && scale * kLog2e < INFINITY) || qs == nullptr || ks == nullptr || vs == nullptr || mask_sb < 0)
     return MLORA_ERR_INVALID;
   st = check_heads(q, qs[0], qs[1], qs[2], B * Lq == 0);
   if (!st) st = check_heads(k, ks[0], ks[1], ks[2], B * Lk == 0);
@@ -1153,9 +1266,9 @@ extern "C" int64_t mlora_cross_attention_backward_workspace_bytes(int dtype, int
                                                                   int64_t Hk, int64_t D) {
   const int st = attn_sizes(dtype, B, Lq, Lk, H, Hk, D);
   if (st) return st;
-  // delta, rounded up to whole 16-byte vectors, then the splits
+  // three values of every row, rounded up to whole 16-byte vectors, then the splits
   const bool f32 = dtype == MLORA_F32;
-  return (B * H * Lq + 3) / 4 * 16 +
+  return (3 * B * H * Lq + 3) / 4 * 16 +
          bwd_part_bytes(dq_plan(B, H / Hk * Lq, Lk, Hk, f32), dkv_plan(B, Lq, Lk, Hk, H / Hk, D, f32), B, Hk, D);
 }
 
@@ -1184,8 +1297,8 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   AttnArgs &a = ba.f;
   const DkvPlan p = dkv_plan(B, Lq, Lk, Hk, a.G, D, f32);
   ba.o = out, ba.g = g, ba.g_sb = g_strides[0], ba.g_sl = g_strides[1], ba.g_sh = g_strides[2], ba.scale = scale;
-  ba.dq = dq, ba.dk = dk, ba.dv = dv, ba.delta = static_cast<float *>(workspace);
-  ba.part = static_cast<f32x4 *>(workspace) + (B * H * Lq + 3) / 4;
+  ba.dq = dq, ba.dk = dk, ba.dv = dv, ba.stats = static_cast<float *>(workspace);
+  ba.part = static_cast<f32x4 *>(workspace) + (3 * B * H * Lq + 3) / 4;
   ba.key_blocks = (int32_t)p.key_blocks, ba.q_tiles = (int32_t)p.q_tiles, ba.head_q_tiles = (int32_t)p.head_q_tiles;
   ba.q_splits = (int32_t)p.splits, ba.q_split_tiles = (int32_t)p.split_tiles;
   const DqPlan qp = dq_plan(B, a.rows, Lk, Hk, f32);

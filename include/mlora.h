@@ -568,14 +568,16 @@ int mlora_joint_backward(const void *x, int x_dtype, int64_t x_stride_b, int64_t
  *
  * out = softmax(scale · q kᵀ) v per head, q [B, Lq, H, D], k and v [B, Lk, Hk, D] (bf16 or float32, one type;
  * unit stride in the head, element strides {batch, token, head}, multiples of 8, token strides below 2^22,
- * 16-byte aligned); query head h reads key head h / (H / Hk). D is a multiple of 8 up to 128, scale > 0.
+ * 16-byte aligned); query head h reads key head h / (H / Hk). D is a multiple of 8 up to 128, scale > 0 and
+ * scale · log2 e finite in float32.
  *   key_lengths  device int32 [B] or NULL: sample b has its first key_lengths[b] keys (clamped to [0, Lk])
  *   key_mask     device bytes [B, Lk] (batch stride in bytes, 0: shared; unit key stride) or NULL: keys
  *                with a zero byte do not count
  * Whatever k and v hold at keys that do not count is not used. A query without keys gets zeros. out
  * [B, Lq, H, D] contiguous; lse [B, H, Lq] float32: base-2 logarithm of the sum of 2^(score · log2 e), +inf for
- * a query without keys (the backward reads it). workspace (16-byte aligned, the queried bytes, 0: may be
- * NULL) holds partial sums where few rows meet many keys.
+ * a query without keys (the backward reads it; from 2^10 on, where it would say little of the sum, the backward
+ * forms maximum and sum again: equal scores weigh alike at any finite size). workspace (16-byte aligned, the
+ * queried bytes, 0: may be NULL) holds partial sums where few rows meet many keys.
  * Reference: flash_attention(q, k, v, k_lens=context_lens) of WanT2VCrossAttention (wan/modules/model.py). */
 int64_t mlora_cross_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk,
                                               int64_t D);
