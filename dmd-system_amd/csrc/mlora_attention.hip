@@ -561,8 +561,7 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
   constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024 / NW;
-  __shared__ u32x4 smem[4 * TB / 16 + 1];  // K, V of buffer 0, K, V of buffer 1; a flag of every wave
-  int *wave_far = (int *)(smem + 4 * TB / 16);
+  __shared__ u32x4 smem[4 * TB / 16];
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
   const int wave = wave_id(), lane = threadIdx.x & 63;
   int id = blockIdx.x;  // heads first: rows of all heads are read together, whole token rows of memory
@@ -573,9 +572,6 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
   const int b = id % a.batches, sp = id / a.batches;
   const int t0 = sp * a.split_tiles, keys = sample_keys(a, b);
   const int end = (int)min((int64_t)(t0 + a.split_tiles) * KT, (int64_t)keys), t1 = (end + KT - 1) / KT;
-  // Few keys, and out's rounding to bf16 tells in delta (5 keys: 1.4e-3 of dq, as much as dS's): it is summed from P and
-  // dP, formed once more, where all the keys are in one tile. From 65 keys on it is below a third of dS's.
-  const bool one = keys <= KT;
   const uint8_t *mask = a.mask == nullptr ? nullptr : a.mask + b * a.mask_sb;
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
@@ -586,30 +582,34 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
     vl.load(vp + (int64_t)t * KT * a.v_sl, bits, lds + buf * 2 * TB + TB);
   };
   uint64_t bits = 0, next = 0;
-  auto start = [&](const KeyMask<KT> &km, int first) __attribute__((always_inline)) {
+  auto start = [&](const KeyMask<KT> &km, int first, int second) __attribute__((always_inline)) {
     bits = km.bits(first, km.byte(first, lane));
     stage(first, 0, bits);
-    next = km.bits(first + 1, km.byte(first + 1, lane));
+    next = km.bits(second, km.byte(second, lane));
   };
   FragReader<T, DP> fr;
   fr.init(lane, lds);
   // body(live bits) for the tiles first .. last - 1 after start(first); tile `last` is asked for too: without live keys
-  auto sweep = [&](const KeyMask<KT> &km, int first, int last, auto body) __attribute__((always_inline)) {
+  auto sweep = [&](const KeyMask<KT> &km, int first, int last, auto tile, auto body) __attribute__((always_inline)) {
     for (int t = first; t < last; ++t) {
       wait_vmcnt<0>();
       lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-      stage(t + 1, (t + 1 - first) & 1, next);  // past the last tile: no live row, nothing is read
-      const int byte = km.byte(t + 2, lane);
+      stage(tile(t + 1), (t + 1 - first) & 1, next);  // past the last tile: no live row, nothing is read
+      const int byte = km.byte(tile(t + 2), lane);
       if (bits != 0) body(bits);
       fr.flip(2 * TB);
       bits = next;
-      next = km.bits(t + 2, byte);
+      next = km.bits(tile(t + 2), byte);
     }
     wait_vmcnt<0>();
   };
-  if (t0 < t1) start(KeyMask<KT>{mask, end}, t0);
+  auto same = [](int t) __attribute__((always_inline)) { return t; };
   const int row0 = (rt * NW + wave) * 32, r = row0 + (lane & 31), rc = min(r, a.rows - 1);
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows;
+  float wg_lse[NW / 2];  // of all the workgroup's rows, in every wave: asked for first, looked at below
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) wg_lse[i] = a.lse[head_rows + min(rt * NW * 32 + 64 * i + lane, a.rows - 1)];
+  if (t0 < t1) start(KeyMask<KT>{mask, end}, t0, t0 + 1);
   const int64_t oat = ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
   Frag<T> q[DP / 16], g[DP / 16];
   float delta = 0.f;
@@ -656,22 +656,50 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
       for (int i = 0; i < 16; ++i) s[i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
     }
   };
+  // Few live keys, and roundings to bf16 do not average away: out's tells in delta, the weights' in their sum (2 to 5
+  // keys: 1.4e-3 to 4e-3 of dq and dk, as much and more than the gradients' own). Then x and delta are measured too. From
+  // 65 keys on delta's share is below a third of that. The keys are counted up to there, with length and mask; lane i
+  // keeps the i-th tile that has one. The measuring takes 2 us of a small backward (2 x 1560 rows, 12 heads of 128, 5 of 512
+  // keys: 52 -> 54 us); its presence costs dq 3 % where it does not run but tiles are few (2 x 32760 x 512: 383 -> 395).
+  int live = 0, live_tiles = 0, list = 0;
+  if constexpr (sizeof(T) == 2) {
+    if (mask == nullptr || keys <= KT) {
+      live = keys, live_tiles = 1;
+    } else {
+      constexpr int kAtOnce = 8;
+      for (int k0 = 0; k0 < keys && live <= KT; k0 += kAtOnce * KT) {
+        uint8_t byte[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) byte[j] = mask[min(k0 + j * KT + lane, keys - 1)];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const uint64_t on = __ballot(byte[j] != 0) & low_bits(keys - k0 - j * KT);
+          if (on == 0) continue;
+          if (lane == live_tiles) list = k0 / KT + j;
+          ++live_tiles, live += __popcll(on);
+        }
+      }
+    }
+  }
+  const bool few = sizeof(T) == 2 && live > 0 && live <= KT;
   // Rows far from zero, whose lse says nothing of log2 l: their maximum, sum and delta are measured over all keys of
   // the sample. The workgroup's waves share the tiles, so that they all do.
-  const bool wave_is_far = __any(fabsf(x) >= kFar && fabsf(x) < INFINITY);
-  if (lane == 0) wave_far[wave] = wave_is_far;
-  lds_pipeline_barrier();
-  int any_far = 0;
+  bool far = false;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) any_far |= wave_far[w];
-  if (__builtin_amdgcn_readfirstlane(any_far)) {
+  for (int i = 0; i < NW / 2; ++i) far |= fabsf(wg_lse[i]) >= kFar && fabsf(wg_lse[i]) < INFINITY;
+  if (few || __any(far)) {
     float m = kNoMax, l = 0.f, pd = 0.f;
     const KeyMask<KT> km{mask, keys};
-    const int last = (keys + KT - 1) / KT;
-    wait_vmcnt<0>();
-    lds_pipeline_barrier();  // what is on its way into the buffers has arrived
-    start(km, 0);
-    sweep(km, 0, last, [&](uint64_t bits) __attribute__((always_inline)) {
+    const int tiles = (keys + KT - 1) / KT, n = few ? live_tiles : tiles;
+    auto tile = [&](int i) __attribute__((always_inline)) { return i >= n ? tiles : few ? __builtin_amdgcn_readlane(list, i) : i; };
+    const bool there = n == 1 && tile(0) == t0 && t0 < t1;  // the only tile is this split's first
+    const uint64_t first = bits;
+    if (!there) {
+      wait_vmcnt<0>();
+      lds_pipeline_barrier();  // what is on its way into the buffers has arrived
+      start(km, tile(0), tile(1));
+    }
+    sweep(km, 0, n, tile, [&](uint64_t bits) __attribute__((always_inline)) {
       static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
         f32x16 s, dp;
         scores(block, bits, s, dp);
@@ -689,9 +717,10 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
         return true;
       });
     });
-    if (last & 1) fr.flip(2 * TB);
+    if (n & 1) fr.flip(2 * TB);
     lds_pipeline_barrier();  // every wave has read the last tile
-    if (t0 < t1) start(KeyMask<KT>{mask, end}, t0);
+    if (there) bits = first, next = 0;  // it lies in the first buffer still, and no other tile has a key
+    else if (t0 < t1) start(KeyMask<KT>{mask, end}, t0, t0 + 1);
     l = half_sum(l), pd = half_sum(pd);
     if (l > 0.f) {
       const RowRef ref = row_ref(m, a.c);
@@ -701,28 +730,21 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
       x = l != l ? l : INFINITY;
     }
   }
-  const bool shifted = __any(shift != 0.f);
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-  auto weights = [&](auto block, uint64_t bits, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {  // P and dP
-    scores(block, bits, s, dp);
-    if (shifted) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] -= shift;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -x));
-  };
-  auto step = [&](uint64_t bits) __attribute__((always_inline)) {
+  auto step = [&](auto shifted, uint64_t bits) __attribute__((always_inline)) {
     static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
       constexpr int kb = decltype(block)::value;
       f32x16 s, dp;
-      weights(block, bits, s, dp);
+      scores(block, bits, s, dp);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
+      for (int i = 0; i < 16; ++i) {
+        const float ds = decltype(shifted)::value ? s[i] - shift : s[i];
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(ds, a.c, -x)) * (dp[i] - delta);
+      }
       static_for<2>([&](auto ks) __attribute__((always_inline)) {
         Frag<T> ds, rest;
         to_frag(s, ks, ds);
@@ -739,20 +761,10 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
       return true;
     });
   };
-  sweep(KeyMask<KT>{mask, end}, t0, t1, [&](uint64_t bits) __attribute__((always_inline)) {
-    if (sizeof(T) == 2 && one) {
-      float sum = 0.f;
-      static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
-        f32x16 s, dp;
-        weights(block, bits, s, dp);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += s[i] * dp[i];
-        return true;
-      });
-      delta = half_sum(sum);
-    }
-    step(bits);
-  });
+  // a loop each: a branch between a block's products and its exponentials would keep the next block's out of them
+  const KeyMask<KT> km{mask, end};
+  if (__any(shift != 0.f)) sweep(km, t0, t1, same, [&](uint64_t bits) __attribute__((always_inline)) { step(std::true_type{}, bits); });
+  else sweep(km, t0, t1, same, [&](uint64_t bits) __attribute__((always_inline)) { step(std::false_type{}, bits); });
   if (lane < 32 && r < a.rows && sp == 0) {
     const int64_t all = (int64_t)a.batches * a.Hk * a.rows;
     float *p = ba.stats + head_rows + r;

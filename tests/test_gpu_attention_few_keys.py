@@ -1,0 +1,80 @@
+"""bf16 gradients of queries whose softmax rests on few keys, given as leading keys, as a mask or both: where few values
+add up, out's rounding to bf16 (which delta = do . out would carry on) and the weights' (which the forward's sum holds)
+do not average away.
+
+Root mean squares: rounding to bf16 moves a value of [2^k, 2^(k+1)) by up to 2^(k-8), uniformly, 2^(k-8) / sqrt(3) in the
+mean square: `rounding` adds that up over the tensor that is wanted. The squares of N uniform errors add up to their mean
+within 0.9 / sqrt(N) of it (one deviation; six are allowed). Beside it stand float32 sums of up to 2^10 terms and what two bf16 parts
+of P and dS leave out: 2^-14 in all."""
+import math
+
+import pytest
+import torch
+
+import block_reference as ref
+from test_gpu_attention import live_keys, make, run
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def rounding(want):
+    """The mean square error, summed, of `want` rounded to bf16."""
+    return float((2.0 ** (torch.floor(torch.log2(want[want != 0].abs())) - 8)).square().sum()) / 3
+
+
+def only_rounded(q, k, v, g, grads, live):
+    """The gradients are the formula's, rounded once."""
+    _, dq, dk, dv, _ = ref.attention(q, k, v, live=live, do=g)
+    found = {}
+    for name, got, want in (("dq", grads[0], dq), ("dk", grads[1], dk), ("dv", grads[2], dv)):
+        off, norm = float((ref.f64(got) - want).square().sum()), float(want.square().sum())
+        most = rounding(want) * (1 + 6 * 0.9 / math.sqrt(int((want != 0).sum())))
+        found[name] = (math.sqrt(off / norm), math.sqrt(most / norm) + 2 ** -14)
+    assert all(off <= most for off, most in found.values()), found
+
+
+@pytest.mark.parametrize("how", ["lengths", "mask", "both", "one mask for all"])
+@pytest.mark.parametrize("Lq, Lk, H, Hk, D, n", [
+    (200, 512, 4, 4, 128, 5),
+    (200, 512, 4, 2, 64, 2),
+    (3, 700, 6, 2, 128, 3),
+    (60, 900, 8, 8, 72, 30),
+    (100, 1000, 8, 8, 128, 64),   # as many as are counted, dq's keys split
+    (40, 20000, 2, 2, 128, 17),   # far apart, many splits
+    (150, 64, 8, 8, 64, 4),       # one tile
+])
+def test_few_live_keys(pkg, dev, Lq, Lk, H, Hk, D, n, how):
+    """The same error whichever way the same number of keys is given, and however many dead ones lie between them."""
+    B = 2
+    q, k, v, g = make(B, Lq, Lk, H, Hk, D, BF, dev, Lq + Lk + n)
+    gen = torch.Generator().manual_seed(n)
+    lengths = mask = None
+    if how == "lengths":
+        lengths = torch.full((B,), n, dtype=torch.int32)
+    else:
+        rows = 1 if how == "one mask for all" else B
+        mask = torch.zeros(rows, Lk, dtype=torch.bool)
+        for b in range(rows):
+            mask[b, torch.randperm(Lk - (how == "both"), generator=gen)[:n]] = True
+        if how == "both":
+            lengths = torch.full((B,), Lk - 1, dtype=torch.int32)
+            mask[:, Lk - 1] = True  # behind the length
+    kw = dict(key_lengths=None if lengths is None else lengths.to(dev), key_mask=None if mask is None else mask.to(dev))
+    _, grads = run(pkg, q, k, v, g, **kw)
+    only_rounded(q, k, v, g, grads, live_keys(B, Lk, lengths, mask))
+
+
+def test_live_keys_at_the_border_of_the_count(pkg, dev):
+    """63, 64 and 65 live keys and none, in one batch, under masks, against the formula value by value."""
+    from test_gpu_attention import check
+
+    B, Lq, Lk = 4, 70, 700
+    q, k, v, g = make(B, Lq, Lk, 2, 2, 64, BF, dev, 3)
+    mask = torch.zeros(B, Lk, dtype=torch.bool)
+    for b, n in enumerate((63, 64, 65, 0)):
+        mask[b, torch.randperm(Lk, generator=torch.Generator().manual_seed(b))[:n]] = True
+    out, grads = run(pkg, q, k, v, g, key_mask=mask.to(dev))
+    check(q, k, v, out, g, grads, live=mask)
+    for t in (out, *grads):
+        assert t[3].abs().sum() == 0
