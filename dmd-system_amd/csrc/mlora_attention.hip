@@ -102,17 +102,20 @@ __device__ __forceinline__ float row_lse(float m, float l, float c) {
   return l > 0.f ? mc + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
 }
 
-// The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step.
-template <class T, int DP, int NQ, int KT>
+// The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step. EXACT: e sums the weights
+// before their rounding to bf16, for lse: the backward forms them unrounded, and where a row rests on few keys the two sums
+// are up to half a bf16 step apart (a factor of all of its gradients). 16 additions more per 32 x 32 block; l is e elsewhere.
+template <class T, int DP, int NQ, int KT, bool EXACT>
 struct Softmax {
+  static constexpr bool kTwoSums = EXACT && sizeof(T) == 2;
   f32x16 o[NQ][DP / 32];
   Frag<T> q[NQ][DP / 16];
-  float m[NQ], l[NQ];  // the largest product so far, the sum relative to row_ref(m)
+  float m[NQ], l[NQ], e[NQ];  // the largest product so far, the sums relative to row_ref(m)
 
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      m[n] = kNoMax, l[n] = 0.f;
+      m[n] = kNoMax, l[n] = 0.f, e[n] = 0.f;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -166,7 +169,7 @@ struct Softmax {
         const RowRef up = row_ref(m[n], c);
         const float f = ref_factor(ref, up, c);
         ref = up;
-        l[n] *= f;
+        l[n] *= f, e[n] *= f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -184,6 +187,12 @@ struct Softmax {
         for (int i = 0; i < 16; ++i) s[n][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][i], c, -ref.r));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) to_frag(s[n][kb], ks, p[n][2 * kb + ks]);
+        if constexpr (kTwoSums) {
+          float t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = (s[n][kb][i] + s[n][kb][4 + i]) + (s[n][kb][8 + i] + s[n][kb][12 + i]);
+          e[n] += (t[0] + t[1]) + (t[2] + t[3]);
+        }
       }
       l[n] += frag_sum(p[n]);
     }
@@ -197,6 +206,16 @@ struct Softmax {
       }
       return true;
     });
+  }
+
+  // The row's whole sums over both halves; f: what makes O a sum of weights that add up to e where they added up to l.
+  __device__ __forceinline__ float sums(int n, float &f) {
+    const float lw = half_sum(l[n]);
+    f = 1.f;
+    if constexpr (!kTwoSums) return lw;
+    const float ew = half_sum(e[n]);
+    if (lw > 0.f) f = ew / lw;
+    return lw > 0.f ? ew : lw;
   }
 
   // The sum of the weights as the product with V sees them (bf16: two per v_dot2_f32_bf16 with ones).
@@ -275,7 +294,7 @@ struct AttnTile {
 // t is multiplied; one barrier per tile. A workgroup takes `turns` row tiles of one head in a row: the key tiles
 // go on loading from one to the next, and the next rows' q arrives under the present ones' products (with one row
 // tile per workgroup and 512 keys, every workgroup waits for q and its first keys, in step with all others).
-template <class T, int DP>
+template <class T, int DP, bool EXACT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(const AttnArgs a) {
   constexpr int KT = AttnTile<T>::KT;
   using Tile = HeadTile<T, DP>;
@@ -310,7 +329,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(c
   }
   FragReader<T, DP> fr;
   fr.init(lane, lds);
-  Softmax<T, DP, 1, KT> sm;
+  Softmax<T, DP, 1, KT, EXACT> sm;
   const T *qp = static_cast<const T *>(a.q) + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
   Frag<T> qn[DP / 16];
   auto load_q = [&](int rt) __attribute__((always_inline)) {
@@ -350,16 +369,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(c
       next = km.bits(after(after(t)), byte);
     }
     const int row0 = (rt * 4 + wave) * 32, r = row0 + (lane & 31);
-    const float l = half_sum(sm.l[0]);
+    float f[1];
+    const float l = sm.sums(0, f[0]);
     if (t1 - t0 == 1) wait_vmcnt<kLoadsQ>();  // the next rows' first tile
     else wait_vmcnt<0>();
     if (a.splits > 1) {
       const int64_t first = sp * all + head_rows;
-      const float one[1] = {1.f};
       if (lane < 32 && r < a.rows) *(float2 *)(a.part_ml + 2 * (first + r)) = float2{sm.m[0], l};
-      store_rows<float, DP, 1>(a.part_o + first * a.D, sm.o, one, row0, a.rows, a.rows, a.D, 0, a.D, lane);
+      store_rows<float, DP, 1>(a.part_o + first * a.D, sm.o, f, row0, a.rows, a.rows, a.D, 0, a.D, lane);
     } else {
-      const float inv[1] = {l > 0.f || l != l ? 1.0f / l : 0.f};
+      const float inv[1] = {l > 0.f || l != l ? f[0] / l : 0.f};
       if (lane < 32 && r < a.rows) a.lse[head_rows + r] = row_lse(sm.m[0], l, a.c);
       store_rows<T, DP, 1>(op, sm.o, inv, row0, a.rows, a.Lq, (int64_t)a.H * a.D, a.D, a.D, lane);
     }
@@ -408,7 +427,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
   }
   FragReader<T, DP> fr;
   fr.init(lane, lds);
-  Softmax<T, DP, NQ, KT> sm;
+  Softmax<T, DP, NQ, KT, true> sm;  // bound by K and V: the second sum costs nothing
   sm.init();
   const T *qp = static_cast<const T *>(a.q) + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
 #pragma unroll
@@ -436,11 +455,11 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
   }
   wait_vmcnt<0>();
   // join the waves: every wave leaves its sums, then sums its share of the 32 x 32 tiles over the waves
-  float l[NQ];
+  float f[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] = half_sum(sm.l[n]);
-    if (lane < 32) ml[wave][n][lane] = float2{sm.m[n], l[n]};
+    const float l = sm.sums(n, f[n]);
+    if (lane < 32) ml[wave][n][lane] = float2{sm.m[n], l};
   }
   __syncthreads();
   f32x4 *sums = (f32x4 *)smem;
@@ -451,7 +470,7 @@ __global__ __launch_bounds__((64 * FewTile<T, DP>::NW), 1) void attn_few_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         sums[(((wave * NQ + n) * ND + d) * 4 + i) * 64 + lane] =
-            f32x4{sm.o[n][d][4 * i], sm.o[n][d][4 * i + 1], sm.o[n][d][4 * i + 2], sm.o[n][d][4 * i + 3]};
+            f32x4{sm.o[n][d][4 * i], sm.o[n][d][4 * i + 1], sm.o[n][d][4 * i + 2], sm.o[n][d][4 * i + 3]} * f[n];
   __syncthreads();
   const int64_t head_rows = ((int64_t)b * a.Hk + hk) * a.rows, all = (int64_t)a.batches * a.Hk * a.rows;
   T *op = static_cast<T *>(a.out) + ((int64_t)b * a.Lq * a.H + (int64_t)hk * a.G) * a.D;
@@ -536,7 +555,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // add up float32 parts of dq per 256 keys (402 MB each at 2 x 32760 rows of 12 x 128: more time than its
 // two products). bf16: P and dS are rounded to bf16 as operands of the products that follow: half a step each,
 // 1.7e-3 of dq, dk and dv in the mean square where few rows add up, as much as their own rounding. FINE: what the
-// rounding left is a second operand, and only the gradients' own rounding remains (dq's error at 512 keys 2.4e-3 ->
+// rounding left is a second operand, and the forward's lse holds the weights' sum before their rounding. Then the
+// gradients' own rounding remains, and beyond 64 live keys delta's from the rounded out: relative to |do| |out|, little where
+// out averages many values, up to half a step where one key has nearly all the weight (dq's error at 512 keys 2.4e-3 ->
 // 1.7e-3). At 2 x 32760 rows x 512 keys, 12 heads of 128, that costs dq 414 -> 456 us and dk alone 460 -> 617:
 // it is done up to 2^30 products of scores and channels, where the backward's kernels take less than the call's host
 // side (500 x 512, 12 heads of 128: 49 -> 59 us, 1000 x 1000, 8 of 64: 41 -> 44). Single rows of a long cache pay
@@ -1012,9 +1033,9 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const AttnBwdArgs ba
 
 // The kernels are named here because hipcc's host pass does not instantiate a kernel that holds generic lambdas
 // from a launch inside one.
-#define MLORA_ATTN(T, DP)                                             \
-  template __global__ void attn_fwd_kernel<T, DP>(const AttnArgs);    \
-  template __global__ void attn_few_kernel<T, DP, 1>(const AttnArgs); \
+#define MLORA_ATTN(T, DP)                                                       \
+  template __global__ void attn_fwd_kernel<T, DP, false>(const AttnArgs);       \
+  template __global__ void attn_few_kernel<T, DP, 1>(const AttnArgs);           \
   template __global__ void attn_dq_kernel<T, DP, 4, false>(const AttnBwdArgs);  \
   template __global__ void attn_dkv_kernel<T, DP, 4, false>(const AttnBwdArgs);
 MLORA_ATTN(uint16_t, 64)
@@ -1022,6 +1043,8 @@ MLORA_ATTN(uint16_t, 128)
 MLORA_ATTN(float, 64)
 MLORA_ATTN(float, 128)
 #undef MLORA_ATTN
+template __global__ void attn_fwd_kernel<uint16_t, 64, true>(const AttnArgs);
+template __global__ void attn_fwd_kernel<uint16_t, 128, true>(const AttnArgs);
 template __global__ void attn_few_kernel<uint16_t, 64, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<uint16_t, 128, 2>(const AttnArgs);
 template __global__ void attn_few_kernel<float, 64, 2>(const AttnArgs);
@@ -1168,6 +1191,11 @@ static int64_t bwd_part_bytes(const DqPlan &q, const DkvPlan &p, int64_t batches
   return dq > dkv ? dq : dkv;
 }
 
+// Whether the backward's products take P and dS in two bf16 parts, and the forward's lse the sum that goes with them.
+static bool fine_call(int64_t B, int64_t H, int64_t Lq, int64_t Lk, int64_t D) {
+  return (double)B * (double)H * (double)Lq * (double)Lk * (double)D <= 1073741824.0;
+}
+
 // Sizes and types shared by every entry. MLORA_OK, or the status.
 static int attn_sizes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D) {
   if (dtype != MLORA_BF16 && dtype != MLORA_F32) return MLORA_ERR_UNSUPPORTED;
@@ -1262,7 +1290,15 @@ extern "C" int mlora_cross_attention(const void *q, const int64_t *q_strides, co
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     if (p.few && p.nq == 1) hipLaunchKernelGGL((attn_few_kernel<T, DP, 1>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
-    else if (!p.few) hipLaunchKernelGGL((attn_fwd_kernel<T, DP>), grid, dim3(256), 0, s, a);
+    else if (!p.few) {
+      if constexpr (sizeof(T) == 2) {
+        if (fine_call(B, H, Lq, Lk, D)) {
+          hipLaunchKernelGGL((attn_fwd_kernel<T, DP, true>), grid, dim3(256), 0, s, a);
+          return;
+        }
+      }
+      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, false>), grid, dim3(256), 0, s, a);
+    }
     else if constexpr (sizeof(T) * DP < 512)
       hipLaunchKernelGGL((attn_few_kernel<T, DP, 2>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
   });
@@ -1315,7 +1351,7 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   ba.q_splits = (int32_t)p.splits, ba.q_split_tiles = (int32_t)p.split_tiles;
   const DqPlan qp = dq_plan(B, a.rows, Lk, Hk, f32);
   a.row_tiles = (int32_t)qp.row_tiles, a.splits = (int32_t)qp.splits, a.split_tiles = (int32_t)qp.split_tiles;
-  const bool fine = (double)B * (double)H * (double)Lq * (double)Lk * (double)D <= 1073741824.0;
+  const bool fine = fine_call(B, H, Lq, Lk, D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (Lq > 0) {
     with_head(f32, D, [&](auto t, auto dp) {

@@ -78,3 +78,33 @@ def test_live_keys_at_the_border_of_the_count(pkg, dev):
     check(q, k, v, out, g, grads, live=mask)
     for t in (out, *grads):
         assert t[3].abs().sum() == 0
+
+
+@pytest.mark.parametrize("Lq, Lk, Hk", [
+    (1, 100, 16),   # few rows
+    (1, 3000, 4),   # ... that share keys, split
+    (40, 200, 16),
+    (70, 100, 16),  # many rows
+    (70, 1500, 16),  # ... split
+])
+def test_weights_add_up_to_one(pkg, dev, Lq, Lk, Hk):
+    """Among many keys too the weights may rest on a few: scores of a spread of 8, and the weights' own rounding (bf16, for
+    their product with v) must not be in the sum that the backward divides by. Only one row of each head has an upstream
+    gradient, so that the sum over the keys of <dv_j, do> / <do, do> is the sum of that row's weights, each dv_j = P_j do
+    rounded to bf16. Those roundings are no noise to be averaged: do is bf16 itself, and where one P is within 2^-9 of 1 every
+    channel of P do rounds to do, all off to one side. So they are computed: weights off by a factor of 1 -+ 2^-14 (the
+    float32 scores and sums) give sums between those of P do (1 -+ 2^-14), each rounded."""
+    B, H, D = 4, 16, 128
+    q, k, v, g = make(B, Lq, Lk, H, Hk, D, BF, dev, 17, loud=8.0)
+    g[:, :Lq // 2] = 0
+    g[:, Lq // 2 + 1:] = 0
+    if Hk < H:
+        g[:, :, torch.arange(H) % (H // Hk) != 0] = 0  # one row for every key head
+    _, (_, _, dv) = run(pkg, q, k, v, g)
+    do = ref.f64(g)[:, Lq // 2, ::H // Hk]  # [B, Hk, D]
+    exact = ref.attention(q, k, v, do=g)[3]  # [B, Lk, Hk, D]
+    total = lambda t: (ref.f64(t) * do.unsqueeze(1)).sum((1, 3)) / do.square().sum(-1) - 1  # noqa: E731
+    low, want, high = (total((exact * (1 + e)).to(BF)) for e in (-(2.0 ** -14), 0.0, 2.0 ** -14))
+    off, room = total(dv) - want, torch.maximum(high - want, want - low)
+    rms = lambda t: float(t.square().mean().sqrt())  # noqa: E731
+    assert rms(off) <= rms(room), (rms(off), rms(room), float(off.abs().max()))
