@@ -8,7 +8,9 @@ length or masked out do not count, whatever they hold; a query without keys gets
 Query heads may share key heads (H a multiple of Hk). Gradients of q, k and v, summed in a fixed order.
 
 bf16: scores, softmax and sums in float32; the weights are rounded to bf16 for their product with v, as they and dS
-are in a backward of more than 2^30 products (below, both enter in two parts, to 16 bits). float32: float32 throughout, on the fp32 matrix core.
+are in the backward of a sample of more than 2^30 products (heads, rows, keys and channels multiplied; below, both
+enter in two parts, to 16 bits, whatever the batch). delta is formed from the rounded output, but from float32 weights
+where a sample has at most 64 keys that count. float32: float32 throughout, on the fp32 matrix core.
 """
 from __future__ import annotations
 

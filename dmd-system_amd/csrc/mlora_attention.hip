@@ -559,10 +559,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // gradients' own rounding remains, and beyond 64 live keys delta's from the rounded out: relative to |do| |out|, little where
 // out averages many values, up to half a step where one key has nearly all the weight (dq's error at 512 keys 2.4e-3 ->
 // 1.7e-3). At 2 x 32760 rows x 512 keys, 12 heads of 128, that costs dq 414 -> 456 us and dk alone 460 -> 617:
-// it is done up to 2^30 products of scores and channels, where the backward's kernels take less than the call's host
-// side (500 x 512, 12 heads of 128: 49 -> 59 us, 1000 x 1000, 8 of 64: 41 -> 44). Single rows of a long cache pay
-// too (4 x 1 x 58981 keys, 40 heads on 4 of 64: 407 -> 513 us): it is there that dv, a sum of few rows, has the most to
-// lose.
+// it is done up to 2^30 products of scores and channels of one sample, whatever the batch, so that a sample's gradients do
+// not depend on what it is batched with. Below that line it costs a backward a tenth to a fifth (500 x 512, 12 heads
+// of 128: 49 -> 59 us; with the forward 64 of them 706 -> 846; 1000 x 1000, 8 of 64: 41 -> 44), and single rows of a
+// long cache a quarter (4 x 1 x 58981 keys, 40 heads on 4 of 64: 407 -> 513 us): it is there that dv, a sum of few rows,
+// has the most to lose.
 
 struct AttnBwdArgs {
   AttnArgs f;
@@ -1191,9 +1192,10 @@ static int64_t bwd_part_bytes(const DqPlan &q, const DkvPlan &p, int64_t batches
   return dq > dkv ? dq : dkv;
 }
 
-// Whether the backward's products take P and dS in two bf16 parts, and the forward's lse the sum that goes with them.
-static bool fine_call(int64_t B, int64_t H, int64_t Lq, int64_t Lk, int64_t D) {
-  return (double)B * (double)H * (double)Lq * (double)Lk * (double)D <= 1073741824.0;
+// Whether the backward's products take P and dS in two bf16 parts, and the forward's lse the sum that goes with them: a
+// matter of one sample's sizes, so that its gradients do not depend on the batch it is in.
+static bool fine_call(int64_t H, int64_t Lq, int64_t Lk, int64_t D) {
+  return (double)H * (double)Lq * (double)Lk * (double)D <= 1073741824.0;
 }
 
 // Sizes and types shared by every entry. MLORA_OK, or the status.
@@ -1292,7 +1294,7 @@ extern "C" int mlora_cross_attention(const void *q, const int64_t *q_strides, co
     if (p.few && p.nq == 1) hipLaunchKernelGGL((attn_few_kernel<T, DP, 1>), grid, dim3(64 * FewTile<T, DP>::NW), 0, s, a);
     else if (!p.few) {
       if constexpr (sizeof(T) == 2) {
-        if (fine_call(B, H, Lq, Lk, D)) {
+        if (fine_call(H, Lq, Lk, D)) {
           hipLaunchKernelGGL((attn_fwd_kernel<T, DP, true>), grid, dim3(256), 0, s, a);
           return;
         }
@@ -1351,7 +1353,7 @@ extern "C" int mlora_cross_attention_backward(const void *q, const int64_t *q_st
   ba.q_splits = (int32_t)p.splits, ba.q_split_tiles = (int32_t)p.split_tiles;
   const DqPlan qp = dq_plan(B, a.rows, Lk, Hk, f32);
   a.row_tiles = (int32_t)qp.row_tiles, a.splits = (int32_t)qp.splits, a.split_tiles = (int32_t)qp.split_tiles;
-  const bool fine = fine_call(B, H, Lq, Lk, D);
+  const bool fine = fine_call(H, Lq, Lk, D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (Lq > 0) {
     with_head(f32, D, [&](auto t, auto dp) {

@@ -108,3 +108,23 @@ def test_weights_add_up_to_one(pkg, dev, Lq, Lk, Hk):
     off, room = total(dv) - want, torch.maximum(high - want, want - low)
     rms = lambda t: float(t.square().mean().sqrt())  # noqa: E731
     assert rms(off) <= rms(room), (rms(off), rms(room), float(off.abs().max()))
+
+
+@pytest.mark.parametrize("B, Lq, Lk, H, Hk, D", [
+    (6, 512, 512, 8, 8, 128),
+    (40, 300, 700, 4, 2, 96),
+    (70, 2000, 130, 1, 1, 64),
+])
+def test_a_samples_gradients_do_not_depend_on_its_batch(pkg, dev, B, Lq, Lk, H, Hk, D):
+    """The first sample alone (below 2^30 products of scores and channels) and among others (beyond in all): as
+    exact as before. Both are the same values but for the order of float32 sums, so that their errors, squared and added up,
+    agree as closely as the errors of N values that are rounded alike."""
+    q, k, v, g = make(B, Lq, Lk, H, Hk, D, BF, dev, 29)
+    assert H * Lq * Lk * D <= 2 ** 30 < B * H * Lq * Lk * D
+    one = [t[:1] for t in (q, k, v, g)]
+    _, alone = run(pkg, *one)
+    _, among = run(pkg, q, k, v, g)
+    wanted = ref.attention(*one[:3], do=one[3])[1:4]
+    for name, a, b, want in zip(("dq", "dk", "dv"), alone, among, wanted):
+        x, y = (float((ref.f64(t[:1]) - want).norm() / want.norm()) for t in (a, b))
+        assert abs(x - y) <= x * 6 * 0.9 / math.sqrt(want.numel()), (name, x, y)
