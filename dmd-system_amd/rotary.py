@@ -28,17 +28,27 @@ def _fail(message: str) -> None:
     raise RuntimeError("rotary axes: " + message)
 
 
+def _whole(name: str, value) -> int:
+    try:
+        whole = int(value)
+    except (TypeError, ValueError, OverflowError, RuntimeError):
+        _fail(f"{name} must be whole numbers, got a {type(value).__name__}")
+    if whole != value:
+        _fail(f"{name} must be whole numbers")
+    return whole
+
+
 def grid_positions(grid_sizes, tokens: int, device=None, start=0) -> torch.Tensor:
-    """int32 [B, tokens, axes]: the coordinates of each sample's grid in row-major order from `start` (a
+    """int32 [B, tokens, axes]: the coordinates of each sample's grid in row-major order from `start` (a whole
     number, or one per axis). Tokens behind a sample's grid get the origin, where the rotation leaves
     them as they are.
 
     grid_sizes: [B, axes] as a tensor (the reference's ``grid_sizes``) or nested sequence."""
-    sizes = [[int(v) for v in row] for row in (grid_sizes.tolist() if isinstance(grid_sizes, torch.Tensor) else grid_sizes)]
+    sizes = [[_whole("grid_sizes", v) for v in row] for row in (grid_sizes.tolist() if isinstance(grid_sizes, torch.Tensor) else grid_sizes)]
     if not sizes or not sizes[0] or any(len(r) != len(sizes[0]) for r in sizes):
         _fail("grid_sizes must be [batch, axes]")
     axes = len(sizes[0])
-    first = [int(start)] * axes if not isinstance(start, (list, tuple)) else [int(v) for v in start]
+    first = [_whole("start", v) for v in (start if isinstance(start, (list, tuple)) else [start] * axes)]
     if len(first) != axes:
         _fail(f"start has {len(first)} values for {axes} axes")
     out = torch.zeros(len(sizes), tokens, axes, dtype=torch.int32)
@@ -47,6 +57,8 @@ def grid_positions(grid_sizes, tokens: int, device=None, start=0) -> torch.Tenso
         if min(row) < 0 or n > tokens:
             _fail(f"grid {row} does not fit {tokens} tokens")
         if n:
+            if min(first) < -2 ** 31 or any(f + s > 2 ** 31 for f, s in zip(first, row)):
+                _fail(f"grid {row} from start {first} leaves int32")
             grid = torch.meshgrid(*(torch.arange(f, f + s, dtype=torch.int32) for f, s in zip(first, row)), indexing="ij")
             out[b, :n] = torch.stack([g.reshape(-1) for g in grid], dim=1)
     return out.to(device) if device is not None else out
@@ -142,7 +154,7 @@ def _apply(xs, ws, names, positions, axis_dims, theta, pairing, eps):
         _fail("positions take no gradient")
     kernels.refuse_tangents((positions,))
     cfg = _plan(names, tuple([_meta(x) for x in xs]), tuple([_meta(w) for w in ws]), _meta(positions),
-                tuple([int(d) for d in axis_dims]), kernels.number("theta", theta, _fail), pairing,
+                tuple([d if type(d) is int else _whole("axis_dims", d) for d in axis_dims]), kernels.number("theta", theta, _fail), pairing,
                 kernels.number("eps", eps, _fail))
     if positions.dim() == 2:
         positions = positions.unsqueeze(0)

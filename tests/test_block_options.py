@@ -124,3 +124,24 @@ def test_forward_mode_numbers_are_refused(pkg, recorded):
         value = forward_ad.make_dual(torch.tensor(0.5), torch.tensor(1.0))
         with pytest.raises(RuntimeError, match="forward-mode"):
             pkg.cross_attention(heads(), heads(), heads(), scale=value)
+
+
+def test_grids_take_whole_numbers(pkg):
+    """A start between two positions (a clip at another rate) was cut to a whole one: positions are int32 here, and a
+    fractional start is refused; so is one whose grid leaves int32."""
+    assert pkg.grid_positions([[1, 2.0]], 2, start=(torch.tensor(3), 4.0))[0].tolist() == [[3, 4], [3, 5]]
+    for kw in (dict(start=0.5), dict(start=(0, 1.25)), dict(start=torch.tensor(0.5)), dict(start=float("nan")),
+               dict(start=2 ** 31 - 2), dict(start=(0, -2 ** 31 - 1)), dict(start="x")):
+        with pytest.raises(RuntimeError, match="start"):
+            pkg.grid_positions([[1, 4]], 5, **kw)
+    with pytest.raises(RuntimeError, match="grid_sizes"):
+        pkg.grid_positions([[1, 2.5]], 5)
+    assert pkg.grid_positions([[1, 2]], 2, start=2 ** 31 - 2)[0].tolist() == [[2 ** 31 - 2, 2 ** 31 - 2], [2 ** 31 - 2, 2 ** 31 - 1]]
+
+
+def test_axis_dims_are_whole_numbers(pkg, recorded):
+    pos = torch.zeros(3, 2, dtype=torch.int32)
+    pkg.rotary_axes(heads(), pos, (8.0, torch.tensor(8)))
+    assert recorded[-1]["axis_dims"] == (8, 8)
+    with pytest.raises(RuntimeError, match="axis_dims"):
+        pkg.rotary_axes(heads(), pos, (8.9, 8.9))
