@@ -902,8 +902,14 @@ def rotary_turns(axis_dims: tuple, theta: float):
     return turns, axis
 
 
+def _check_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> None:
+    """The checks' last: everything lies on one ROCm device."""
+    _require(first.is_cuda and all([t is None or t.device == first.device for t in tensors]),
+             "the tensors must be on one ROCm device")
+
+
 def _check_heads(name: str, t: torch.Tensor, dtype, lead) -> None:
-    _require(t.is_cuda and t.dtype == dtype, f"{name} must be a {dtype} device tensor")
+    _require(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
     _require(t.dim() == 4 and tuple(t.shape[:2]) == tuple(lead), f"{name} must be [{lead[0]}, {lead[1]}, heads, head_dim]")
     _require(rows_layout(t), f"{name} needs unit stride in the head and 16-byte aligned heads (strides multiples of 8)")
 
@@ -940,13 +946,9 @@ def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: 
     """The normed and rotated tensors (one or two [B, L, H_i, D] of one dtype), contiguous. checked: the caller
     has made the checks of layout and type."""
     first = xs[0]
-    B, L, _, D = first.shape
     if not checked:
-        for i, x in enumerate(xs):
-            _check_heads(f"tensor {i}", x, first.dtype, (B, L))
-            _require(x.shape[3] == D and x.shape[2] >= 1, "the tensors have heads of one head_dim")
-        _check_weights(weights, norm, first)
-        _check_positions(positions, B, L)
+        _check_rotary(xs, positions, axis_dims, norm, weights)
+    B, L, _, D = first.shape
     ys = [_new(x) for x in xs]
     if B * L == 0:
         return ys
@@ -960,18 +962,32 @@ def rotary_axes(xs: Sequence[torch.Tensor], positions: torch.Tensor, axis_dims: 
     return ys
 
 
-def _check_weights(weights, norm: int, x: torch.Tensor) -> None:
+def _check_rotary(xs, positions: torch.Tensor, axis_dims: tuple, norm: int, weights, gs=None) -> None:
+    first = xs[0]
+    _require(len(xs) in (1, 2) and first.dtype in _DT and first.dim() == 4,
+             "one or two bfloat16 or float32 tensors [batch, tokens, heads, head_dim]")
+    B, L, _, D = first.shape
+    for i, x in enumerate(xs):
+        _check_heads(f"tensor {i}", x, first.dtype, (B, L))
+        _require(x.shape[3] == D and x.shape[2] >= 1, "the tensors have heads of one head_dim")
+    _require(gs is None or len(gs) == len(xs), "a gradient for every tensor")
+    for i, g in enumerate(gs or ()):
+        _check_heads(f"gradient {i}", g, first.dtype, (B, L))
+        _require(g.shape == xs[i].shape, "a gradient has its tensor's shape")
+    _require(sum(axis_dims) == D and all([d >= 0 and d % 2 == 0 for d in axis_dims]),
+             f"axis_dims must be even and add up to {D}, got {axis_dims}")
     _require(norm in (NORM_NONE, NORM_HEAD, NORM_ROW), "norm is NORM_NONE, NORM_HEAD or NORM_ROW")
-    for w in weights if norm else ():
-        _require(w is not None and w.is_cuda and w.dtype in _DT and w.dtype == weights[0].dtype and w.dim() == 1
-                 and rows_layout(w), "norm weights must be 16-byte aligned contiguous device vectors of one dtype")
-
-
-def _check_positions(positions: torch.Tensor, B: int, L: int) -> None:
-    _require(positions.is_cuda and positions.dtype in _POS_TYPES, "positions must be an int32, int64 or float32 device tensor")
-    _require(positions.dim() == 3 and positions.shape[0] in (1, B) and positions.shape[1] == L
-             and positions.shape[2] >= 1 and (positions.stride(2) == 1 or positions.shape[2] == 1),
-             f"positions must be [{B} or 1, {L}, axes] with unit axis stride")
+    if norm:
+        _require(len(weights) == len(xs), "a norm weight for every tensor")
+        for x, w in zip(xs, weights):
+            _require(w is not None and w.dtype in _DT and w.dtype == weights[0].dtype and rows_layout(w)
+                     and tuple(w.shape) == (D if norm == NORM_HEAD else x.shape[2] * D,),
+                     "norm weights must be 16-byte aligned contiguous vectors of one dtype, of a head's or the row's width")
+    _require(positions.dtype in _POS_TYPES, "positions must be int32, int64 or float32")
+    _require(positions.dim() == 3 and positions.shape[0] in (1, B) and tuple(positions.shape[1:]) == (L, len(axis_dims))
+             and (positions.stride(2) == 1 or positions.shape[2] == 1),
+             f"positions must be [{B} or 1, {L}, {len(axis_dims)}] with unit axis stride")
+    _check_device(*xs, *(gs or ()), positions, *(weights if norm else ()))
 
 
 def rotary_axes_backward(xs: Sequence[torch.Tensor] | None, gs: Sequence[torch.Tensor], positions: torch.Tensor,
@@ -980,15 +996,10 @@ def rotary_axes_backward(xs: Sequence[torch.Tensor] | None, gs: Sequence[torch.T
                          want_dw: Sequence[bool], checked: bool = False) -> tuple[list, list]:
     """(dx, dw) lists of rotary_axes; None where not wanted."""
     first = gs[0]
-    B, L, _, D = first.shape
     if not checked:
-        for i, g in enumerate(gs):
-            _check_heads(f"gradient {i}", g, first.dtype, (B, L))
-            if norm:
-                _check_heads(f"tensor {i}", xs[i], first.dtype, (B, L))
-                _require(xs[i].shape == g.shape, "a gradient has its tensor's shape")
-        _check_weights(weights, norm, first)
-        _check_positions(positions, B, L)
+        _check_rotary(xs if norm else gs, positions, axis_dims, norm, weights, gs)
+        _require(len(want_dx) == len(gs) and len(want_dw) == (len(gs) if norm else 0), "a wish for every gradient")
+    B, L, _, D = first.shape
     dev = first.device
     dxs = [_new(g) if w else None for g, w in zip(gs, want_dx)]
     dws = [_new(w) if k else None for w, k in zip(weights, want_dw)]
@@ -1022,16 +1033,18 @@ def _vec(v: torch.Tensor | None) -> tuple:
 
 
 def _check_joint(x, y, gate, scale, shift, post_w, norm, post) -> None:
+    _require(x.dim() == 3, "x must be [batch, tokens, width]")
     B, T, W = x.shape
     for name, t in (("x", x), ("y", y)):
-        _require(t.is_cuda and t.dtype in _DT and tuple(t.shape) == (B, T, W) and rows_layout(t),
-                 f"{name} must be a bfloat16 or float32 [{B}, {T}, {W}] device tensor with 16-byte aligned rows")
+        _require(t.dtype in _DT and tuple(t.shape) == (B, T, W) and rows_layout(t),
+                 f"{name} must be bfloat16 or float32 [{B}, {T}, {W}] with 16-byte aligned rows")
     for name, v in (("gate", gate), ("scale", scale), ("shift", shift), ("post weight", post_w)):
-        _require(v is None or (v.is_cuda and v.dtype in _DT and vector_layout(v, B, W) and rows_layout(v)),
-                 f"{name} must be a bfloat16 or float32 device vector [{W}], [{B}, {W}] or [{B}, 1, {W}], 16-byte aligned")
+        _require(v is None or (v.dtype in _DT and vector_layout(v, B, W) and rows_layout(v)),
+                 f"{name} must be a bfloat16 or float32 vector [{W}], [{B}, {W}] or [{B}, 1, {W}], 16-byte aligned")
     _require(post_w is None or post_w.numel() == W, "the post weight is shared by the samples")
     _require(scale is None or shift is None or scale.dtype == shift.dtype, "scale and shift share a dtype")
     _require(norm in NORM_KINDS and (post is None or post in NORM_KINDS), "norm and post are 'layer' or 'rms'")
+    _check_device(x, y, gate, scale, shift, post_w)
 
 
 def _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps):
@@ -1067,8 +1080,9 @@ def joint_backward(x: torch.Tensor, y: torch.Tensor, gx: torch.Tensor | None, go
     if not checked:
         _check_joint(x, y, gate, scale, shift, post_w, norm, post)
         for name, t, like in (("gx", gx, x), ("go", go, y)):
-            _require(t is None or (t.is_cuda and t.dtype == like.dtype and t.shape == x.shape and rows_layout(t)),
+            _require(t is None or (t.dtype == like.dtype and t.shape == x.shape and rows_layout(t)),
                      f"{name} must have its output's shape and dtype, with 16-byte aligned rows")
+        _check_device(x, gx, go)
     B, T, W = x.shape
     head, tail = _joint_args(x, y, gate, scale, shift, post_w, norm, post, unit_offset, alpha, eps)
     outs = [_new(t) if w else None for t, w in zip((x, y, gate, scale, shift, post_w), want)]
@@ -1093,19 +1107,21 @@ def attention_layout(t: torch.Tensor) -> bool:
 
 
 def _check_attention(q, k, v, key_lengths, key_mask) -> None:
+    _require(q.dim() == 4 and k.dim() == 4, "q, k and v must be [batch, tokens, heads, head_dim]")
     B, Lq, H, D = q.shape
     Lk, Hk = k.shape[1:3]
     for name, t, shape in (("q", q, (B, Lq, H, D)), ("k", k, (B, Lk, Hk, D)), ("v", v, (B, Lk, Hk, D))):
-        _require(t.is_cuda and t.dtype == q.dtype and t.dtype in _DT and tuple(t.shape) == shape and attention_layout(t),
-                 f"{name} must be a [batch, tokens, heads, head_dim] device tensor of q's dtype with 16-byte aligned heads "
-                 f"and a token stride below {ATTENTION_MAX_STRIDE}")
-    _require(key_lengths is None or (key_lengths.is_cuda and key_lengths.dtype == torch.int32
-                                     and tuple(key_lengths.shape) == (B,) and key_lengths.is_contiguous()),
-             f"key_lengths must be a contiguous int32 device vector of {B}")
-    _require(key_mask is None or (key_mask.is_cuda and key_mask.dtype == torch.bool and key_mask.dim() == 2
+        _require(t.dtype == q.dtype and t.dtype in _DT and tuple(t.shape) == shape and attention_layout(t),
+                 f"{name} must be [batch, tokens, heads, head_dim] of q's dtype with 16-byte aligned heads and a token stride "
+                 f"below {ATTENTION_MAX_STRIDE}")
+    _require(key_lengths is None or (key_lengths.dtype == torch.int32 and tuple(key_lengths.shape) == (B,)
+                                     and key_lengths.is_contiguous()),
+             f"key_lengths must be a contiguous int32 vector of {B}")
+    _require(key_mask is None or (key_mask.dtype == torch.bool and key_mask.dim() == 2
                                   and key_mask.shape[0] in (1, B) and key_mask.shape[1] == Lk
                                   and (key_mask.stride(1) == 1 or Lk < 2)),
-             f"key_mask must be a bool device tensor [{B} or 1, {Lk}] with unit stride")
+             f"key_mask must be bool [{B} or 1, {Lk}] with unit stride")
+    _check_device(q, k, v, key_lengths, key_mask)
 
 
 def _attention_args(q, k, v, key_lengths, key_mask, scale):
@@ -1141,10 +1157,11 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     if not checked:
         _check_attention(q, k, v, key_lengths, key_mask)
         for name, t in (("out", out), ("g", g)):
-            _require(t.is_cuda and t.dtype == q.dtype and t.shape == q.shape, f"{name} must have q's shape and dtype")
+            _require(t.dtype == q.dtype and t.shape == q.shape, f"{name} must have q's shape and dtype")
         _require(out.is_contiguous() and attention_layout(g), "out is contiguous, g's heads are 16-byte aligned")
         _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == q.shape[0] * q.shape[1] * q.shape[2],
                  "lse is the forward's [batch, heads, tokens]")
+        _check_device(q, out, lse, g)
     args, sizes = _attention_args(q, k, v, key_lengths, key_mask, scale)
     dq, dk, dv = _new(q), _new(k), _new(v)
     nbytes = _bytes("mlora_cross_attention_backward_workspace_bytes", _DT[q.dtype], *sizes)
