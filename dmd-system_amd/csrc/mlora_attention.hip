@@ -20,10 +20,13 @@
 //
 // What bounds it, bf16 with 128 channels: a 32 x 32 block of scores costs the SIMD's matrix core 16 products of
 // 32 cycles and its vector unit about as many cycles (16 exp2 at a quarter of the rate, the maximum, fma, packing);
-// the two waves of a SIMD overlap the two only in part. Counters at 2 x 32760 rows x 512 keys, 12 heads: matrix
-// cores busy 34 % of the cycles, no LDS bank conflict. Measured there: forward 273 us (755 TFLOP/s), dq 382 (810),
-// dk / dv 420 (980); forward at 4096 keys 990 TFLOP/s, dq 1140. Few rows are bound by reading K and V: 48 rows per
-// key head x 65520 keys, 8 key heads, 268 MB: 50 us, 5.4 TB/s, and 5 us for the join of its 32 splits.
+// the two waves of a SIMD overlap the two only in part. dk / dv has fewer vector instructions per product (4.3; forward 7.6,
+// dq 6.8) but two LDS reads (1.5, 1.3), since every fragment it reads feeds one product, and it spills six registers. Counters at
+// 2 x 32760 rows x 512 keys, 12 heads: matrix cores busy 34 % of the cycles forward, 37 % in dq, 46 % in dk / dv, no
+// LDS bank conflict. Measured there, averages of 20 calls (minima): forward 302 us (275; 680 TFLOP/s), dq 425 (392;
+// 730), dk / dv 470 (424; 880). 16380 rows x 4096 keys: forward 433 us (950), dq 562 (1100). Few rows are bound by
+// reading K and V: 48 rows per key head x 65520 keys, 8 key heads, 268 MB: 52 us, 5.1 TB/s, and 5 us for the join of
+// its 32 splits.
 #include "mlora_attention.h"
 
 namespace mlora {
@@ -1072,7 +1075,7 @@ struct AttnPlan {
 
 // Row tiles per workgroup: up to 4 where few key tiles leave a workgroup mostly waiting for its first loads and
 // at least 1024 workgroups (two for every place) remain. 2 x 32760 rows of 12 heads of 128: 512 keys 285 us with
-// one, 263 with four; 64 keys 141 and 120; 1024 keys 494 and 451; at 4096 keys one row's tile is best (819, 909).
+// one, 263 with four; 64 keys 141 and 120; 1024 keys 494 and 451; at 4096 keys one row's tile is best (819, 909; minima).
 static int64_t row_turns(int64_t tiles, int64_t key_tiles) {
   const int64_t most = key_tiles <= 16 ? 4 : 1, turns = tiles / 1024;
   return turns < 1 ? 1 : turns > most ? most : turns;
@@ -1081,7 +1084,10 @@ static int64_t row_turns(int64_t tiles, int64_t key_tiles) {
 // How a forward is cut: few rows per key head run waves over different keys, more rows 128 per workgroup;
 // the keys are split where that leaves less than a workgroup for every compute unit and there are enough of them:
 // a float32 tile takes about as long as a join, a bf16 tile a sixth of it (2 x 64 rows x 512 keys, 12 heads of 128,
-// float32: 47 us where a split takes 8 tiles at least, 31 with 4, 23 with 2; bf16 14.7, 16.3 and 15.6).
+// float32: 47 us where a split takes 8 tiles at least, 31 with 4, 23 with 2; bf16 14.7, 16.3 and 15.6). 129 to 255
+// workgroups stay whole, and a second place per compute unit, which bf16 and float32 up to 64 channels have, is not
+// counted: one frame of 1560 rows, 12 heads of 128, is 156 workgroups (9360 keys 245 us, 62 at the matrix cores' rate;
+// 32760 keys 799 and 217).
 static AttnPlan attn_plan(int64_t batches, int64_t rows, int64_t Lk, int64_t Hk, int64_t D, bool f32) {
   AttnPlan p{};
   p.few = rows <= (f32 && D > 64 ? 32 : 64);

@@ -17,7 +17,8 @@
 // 12 heads of 128).
 //
 // HBM-bound: 2 x 32760 tokens, q and k of 12 heads of 128, bf16, normed over the row: forward 181 us for 805 MB
-// (4.4 TB/s), backward 291 for 1208 MB (4.2 TB/s); one frame of 1560 tokens 10 us.
+// (4.4 TB/s), backward 291 for 1208 MB (4.2 TB/s); one frame of 1560 tokens 10 us for 19 MB: a row per wave, whose loads,
+// sum, angles and stores wait for each other, of which a launch is 3 to 4.
 //
 // A unit is 8 pairs (16 values: two 16-byte loads of bf16): chunks 2j and 2j + 1 of a head, or chunks j and
 // j + D/16 where halves are paired. WPR waves hold a row's units, NU per lane; a wave writes
