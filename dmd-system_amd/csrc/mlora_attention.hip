@@ -43,6 +43,18 @@ struct AttnArgs {
   float c;            // scale · log2 e
 };
 
+// How many of 16 mask bytes are set, without the first `skip`.
+typedef uint32_t unaligned_u4 __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ int live_bytes(const u32x4 &v, int skip) {
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t set = (((v[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v[j]) & 0x80808080u;  // a byte's top bit: it is not 0
+    n += __popc(set & (uint32_t)(0xffffffffull << (8 * min(max(skip - 4 * j, 0), 4))));
+  }
+  return n;
+}
+
 // A sample's live keys, 64 (or KT) at a time.
 template <int KT>
 struct KeyMask {
@@ -685,23 +697,33 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void attn_dq_k
   // keys: 1.4e-3 to 4e-3 of dq and dk, as much and more than the gradients' own). Then x and delta are measured too. From
   // 65 keys on delta's share is below a third of that. The keys are counted up to there, with length and mask; lane i
   // keeps the i-th tile that has one. The measuring takes 2 us of a small backward (2 x 1560 rows, 12 heads of 128, 5 of 512
-  // keys: 52 -> 54 us); its presence costs dq 3 % where it does not run but tiles are few (2 x 32760 x 512: 383 -> 395).
+  // keys: 52 -> 54 us) and 2 per tile where the keys lie far apart (40 of 65520, 16 rows, 24 heads on 8: 124 -> 241); its
+  // presence costs dq 3 % where it does not run but tiles are few (2 x 32760 x 512: 383 -> 395).
   int live = 0, live_tiles = 0, list = 0;
   if constexpr (sizeof(T) == 2) {
     if (mask == nullptr || keys <= KT) {
       live = keys, live_tiles = 1;
     } else {
-      constexpr int kAtOnce = 8;
-      for (int k0 = 0; k0 < keys && live <= KT; k0 += kAtOnce * KT) {
-        uint8_t byte[kAtOnce];
+      // 16 keys per lane and load, unaligned; the row's last load begins at keys − 16 and leaves out what came before
+      constexpr int kAtOnce = 4;
+      for (int k0 = 0; k0 < keys && live <= KT; k0 += kAtOnce * 1024) {
+        u32x4 bytes[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) byte[j] = mask[min(k0 + j * KT + lane, keys - 1)];
+        for (int j = 0; j < kAtOnce; ++j) bytes[j] = *(const unaligned_u4 *)(mask + min(k0 + 1024 * j + 16 * lane, keys - 16));
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          const uint64_t on = __ballot(byte[j] != 0) & low_bits(keys - k0 - j * KT);
+          const int key = k0 + 1024 * j + 16 * lane;
+          const int n = live_bytes(bytes[j], max(key - (keys - 16), 0));
+          const uint64_t on = __ballot(n != 0);
           if (on == 0) continue;
-          if (lane == live_tiles) list = k0 / KT + j;
-          ++live_tiles, live += __popcll(on);
+#pragma unroll
+          for (int bit = 0; bit < 5; ++bit) live += __popcll(__ballot((n >> bit) & 1)) << bit;
+          if (live > KT) break;
+          for (int t = 0; t < 16; ++t)  // four lanes hold a tile
+            if ((on >> (4 * t)) & 15) {
+              if (lane == live_tiles) list = k0 / KT + 16 * j + t;
+              ++live_tiles;
+            }
         }
       }
     }

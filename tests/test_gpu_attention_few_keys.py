@@ -128,3 +128,36 @@ def test_a_samples_gradients_do_not_depend_on_its_batch(pkg, dev, B, Lq, Lk, H, 
     for name, a, b, want in zip(("dq", "dk", "dv"), alone, among, wanted):
         x, y = (float((ref.f64(t[:1]) - want).norm() / want.norm()) for t in (a, b))
         assert abs(x - y) <= x * 6 * 0.9 / math.sqrt(want.numel()), (name, x, y)
+
+
+@pytest.mark.parametrize("Lk", [65, 79, 80, 81, 1023, 1025, 4097, 9001])
+@pytest.mark.parametrize("n", [1, 20, 64])
+def test_few_keys_of_masks_at_any_address(pkg, dev, Lk, n):
+    """Rows of a mask that begin at any byte, live keys at both ends, and set bytes behind the row's end and behind the
+    sample's length, which do not count: as exact as the same keys by themselves."""
+    B, Lq, H, D = 3, 33, 2, 64
+    q, k, v, g = make(B, Lq, Lk, H, H, D, BF, dev, Lk + n)
+    gen = torch.Generator().manual_seed(Lk)
+    wide = torch.ones(B, Lk + 5, dtype=torch.bool)
+    mask = wide[:, 3:3 + Lk]
+    mask[:] = False
+    lengths = torch.tensor([Lk, Lk - 1, Lk], dtype=torch.int32)
+    for b in range(B):
+        end = int(lengths[b])
+        mask[b, torch.randperm(end - 1, generator=gen)[:n - 1]] = True
+        mask[b, end - 1] = True
+        mask[b, end:] = True
+    kw = dict(key_lengths=lengths.to(dev), key_mask=wide.to(dev)[:, 3:3 + Lk])
+    assert kw["key_mask"].stride(0) == Lk + 5
+    _, grads = run(pkg, q, k, v, g, **kw)
+    live = live_keys(B, Lk, lengths, mask)
+    assert live.sum(1).tolist() == [n] * B
+    if n > 1:
+        only_rounded(q, k, v, g, grads, live)
+    else:  # a lone key: dq and dk are zero in mathematics, and dv the sum of do with weights off by 2^-18 at most (the logarithm's
+        # rounding, scores below 2^6, and the sum of 33 rows)
+        want, g64 = ref.attention(q, k, v, live=live, do=g)[3], ref.f64(g)
+        room = ref.half_step(BF) * want.abs() + 2 ** -18 * g64.abs().sum(1, keepdim=True)
+        assert ((ref.f64(grads[2]) - want).abs() <= room).all()
+    for d in grads[1:]:
+        assert d[~live.to(dev)].abs().sum() == 0
