@@ -37,12 +37,30 @@ SCORES = {"5*2^34": (5 * 2.0 ** 14, 2.0 ** 15), "-5*2^34": (-5 * 2.0 ** 14, 2.0 
     (130, 2500, "lengths"),  # the keys of the forward and of dq split
 ])
 def test_equal_scores_of_any_size(pkg, dev, Lq, Lk, keys, score, dtype):
-    B, H, D = 2, 2, 32
+    equal_scores(pkg, dev, Lq, Lk, keys, score, dtype, 2, 2, 32)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("score", ["-5*2^34", "3*2^28", "3*2^9"])
+@pytest.mark.parametrize("Lq, Lk, keys, H, Hk, D", [
+    (2, 40, "all", 4, 2, 128),        # few rows and keys
+    (40, 900, "mask", 2, 2, 128),
+    (150, 100, "lengths", 3, 1, 128),  # one tile of query rows ends within a head
+    (150, 300, "mask", 2, 2, 72),
+    (2600, 140, "all", 1, 1, 128),     # ... the rows of dk and dv split
+    (90, 60, "lengths", 2, 1, 104),    # at most 64 keys
+])
+def test_equal_scores_of_wide_heads(pkg, dev, Lq, Lk, keys, H, Hk, D, score, dtype):
+    equal_scores(pkg, dev, Lq, Lk, keys, score, dtype, H, Hk, D)
+
+
+def equal_scores(pkg, dev, Lq, Lk, keys, score, dtype, H, Hk, D):
+    B, G = 2, H // Hk
     gen = torch.Generator().manual_seed(Lq + Lk)
     r = lambda *s: torch.randn(*s, generator=gen).to(dtype)  # noqa: E731
     qe, ke = SCORES[score]
-    q, k = torch.full((B, Lq, H, D), qe, dtype=dtype), torch.full((B, Lk, H, D), ke, dtype=dtype)
-    v, g = r(B, Lk, H, D), r(B, Lq, H, D)
+    q, k = torch.full((B, Lq, H, D), qe, dtype=dtype), torch.full((B, Lk, Hk, D), ke, dtype=dtype)
+    v, g = r(B, Lk, Hk, D), r(B, Lq, H, D)
     live = torch.ones(B, Lk, dtype=torch.bool)
     kw = {}
     if keys == "mask":
@@ -60,16 +78,18 @@ def test_equal_scores_of_any_size(pkg, dev, Lq, Lk, keys, score, dtype):
     n = live.sum(1).view(B, 1, 1, 1)
     on = live.view(B, Lk, 1, 1).double()
     v64, g64 = ref.f64(v) * on, ref.f64(g)
-    mean = v64.abs().sum(1, keepdim=True) / n
+    wide = lambda t: t.repeat_interleave(G, dim=2)  # noqa: E731
+    fold = lambda t, dim: t.unflatten(dim, (Hk, G)).sum(dim + 1)  # noqa: E731
+    mean = wide(v64.abs().sum(1, keepdim=True) / n)
     assert ((ref.f64(out) - want).abs() <= u * want.abs() + (e + Lk * 2 ** -24) * mean).all()
-    share = on * g64.abs().sum(1, keepdim=True) / n  # what dv adds up
-    assert ((grads[2] - dv).abs() <= u * dv.abs() + (e + Lq * 2 ** -24) * share).all()
+    share = on * fold(g64.abs().sum(1, keepdim=True), 2) / n  # what dv adds up
+    assert ((grads[2] - dv).abs() <= u * dv.abs() + (e + G * Lq * 2 ** -24) * share).all()
     # dS of row i and key j: at most (|do| |v| + |do| mean |v|) / n off by these shares
     off = e + 2 * D * 2 ** -24 + (u if dtype is BF else 0)
-    size = (torch.einsum("bqhd,bkhd->bhqk", g64.abs(), v64.abs()) + (g64.abs() * mean).sum(-1).transpose(1, 2).unsqueeze(-1)) / n
+    size = (torch.einsum("bqhd,bkhd->bhqk", g64.abs(), wide(v64.abs())) + (g64.abs() * mean).sum(-1).transpose(1, 2).unsqueeze(-1)) / n
     size = size * on.view(B, 1, 1, Lk)
-    room_k = size.sum(2).transpose(1, 2).unsqueeze(-1) * abs(qe)
-    assert ((grads[1] - dk).abs() <= u * dk.abs() + (off + Lq * 2 ** -24) * room_k).all()
+    room_k = fold(size.sum(2), 1).transpose(1, 2).unsqueeze(-1) * abs(qe)
+    assert ((grads[1] - dk).abs() <= u * dk.abs() + (off + G * Lq * 2 ** -24) * room_k).all()
     room_q = size.sum(3).transpose(1, 2).unsqueeze(-1) * abs(ke)
     assert (grads[0].abs() <= (off + Lk * 2 ** -24) * room_q * (1 + 2 * u)).all()
 
@@ -133,3 +153,40 @@ def test_a_scale_whose_base_two_form_overflows_is_refused(pkg, dev):
     with pytest.raises(RuntimeError):
         pkg.cross_attention(q, q, q, scale=3e38)
     assert math.isfinite(float(pkg.cross_attention(q, q, q, scale=2e38).sum()))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_far_and_few_in_a_captured_graph(pkg, dev, dtype):
+    """One capture replayed with scores near and far from zero and with many, few and no live keys: what the backward measures
+    is decided on the device, and every replay equals the eager call."""
+    B, Lq, Lk, H, D = 2, 140, 300, 2, 64
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(len(s))).to(dtype).to(dev)  # noqa: E731
+    q, k, v, g = r(B, Lq, H, D), r(B, Lk, H, D), r(B, Lk, H, D), r(B, Lq, H, D)
+    mask = torch.ones(B, Lk, dtype=torch.bool, device=dev)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+
+    def step():
+        out = pkg.cross_attention(q, k, v, key_mask=mask, scale=1.0)
+        return [out.detach(), *torch.autograd.grad(out, [q, k, v], [g])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for turn, (size, keep) in enumerate(((1.0, 0.8), (2.0 ** 30, 0.8), (1.0, 0.02), (2.0 ** 30, 0.02), (1.0, 0.0), (2.0, 0.9))):
+        gen = torch.Generator().manual_seed(turn)
+        with torch.no_grad():
+            for t in (q, k, v, g):
+                t.copy_(torch.randn(t.shape, generator=gen))
+            q.mul_(size)
+            mask.copy_(torch.rand(B, Lk, generator=gen) < keep)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b) and torch.isfinite(a).all()
