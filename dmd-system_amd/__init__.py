@@ -22,6 +22,8 @@ Public API:
     ModulatedLayerNormFunction, modulated_layer_norm   the same as one autograd op
     rotary_axes, rotary_axes_qk, grid_positions, RotaryAxesFunction   rotary positions with several axes, q / k norms
     cross_attention, CrossAttentionFunction   attention to an encoder's states of another length
+    window_attention, prefix_attention, PastAttentionFunction   attention of a stream's tokens to their own past: a sliding
+        window with sinks, a prefix that samples share
     gated_residual_norm, GatedResidualNormFunction   the joint of two sublayers: norm after, gate, residual, norm before
     load_library()                       load libmlora.so (raises if missing)
 
@@ -50,6 +52,7 @@ from .modulated_norm import (ModulatedLayerNormFunction, fused_bf16_layernorm_mo
                              fused_tensor4d_component_gradient, modulated_layer_norm)
 from .rotary import RotaryAxesFunction, grid_positions, rotary_axes, rotary_axes_qk
 from .attention import CrossAttentionFunction, cross_attention
+from .past_attention import PastAttentionFunction, prefix_attention, window_attention
 from .joint import GatedResidualNormFunction, gated_residual_norm
 
 
@@ -73,4 +76,5 @@ __all__ = [
     "fused_tensor4d_component_gradient", "ModulatedLayerNormFunction", "modulated_layer_norm",
     "RotaryAxesFunction", "grid_positions", "rotary_axes", "rotary_axes_qk", "GatedResidualNormFunction",
     "gated_residual_norm", "CrossAttentionFunction", "cross_attention",
+    "PastAttentionFunction", "prefix_attention", "window_attention",
 ]

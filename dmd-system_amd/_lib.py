@@ -34,6 +34,17 @@ _pf32 = ctypes.POINTER(ctypes.c_float)
 _pf64 = ctypes.POINTER(ctypes.c_double)
 _f32 = ctypes.c_float
 
+
+class PastShape(ctypes.Structure):
+    """``mlora_past_shape``: the sizes and options of an attention of tokens to their own past."""
+    _fields_ = [("dtype", _i32), ("from_end", _i32),
+                *[(name, _i64) for name in ("B", "Lq", "Lk", "H", "Hk", "D", "groups", "Lp", "window", "sinks", "chunk", "first")],
+                *[(name, _i64 * 3) for name in ("q_strides", "k_strides", "v_strides", "pk_strides", "pv_strides")],
+                ("scale", _f32)]
+
+
+_pshape = ctypes.POINTER(PastShape)
+
 SIGNATURES = {
     "mlora_abi_version": (_int, []),
     "mlora_status_string": (ctypes.c_char_p, [_int]),
@@ -110,6 +121,10 @@ SIGNATURES = {
     "mlora_cross_attention_backward": (_int, [_vp, _pi64, _vp, _pi64, _vp, _pi64, _int, _vp, _vp, _i64, _f32, _vp, _vp,
                                               _vp, _pi64, _vp, _vp, _vp, _vp, _i64,
                                               _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "mlora_past_attention_workspace_bytes": (_i64, [_pshape]),
+    "mlora_past_attention": (_int, [_pshape, *[_vp] * 8, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mlora_past_attention_backward_workspace_bytes": (_i64, [_pshape]),
+    "mlora_past_attention_backward": (_int, [_pshape, *[_vp] * 8, _vp, _vp, _vp, _vp, _pi64, *[_vp] * 5, _vp, _i64, _vp]),
 }
 
 _LIB = None

@@ -194,4 +194,233 @@ __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 8 elements at base + off, or zeros (base itself is always readable: no branch around the load).
+__device__ __forceinline__ void load_frag(const uint16_t *base, int64_t off, bool on, Frag<uint16_t> &f) {
+  const u32x4 v = *(const MLORA_GLOBAL u32x4 *)(base + (on ? off : 0));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f.v[j] = on ? v[j] : 0;
+}
+__device__ __forceinline__ void load_frag(const float *base, int64_t off, bool on, Frag<float> &f) {
+  const float *p = base + (on ? off : 0);
+  const f32x4 a = *(const MLORA_GLOBAL f32x4 *)p, b = *(const MLORA_GLOBAL f32x4 *)(p + 4);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f.v[j] = on ? a[j] : 0.f, f.v[j + 4] = on ? b[j] : 0.f;
+}
+
+// The running maximum before any key: below every other score, but finite, so that 2^(−inf − m) is 0 and not NaN where
+// a block has no live key.
+constexpr float kNoMax = -3.4028234664e38f;
+
+// What a row's exponents are relative to: P = 2^((s − a)·c − r), a function of the row's largest product m alone. Near
+// zero a = 0 and r = m·c rounded, off by 2^-15 at most, the same for the whole row; far from zero a = m and r = 0, since
+// the rounding of m·c would grow with it and end in 2^128 or 0 (at |m·c| of 3e9).
+struct RowRef {
+  float a, r;
+};
+constexpr float kFar = 1024.f;
+__device__ __forceinline__ RowRef row_ref(float m, float c) {
+  const float mc = m * c;
+  const bool far = !(fabsf(mc) < kFar);
+  return {far ? m : 0.f, far ? 0.f : mc};
+}
+// 2^(x − y): what sums relative to x become relative to y.
+__device__ __forceinline__ float ref_factor(const RowRef &x, const RowRef &y, float c) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x.a - y.a, c, x.r - y.r));
+}
+// The logarithm of a row's sum l relative to row_ref(m): +inf without keys, finite for finite scores.
+__device__ __forceinline__ float row_lse(float m, float l, float c) {
+  const float mc = fminf(fmaxf(m * c, kNoMax), -kNoMax);
+  return l > 0.f ? mc + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+}
+
+// The running softmax of NQ x 32 queries (a column per lane and half) against KT keys per step. EXACT: e sums the weights
+// before their rounding to bf16, for lse: the backward forms them unrounded, and where a row rests on few keys the two sums
+// are up to half a bf16 step apart (a factor of all of its gradients). 16 additions more per 32 x 32 block; l is e elsewhere.
+template <class T, int DP, int NQ, int KT, bool EXACT>
+struct Softmax {
+  static constexpr bool kTwoSums = EXACT && sizeof(T) == 2;
+  f32x16 o[NQ][DP / 32];
+  Frag<T> q[NQ][DP / 16];
+  float m[NQ], l[NQ], e[NQ];  // the largest product so far, the sums relative to row_ref(m)
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      m[n] = kNoMax, l[n] = 0.f, e[n] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][d][i] = 0.f;
+    }
+  }
+
+  // One tile of keys KOFF bytes from the reader's base, V at VOFF. bits: the keys that count, the same for every lane; or
+  // (`masked` then says whether any query lacks one) those of the lane's queries.
+  template <int KOFF, int VOFF>
+  __device__ __forceinline__ void step(const FragReader<T, DP> &fr, uint64_t bits, float c, int lane) {
+    uint64_t all[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) all[n] = bits;
+    step<KOFF, VOFF>(fr, bits != low_bits(KT), all, c, lane);
+  }
+  template <int KOFF, int VOFF>
+  __device__ __forceinline__ void step(const FragReader<T, DP> &fr, bool masked, const uint64_t (&bits)[NQ], float c, int lane) {
+    constexpr int NB = KT / 32;
+    f32x16 s[NQ][NB];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][kb][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)  // the blocks' sums in turn: a sum waits for its last product
+      static_for<NB>([&](auto kb) __attribute__((always_inline)) {
+        Frag<T> kf;
+        fr.template rows<KOFF, 32 * decltype(kb)::value>(ks, kf);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][kb] = mma16(kf, q[n][ks], s[n][kb]);
+        return true;
+      });
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const uint64_t mine = bits[n] >> (4 * (lane >> 5));
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[n][kb][i] = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1 ? s[n][kb][i] : -INFINITY;
+      }
+    }
+    Frag<T> p[NQ][KT / 16];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float mx = s[n][0][0];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][kb][i]);
+      mx = half_max(mx);
+      RowRef ref = row_ref(m[n], c);
+      if (__any(__builtin_fmaf(mx - ref.a, c, -ref.r) > 8.f)) {
+        m[n] = fmaxf(m[n], mx);
+        const RowRef up = row_ref(m[n], c);
+        const float f = ref_factor(ref, up, c);
+        ref = up;
+        l[n] *= f, e[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[n][d][i] *= f;
+      }
+      if (__any(ref.a != 0.f)) {
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[n][kb][i] -= ref.a;
+      }
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][i], c, -ref.r));
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) to_frag(s[n][kb], ks, p[n][2 * kb + ks]);
+        if constexpr (kTwoSums) {
+          float t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = (s[n][kb][i] + s[n][kb][4 + i]) + (s[n][kb][8 + i] + s[n][kb][12 + i]);
+          e[n] += (t[0] + t[1]) + (t[2] + t[3]);
+        }
+      }
+      l[n] += frag_sum(p[n]);
+    }
+    static_for<KT / 16>([&](auto ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        Frag<T> vf;
+        fr.template cols<VOFF, 16 * decltype(ks)::value>(d, vf);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][d] = mma16(vf, p[n][ks], o[n][d]);
+      }
+      return true;
+    });
+  }
+
+  // The row's whole sums over both halves; f: what makes O a sum of weights that add up to e where they added up to l.
+  __device__ __forceinline__ float sums(int n, float &f) {
+    const float lw = half_sum(l[n]);
+    f = 1.f;
+    if constexpr (!kTwoSums) return lw;
+    const float ew = half_sum(e[n]);
+    if (lw > 0.f) f = ew / lw;
+    return lw > 0.f ? ew : lw;
+  }
+
+  // The sum of the weights as the product with V sees them (bf16: two per v_dot2_f32_bf16 with ones).
+  static __device__ __forceinline__ float frag_sum(const Frag<T> (&p)[KT / 16]) {
+    float t = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KT / 16; ++ks) {
+      if constexpr (sizeof(T) == 2) {
+        const auto ones = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)p[ks].v[j]), ones, t, false);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t += p[ks].v[j];
+      }
+    }
+    return t;
+  }
+};
+
+// Writes NQ x 32 rows of the O^T registers (times f[n]) to base, row r at element at_row(r) of it. The halves of a column hold alternating groups of
+// four channels; they swap groups, so that a lane has eight neighbouring channels: one 16-byte store of bf16.
+template <class T, int DP, int NQ, class At>
+__device__ __forceinline__ void store_rows(T *base, const f32x16 (&o)[NQ][DP / 32], const float (&f)[NQ], int row0, int rows,
+                                           At &&at_row, int D, int lane) {
+  auto swap = [](uint32_t &x, uint32_t &y) __attribute__((always_inline)) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0], y = r[1];
+  };
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = row0 + 32 * n + (lane & 31);
+    T *p = base + at_row(min(r, rows - 1)) + 8 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const int at = 32 * d + 8 * i + 8 * (lane >> 5);  // the head dimension is a multiple of 8
+        uint32_t x[4], y[4];
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[j] = pack2_bf16(o[n][d][4 * i + 2 * j] * f[n], o[n][d][4 * i + 2 * j + 1] * f[n]);
+            y[j] = pack2_bf16(o[n][d][4 * i + 4 + 2 * j] * f[n], o[n][d][4 * i + 5 + 2 * j] * f[n]);
+            swap(x[j], y[j]);
+          }
+          if (r < rows && at < D) *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i) = u32x4{x[0], x[1], y[0], y[1]};
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = __float_as_uint(o[n][d][4 * i + j] * f[n]), y[j] = __float_as_uint(o[n][d][4 * i + 4 + j] * f[n]);
+            swap(x[j], y[j]);
+          }
+          if (r < rows && at < D) {
+            *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i) = u32x4{x[0], x[1], x[2], x[3]};
+            *(MLORA_GLOBAL u32x4 *)(p + 32 * d + 8 * i + 4) = u32x4{y[0], y[1], y[2], y[3]};
+          }
+        }
+      }
+  }
+}
+
+template <class T>
+struct AttnTile {
+  static constexpr int KT = sizeof(T) == 2 ? 64 : 32;  // keys per tile: 16 KB of K and of V at 128 channels
+};
+
 }  // namespace mlora

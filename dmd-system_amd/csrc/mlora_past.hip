@@ -1,0 +1,1257 @@
+// Attention of a stream's tokens to their own past: a window, the first tokens, a prefix that samples share.
+//
+// A query at position p of a sample with n keys, chunks of C tokens, a window of W and S sinks sees its sample's keys
+//   j < min(e, n) with j >= e − W or j < S,   e = (⌊p / C⌋ + 1)·C the end of its chunk,
+// and all keys of its group's prefix. out = Σ_j P_j v_j, P = softmax(scale · q·k_j) over the keys that it sees; queries
+// with p < 0 or p >= n belong to no token and get zeros.
+//
+// One pass over the key tiles that some row of a workgroup sees: the prefix's, the sinks', then the window's from its first
+// tile on, with a running maximum and sum per row (Softmax). Everything between them is never read. Only the tiles at the edges of
+// a wave's rows need masks; keys that no row of the workgroup sees are loaded as zeros, whatever lies there.
+//
+// Rows: the G = heads / kv_heads query heads that share a key head are packed token by token, row r = i·G + g of token i,
+// so that 32 rows are 32 / G neighbouring tokens and see almost the same keys.
+#include "mlora_attention.h"
+
+namespace mlora {
+
+struct PastArgs {
+  const void *q, *k, *v, *pk, *pv;
+  void *out;        // [B, Lq, H, D] contiguous
+  uint16_t *rest;   // bf16 and a backward to come: what out's rounding left, [B, Lq, H, D]
+  float *stats;     // a backward to come: [2][B·Hk·rows], x and a of every row: P = 2^((s − a)·c − x)
+  const int32_t *lengths, *starts, *prefix_lengths;
+  float *part_o, *part_ml;  // [slots][B·Hk·rows][D] sums and [slots][B·Hk·rows][2] (m, l)
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, pk_sb, pk_sl, pk_sh, pv_sb, pv_sl, pv_sh;
+  int32_t B, Lq, Lk, H, Hk, G, D, Lp, each;  // each: samples per prefix
+  int32_t window, sinks, chunk, first, from_end, rows;
+  int32_t packed_blocks;  // workgroups at the grid's start that take the prefix alone, for the rows of all its samples
+  int32_t packed_tiles, packed_splits, row_tiles, splits, slots;
+  int32_t with_prefix;    // the other workgroups take the prefix too
+  float c;                // scale · log2 e
+};
+
+constexpr int kEver = 1 << 30;  // past every position; lengths, windows and chunks are limited so that sums of two stay in int32
+
+struct Sample {
+  int n, start;  // its keys; the position of its first query
+};
+__device__ __forceinline__ Sample sample_of(const PastArgs &a, int b) {
+  Sample s;
+  s.n = a.lengths == nullptr ? a.Lk : min(max(a.lengths[b], 0), a.Lk);
+  const int first = a.starts != nullptr ? a.starts[b] : a.from_end ? s.n - a.Lq : a.first;
+  s.start = min(max(first, -a.Lq), a.Lk);  // beyond these no query has a token
+  return s;
+}
+__device__ __forceinline__ Sample uniform(const Sample &s) {
+  return {__builtin_amdgcn_readfirstlane(s.n), __builtin_amdgcn_readfirstlane(s.start)};
+}
+__device__ __forceinline__ int prefix_keys(const PastArgs &a, int group) {
+  if (a.prefix_lengths == nullptr) return a.Lp;
+  return __builtin_amdgcn_readfirstlane(min(max(a.prefix_lengths[group], 0), a.Lp));
+}
+
+// The own keys [lo, hi) that a token sees beside the sinks; lo may be negative.
+struct Span {
+  int lo, hi;
+};
+__device__ __forceinline__ Span span_of(const PastArgs &a, int n, int p) {
+  const int end = (int)((uint32_t)p / (uint32_t)a.chunk + 1) * a.chunk;
+  return {end - a.window, min(end, n)};
+}
+
+// The key tiles that the tokens pa .. pb of a sample see, in the order they are taken.
+template <int KT>
+struct KeyTiles {
+  int plen, lo, hi, sink_end;       // prefix keys; own keys [lo, hi) and [0, sink_end)
+  int np, ns, w0, count;            // tiles of the prefix, of the sinks before tile w0, all
+  __device__ __forceinline__ void init(const PastArgs &a, int plen_, int n, int pa, int pb) {
+    plen = pa <= pb ? plen_ : 0, np = (plen + KT - 1) / KT, lo = hi = sink_end = ns = w0 = 0, count = np;
+    if (pa > pb || n == 0) return;
+    lo = max(span_of(a, n, pa).lo, 0), hi = span_of(a, n, pb).hi, sink_end = min(a.sinks, hi);
+    w0 = lo / KT, ns = min((sink_end + KT - 1) / KT, w0);
+    count = np + ns + (hi + KT - 1) / KT - w0;
+  }
+  __device__ __forceinline__ bool own(int t) const { return t >= np; }
+  __device__ __forceinline__ int key0(int t) const {
+    const int u = t - np;
+    return (u < 0 ? t : u < ns ? u : w0 + u - ns) * KT;
+  }
+  // the tile's keys that some row may see; none past the last tile
+  __device__ __forceinline__ uint64_t bits(int t, int end) const {
+    const int k0 = key0(t);
+    const uint64_t b = t < np ? low_bits(plen - k0) : low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(sink_end - k0));
+    return t < end ? b & low_bits(KT) : 0;
+  }
+};
+
+// What the rows of one wave (or 32 of them) see of an own tile.
+struct WaveRows {
+  int none;              // no row belongs to a token
+  int lo_a, hi_a, lo_b, hi_b;  // the spans of the first and the last token
+  __device__ __forceinline__ void init(const PastArgs &a, const Sample &s, int r0, int r1) {  // rows r0 .. r1 - 1
+    const int pa = max(s.start + r0 / a.G, 0), pb = min(s.start + (r1 - 1) / a.G, s.n - 1);
+    none = r0 >= r1 || pa > pb;
+    if (none) return;
+    const Span x = span_of(a, s.n, pa), y = span_of(a, s.n, pb);
+    lo_a = x.lo, hi_a = x.hi, lo_b = y.lo, hi_b = y.hi;
+  }
+  __device__ __forceinline__ bool nothing(const PastArgs &a, int k0, int KT) const {
+    return k0 >= hi_b || (k0 + KT <= lo_a && k0 >= a.sinks);
+  }
+  __device__ __forceinline__ bool everything(const PastArgs &a, int k0, int KT) const {
+    return k0 + KT <= hi_a && (k0 >= lo_b || k0 + KT <= a.sinks);
+  }
+};
+
+// A lane's row.
+struct Row {
+  int b, i, g;   // sample, token, head within the key head's
+  int lo, hi;    // its span
+  bool on;       // it belongs to a token
+  int64_t at;    // (sample, key head, row)
+  __device__ __forceinline__ uint64_t bits(const PastArgs &a, int k0) const {
+    return low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(a.sinks - k0));
+  }
+};
+// Row r (of `rows`) of sample b, or of the samples of group b one after the other.
+__device__ __forceinline__ Row row_of(const PastArgs &a, bool packed, int b, int hk, int r, int rows, const Sample &s) {
+  Row x;
+  const int rc = min(r, rows - 1);
+  int in = rc;
+  x.b = b;
+  Sample mine = s;
+  if (packed) {
+    x.b = b * a.each + rc / a.rows, in = rc % a.rows;
+    mine = sample_of(a, x.b);
+  }
+  x.i = in / a.G, x.g = in - x.i * a.G;
+  const int p = mine.start + x.i;
+  x.on = r < rows && p >= 0 && p < mine.n;
+  x.at = ((int64_t)x.b * a.Hk + hk) * a.rows + in;
+  const Span w = span_of(a, mine.n, max(p, 0));
+  x.lo = x.on ? w.lo : 0, x.hi = x.on ? w.hi : 0;
+  return x;
+}
+// Its place in a [B, Lq, H, D] tensor.
+__device__ __forceinline__ int64_t row_place(const PastArgs &a, const Row &x, int hk, int64_t sb, int64_t sl, int64_t sh) {
+  return x.b * sb + x.i * sl + (int64_t)(hk * a.G + x.g) * sh;
+}
+
+// Which rows a workgroup takes, and which share of their key tiles.
+struct Job {
+  bool packed;
+  int hk, rt, b, slot, rows;
+  int sp, splits;
+  __device__ __forceinline__ void init(const PastArgs &a, int id) {
+    packed = id < a.packed_blocks;
+    if (!packed) id -= a.packed_blocks;
+    const int tiles = packed ? a.packed_tiles : a.row_tiles;
+    splits = packed ? a.packed_splits : a.splits;
+    rows = packed ? a.each * a.rows : a.rows;
+    hk = id % a.Hk, id /= a.Hk;  // heads first: rows of all heads are read together, whole token rows of memory
+    rt = tiles - 1 - id % tiles, id /= tiles;  // the last rows see the most keys
+    sp = id % splits, b = id / splits;
+    slot = packed ? sp : a.packed_splits + sp;
+  }
+  __device__ __forceinline__ int share(int count, int s) const { return (int)((int64_t)count * s / splits); }
+};
+
+// Writes 32 rows of the O^T registers: the lane's row at base + at.
+template <class T, int DP>
+__device__ __forceinline__ void store_row(T *base, int64_t at, bool on, const f32x16 (&o)[1][DP / 32], float f, int D, int lane) {
+  const float fs[1] = {f};
+  store_rows<T, DP, 1>(base, o, fs, on ? 0 : 1, 1, [&](int) { return at; }, D, lane & 32);
+}
+
+// The rows of a wave that are done: out, what its rounding left, and the statistics for the backward.
+template <class T, int DP>
+__device__ __forceinline__ void finish_rows(const PastArgs &a, const Row &x, bool there, int hk, f32x16 (&o)[1][DP / 32], float inv,
+                                            float m, float l, int lane) {
+  const int64_t at = row_place(a, x, hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
+  if (__any(!x.on)) {  // whatever v held
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[0][d][i] = x.on ? o[0][d][i] : 0.f;
+  }
+  store_row<T, DP>(static_cast<T *>(a.out), at, there, o, inv, a.D, lane);
+  if (a.stats == nullptr) return;
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+  if (lane < 32 && there) {
+    const RowRef ref = row_ref(m, a.c);
+    const bool some = l > 0.f;
+    a.stats[x.at] = some ? ref.r + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+    a.stats[all + x.at] = some ? ref.a : 0.f;
+  }
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float y = o[0][d][i] * inv;
+        o[0][d][i] = y - bf16_to_f32(f32_to_bf16_rne(y));
+      }
+    store_row<uint16_t, DP>(a.rest, at, there, o, 1.f, a.D, lane);
+  }
+}
+
+// Four waves of 32 rows each against the same key tiles, two buffers of K and V in LDS: tile t + 1 loads while tile
+// t is multiplied; one barrier per tile.
+template <class T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_fwd_kernel(const PastArgs a) {
+  constexpr int KT = AttnTile<T>::KT;
+  using Tile = HeadTile<T, DP>;
+  constexpr int TB = KT * Tile::RB, N = TB / 1024 / 4;
+  __shared__ u32x4 smem[4 * TB / 16];  // K, V of buffer 0, K, V of buffer 1
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  Job job;
+  job.init(a, blockIdx.x);
+  const int hk = job.hk, r0 = job.rt * 128, group = job.packed ? job.b : job.b / a.each;
+  Sample s{1, 0};
+  KeyTiles<KT> tiles;
+  WaveRows wr;
+  wr.none = 0;
+  if (job.packed) {
+    tiles.init(a, prefix_keys(a, group), 0, 0, 0);
+  } else {
+    s = uniform(sample_of(a, job.b));
+    tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start + r0 / a.G, 0),
+               min(s.start + min(r0 + 127, a.rows - 1) / a.G, s.n - 1));
+    wr.init(a, s, r0 + wave * 32, min(r0 + wave * 32 + 32, a.rows));
+  }
+  const int t0 = job.share(tiles.count, job.sp), t1 = job.share(tiles.count, job.sp + 1);
+  const T *kp = static_cast<const T *>(a.k) + job.b * a.k_sb + hk * a.k_sh, *vp = static_cast<const T *>(a.v) + job.b * a.v_sb + hk * a.v_sh;
+  const T *pkp = static_cast<const T *>(a.pk) + group * a.pk_sb + hk * a.pk_sh, *pvp = static_cast<const T *>(a.pv) + group * a.pv_sb + hk * a.pv_sh;
+  TileLoader<T, DP, N> kl, vl;
+  bool own = false;
+  auto aim = [&](bool o) __attribute__((always_inline)) {
+    own = o;
+    kl.init(lane, wave, 4, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, wave, 4, o ? a.v_sl : a.pv_sl, a.D);
+  };
+  auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+    const bool o = tiles.own(t);
+    if (o != own) aim(o);  // at the end of the prefix
+    const int64_t k0 = tiles.key0(t);
+    const uint64_t bits = tiles.bits(t, t1);  // behind the last one nothing is read
+    kl.load(o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, bits, lds + buf * 2 * TB);
+    vl.load(o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl, bits, lds + buf * 2 * TB + TB);
+  };
+  aim(tiles.own(t0));
+  if (t0 < t1) stage(t0, 0);
+  FragReader<T, DP> fr;
+  fr.init(lane, lds);
+  Softmax<T, DP, 1, KT, true> sm;
+  sm.init();
+  const Row x = row_of(a, job.packed, job.b, hk, r0 + wave * 32 + (lane & 31), job.rows, s);
+  const bool there = r0 + wave * 32 + (lane & 31) < job.rows;
+  {
+    const T *p = static_cast<const T *>(a.q) + row_place(a, x, hk, a.q_sb, a.q_sl, a.q_sh);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int d = 16 * ks + 8 * (lane >> 5);
+      load_frag(p, d, x.on && d < a.D, sm.q[0][ks]);
+    }
+  }
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    lds_pipeline_barrier();  // tile t is in LDS, and every wave has read the tile before it
+    stage(t + 1, (t + 1 - t0) & 1);
+    const int k0 = tiles.key0(t);
+    const bool o = tiles.own(t);
+    if (!wr.none && !(o && wr.nothing(a, k0, KT))) {
+      const uint64_t all = tiles.bits(t, t1);
+      uint64_t bits[1] = {all};
+      bool masked = all != low_bits(KT);
+      if (o && !wr.everything(a, k0, KT)) masked = true, bits[0] = x.bits(a, k0);
+      sm.template step<0, TB>(fr, masked, bits, a.c, lane);
+    }
+    fr.flip(2 * TB);
+  }
+  wait_vmcnt<0>();
+  float f;
+  const float l = sm.sums(0, f);
+  if (a.slots > 1) {
+    const int64_t first = job.slot * ((int64_t)a.B * a.Hk * a.rows);
+    if (lane < 32 && there) *(float2 *)(a.part_ml + 2 * (first + x.at)) = x.on ? float2{sm.m[0], l} : float2{kNoMax, 0.f};
+    store_row<float, DP>(a.part_o + first * a.D, x.at * a.D, there, sm.o, f, a.D, lane);
+  } else {
+    const bool some = x.on && (l > 0.f || l != l);
+    finish_rows<T, DP>(a, x, there, hk, sm.o, some ? f / l : 0.f, sm.m[0], x.on ? l : 0.f, lane);
+  }
+}
+
+// Few rows (at most 32 NQ): the NW waves take different key tiles, each with its own buffers (no barrier in the loop),
+// and their running softmaxes are joined through LDS. Bound by the reading of K and V.
+template <class T, int DP>
+struct PastFew {
+  static constexpr int KT = 32, NW = sizeof(T) * DP == 512 ? 2 : 4;  // 128 KB of LDS at most
+};
+
+template <class T, int DP, int NQ>
+__global__ __launch_bounds__((64 * PastFew<T, DP>::NW), 1) void past_few_kernel(const PastArgs a) {
+  constexpr int KT = PastFew<T, DP>::KT, NW = PastFew<T, DP>::NW, ND = DP / 32;
+  using Tile = HeadTile<T, DP>;
+  constexpr int TB = KT * Tile::RB, N = TB / 1024;
+  static_assert(NW * NQ * ND * 4 * 64 * 16 <= 4 * TB * NW, "the waves' sums fit the buffers");
+  // one array, so that the readers' buffers start at multiples of 4 TB; (m, l) of [wave][n][query] behind them
+  __shared__ u32x4 smem[4 * TB * NW / 16 + NW * NQ * 16];
+  float2 (&ml)[NW][NQ][32] = *(float2 (*)[NW][NQ][32])(smem + 4 * TB * NW / 16);
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 4 * TB;
+  Job job;
+  job.init(a, blockIdx.x);
+  const int hk = job.hk, group = job.packed ? job.b : job.b / a.each;
+  Sample s{1, 0};
+  KeyTiles<KT> tiles;
+  WaveRows wr;
+  wr.none = 0;
+  if (job.packed) {
+    tiles.init(a, prefix_keys(a, group), 0, 0, 0);
+  } else {
+    s = uniform(sample_of(a, job.b));
+    tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start, 0), min(s.start + a.Lq - 1, s.n - 1));
+    wr.init(a, s, 0, a.rows);
+  }
+  const int t1 = job.share(tiles.count, job.sp + 1), t0 = min(job.share(tiles.count, job.sp) + wave, t1);
+  const T *kp = static_cast<const T *>(a.k) + job.b * a.k_sb + hk * a.k_sh, *vp = static_cast<const T *>(a.v) + job.b * a.v_sb + hk * a.v_sh;
+  const T *pkp = static_cast<const T *>(a.pk) + group * a.pk_sb + hk * a.pk_sh, *pvp = static_cast<const T *>(a.pv) + group * a.pv_sb + hk * a.pv_sh;
+  TileLoader<T, DP, N> kl, vl;
+  bool own = false;
+  auto aim = [&](bool o) __attribute__((always_inline)) {
+    own = o;
+    kl.init(lane, 0, 1, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, 0, 1, o ? a.v_sl : a.pv_sl, a.D);
+  };
+  auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+    const bool o = tiles.own(t);
+    if (o != own) aim(o);  // at the end of the prefix
+    const int64_t k0 = tiles.key0(t);
+    const uint64_t bits = tiles.bits(t, t1);  // behind the last one nothing is read
+    kl.load(o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, bits, lds + buf * 2 * TB);
+    vl.load(o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl, bits, lds + buf * 2 * TB + TB);
+  };
+  aim(tiles.own(t0));
+  if (t0 < t1) stage(t0, 0);
+  FragReader<T, DP> fr;
+  fr.init(lane, lds);
+  Softmax<T, DP, NQ, KT, true> sm;
+  sm.init();
+  Row x[NQ];
+  bool there[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    x[n] = row_of(a, job.packed, job.b, hk, 32 * n + (lane & 31), job.rows, s);
+    there[n] = 32 * n + (lane & 31) < job.rows;
+    const T *p = static_cast<const T *>(a.q) + row_place(a, x[n], hk, a.q_sb, a.q_sl, a.q_sh);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int d = 16 * ks + 8 * (lane >> 5);
+      load_frag(p, d, x[n].on && d < a.D, sm.q[n][ks]);
+    }
+  }
+  auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
+    constexpr int B = decltype(buf)::value;
+    wait_vmcnt<0>();  // tile t is in this wave's buffer
+    asm volatile("" ::: "memory");
+    stage(t + NW, 1 - B);
+    const int k0 = tiles.key0(t);
+    const bool o = tiles.own(t);
+    const uint64_t all = tiles.bits(t, t1);
+    uint64_t bits[NQ];
+    bool masked = all != low_bits(KT);
+    const bool rows = o && !wr.everything(a, k0, KT);
+    masked |= rows;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) bits[n] = rows ? x[n].bits(a, k0) : all;
+    sm.template step<2 * B * TB, 2 * B * TB + TB>(fr, masked, bits, a.c, lane);
+  };
+  for (int t = t0; t < t1; t += 2 * NW) {
+    turn(std::integral_constant<int, 0>{}, t);
+    if (t + NW < t1) turn(std::integral_constant<int, 1>{}, t + NW);
+  }
+  wait_vmcnt<0>();
+  // join the waves: every wave leaves its sums, then sums its share of the 32 x 32 tiles over the waves
+  float f[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const float l = sm.sums(n, f[n]);
+    if (lane < 32) ml[wave][n][lane] = float2{sm.m[n], l};
+  }
+  __syncthreads();
+  f32x4 *sums = (f32x4 *)smem;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sums[(((wave * NQ + n) * ND + d) * 4 + i) * 64 + lane] =
+            f32x4{sm.o[n][d][4 * i], sm.o[n][d][4 * i + 1], sm.o[n][d][4 * i + 2], sm.o[n][d][4 * i + 3]} * f[n];
+  __syncthreads();
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float m = kNoMax, lsum = 0.f, w[NW];
+#pragma unroll
+    for (int q = 0; q < NW; ++q) m = fmaxf(m, ml[q][n][lane & 31].x);
+    const RowRef top = row_ref(m, a.c);
+#pragma unroll
+    for (int q = 0; q < NW; ++q) {
+      const float2 v = ml[q][n][lane & 31];
+      w[q] = ref_factor(row_ref(v.x, a.c), top, a.c);
+      lsum += w[q] * v.y;
+    }
+    if (!x[n].on) lsum = 0.f;
+    const bool some = lsum > 0.f || lsum != lsum;
+    const float inv = a.slots > 1 ? 1.f : some ? 1.0f / lsum : 0.f;
+    if (wave == 0 && lane < 32 && there[n]) {
+      if (a.slots > 1) *(float2 *)(a.part_ml + 2 * (job.slot * all + x[n].at)) = float2{some ? m : kNoMax, lsum};
+      else if (a.stats != nullptr) {
+        a.stats[x[n].at] = lsum > 0.f ? top.r + __builtin_amdgcn_logf(lsum) : lsum != lsum ? lsum : INFINITY;
+        a.stats[all + x[n].at] = lsum > 0.f ? top.a : 0.f;
+      }
+    }
+    const int64_t at = row_place(a, x[n], hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
+    for (int u = wave; u < 4 * ND; u += NW) {  // 4 consecutive channels per lane
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < NW; ++q) o += w[q] * sums[((q * NQ + n) * 4 * ND + u) * 64 + lane];
+      const int ch = 32 * (u / 4) + 8 * (u % 4) + 4 * (lane >> 5);
+      if (!there[n] || ch >= a.D) continue;
+      o *= inv;
+      if (!some) o = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (a.slots > 1) *(MLORA_GLOBAL f32x4 *)(a.part_o + (job.slot * all + x[n].at) * a.D + ch) = o;
+      else if constexpr (sizeof(T) == 2) {
+        *(MLORA_GLOBAL u32x2 *)(static_cast<T *>(a.out) + at + ch) = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+        if (a.stats != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] -= bf16_to_f32(f32_to_bf16_rne(o[j]));
+          *(MLORA_GLOBAL u32x2 *)(a.rest + at + ch) = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+        }
+      } else *(MLORA_GLOBAL f32x4 *)(static_cast<T *>(a.out) + at + ch) = o;
+    }
+  }
+}
+
+// Joins the shares of a row, one workgroup per row: weights 2^((m_s − max m)·c). Eight groups of 32 lanes (4 channels
+// each) take every eighth share, and their sums are added in order through LDS.
+template <class T>
+__global__ __launch_bounds__(256) void past_join_kernel(const PastArgs a) {
+  __shared__ f32x4 sums[8][32];
+  __shared__ float ls[8];
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows, row = blockIdx.x;
+  const int at = threadIdx.x % 32, g = threadIdx.x / 32;
+  float m = kNoMax;
+  for (int s = at; s < a.slots; s += 32) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
+#pragma unroll
+  for (int i = 16; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+  const RowRef top = row_ref(m, a.c);
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = g; s < a.slots; s += 8) {
+    const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * all + row));
+    const float w = ref_factor(row_ref(ml.x, a.c), top, a.c);
+    l += w * ml.y;
+    if (4 * at < a.D && ml.y != 0.f) o += w * *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + 4 * at);
+  }
+  sums[g][at] = o;
+  if (at == 0) ls[g] = l;
+  __syncthreads();
+  if (g != 0) return;
+  l = ls[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) o += sums[i][at], l += ls[i];
+  if (at == 0 && a.stats != nullptr) {
+    a.stats[row] = l > 0.f ? top.r + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+    a.stats[all + row] = l > 0.f ? top.a : 0.f;
+  }
+  if (4 * at >= a.D) return;
+  const int r = (int)(row % a.rows), hk = (int)(row / a.rows % a.Hk);
+  const int64_t b = row / a.rows / a.Hk;
+  const int64_t place = (b * a.Lq + r / a.G) * a.H * a.D + (int64_t)(hk * a.G + r % a.G) * a.D + 4 * at;
+  o *= l > 0.f || l != l ? 1.0f / l : 0.f;
+  T *p = static_cast<T *>(a.out) + place;
+  if constexpr (sizeof(T) == 2) {
+    *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+    if (a.stats == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] -= bf16_to_f32(f32_to_bf16_rne(o[j]));
+    *(MLORA_GLOBAL u32x2 *)(a.rest + place) = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+  } else *(MLORA_GLOBAL f32x4 *)p = o;
+}
+
+// ------------------------------------------------------------------ backward
+//
+//   P = 2^((s − a)·c − x),  delta = Σ_d do·(out + rest),  dP = do·Vᵀ,  dS = P·(dP − delta)
+//   dq = scale · dS·K,   dk = scale · dSᵀ·q,   dv = Pᵀ·do
+// Two kernels form P again: one owns query rows (dq, and delta on the way), one owns keys (dk, dv; a prefix's keys meet
+// the rows of all its samples). That is 7 products instead of 5, and no atomics: every sum has a fixed order. rest holds what
+// the rounding of out to bf16 left, so that delta is as good as float32 sums: a row that rests on one key has dS = 0, and
+// half a bf16 step of out in delta would be its whole gradient. P and dS are rounded to bf16 as operands of the
+// products that follow: half a step each.
+
+struct PastBwdArgs {
+  PastArgs f;
+  const void *g;             // the output's gradient
+  void *dq, *dk, *dv, *dpk, *dpv;  // contiguous
+  float *delta;              // [B·Hk·rows]
+  f32x4 *part;               // shares of dq, then of dk and dv, in register order
+  int64_t g_sb, g_sl, g_sh;
+  float scale;
+  int32_t key_blocks, prefix_blocks, sink_blocks;  // of 32 NW keys: all own ones, the prefix's, those with a sink
+  int32_t prefix_splits, sink_splits, own_splits;
+  int64_t sink_part, own_part;  // where a class's shares begin, in 16-byte vectors
+};
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_dq_kernel(const PastBwdArgs ba) {
+  const PastArgs &a = ba.f;
+  constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
+  using Tile = HeadTile<T, DP>;
+  constexpr int TB = KT * Tile::RB, N = TB / 1024 / 4;
+  __shared__ u32x4 smem[4 * TB / 16];
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  Job job;
+  job.init(a, blockIdx.x);
+  const int hk = job.hk, r0 = job.rt * 128, group = job.b / a.each;
+  const Sample s = uniform(sample_of(a, job.b));
+  KeyTiles<KT> tiles;
+  WaveRows wr;
+  tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start + r0 / a.G, 0),
+             min(s.start + min(r0 + 127, a.rows - 1) / a.G, s.n - 1));
+  wr.init(a, s, r0 + wave * 32, min(r0 + wave * 32 + 32, a.rows));
+  const int t0 = job.share(tiles.count, job.sp), t1 = job.share(tiles.count, job.sp + 1);
+  const T *kp = static_cast<const T *>(a.k) + job.b * a.k_sb + hk * a.k_sh, *vp = static_cast<const T *>(a.v) + job.b * a.v_sb + hk * a.v_sh;
+  const T *pkp = static_cast<const T *>(a.pk) + group * a.pk_sb + hk * a.pk_sh, *pvp = static_cast<const T *>(a.pv) + group * a.pv_sb + hk * a.pv_sh;
+  TileLoader<T, DP, N> kl, vl;
+  bool own = false;
+  auto aim = [&](bool o) __attribute__((always_inline)) {
+    own = o;
+    kl.init(lane, wave, 4, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, wave, 4, o ? a.v_sl : a.pv_sl, a.D);
+  };
+  auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+    const bool o = tiles.own(t);
+    if (o != own) aim(o);
+    const int64_t k0 = tiles.key0(t);
+    const uint64_t bits = tiles.bits(t, t1);
+    kl.load(o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, bits, lds + buf * 2 * TB);
+    vl.load(o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl, bits, lds + buf * 2 * TB + TB);
+  };
+  aim(tiles.own(t0));
+  if (t0 < t1) stage(t0, 0);
+  FragReader<T, DP> fr;
+  fr.init(lane, lds);
+  const Row row = row_of(a, false, job.b, hk, r0 + wave * 32 + (lane & 31), a.rows, s);
+  const bool there = r0 + wave * 32 + (lane & 31) < a.rows;
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+  const int64_t oat = row_place(a, row, hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
+  Frag<T> q[DP / 16], g[DP / 16];
+  float delta = 0.f;
+  {
+    const T *qp = static_cast<const T *>(a.q) + row_place(a, row, hk, a.q_sb, a.q_sl, a.q_sh);
+    const T *gp_ = static_cast<const T *>(ba.g) + row_place(a, row, hk, ba.g_sb, ba.g_sl, ba.g_sh);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int d = 16 * ks + 8 * (lane >> 5);
+      const bool on = row.on && d < a.D;
+      Frag<T> of;
+      load_frag(qp, d, on, q[ks]);
+      load_frag(gp_, d, on, g[ks]);
+      load_frag(static_cast<const T *>(a.out) + oat, d, on, of);
+      if constexpr (sizeof(T) == 2) {
+        Frag<T> rf;
+        load_frag(a.rest + oat, d, on, rf);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          delta += __uint_as_float(g[ks].v[j] << 16) * (__uint_as_float(of.v[j] << 16) + __uint_as_float(rf.v[j] << 16));
+          delta += __uint_as_float(g[ks].v[j] & 0xffff0000u) * (__uint_as_float(of.v[j] & 0xffff0000u) + __uint_as_float(rf.v[j] & 0xffff0000u));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta += g[ks].v[j] * of.v[j];
+      }
+    }
+  }
+  delta = half_sum(delta);
+  const float x = row.on ? a.stats[row.at] : INFINITY, shift = row.on ? a.stats[all + row.at] : 0.f;
+  if (job.sp == 0 && lane < 32 && there) ba.delta[row.at] = delta;
+  const bool shifted = __any(shift != 0.f);
+  f32x16 dq[1][ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dq[0][d][i] = 0.f;
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    lds_pipeline_barrier();  // tile t is in LDS, and every wave has read the tile before it
+    stage(t + 1, (t + 1 - t0) & 1);
+    const int k0 = tiles.key0(t);
+    const bool o = tiles.own(t);
+    if (!wr.none && !(o && wr.nothing(a, k0, KT))) {
+      uint64_t bits = tiles.bits(t, t1);
+      bool masked = bits != low_bits(KT);
+      if (o && !wr.everything(a, k0, KT)) masked = true, bits = row.bits(a, k0);
+      static_for<KT / 32>([&](auto block) __attribute__((always_inline)) {
+        constexpr int kb = decltype(block)::value;
+        f32x16 sc, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          Frag<T> kf, vf;
+          fr.template rows<0, 32 * kb>(ks, kf);
+          sc = mma16(kf, q[ks], sc);
+          fr.template rows<TB, 32 * kb>(ks, vf);
+          dp = mma16(vf, g[ks], dp);
+        }
+        if (masked) {
+          const uint64_t mine = bits >> (4 * (lane >> 5));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool on = (mine >> (32 * kb + 8 * (i / 4) + i % 4)) & 1;
+            sc[i] = on ? sc[i] : -INFINITY, dp[i] = on ? dp[i] : 0.f;
+          }
+        }
+        if (shifted) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] -= shift;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -x)) * (dp[i] - delta);
+        static_for<2>([&](auto ks) __attribute__((always_inline)) {
+          Frag<T> ds;
+          to_frag(sc, ks, ds);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            Frag<T> kf;
+            fr.template cols<0, 32 * kb + 16 * decltype(ks)::value>(d, kf);
+            dq[0][d] = mma16(kf, ds, dq[0][d]);
+          }
+          return true;
+        });
+        return true;
+      });
+    }
+    fr.flip(2 * TB);
+  }
+  wait_vmcnt<0>();
+  if (__any(!row.on)) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dq[0][d][i] = row.on ? dq[0][d][i] : 0.f;
+  }
+  if (a.splits > 1) {
+    f32x4 *p = ba.part + ((((int64_t)job.sp * a.B + job.b) * a.row_tiles + job.rt) * a.Hk + hk) * (4 * ND * 4 * 64) + wave * (ND * 4 * 64) + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dq[0][d][4 * i], dq[0][d][4 * i + 1], dq[0][d][4 * i + 2], dq[0][d][4 * i + 3]};
+    return;
+  }
+  store_row<T, DP>(static_cast<T *>(ba.dq), oat, there, dq, ba.scale, a.D, lane);
+}
+
+// Adds the shares of dq in order and writes them out.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void past_dq_join_kernel(const PastBwdArgs ba) {
+  const PastArgs &a = ba.f;
+  constexpr int ND = DP / 32;
+  const int64_t per = (int64_t)a.B * a.row_tiles * a.Hk * 4 * ND * 4 * 64;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
+  int64_t u = e / 64;
+  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % 4);
+  u /= 4 * ND * 4;  // (b, row tile, hk)
+  const int hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * 128 + wave * 32 + (lane & 31);
+  const int64_t b = u / a.Hk / a.row_tiles;
+  const int ch = 32 * d + 8 * i + 4 * (lane >> 5);
+  if (r >= a.rows || ch >= a.D) return;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(ba.part + s * per + e);
+  x *= ba.scale;
+  T *p = static_cast<T *>(ba.dq) + (b * a.Lq + r / a.G) * a.H * a.D + (int64_t)(hk * a.G + r % a.G) * a.D + ch;
+  if constexpr (sizeof(T) == 2) *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
+  else *(MLORA_GLOBAL f32x4 *)p = x;
+}
+
+// NW waves own 32 keys each (K fragments in registers; V in LDS for bf16, whose two waves per SIMD leave no room
+// for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient and the rows'
+// x, delta and a.
+template <class T, int DP, int NW>
+struct PastDkv {
+  static constexpr int QT = sizeof(T) == 2 && !(DP == 128 && NW == 4) ? 64 : 32;
+};
+
+// A workgroup of dk / dv: which keys, and which share of the rows that see them. Blocks of the prefix come first, then those
+// that hold a sink (both meet many rows and are shared out), then the other own ones.
+struct KeyJob {
+  int prefix, block, o, hk, sp, splits;
+  int64_t part;  // index of the first share's tile in its class
+  __device__ __forceinline__ void init(const PastBwdArgs &ba, int id) {
+    const PastArgs &a = ba.f;
+    const int groups = a.B / a.each;
+    const int np = groups * a.Hk * ba.prefix_blocks * ba.prefix_splits, ns = a.B * a.Hk * ba.sink_blocks * ba.sink_splits;
+    prefix = id < np;
+    const bool sink = !prefix && id < np + ns;
+    id -= prefix ? 0 : sink ? np : np + ns;
+    const int first = prefix || sink ? 0 : ba.sink_blocks;
+    const int blocks = prefix ? ba.prefix_blocks : sink ? ba.sink_blocks : ba.key_blocks - ba.sink_blocks;
+    splits = prefix ? ba.prefix_splits : sink ? ba.sink_splits : ba.own_splits;
+    hk = id % a.Hk, id /= a.Hk;
+    block = id % blocks, id /= blocks;
+    sp = id % splits, o = id / splits;
+    part = (prefix ? 0 : sink ? ba.sink_part : ba.own_part);
+    items = (int64_t)(prefix ? groups : a.B) * a.Hk * blocks;
+    item = ((int64_t)o * a.Hk + hk) * blocks + block;
+    block += first;
+  }
+  int64_t items, item;
+};
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void past_dkv_kernel(const PastBwdArgs ba) {
+  const PastArgs &a = ba.f;
+  constexpr int QT = PastDkv<T, DP, NW>::QT, ND = DP / 32, NS = DP / 16;
+  constexpr bool VLDS = sizeof(T) == 2;
+  using Tile = HeadTile<T, DP>;
+  constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = VLDS ? 32 * Tile::RB : 0;
+  static_assert(64 * NW >= 3 * QT, "a thread loads one of a row's three values");
+  // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then x, delta and a per buffer
+  __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + 3 * QT / 2];
+  f32x4 (&stats)[2][3][QT / 4] = *(f32x4 (*)[2][3][QT / 4])(smem + (4 * TB + NW * VB) / 16);
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  KeyJob job;
+  job.init(ba, blockIdx.x);
+  const int hk = job.hk;
+  Sample s{0, 0};
+  if (!job.prefix) s = uniform(sample_of(a, job.o));
+  const int len = job.prefix ? prefix_keys(a, job.o) : s.n;
+  const int key0 = (job.block * NW + wave) * 32, key = key0 + (lane & 31);
+  const bool live = key < len;
+  const uint64_t live_bits = low_bits(min(len - key0, 32));
+  const T *kp = static_cast<const T *>(job.prefix ? a.pk : a.k) + job.o * (job.prefix ? a.pk_sb : a.k_sb) + hk * (job.prefix ? a.pk_sh : a.k_sh);
+  const T *vp = static_cast<const T *>(job.prefix ? a.pv : a.v) + job.o * (job.prefix ? a.pv_sb : a.v_sb) + hk * (job.prefix ? a.pv_sh : a.v_sh);
+  const int64_t k_sl = job.prefix ? a.pk_sl : a.k_sl, v_sl = job.prefix ? a.pv_sl : a.v_sl;
+  Frag<T> k[NS], v[VLDS ? 1 : NS];
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks) {
+    const int d = 16 * ks + 8 * (lane >> 5);
+    load_frag(kp, key * k_sl + d, live && d < a.D, k[ks]);
+    if constexpr (!VLDS) load_frag(vp, key * v_sl + d, live && d < a.D, v[ks]);
+  }
+  MLORA_LDS char *vt = lds + 4 * TB + wave * VB;
+  if constexpr (VLDS) {
+    TileLoader<T, DP, VB / 1024> vl;
+    vl.init(lane, 0, 1, v_sl, a.D);
+    vl.load(vp + (int64_t)key0 * v_sl, live_bits, vt);
+  }
+  f32x16 dk[1][ND], dv[1][ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[0][d][i] = 0.f, dv[0][d][i] = 0.f;
+  // the tokens whose rows see a key: those from the key's chunk on, to the last whose window reaches it (positions)
+  auto from = [&](int j) __attribute__((always_inline)) { return (int)((uint32_t)j / (uint32_t)a.chunk) * a.chunk; };
+  auto to = [&](int j) __attribute__((always_inline)) {
+    return job.prefix || j < a.sinks ? kEver : (int)((uint32_t)(j + a.window) / (uint32_t)a.chunk) * a.chunk;
+  };
+  const int bk0 = job.block * NW * 32, bk1 = min(bk0 + NW * 32, len) - 1;  // the block's keys
+  int i0 = 0, i1 = bk0 < len ? a.Lq : 0;  // the block's tokens, of an own block
+  if (!job.prefix && bk0 < len) {
+    const int last = bk0 < a.sinks ? kEver : to(bk1);
+    i0 = max(from(bk0) - s.start, 0), i1 = max(min(min(last, s.n) - s.start, a.Lq), i0);
+  }
+  const int tile0 = i0 / QT, head_tiles = max((i1 + QT - 1) / QT - tile0, 0), tiles = head_tiles * a.G * (job.prefix ? a.each : 1);
+  const int t0 = (int)((int64_t)tiles * job.sp / job.splits), t1 = (int)((int64_t)tiles * (job.sp + 1) / job.splits);
+  // rows of the wave's keys: all of them see tokens [full_a, full_b), none of them any outside [some_a, some_b)
+  int full_a = 0, full_b = kEver, some_a = 0, some_b = kEver, mine_a = 0, mine_b = kEver;
+  if (!job.prefix && key0 < len) {
+    const int k1 = min(key0 + 31, len - 1), k2 = max(key0, min(a.sinks, k1));
+    some_a = from(key0), full_a = from(k1), full_b = to(k2), some_b = key0 < a.sinks ? kEver : to(k1);
+    mine_a = from(key), mine_b = to(key);
+  }
+  TileLoader<T, DP, N> ql, gl;
+  ql.init(lane, wave, NW, a.q_sl, a.D), gl.init(lane, wave, NW, ba.g_sl, a.D);
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+  FragReader<T, DP> fr, vr;
+  fr.init(lane, lds), vr.init(lane, vt);
+  struct Tokens {
+    int b, g, i;  // sample, head, first token
+  };
+  auto tokens = [&](int t) __attribute__((always_inline)) {
+    const int h = t / head_tiles, m = h / a.G;
+    return Tokens{job.prefix ? job.o * a.each + m : job.o, h - m * a.G, (tile0 + t - h * head_tiles) * QT};
+  };
+  // a tile's rows into LDS, those that are tokens as bits in `rows`; returns x (threads 0 .. QT - 1), delta (QT .. 2 QT - 1) or
+  // a (.. 3 QT - 1) of the thread's row
+  uint64_t rows = 0, next = 0;
+  auto stage = [&](int t, int buf) __attribute__((always_inline)) -> float {
+    const int i = threadIdx.x % QT, which = threadIdx.x / QT;
+    float x = which == 0 ? INFINITY : 0.f;  // rows without a token: P = 0
+    if (t >= t1) return x;
+    const Tokens k = tokens(t);
+    const Sample ks = job.prefix ? uniform(sample_of(a, k.b)) : s;
+    next = low_bits(min(min(a.Lq, ks.n - ks.start) - k.i, QT)) & ~low_bits(-ks.start - k.i);
+    const int h = hk * a.G + k.g;
+    ql.load(static_cast<const T *>(a.q) + k.b * a.q_sb + h * a.q_sh + k.i * a.q_sl, next, lds + buf * 2 * TB);
+    gl.load(static_cast<const T *>(ba.g) + k.b * ba.g_sb + h * ba.g_sh + k.i * ba.g_sl, next, lds + buf * 2 * TB + TB);
+    const int64_t at = ((int64_t)k.b * a.Hk + hk) * a.rows + (int64_t)(k.i + i) * a.G + k.g;
+    if (which < 3 && ((next >> i) & 1)) x = which == 1 ? ba.delta[at] : a.stats[(which / 2) * all + at];
+    return x;
+  };
+  auto keep = [&](int buf, float x) __attribute__((always_inline)) {
+    if (threadIdx.x < 3 * QT) ((float *)stats[buf][threadIdx.x / QT])[threadIdx.x % QT] = x;
+  };
+  auto step = [&](int buf, int p0) __attribute__((always_inline)) {  // p0: the position of the tile's first token
+    if (!job.prefix && (p0 + QT <= some_a || p0 >= some_b)) return;
+    // rows that are no tokens too: a key that none of the tokens sees may hold anything
+    const bool masked = rows != low_bits(QT) || (!job.prefix && (p0 < full_a || p0 + QT > full_b));
+    uint64_t mine = rows;
+    if (masked && !job.prefix) mine &= low_bits(mine_b - p0) & ~low_bits(mine_a - p0);
+    mine >>= 4 * (lane >> 5);
+    static_for<QT / 32>([&](auto block) __attribute__((always_inline)) {
+      constexpr int qb = decltype(block)::value;
+      __builtin_amdgcn_sched_barrier(0);  // between the phases too: interleaved, they spill
+      f32x16 sc, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {  // the two sums in turn: a sum waits for its last product
+        Frag<T> qf, gf, vf;
+        fr.template rows<0, 32 * qb>(ks, qf);
+        sc = mma16(qf, k[ks], sc);
+        fr.template rows<TB, 32 * qb>(ks, gf);
+        if constexpr (VLDS) vr.template rows<0, 0>(ks, vf);
+        else vf = v[ks];
+        dp = mma16(gf, vf, dp);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool on = (mine >> (32 * qb + 8 * (i / 4) + i % 4)) & 1;
+          sc[i] = on ? sc[i] : -INFINITY, dp[i] = on ? dp[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 x = stats[buf][0][8 * qb + 2 * i4 + (lane >> 5)], delta = stats[buf][1][8 * qb + 2 * i4 + (lane >> 5)];
+        const f32x4 shift = stats[buf][2][8 * qb + 2 * i4 + (lane >> 5)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * i4 + j] - shift[j], a.c, -x[j]));
+          sc[4 * i4 + j] = p;
+          dp[4 * i4 + j] = p * (dp[4 * i4 + j] - delta[j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<2>([&](auto ks) __attribute__((always_inline)) {
+        Frag<T> pf;
+        to_frag(sc, ks, pf);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          Frag<T> f;
+          fr.template cols<TB, 32 * qb + 16 * decltype(ks)::value>(d, f);
+          dv[0][d] = mma16(f, pf, dv[0][d]);
+        }
+        return true;
+      });
+      static_for<2>([&](auto ks) __attribute__((always_inline)) {
+        Frag<T> df;
+        to_frag(dp, ks, df);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          Frag<T> f;
+          fr.template cols<0, 32 * qb + 16 * decltype(ks)::value>(d, f);
+          dk[0][d] = mma16(f, df, dk[0][d]);
+        }
+        return true;
+      });
+      return true;
+    });
+  };
+  if (t0 < t1) keep(0, stage(t0, 0)), rows = next;
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    wait_vmcnt<0>();
+    lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
+    const float x = stage(t + 1, buf ^ 1);
+    if (key0 < len) step(buf, s.start + tokens(t).i);
+    keep(buf ^ 1, x);
+    rows = next;
+    fr.flip(2 * TB);
+  }
+  wait_vmcnt<0>();
+  if (!live) {  // a column of keys that are none holds whatever its zeroed fragments gave
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[0][d][i] = 0.f, dv[0][d][i] = 0.f;
+  }
+  if (job.splits > 1) {
+    f32x4 *p = ba.part + job.part + ((job.sp * job.items + job.item) * NW + wave) * (2 * ND * 4 * 64) + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dk[0][d][4 * i], dk[0][d][4 * i + 1], dk[0][d][4 * i + 2], dk[0][d][4 * i + 3]};
+        *(MLORA_GLOBAL f32x4 *)(p + ((ND + d) * 4 + i) * 64) = f32x4{dv[0][d][4 * i], dv[0][d][4 * i + 1], dv[0][d][4 * i + 2], dv[0][d][4 * i + 3]};
+      }
+    return;
+  }
+  const int L = job.prefix ? a.Lp : a.Lk;
+  const int64_t at = ((int64_t)job.o * L * a.Hk + hk) * a.D;
+  const float fk[1] = {ba.scale}, fv[1] = {1.f};
+  auto key_at = [&](int key) { return (int64_t)key * a.Hk * a.D; };
+  store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpk : ba.dk) + at, dk, fk, key0, L, key_at, a.D, lane);
+  store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpv : ba.dv) + at, dv, fv, key0, L, key_at, a.D, lane);
+}
+
+// Adds the shares of a class of key blocks in order and writes them out: 0 the prefix's, 1 those with a sink, 2 the others.
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba, int which_class) {
+  const PastArgs &a = ba.f;
+  constexpr int ND = DP / 32;
+  const bool prefix = which_class == 0;
+  const int blocks = prefix ? ba.prefix_blocks : which_class == 1 ? ba.sink_blocks : ba.key_blocks - ba.sink_blocks;
+  const int splits = prefix ? ba.prefix_splits : which_class == 1 ? ba.sink_splits : ba.own_splits;
+  const f32x4 *part = ba.part + (prefix ? 0 : which_class == 1 ? ba.sink_part : ba.own_part);
+  const int64_t per = (int64_t)(prefix ? a.B / a.each : a.B) * a.Hk * blocks * NW * 2 * ND * 4 * 64;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(part + s * per + e);
+  int64_t u = e / 64;
+  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), value = (int)(u / 4 / ND % 2);
+  u /= 4 * ND * 2;  // (sample or group, hk, block, wave)
+  const int64_t key = (u % (NW * blocks) + (which_class == 2 ? NW * ba.sink_blocks : 0)) * 32 + (lane & 31), bh = u / (NW * blocks);
+  const int ch = 32 * d + 8 * i + 4 * (lane >> 5), L = prefix ? a.Lp : a.Lk;
+  if (key >= L || ch >= a.D) return;
+  void *base = value ? (prefix ? ba.dpv : ba.dv) : prefix ? ba.dpk : ba.dk;
+  T *p = static_cast<T *>(base) + ((bh / a.Hk * L + key) * a.Hk + bh % a.Hk) * a.D + ch;
+  if (!value) x *= ba.scale;
+  if constexpr (sizeof(T) == 2) *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
+  else *(MLORA_GLOBAL f32x4 *)p = x;
+}
+
+// The kernels are named here because hipcc's host pass does not instantiate a kernel that holds generic lambdas
+// from a launch inside one.
+#define MLORA_PAST(T, DP)                                             \
+  template __global__ void past_fwd_kernel<T, DP>(const PastArgs);    \
+  template __global__ void past_few_kernel<T, DP, 1>(const PastArgs); \
+  template __global__ void past_dq_kernel<T, DP>(const PastBwdArgs);  \
+  template __global__ void past_dkv_kernel<T, DP, 4>(const PastBwdArgs);
+MLORA_PAST(uint16_t, 64)
+MLORA_PAST(uint16_t, 128)
+MLORA_PAST(float, 64)
+MLORA_PAST(float, 128)
+#undef MLORA_PAST
+template __global__ void past_few_kernel<uint16_t, 64, 2>(const PastArgs);
+template __global__ void past_few_kernel<uint16_t, 128, 2>(const PastArgs);
+template __global__ void past_few_kernel<float, 64, 2>(const PastArgs);
+template __global__ void past_dkv_kernel<uint16_t, 128, 8>(const PastBwdArgs);
+
+// ------------------------------------------------------------------ host
+
+constexpr int64_t kPastMostTokens = 1 << 28;
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// A call's sizes with options brought into the range where they differ, or a status.
+struct PastSizes {
+  bool f32;
+  int64_t B, Lq, Lk, H, Hk, G, D, groups, each, Lp, rows, window, sinks, chunk, first;
+};
+
+static int past_sizes(PastSizes &z, const mlora_past_shape *s) {
+  if (s == nullptr) return MLORA_ERR_INVALID;
+  if (s->dtype != MLORA_BF16 && s->dtype != MLORA_F32) return MLORA_ERR_UNSUPPORTED;
+  if (s->B < 0 || s->Lq < 0 || s->Lk < 0 || s->H < 1 || s->Hk < 1 || s->H % s->Hk != 0) return MLORA_ERR_INVALID;
+  if (s->D < 8 || s->D % 8 != 0 || s->D > 128) return MLORA_ERR_UNSUPPORTED;
+  if (s->window < 0 || s->sinks < 0 || s->chunk < 1 || (s->window > 0 && s->window < s->chunk)) return MLORA_ERR_INVALID;
+  if (s->groups < 0 || s->Lp < 0 || (s->groups == 0 && s->Lp > 0) || (s->groups > 0 && s->B % s->groups != 0)) return MLORA_ERR_INVALID;
+  if (!(s->scale > 0.f && s->scale * kLog2e < INFINITY)) return MLORA_ERR_INVALID;
+  z.f32 = s->dtype == MLORA_F32;
+  z.B = s->B, z.Lq = s->Lq, z.Lk = s->Lk, z.H = s->H, z.Hk = s->Hk, z.D = s->D, z.G = s->H / s->Hk, z.Lp = s->Lp;
+  if (z.Lq > kPastMostTokens || z.Lk > kPastMostTokens || z.Lp > kPastMostTokens || z.H > 65536) return MLORA_ERR_LIMIT;
+  z.groups = s->groups > 0 ? s->groups : z.B, z.each = z.groups > 0 ? z.B / z.groups : 1;
+  z.rows = z.G * z.Lq;
+  // workgroups: one per (sample, key head, 128 rows or keys), a few thousand shares beside them; rows of a group
+  const int64_t most = INT32_MAX - 65536, blocks = ceil_div(z.rows, 128) + ceil_div(z.Lk, 128) + ceil_div(z.Lp, 128) + 1;
+  if (z.rows > most || (z.B > 0 && (z.Hk > most / z.B || blocks + 4096 > most / (z.B * z.Hk) || z.rows > most / z.B))) return MLORA_ERR_LIMIT;
+  z.chunk = between(s->chunk, 1, z.Lk > 1 ? z.Lk : 1);  // from there on all keys are one chunk
+  z.window = s->window > 0 ? between(s->window, z.chunk, z.Lk + z.chunk) : z.Lk + z.chunk;
+  z.sinks = between(s->sinks, 0, z.Lk);
+  z.first = between(s->first, -z.Lq, z.Lk);
+  return MLORA_OK;
+}
+
+// Key tiles of kt keys that `rows` neighbouring rows of a sample see at most, the prefix aside.
+static int64_t own_tiles(const PastSizes &z, int64_t rows, int64_t kt) {
+  const int64_t all = ceil_div(z.Lk, kt), some = ceil_div(z.window + z.chunk + rows / z.G, kt) + 1 + ceil_div(z.sinks, kt);
+  return some < all ? some : all;
+}
+
+// How a forward is cut. Few rows per key head run waves over different keys, more rows 128 per workgroup. Few rows
+// of samples that share a prefix take it together, in workgroups of its own: then all shares are joined. Keys are shared
+// out where there is less than a workgroup for every compute unit.
+struct PastPlan {
+  bool few, packed, packed_few;
+  int64_t packed_tiles, packed_splits, row_tiles, splits, slots;
+};
+
+static PastPlan past_plan(const PastSizes &z) {
+  PastPlan p{};
+  const int64_t few_rows = z.f32 && z.D > 64 ? 32 : 64, waves = z.f32 && z.D > 64 ? 2 : 4, e = z.f32 ? 4 : 2;
+  p.few = z.rows <= few_rows;
+  p.packed = p.few && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
+  p.row_tiles = p.few ? 1 : ceil_div(z.rows, 128);
+  auto share = [&](int64_t items, int64_t tiles, bool few) {
+    const int64_t least = few ? (z.f32 ? waves : 4 * waves) : z.f32 ? 2 : 8;  // tiles that a share is worth its join for
+    return items > 0 ? between(between(256 / items, 1, 64), 1, between(tiles / least, 1, 64)) : 1;
+  };
+  const int64_t kt = p.few || z.f32 ? 32 : 64;
+  const int64_t prefix_tiles = p.packed ? 0 : ceil_div(z.Lp, kt);
+  p.splits = share(z.B * z.Hk * p.row_tiles, own_tiles(z, p.few ? z.rows : 128, kt) + prefix_tiles, p.few);
+  if (p.packed) {
+    const int64_t rows = z.each * z.rows;
+    p.packed_few = rows <= few_rows;
+    p.packed_tiles = p.packed_few ? 1 : ceil_div(rows, 128);
+    p.packed_splits = share(z.groups * z.Hk * p.packed_tiles, ceil_div(z.Lp, p.packed_few || z.f32 ? 32 : 64), p.packed_few);
+  }
+  p.slots = p.splits + p.packed_splits;
+  return p;
+}
+
+static int64_t past_floats(const PastPlan &p, const PastSizes &z) {
+  return p.slots > 1 ? p.slots * ceil_div(z.B * z.Hk * z.rows * (z.D + 2), 4) * 4 : 0;
+}
+
+struct PastBwdPlan {
+  int nw;  // waves of dk / dv, 32 keys each
+  int64_t row_tiles, splits;
+  int64_t key_blocks, prefix_blocks, sink_blocks, prefix_splits, sink_splits, own_splits;
+  int64_t prefix_vectors, sink_vectors, own_vectors;  // 16-byte vectors of all shares of a class, 0 where it has one
+  int64_t dq_vectors;                                 // of one share of dq
+};
+
+static PastBwdPlan past_bwd_plan(const PastSizes &z) {
+  PastBwdPlan p{};
+  const int64_t kt = z.f32 ? 32 : 64, dp = z.D > 64 ? 128 : 64;
+  p.row_tiles = ceil_div(z.rows, 128);
+  const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, 128, kt) + ceil_div(z.Lp, kt), places = z.f32 ? 256 : 512;
+  p.splits = items > 0 ? between(places / items, 1, between(tiles / (z.f32 ? 1 : 4), 1, 64)) : 1;
+  p.dq_vectors = items * 4 * (dp / 32) * 4 * 64;
+  const int64_t longest = z.Lk > z.Lp ? z.Lk : z.Lp;
+  p.nw = !z.f32 && z.D > 64 && longest > 128 ? 8 : 4;
+  const int64_t qt = z.f32 || (z.D > 64 && p.nw == 4) ? 32 : 64, keys = 32 * p.nw;
+  p.key_blocks = ceil_div(z.Lk, keys), p.prefix_blocks = ceil_div(z.Lp, keys);
+  const bool bounded = z.window < z.Lk;
+  p.sink_blocks = bounded ? between(ceil_div(z.sinks, keys), 0, p.key_blocks) : 0;  // without a window all blocks are alike
+  const int64_t head_tiles = ceil_div(z.Lq, qt), seen = z.window + z.chunk + keys;
+  const int64_t prefix_work = z.each * z.G * head_tiles, sink_work = z.G * head_tiles;
+  const int64_t own_work = z.G * (bounded && seen < z.Lq ? ceil_div(seen, qt) + 1 : head_tiles);
+  const int64_t prefix_items = z.groups * z.Hk * p.prefix_blocks, sink_items = z.B * z.Hk * p.sink_blocks,
+                own_items = z.B * z.Hk * (p.key_blocks - p.sink_blocks);
+  const int64_t total = prefix_items * prefix_work + sink_items * sink_work + own_items * own_work;
+  const int64_t slots = p.nw == 8 || z.f32 ? 256 : 512;
+  int64_t target = ceil_div(total, slots);
+  const int64_t least = z.f32 ? 2 : 4;
+  if (target < least) target = least;
+  auto cut = [&](int64_t work, int64_t n) { return n > 0 ? between(work / target, 1, 64) : 1; };
+  p.prefix_splits = cut(prefix_work, prefix_items), p.sink_splits = cut(sink_work, sink_items), p.own_splits = cut(own_work, own_items);
+  const int64_t per = p.nw * 2 * (dp / 32) * 4 * 64;
+  p.prefix_vectors = p.prefix_splits > 1 ? prefix_items * p.prefix_splits * per : 0;
+  p.sink_vectors = p.sink_splits > 1 ? sink_items * p.sink_splits * per : 0;
+  p.own_vectors = p.own_splits > 1 ? own_items * p.own_splits * per : 0;
+  return p;
+}
+
+// The rows' deltas, then the shares of dq, and after they are joined those of dk and dv in the same place.
+static int64_t past_bwd_bytes(const PastBwdPlan &p, const PastSizes &z) {
+  const int64_t dq = p.splits > 1 ? p.splits * p.dq_vectors : 0, dkv = p.prefix_vectors + p.sink_vectors + p.own_vectors;
+  return (ceil_div(z.B * z.Hk * z.rows, 4) + (dq > dkv ? dq : dkv)) * 16;
+}
+
+// A [B, L, heads, D] operand: 16-byte aligned heads, token strides whose tiles stay within 32-bit offsets.
+static int past_operand(const void *p, const int64_t *st, bool empty) {
+  if (empty) return MLORA_OK;
+  if (p == nullptr) return MLORA_ERR_INVALID;
+  if (!aligned16(p) || st[0] < 0 || st[1] < 0 || st[2] < 0 || st[0] % 8 != 0 || st[1] % 8 != 0 || st[2] % 8 != 0) return MLORA_ERR_UNSUPPORTED;
+  if (st[1] >= (int64_t)1 << 22) return MLORA_ERR_LIMIT;  // 64 rows of 2^22 floats: 2^30 bytes
+  return MLORA_OK;
+}
+
+static int past_args(PastArgs &a, const PastSizes &z, const mlora_past_shape *s, const void *q, const void *k, const void *v,
+                     const void *pk, const void *pv, const int32_t *lengths, const int32_t *starts, const int32_t *prefix_lengths) {
+  int st = past_operand(q, s->q_strides, z.B * z.Lq == 0);
+  if (!st) st = past_operand(k, s->k_strides, z.B * z.Lk == 0);
+  if (!st) st = past_operand(v, s->v_strides, z.B * z.Lk == 0);
+  if (!st) st = past_operand(pk, s->pk_strides, z.groups * z.Lp == 0);
+  if (!st) st = past_operand(pv, s->pv_strides, z.groups * z.Lp == 0);
+  if (st) return st;
+  a = PastArgs{};
+  a.q = q, a.k = k, a.v = v, a.pk = pk, a.pv = pv, a.lengths = lengths, a.starts = starts, a.prefix_lengths = prefix_lengths;
+  a.q_sb = s->q_strides[0], a.q_sl = s->q_strides[1], a.q_sh = s->q_strides[2];
+  a.k_sb = s->k_strides[0], a.k_sl = s->k_strides[1], a.k_sh = s->k_strides[2];
+  a.v_sb = s->v_strides[0], a.v_sl = s->v_strides[1], a.v_sh = s->v_strides[2];
+  a.pk_sb = s->pk_strides[0], a.pk_sl = s->pk_strides[1], a.pk_sh = s->pk_strides[2];
+  a.pv_sb = s->pv_strides[0], a.pv_sl = s->pv_strides[1], a.pv_sh = s->pv_strides[2];
+  a.B = (int32_t)z.B, a.Lq = (int32_t)z.Lq, a.Lk = (int32_t)z.Lk, a.H = (int32_t)z.H, a.Hk = (int32_t)z.Hk, a.G = (int32_t)z.G;
+  a.D = (int32_t)z.D, a.Lp = (int32_t)z.Lp, a.each = (int32_t)z.each, a.rows = (int32_t)z.rows;
+  a.window = (int32_t)z.window, a.sinks = (int32_t)z.sinks, a.chunk = (int32_t)z.chunk, a.first = (int32_t)z.first;
+  a.from_end = s->from_end != 0, a.c = s->scale * kLog2e, a.with_prefix = z.Lp > 0, a.splits = 1;
+  return MLORA_OK;
+}
+
+template <class F>
+static void with_head(bool f32, int64_t D, F &&f) {
+  using std::integral_constant;
+  auto small = integral_constant<int, 64>{};
+  auto large = integral_constant<int, 128>{};
+  if (f32 && D <= 64) f(float{}, small);
+  else if (f32) f(float{}, large);
+  else if (D <= 64) f(uint16_t{}, small);
+  else f(uint16_t{}, large);
+}
+
+}  // namespace mlora
+
+using namespace mlora;
+
+extern "C" int64_t mlora_past_attention_workspace_bytes(const mlora_past_shape *shape) {
+  PastSizes z;
+  const int st = past_sizes(z, shape);
+  return st ? st : past_floats(past_plan(z), z) * (int64_t)sizeof(float);
+}
+
+extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q, const void *k, const void *v, const void *pk,
+                                    const void *pv, const int32_t *key_lengths, const int32_t *query_start,
+                                    const int32_t *prefix_lengths, void *out, void *rest, float *stats, void *workspace,
+                                    int64_t workspace_bytes, void *stream) {
+  PastSizes z;
+  int st = past_sizes(z, shape);
+  if (st) return st;
+  PastArgs a;
+  st = past_args(a, z, shape, q, k, v, pk, pv, key_lengths, query_start, prefix_lengths);
+  if (st || z.B * z.Lq == 0) return st;
+  if (out == nullptr || (stats != nullptr && !z.f32 && rest == nullptr)) return MLORA_ERR_INVALID;
+  if (!aligned16(out) || !aligned16(rest) || (reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return MLORA_ERR_UNSUPPORTED;
+  const PastPlan p = past_plan(z);
+  const int64_t floats = past_floats(p, z);
+  if (floats > 0) {
+    if (workspace == nullptr || workspace_bytes < floats * (int64_t)sizeof(float)) return MLORA_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
+  }
+  a.out = out, a.rest = static_cast<uint16_t *>(rest), a.stats = stats;
+  a.part_o = static_cast<float *>(workspace);
+  a.part_ml = a.part_o + p.slots * z.B * z.Hk * z.rows * z.D;
+  a.row_tiles = (int32_t)p.row_tiles, a.splits = (int32_t)p.splits, a.slots = (int32_t)p.slots;
+  a.packed_tiles = (int32_t)p.packed_tiles, a.packed_splits = (int32_t)p.packed_splits;
+  const int64_t packed = z.groups * z.Hk * p.packed_tiles * p.packed_splits, blocks = z.B * z.Hk * p.row_tiles * p.splits;
+  if (p.packed) a.with_prefix = 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  with_head(z.f32, z.D, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value, NW = PastFew<T, DP>::NW;
+    if (!p.few) {
+      hipLaunchKernelGGL((past_fwd_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+      return;
+    }
+    if (p.packed && !p.packed_few) {  // the prefix's workgroups are of the other kernel
+      a.packed_blocks = (int32_t)packed;
+      hipLaunchKernelGGL((past_fwd_kernel<T, DP>), dim3((unsigned)packed), dim3(256), 0, s, a);
+    }
+    a.packed_blocks = p.packed_few ? (int32_t)packed : 0;
+    const dim3 grid((unsigned)(blocks + a.packed_blocks));
+    const bool two = (p.packed_few ? z.each * z.rows : z.rows) > 32;
+    if constexpr (sizeof(T) * DP < 512) {
+      if (two) hipLaunchKernelGGL((past_few_kernel<T, DP, 2>), grid, dim3(64 * NW), 0, s, a);
+    }
+    if (!two) hipLaunchKernelGGL((past_few_kernel<T, DP, 1>), grid, dim3(64 * NW), 0, s, a);
+  });
+  st = launch_status();
+  if (st || p.slots == 1) return st;
+  const dim3 joins((unsigned)(z.B * z.Hk * z.rows));
+  if (z.f32) hipLaunchKernelGGL(past_join_kernel<float>, joins, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(past_join_kernel<uint16_t>, joins, dim3(256), 0, s, a);
+  return launch_status();
+}
+
+extern "C" int64_t mlora_past_attention_backward_workspace_bytes(const mlora_past_shape *shape) {
+  PastSizes z;
+  const int st = past_sizes(z, shape);
+  return st ? st : past_bwd_bytes(past_bwd_plan(z), z);
+}
+
+extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, const void *q, const void *k, const void *v,
+                                             const void *pk, const void *pv, const int32_t *key_lengths,
+                                             const int32_t *query_start, const int32_t *prefix_lengths, const void *out,
+                                             const void *rest, const float *stats, const void *g, const int64_t *g_strides,
+                                             void *dq, void *dk, void *dv, void *dpk, void *dpv, void *workspace,
+                                             int64_t workspace_bytes, void *stream) {
+  PastSizes z;
+  int st = past_sizes(z, shape);
+  if (st) return st;
+  PastBwdArgs ba{};
+  PastArgs &a = ba.f;
+  st = past_args(a, z, shape, q, k, v, pk, pv, key_lengths, query_start, prefix_lengths);
+  if (st || z.B == 0) return st;
+  if (g_strides == nullptr) return MLORA_ERR_INVALID;
+  st = past_operand(g, g_strides, z.Lq == 0);
+  if (st) return st;
+  if ((z.Lq > 0 && (out == nullptr || stats == nullptr || dq == nullptr || (!z.f32 && rest == nullptr))) ||
+      (z.Lk > 0 && (dk == nullptr || dv == nullptr)) || (z.groups * z.Lp > 0 && (dpk == nullptr || dpv == nullptr)))
+    return MLORA_ERR_INVALID;
+  for (const void *p : {out, rest, (const void *)dq, (const void *)dk, (const void *)dv, (const void *)dpk, (const void *)dpv})
+    if (!aligned16(p)) return MLORA_ERR_UNSUPPORTED;
+  const PastBwdPlan p = past_bwd_plan(z);
+  if (workspace_bytes < past_bwd_bytes(p, z) || (workspace == nullptr && workspace_bytes > 0)) return MLORA_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
+  a.out = const_cast<void *>(out), a.rest = static_cast<uint16_t *>(const_cast<void *>(rest)), a.stats = const_cast<float *>(stats);
+  a.row_tiles = (int32_t)p.row_tiles, a.splits = (int32_t)p.splits, a.slots = (int32_t)p.splits;
+  ba.g = g, ba.g_sb = g_strides[0], ba.g_sl = g_strides[1], ba.g_sh = g_strides[2], ba.scale = shape->scale;
+  ba.dq = dq, ba.dk = dk, ba.dv = dv, ba.dpk = dpk, ba.dpv = dpv, ba.delta = static_cast<float *>(workspace);
+  ba.part = static_cast<f32x4 *>(workspace) + ceil_div(z.B * z.Hk * z.rows, 4);
+  ba.key_blocks = (int32_t)p.key_blocks, ba.prefix_blocks = (int32_t)p.prefix_blocks, ba.sink_blocks = (int32_t)p.sink_blocks;
+  ba.prefix_splits = (int32_t)p.prefix_splits, ba.sink_splits = (int32_t)p.sink_splits, ba.own_splits = (int32_t)p.own_splits;
+  ba.sink_part = p.prefix_vectors, ba.own_part = p.prefix_vectors + p.sink_vectors;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (z.Lq > 0) {
+    with_head(z.f32, z.D, [&](auto t, auto dp) {
+      using T = decltype(t);
+      constexpr int DP = decltype(dp)::value;
+      hipLaunchKernelGGL((past_dq_kernel<T, DP>), dim3((unsigned)(z.B * z.Hk * p.row_tiles * p.splits)), dim3(256), 0, s, ba);
+      if (p.splits > 1) hipLaunchKernelGGL((past_dq_join_kernel<T, DP>), dim3((unsigned)(p.dq_vectors / 256)), dim3(256), 0, s, ba);
+    });
+    st = launch_status();
+    if (st) return st;
+  }
+  const int64_t items[3] = {z.groups * z.Hk * p.prefix_blocks, z.B * z.Hk * p.sink_blocks, z.B * z.Hk * (p.key_blocks - p.sink_blocks)};
+  const int64_t splits[3] = {p.prefix_splits, p.sink_splits, p.own_splits};
+  const int64_t blocks = items[0] * splits[0] + items[1] * splits[1] + items[2] * splits[2];
+  if (blocks == 0) return MLORA_OK;
+  with_head(z.f32, z.D, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    auto go = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      hipLaunchKernelGGL((past_dkv_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, ba);
+      for (int c = 0; c < 3; ++c)
+        if (splits[c] > 1)
+          hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, NW>), dim3((unsigned)(items[c] * NW * 2 * (DP / 32))), dim3(256), 0, s, ba, c);
+    };
+    if constexpr (sizeof(T) == 2 && DP == 128) {
+      if (p.nw == 8) return go(std::integral_constant<int, 8>{});
+    }
+    go(std::integral_constant<int, 4>{});
+  });
+  return launch_status();
+}

@@ -1,0 +1,200 @@
+"""Attention of a stream's tokens to their own past.
+
+A streaming student generates a clip chunk by chunk (a few latent frames at a time, or token by token): a token attends
+to its own chunk and to what was generated before it, mostly to the last chunks (a sliding window) and to the first ones
+(sinks), and several samples may continue one past (conditional and unconditional passes, rollouts of one history).
+
+``window_attention(q, k, v, window=..., sinks=..., chunk=...)`` covers whole sequences (training, prompts) and the newest
+tokens of a cache; ``prefix_attention(q, k, v, prefix_k, prefix_v, ...)`` adds a prefix that the samples of a group share,
+read once for all of them where they have few tokens each. Both with gradients of every tensor, the prefix's summed over its
+samples, all in a fixed order. Query heads may share key heads (H a multiple of Hk).
+
+A token at position p of a sample with n keys sees the own keys j < min(e, n) with j >= e - window or j < sinks, where
+e = (p // chunk + 1) * chunk is the end of its chunk, and all keys of its prefix. Queries that are no token of the sample
+(p < 0 or p >= n: padding) get zeros, and so do their gradients, whatever they hold; so do keys behind n. What lies in
+k and v where no token of the sample sees it is not used. A NaN or infinity in v where only some tokens see it may reach
+others among the 128 rows computed with them, as a product with weight zero does.
+
+bf16: scores, softmax and sums in float32; the weights are rounded to bf16 for their products (dS too); out is rounded
+once, and what that rounding left is kept for the backward (bf16, the size of out). float32: float32 throughout, on
+the fp32 matrix core.
+"""
+from __future__ import annotations
+
+import functools
+import math
+
+import torch
+
+from . import kernels
+
+_DTYPES = (torch.bfloat16, torch.float32)
+_MOST = 1 << 28  # tokens
+
+
+def _fail(message: str) -> None:
+    raise RuntimeError("past attention: " + message)
+
+
+def _whole(name: str, value) -> int:
+    if type(value) is int:
+        return value
+    try:
+        whole = int(value)
+    except (TypeError, ValueError, OverflowError, RuntimeError):
+        _fail(f"{name} must be a whole number, got a {type(value).__name__}")
+    if whole != value:
+        _fail(f"{name} must be a whole number")
+    return whole
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    if kernels.attention_layout(t):
+        return t
+    t = t.contiguous()
+    return t if kernels.attention_layout(t) else t.clone()
+
+
+class PastAttentionFunction(torch.autograd.Function):
+    """``apply(cfg, key_lengths, query_start, prefix_lengths, q, k, v[, prefix_k, prefix_v])`` -> out; cfg as _plan
+    gives it."""
+
+    @staticmethod
+    def forward(ctx, cfg, key_lengths, query_start, prefix_lengths, *tensors):
+        tensors = [_aligned(t) for t in tensors]
+        out, rest, stats = kernels.past_attention(*tensors, key_lengths=key_lengths, query_start=query_start,
+                                                  prefix_lengths=prefix_lengths, for_backward=True, checked=True, **cfg)
+        ctx.save_for_backward(key_lengths, query_start, prefix_lengths, out, rest, stats, *tensors)
+        ctx.cfg = cfg
+        return out
+
+    @staticmethod
+    @kernels.first_order
+    def backward(ctx, g):
+        key_lengths, query_start, prefix_lengths, out, rest, stats, *tensors = ctx.saved_tensors
+        g = _aligned(g if g.dtype is out.dtype else g.to(out.dtype))
+        grads = kernels.past_attention_backward(out, rest, stats, g, *tensors, key_lengths=key_lengths, query_start=query_start,
+                                                prefix_lengths=prefix_lengths, checked=True, **ctx.cfg)
+        return (None, None, None, None, *[d if want else None for d, want in zip(grads, ctx.needs_input_grad[4:])])
+
+
+def _meta(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+def _check_vector(name: str, meta, n: int, device) -> None:
+    if meta is not None:
+        shape, dtype, dev = meta
+        if dev != device or dtype not in (torch.int32, torch.int64) or tuple(shape) != (n,):
+            _fail(f"{name} must be int32 or int64 [{n}] on q's device")
+
+
+# What a call's shapes, types and options allow, checked once per combination of them.
+@functools.lru_cache(maxsize=512)
+def _plan(q, k, v, pk, pv, key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale) -> dict:
+    for name, (shape, dtype, device) in (("q", q), ("k", k), ("v", v)):
+        if len(shape) != 4:
+            _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(shape)}")
+        if dtype not in _DTYPES:
+            _fail(f"{name} must be bfloat16 or float32, got {dtype}")
+        if dtype != q[1] or device != q[2]:
+            _fail("q, k and v share one dtype and device")
+    (B, Lq, H, D), dtype, device = q
+    Lk, Hk = k[0][1:3]
+    if k[0] != v[0] or k[0][0] != B or k[0][3] != D:
+        _fail(f"k and v must be [{B}, tokens, heads, {D}], got {tuple(k[0])} and {tuple(v[0])}")
+    if Hk < 1 or H < 1 or H % Hk:
+        _fail(f"{H} query heads do not share {Hk} key heads evenly")
+    if D % 8 or not 8 <= D <= 128:
+        _fail(f"head_dim must be a multiple of 8 up to 128, got {D}")
+    if max(Lq, Lk) > _MOST:
+        _fail(f"at most {_MOST} tokens")
+    if pk is not None:
+        if pk[1:] != q[1:] or pv[1:] != q[1:]:
+            _fail("prefix_k and prefix_v have q's dtype and device")
+        if pk[0] != pv[0] or len(pk[0]) != 4 or tuple(pk[0][2:]) != (Hk, D):
+            _fail(f"prefix_k and prefix_v must be [tokens, {Hk}, {D}] or [groups, tokens, {Hk}, {D}], got {tuple(pk[0])} and {tuple(pv[0])}")
+        if pk[0][0] < 1 or B % pk[0][0]:
+            _fail(f"{B} samples do not share {pk[0][0]} prefixes evenly")
+        if pk[0][1] > _MOST:
+            _fail(f"at most {_MOST} tokens")
+        _check_vector("prefix_lengths", prefix_lengths, pk[0][0], device)
+    if chunk < 1:
+        _fail(f"chunk must be at least 1, got {chunk}")
+    if window is not None and window < chunk:
+        _fail(f"window must be at least chunk ({chunk}), so that every token sees its own chunk; got {window}")
+    if sinks < 0:
+        _fail(f"sinks must not be negative, got {sinks}")
+    _check_vector("key_lengths", key_lengths, B, device)
+    if isinstance(query_start, tuple):
+        _check_vector("query_start", query_start, B, device)
+    elif query_start is None and Lq > Lk:
+        _fail(f"{Lq} queries are no tokens of {Lk} keys: give query_start")
+    scale = D ** -0.5 if scale is None else scale
+    if not (math.isfinite(scale) and scale > 0):
+        _fail("scale must be positive")
+    if device.type != "cuda":
+        _fail("the tensors must be ROCm device tensors")
+    # past these nothing changes, and they fit the kernels' integers
+    start = 0 if isinstance(query_start, tuple) else Lk - Lq if query_start is None else max(-Lq, min(query_start, Lk))
+    chunk = min(chunk, max(Lk, 1))
+    return dict(window=0 if window is None else min(max(window, chunk), Lk + chunk), sinks=min(sinks, Lk), chunk=chunk, scale=scale,
+                first=start, from_end=query_start is None and key_lengths is not None and Lq < Lk)
+
+
+def _int32(t: torch.Tensor | None, low: int, high: int) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype is torch.int64:
+        t = t.clamp(low, high).to(torch.int32)
+    return t.contiguous()
+
+
+def _attend(tensors, key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale):
+    if scale is not None:
+        scale = kernels.number("scale", scale, _fail)
+    start = query_start
+    if isinstance(start, torch.Tensor) and start.dim():
+        start = _meta(start)
+    elif start is not None:
+        start, query_start = _whole("query_start", start), None
+    metas = [_meta(t) for t in tensors]
+    cfg = _plan(*metas, *(() if len(tensors) == 5 else (None, None)), _meta(key_lengths), start, _meta(prefix_lengths),
+                None if window is None else _whole("window", window), _whole("sinks", sinks), _whole("chunk", chunk), scale)
+    Lq, Lk = tensors[0].shape[1], tensors[1].shape[1]
+    key_lengths = _int32(key_lengths, 0, Lk)
+    query_start = _int32(query_start, -Lq, Lk)
+    if prefix_lengths is not None:
+        prefix_lengths = _int32(prefix_lengths, 0, tensors[3].shape[1])
+    if kernels.wants_grad(tensors):
+        return PastAttentionFunction.apply(cfg, key_lengths, query_start, prefix_lengths, *tensors)
+    return kernels.past_attention(*[_aligned(t) for t in tensors], key_lengths=key_lengths, query_start=query_start,
+                                  prefix_lengths=prefix_lengths, checked=True, **cfg)[0]
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                     chunk: int = 1, key_lengths: torch.Tensor | None = None, query_start: torch.Tensor | int | None = None,
+                     scale: float | None = None) -> torch.Tensor:
+    """softmax(scale q kᵀ) v per head over the keys that a token sees, [B, Lq, H, D] contiguous in q's dtype.
+
+    q [B, Lq, H, D], k and v [B, Lk, Hk, D], bfloat16 or float32, D a multiple of 8 up to 128. window: how many keys up
+    to the end of its own chunk a token sees (at least chunk; None: all before it too). sinks: the first keys that stay visible.
+    chunk: tokens that see each other (1: each sees itself and those before it). key_lengths: int32 or int64 [B] on q's device,
+    the number of leading keys a sample has (clamped to [0, Lk]). query_start: the position of q's first token, a whole
+    number or int32 / int64 [B] on q's device; if not given, the queries are the last Lq of Lk tokens, and with key_lengths and
+    Lq < Lk the last Lq of each sample's (a cache). scale > 0, 1 / sqrt(D) if not given."""
+    return _attend((q, k, v), key_lengths, query_start, None, window, sinks, chunk, scale)
+
+
+def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, *,
+                     window: int | None = None, chunk: int = 1, key_lengths: torch.Tensor | None = None,
+                     prefix_lengths: torch.Tensor | None = None, query_start: torch.Tensor | int | None = None,
+                     scale: float | None = None) -> torch.Tensor:
+    """window_attention of samples that continue a common prefix: every token sees all keys of its prefix as well.
+
+    prefix_k and prefix_v: [Lp, Hk, D] for all samples, or [groups, Lp, Hk, D], each for B / groups samples in a row.
+    prefix_lengths: int32 or int64 [groups] on q's device, the leading keys a prefix has (clamped to [0, Lp]). k and v hold the
+    samples' own keys; positions, window, chunk and key_lengths count these alone."""
+    if prefix_k.dim() == 3 and prefix_v.dim() == 3:
+        prefix_k, prefix_v = prefix_k.unsqueeze(0), prefix_v.unsqueeze(0)
+    return _attend((q, k, v, prefix_k, prefix_v), key_lengths, query_start, prefix_lengths, window, 0, chunk, scale)

@@ -598,6 +598,46 @@ int mlora_cross_attention_backward(const void *q, const int64_t *q_strides, cons
                                    void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes,
                                    int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, void *stream);
 
+/* ------------------------------------------------------------------ attention of tokens to their own past
+ *
+ * q [B, Lq, H, D], k and v [B, Lk, Hk, D] (bf16 or float32, one type; unit stride in the head, element strides {batch,
+ * token, head}, multiples of 8, token strides below 2^22, 16-byte aligned); query head h reads key head h / (H / Hk). Sample b
+ * has its first n = key_lengths[b] keys (NULL: Lk; clamped to [0, Lk]); its query i sits at position p = start + i,
+ * start = query_start[b], or, with query_start NULL, n - Lq where from_end is set, else first. With
+ * e = (p / chunk + 1) * chunk, the end of the query's chunk, it sees
+ *   the keys j < min(e, n) with j >= e - window (window 0: all of them) or j < sinks, and
+ *   with groups > 0 its prefix: the first prefix_lengths[g] (NULL: Lp; clamped) keys of pk / pv [groups, Lp, Hk, D],
+ *   g = b / (B / groups), shared by the group's samples.
+ * out = softmax(scale * q kT) v over these keys. Queries with p < 0 or p >= n belong to no token: zeros. Keys that no query
+ * of a sample sees may hold anything. window is 0 or at least chunk; D a multiple of 8 up to 128; Lq, Lk and Lp up to 2^28;
+ * scale > 0 and scale * log2 e finite in float32.
+ *   out    [B, Lq, H, D] contiguous
+ *   stats  NULL, or float [2 * B * H * Lq] for the backward; rest then takes what out's rounding to bf16 left ([B, Lq, H, D]
+ *          bf16; NULL for float32)
+ * workspace (16-byte aligned, the queried bytes, 0: may be NULL) holds partial sums. */
+typedef struct mlora_past_shape {
+  int32_t dtype, from_end;
+  int64_t B, Lq, Lk, H, Hk, D, groups, Lp, window, sinks, chunk, first;
+  int64_t q_strides[3], k_strides[3], v_strides[3], pk_strides[3], pv_strides[3];
+  float scale;
+} mlora_past_shape;
+
+int64_t mlora_past_attention_workspace_bytes(const mlora_past_shape *shape);
+int mlora_past_attention(const mlora_past_shape *shape, const void *q, const void *k, const void *v, const void *pk,
+                         const void *pv, const int32_t *key_lengths, const int32_t *query_start,
+                         const int32_t *prefix_lengths, void *out, void *rest, float *stats, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+
+/* Its gradients for the upstream g ([B, Lq, H, D], strided like q): dq, dk, dv and, with a prefix, dpk and dpv (summed over
+ * the group's samples), contiguous, zeros where nothing counts. out, rest and stats are the forward's. Sums have a fixed
+ * order. */
+int64_t mlora_past_attention_backward_workspace_bytes(const mlora_past_shape *shape);
+int mlora_past_attention_backward(const mlora_past_shape *shape, const void *q, const void *k, const void *v, const void *pk,
+                                  const void *pv, const int32_t *key_lengths, const int32_t *query_start,
+                                  const int32_t *prefix_lengths, const void *out, const void *rest, const float *stats,
+                                  const void *g, const int64_t *g_strides, void *dq, void *dk, void *dv, void *dpk, void *dpv,
+                                  void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

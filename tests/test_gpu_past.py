@@ -1,0 +1,332 @@
+"""Windowed attention with sinks and attention to a shared prefix against the 64-bit definition (past_reference.check derives
+the tolerances)."""
+import math
+
+import pytest
+import torch
+
+import past_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF, F = torch.bfloat16, torch.float32
+
+
+def make(dtype, dev, seed, B, Lq, Lk, H, Hk, D, groups=0, Lp=0, loud=1.5):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(dtype).to(dev)  # noqa: E731
+    t = [r(B, Lq, H, D, std=loud), r(B, Lk, Hk, D), r(B, Lk, Hk, D)]
+    if groups:
+        t += [r(groups, Lp, Hk, D), r(groups, Lp, Hk, D)]
+    return t, r(B, Lq, H, D)
+
+
+def run(pkg, tensors, g=None, *, plens=None, lengths=None, start=None, **kw):
+    """{"out": ..., "dq": ...} through the public entry points."""
+    dev = tensors[0].device
+    on = lambda t: t.to(dev) if isinstance(t, torch.Tensor) else t  # noqa: E731
+    leaves = [t.detach().requires_grad_(g is not None) for t in tensors]
+    if len(tensors) == 3:
+        out = pkg.window_attention(*leaves, key_lengths=on(lengths), query_start=on(start), **kw)
+    else:
+        out = pkg.prefix_attention(*leaves, key_lengths=on(lengths), query_start=on(start), prefix_lengths=on(plens), **kw)
+    got = {"out": out.detach()}
+    if g is not None:
+        got.update(zip(("dq", "dk", "dv", "dpk", "dpv"), torch.autograd.grad(out, leaves, [g])))
+    return got
+
+
+def both(pkg, tensors, g, **kw):
+    got = run(pkg, tensors, g, **kw)
+    ref.check(got, *tensors, do=g, **kw)
+    with torch.no_grad():
+        assert torch.equal(run(pkg, tensors, **kw)["out"], got["out"])
+    return got
+
+
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+
+SEQUENCES = [  # B, L, H, Hk, D, options
+    (1, 1, 1, 1, 8, dict(window=1)),
+    (2, 2, 2, 1, 16, dict(window=1, sinks=1)),
+    (1, 33, 4, 4, 64, dict()),                                   # causal alone
+    (2, 64, 4, 2, 40, dict(window=64)),
+    (1, 65, 6, 2, 72, dict(window=7, sinks=2)),                  # three heads to a key head: tokens end inside a wave
+    (2, 130, 3, 1, 128, dict(window=40, sinks=3, chunk=13)),
+    (1, 300, 2, 2, 96, dict(window=128, sinks=70, chunk=64)),    # sinks past a tile
+    (1, 517, 5, 1, 64, dict(window=100, sinks=130, chunk=1)),    # sinks and window meet in the first tokens
+    (2, 257, 1, 1, 128, dict(window=300, sinks=5, chunk=300)),   # one chunk: everything
+    (1, 700, 2, 1, 128, dict(window=33, sinks=1, chunk=32)),
+    (1, 1030, 2, 2, 32, dict(window=256, sinks=4)),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", SEQUENCES, ids=str)
+def test_sequences(pkg, dev, case, ragged, dtype):
+    B, L, H, Hk, D, kw = case
+    tensors, g = make(dtype, dev, L + H, B, L, L, H, Hk, D)
+    lengths = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(L)) if ragged else None
+    both(pkg, tensors, g, lengths=lengths, **kw)
+
+
+CACHES = [  # B, Lq, Lk, H, Hk, D, options
+    (3, 1, 700, 8, 2, 128, dict(window=100, sinks=4)),
+    (1, 1, 5000, 4, 4, 64, dict(window=4000, sinks=40)),          # shared out and joined
+    (2, 5, 333, 6, 2, 72, dict(window=64, sinks=9, chunk=4)),
+    (2, 40, 260, 2, 2, 128, dict(window=50, sinks=1)),            # 40 rows: two blocks of rows per wave
+    (1, 70, 2100, 4, 2, 96, dict(window=900, sinks=64, chunk=35)),  # more rows than one wave's, shared out
+    (2, 156, 999, 3, 3, 128, dict(window=468, sinks=156, chunk=156)),
+    (2, 3, 90, 4, 1, 8, dict()),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("where", ["end", "lengths", "start", "number"])
+@pytest.mark.parametrize("case", CACHES, ids=str)
+def test_caches(pkg, dev, case, where, dtype):
+    B, Lq, Lk, H, Hk, D, kw = case
+    tensors, g = make(dtype, dev, Lk + Lq, B, Lq, Lk, H, Hk, D)
+    lengths = i32(*[Lk, Lk // 3, Lq // 2][:B]) if where == "lengths" else None  # fewer keys than queries: padding in front
+    start = {"start": i32(*[Lk - 2 * Lq, 0, -1][:B]), "number": Lk // 2}.get(where)
+    both(pkg, tensors, g, lengths=lengths, start=start, **kw)
+
+
+PREFIXES = [  # groups, each, Lq, Lk, Lp, H, Hk, D, options
+    (1, 1, 1, 1, 1, 1, 1, 8, dict()),
+    (1, 3, 1, 9, 100, 4, 4, 64, dict()),
+    (2, 2, 7, 50, 333, 6, 2, 72, dict(window=20)),
+    (1, 8, 1, 70, 20000, 8, 8, 128, dict()),                      # computed once for eight samples
+    (2, 5, 2, 33, 9001, 8, 4, 128, dict(window=16)),              # 20 rows to a group's key head
+    (1, 40, 1, 12, 4100, 8, 2, 128, dict()),                      # 160 rows: the prefix on 128 rows per workgroup
+    (3, 2, 65, 65, 130, 2, 1, 128, dict(chunk=65)),
+    (1, 2, 200, 200, 515, 3, 3, 40, dict(chunk=50, window=100)),
+    (1, 4, 129, 129, 0, 2, 2, 64, dict()),                        # no prefix at all
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", PREFIXES, ids=str)
+def test_prefixes(pkg, dev, case, ragged, dtype):
+    groups, each, Lq, Lk, Lp, H, Hk, D, kw = case
+    B = groups * each
+    tensors, g = make(dtype, dev, Lp + Lq, B, Lq, Lk, H, Hk, D, groups, Lp)
+    gen = torch.Generator().manual_seed(Lp)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=gen) if ragged else None
+    plens = torch.randint(0, Lp + 1, (groups,), generator=gen, dtype=torch.int32) if ragged else None
+    both(pkg, tensors, g, lengths=lengths, plens=plens, **kw)
+    if groups == 1 and not ragged:  # a prefix without a group axis
+        flat = [*tensors[:3], tensors[3][0], tensors[4][0]]
+        with torch.no_grad():
+            assert torch.equal(pkg.prefix_attention(*flat, **kw), run(pkg, tensors, **kw)["out"])
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq", [1, 40, 150])
+def test_what_no_token_sees_may_hold_anything(pkg, dev, Lq, dtype):
+    """Keys behind a sample's length, between the sinks and the window of its first token, and behind its last token's chunk;
+    padding queries and their upstream gradients: NaN, infinities, the type's lowest value. Samples without a key or whose
+    queries are all padding give zeros."""
+    B, Lk, H, D = 4, 400, 2, 64
+    tensors, g = make(dtype, dev, 5, B, Lq, Lk, H, H, D, 2, 90)
+    lengths, plens = i32(400, 390, 0, 300), i32(90, 33)
+    start = i32(200, 390 - Lq // 2, 0, -Lq)
+    kw = dict(window=60, chunk=4, lengths=lengths, start=start)
+    for t, more in ((tensors[:3], dict(sinks=5)), (tensors, dict(plens=plens))):
+        got = run(pkg, t, g, **kw, **more)
+        ref.check(got, *t, do=g, **kw, **more)
+        for name in ("out", "dq", "dk", "dv"):
+            assert got[name][2].abs().sum() == 0 and got[name][3].abs().sum() == 0
+        dirty, dg = [x.clone() for x in t], g.clone()
+        for bad_k, bad_v in ((math.nan, math.inf), (math.inf, math.nan), (torch.finfo(dtype).min, -math.inf)):
+            for b, (n, first) in enumerate(ref.starts_of(B, Lq, Lk, lengths, start)):
+                vis = ref.seen(Lq, Lk, n, first, 60, more.get("sinks", 0), 4)
+                dirty[1][b, ~vis.any(0).to(dev)], dirty[2][b, ~vis.any(0).to(dev)] = bad_k, bad_v
+                dirty[0][b, ~vis.any(1).to(dev)], dg[b, ~vis.any(1).to(dev)] = bad_v, bad_k
+            if len(t) == 5:
+                dirty[3][1, 33:], dirty[4][1, 33:] = bad_k, bad_v
+            again = run(pkg, dirty, dg, **kw, **more)
+            assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+def test_int64_vectors_and_values_out_of_range(pkg, dev):
+    tensors, g = make(BF, dev, 6, 3, 9, 50, 2, 2, 64, 3, 20)
+    for dt in (torch.int32, torch.int64):
+        far = 2 ** 31 - 1 if dt is torch.int32 else 2 ** 40
+        lengths, plens, start = (torch.tensor(v, dtype=dt) for v in ([-5, far, 17], [far, -1, 3], [41, -far, far]))
+        both(pkg, tensors, g, lengths=lengths, plens=plens, start=start, window=8)
+        got = both(pkg, tensors, g, start=far)
+        assert got["out"].abs().sum() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq", [2, 100])
+def test_options_past_the_range(pkg, dev, Lq, dtype):
+    """Windows, chunks and sinks of any size mean all keys; a given scale; loud scores that rise and fall along the keys."""
+    tensors, g = make(dtype, dev, 8, 2, Lq, 150, 2, 1, 32, loud=6.0)
+    big = 2 ** 40
+    whole = both(pkg, tensors, g, scale=0.3)
+    for kw in (dict(window=big), dict(window=1, sinks=big)):
+        got = run(pkg, tensors, g, scale=0.3, **kw)
+        assert torch.equal(got["out"], whole["out"]) or kw.get("window") == 1
+        ref.check(got, *tensors, do=g, scale=0.3, **kw)
+    ramp = torch.linspace(0.1, 8.0, 150, device=dev).view(1, 150, 1, 1).to(dtype)
+    for r in (ramp, ramp.flip(1)):
+        both(pkg, [tensors[0], tensors[1] * r, tensors[2]], g, window=big, chunk=big)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq, Lk", [(3, 50), (3, 3000), (200, 200)])
+def test_very_low_scores_are_scores(pkg, dev, Lq, Lk, dtype):
+    """Every score -2^103 (exact in bf16 and float32): all visible keys weigh the same, forward and backward: dv is the sum of
+    do over the rows that see the key, each with weight 1 / its number of keys."""
+    (q, k, v), g = make(dtype, dev, 5, 1, Lq, Lk, 2, 2, 32)
+    q, k = torch.full_like(q, 2.0 ** 49), torch.full_like(k, -(2.0 ** 49))
+    got = run(pkg, [q, k, v], g, window=40, sinks=3, scale=1.0)
+    vis = ref.seen(Lq, Lk, Lk, Lk - Lq, 40, 3, 1).double()
+    p = vis / vis.sum(1, keepdim=True)
+    u = ref.half_step(dtype)
+    for name, w, t in (("out", p, v), ("dv", p.T, g)):
+        t = ref.f64(t)[0]
+        want, size = (torch.einsum("ij,jhd->ihd", w, x) for x in (t, t.abs()))
+        room = u * want.abs() + (2 ** -20 + 50 * 2 ** -24 + (u if dtype is BF else 0)) * size
+        assert ((ref.f64(got[name])[0] - want).abs() <= room).all(), name
+
+
+def test_layouts(pkg, dev):
+    """q of one packed [B, L, 3, H, D], k and v slices of a joint cache, head-major storage, misaligned storage, token strides
+    past the kernels' limit, an expanded batch, a transposed gradient."""
+    H, D = 4, 64
+    gen = torch.Generator().manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev).to(BF)  # noqa: E731
+    q, kv, g = r(2, 50, 3, H, D)[:, :, 1], r(2, 90, 2, H, D), r(2, H, 50, D).transpose(1, 2)
+    both(pkg, [q, kv[:, :, 0], kv[:, :, 1]], g, window=20, sinks=2)
+    head_major = r(2, H, 90, D).transpose(1, 2)
+    odd = r(2 * 90 * H * D + 3)[3:].view(2, 90, H, D)
+    both(pkg, [q, head_major, odd], g, window=20)
+    one = r(1, 90, H, D).expand(2, 90, H, D)
+    both(pkg, [q, one, kv[:, :, 1], r(1, 40, 2, H, D)[:, :, 1], r(1, H, 40, D).transpose(1, 2)], g, chunk=10)
+    wide = r(3, (1 << 22) + 8).as_strided((1, 3, H, D), (0, (1 << 22) + 8, D, 1))
+    both(pkg, [wide, wide, wide], torch.ones_like(wide), window=2)
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 7, 3), (2, 0, 7, 3), (2, 5, 0, 3), (2, 5, 7, 0), (2, 0, 0, 0)])
+def test_empty(pkg, dev, shape):
+    B, Lq, Lk, Lp = shape
+    tensors, g = make(BF, dev, 1, B, Lq, Lk, 4, 2, 64, 1, Lp)
+    for t in (tensors[:3], tensors):
+        got = run(pkg, t, g, start=0)
+        ref.check(got, *t, do=g, start=0)
+
+
+def test_fixed_order_and_partial_gradients(pkg, dev):
+    tensors, g = make(BF, dev, 3, 4, 130, 130, 4, 2, 128, 2, 300)
+    first = run(pkg, tensors, g, chunk=10)
+    again = run(pkg, tensors, g, chunk=10)
+    assert all(torch.equal(first[n], again[n]) for n in first)
+    for i, name in enumerate(("dq", "dk", "dv", "dpk", "dpv")):
+        leaves = [t.detach().requires_grad_(j == i) for j, t in enumerate(tensors)]
+        got, = torch.autograd.grad(pkg.prefix_attention(*leaves, chunk=10), [leaves[i]], [g])
+        assert torch.equal(got, first[name])
+    x = tensors[0].detach().requires_grad_(True)
+    with pytest.raises(RuntimeError):  # the backward itself is not differentiable, and says so
+        (d,) = torch.autograd.grad(pkg.window_attention(x, *tensors[1:3]), [x], [g], create_graph=True)
+        d.float().sum().backward()
+
+
+def test_gradient_against_differences(pkg, dev):
+    """The kernel's float32 gradients against differences of the 64-bit definition."""
+    from block_reference import finite_difference
+    tensors, g = make(F, dev, 13, 4, 9, 21, 4, 2, 32, 2, 6)
+    kw = dict(window=5, chunk=2, lengths=i32(21, 12, 9, 4), plens=i32(6, 2))
+    got = run(pkg, tensors, g, **kw)
+    args = [ref.f64(t) for t in tensors]
+    for i, name in enumerate(("dq", "dk", "dv", "dpk", "dpv")):
+        d = torch.randn(args[i].shape, generator=torch.Generator().manual_seed(i)).double()
+
+        def f(x, i=i):
+            return float((ref.attention(*(x if j == i else t for j, t in enumerate(args)), **kw)[0]["out"] * ref.f64(g)).sum())
+
+        want = finite_difference(f, args[i], d, 1e-5)
+        have = ref.f64(got[name]) * d
+        assert abs(float(have.sum()) - want) <= 2 ** -15 * float(have.abs().sum()) + 1e-6
+
+
+def test_captured_and_replayed(pkg, dev):
+    """Training, a cache's next token and a shared prefix in one HIP graph, replayed with other inputs and lengths."""
+    train, g = make(BF, dev, 19, 2, 300, 300, 2, 1, 128)
+    token, _ = make(BF, dev, 20, 2, 1, 6000, 4, 2, 128)
+    shared, _ = make(BF, dev, 21, 8, 1, 30, 8, 8, 128, 1, 9000)
+    lengths = torch.tensor([300, 200], dtype=torch.int32, device=dev)
+    filled = torch.tensor([6000, 10], dtype=torch.int32, device=dev)
+    for t in train:
+        t.requires_grad_(True)
+
+    def step():
+        out = pkg.window_attention(*train, window=70, sinks=2, key_lengths=lengths)
+        with torch.no_grad():
+            more = [pkg.window_attention(*token, window=4000, sinks=4, key_lengths=filled), pkg.prefix_attention(*shared)]
+        return [out.detach(), *more, *torch.autograd.grad(out, train, [g])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(4):
+        gen = torch.Generator().manual_seed(seed)
+        with torch.no_grad():
+            for t in (*train, g, *token, *shared):
+                t.copy_(torch.randn(t.shape, generator=gen))
+            lengths.fill_(90 * seed)
+            filled.copy_(torch.tensor([1500 * seed + 1, 5000 - seed]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(pkg, dev):
+    """Calls on two streams have workspaces of their own."""
+    a, ga = make(BF, dev, 31, 1, 500, 500, 4, 4, 128)
+    b, gb = make(BF, dev, 32, 8, 1, 40, 8, 8, 128, 1, 9000)
+    want = run(pkg, a, ga, window=100, sinks=3), run(pkg, b, gb)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(3):
+        for s, args, kw in ((streams[0], (a, ga), dict(window=100, sinks=3)), (streams[1], (b, gb), {})):
+            with torch.cuda.stream(s):
+                got.append(run(pkg, *args, **kw))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert all(torch.equal(x[n], want[i % 2][n]) for n in x)
+
+
+def test_a_frame_of_a_long_clip(pkg, dev):
+    """A late frame of a Wan clip, tokens and keys of whole frames, two heads of it in 64 bits."""
+    L, C, H, D = 12480, 1560, 2, 128
+    tensors, _ = make(BF, dev, 23, 1, C, L, H, H, D)
+    got = run(pkg, tensors, window=4 * C, sinks=C, chunk=C)
+    keys = [*range(C), *range(L - 4 * C, L)]
+    q, k, v = (t[:, keys] if t.shape[1] == L else t for t in tensors)
+    ref.check(got, q, k, v, chunk=len(keys), start=0)
+
+
+def test_offsets_past_32_bits(pkg, dev):
+    """The last tokens of a cache of 2^31 + elements per sample and a prefix behind 2^31 elements."""
+    H, D, Lk = 8, 128, 1100000  # 1.13e9 elements a sample: 4.5 GB for k and v in bf16
+    base = torch.zeros(2 * Lk, 2, H, D, dtype=BF, device=dev)
+    tail, g = make(BF, dev, 29, 1, 4, 600, H, H, D)
+    base[-600:, 0], base[-600:, 1] = tail[1][0], tail[2][0]
+    k, v = base[Lk:, 0].unsqueeze(0), base[Lk:, 1].unsqueeze(0)
+    got = run(pkg, [tail[0], k, v], window=500, sinks=0)
+    ref.check(got, *tail, window=500)
+    whole = base.view(1, 2 * Lk, 2, H, D)  # token offsets of 4.5e9 elements
+    got = run(pkg, [tail[0], whole[:, :, 0], whole[:, :, 1]], window=500)
+    ref.check(got, *tail, window=500)
