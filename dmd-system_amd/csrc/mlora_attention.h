@@ -188,6 +188,12 @@ struct TileLoader {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (MLORA_LDS void *)(lds + blk * 1024), 16, on ? off[i] : kOOB, 0, 0, 0);
     }
   }
+  __device__ __forceinline__ void load_all(const void *base, MLORA_LDS char *lds) const {  // every row is live
+    const auto rsrc = make_rsrc(base, (int64_t)kOOB);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (MLORA_LDS void *)(lds + (first + i * step) * 1024), 16, off[i], 0, 0, 0);
+  }
 };
 
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }

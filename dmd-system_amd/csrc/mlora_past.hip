@@ -282,27 +282,206 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_fwd_kernel(c
   }
 }
 
-// Few rows (at most 32 NQ): the NW waves take different key tiles, each with its own buffers (no barrier in the loop),
-// and their running softmaxes are joined through LDS. Bound by the reading of K and V.
+// ---------------------------------------------------------------- few rows
+//
+// Blocks of 16 rows on 16 x 16 products: D[16 x 16] += A[16 x 32] B[32 x 16], a lane holds row (or column) lane % 16 and 8 of the
+// step's 32 contraction elements, its quarter lane / 16 decides which; the result leaves it column lane % 16 and rows
+// 4·(lane / 16) + i. S^T = K·Q^T of 16 keys leaves a lane four keys of its query; two such blocks are the eight
+// contraction elements of O^T += V^T·P^T, keys 4g + j and 16 + 4g + j of 32.
+__device__ __forceinline__ f32x4 mma32(const Frag<uint16_t> &a, const Frag<uint16_t> &b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a.v), as_bf16x8(b.v), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma32(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+// over the four quarters of a column
+__device__ __forceinline__ float quarter_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// A lane's addresses for such fragments of a HeadTile. keys: row R0 + lane % 16, elements 32s + 8·(lane / 16) .. + 7; values: column
+// 16d + lane % 16 of the 32 rows in the order above.
 template <class T, int DP>
-struct PastFew {
-  static constexpr int KT = 32, NW = sizeof(T) * DP == 512 ? 2 : 4;  // 128 KB of LDS at most
+struct FewReader;
+template <int DP>
+struct FewReader<uint16_t, DP> {
+  using Tile = HeadTile<uint16_t, DP>;
+  int32_t row[DP / 32], col[DP / 16];
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
+    const int32_t at = (int32_t)(uintptr_t)base;
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) row[s] = at + r * Tile::RB + (((4 * s + g) ^ Tile::swz(r)) << 4);
+    const int key = 4 * g + (r >> 2), c = r & 3;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) col[d] = at + key * Tile::RB + (((2 * d + (c >> 1)) ^ Tile::swz(key)) << 4) + 8 * (c & 1);
+  }
+  template <int OFF, int R0>  // swz(r + 16) = swz(r)
+  __device__ __forceinline__ void keys(int s, Frag<uint16_t> &f) const {
+    f.v = *(const lds_u4 *)((const MLORA_LDS char *)(uintptr_t)(uint32_t)row[s] + OFF + R0 * Tile::RB);
+  }
+  template <int OFF>
+  __device__ __forceinline__ void values(int d, Frag<uint16_t> &f) const {
+    typedef MLORA_LDS bf16x4 lds_b4;
+    const MLORA_LDS char *p = (const MLORA_LDS char *)(uintptr_t)(uint32_t)col[d] + OFF;
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)p));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)(p + 16 * Tile::RB)));
+    f.v = u32x4{x[0], x[1], y[0], y[1]};
+  }
+};
+template <int DP>
+struct FewReader<float, DP> {
+  using Tile = HeadTile<float, DP>;
+  int32_t row, at, sw, r, g;
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
+    r = lane & 15, g = lane >> 4, sw = Tile::swz(r);
+    at = (int32_t)(uintptr_t)base, row = at + r * Tile::RB;
+  }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void keys(int s, Frag<float> &f) const {
+    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)row + OFF + R0 * Tile::RB;
+    const f32x4 a = *(const lds_f4 *)(t + (((8 * s + 2 * g) ^ sw) << 4)), b = *(const lds_f4 *)(t + (((8 * s + 2 * g + 1) ^ sw) << 4));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.v[j] = a[j], f.v[j + 4] = b[j];
+  }
+  template <int OFF>
+  __device__ __forceinline__ void values(int d, Frag<float> &f) const {
+    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)at + OFF;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = 16 * (j / 4) + 4 * g + j % 4, chunk = 4 * d + (r >> 2);
+      f.v[j] = *(const MLORA_LDS float *)(t + key * Tile::RB + ((chunk ^ Tile::swz(key)) << 4) + 4 * (r & 3));
+    }
+  }
 };
 
-template <class T, int DP, int NQ>
-__global__ __launch_bounds__((64 * PastFew<T, DP>::NW), 1) void past_few_kernel(const PastArgs a) {
-  constexpr int KT = PastFew<T, DP>::KT, NW = PastFew<T, DP>::NW, ND = DP / 32;
+// The running softmax of NC x 16 rows against 32 keys per step, as Softmax does it (two sums: e of the weights before their
+// rounding to bf16, l of what the product with V sees).
+template <class T, int DP, int NC>
+struct FewSoftmax {
+  static constexpr int ND = DP / 16, NS = DP / 32;
+  f32x4 o[NC][ND];
+  Frag<T> q[NC][NS];
+  float m[NC], l[NC], e[NC];
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      m[n] = kNoMax, l[n] = 0.f, e[n] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  template <int KOFF, int VOFF>
+  __device__ __forceinline__ void step(const FewReader<T, DP> &fr, bool masked, const uint32_t (&bits)[NC], float c, int lane) {
+    f32x4 s[NC][2];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks)
+      static_for<2>([&](auto kb) __attribute__((always_inline)) {
+        Frag<T> kf;
+        fr.template keys<KOFF, 16 * decltype(kb)::value>(ks, kf);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][kb] = mma32(kf, q[n][ks], s[n][kb]);
+        return true;
+      });
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const uint32_t mine = bits[n] >> (4 * (lane >> 4));
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][kb][i] = (mine >> (16 * kb + i)) & 1 ? s[n][kb][i] : -INFINITY;
+      }
+    }
+    Frag<T> p[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                       fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+      mx = quarter_max(mx);
+      RowRef ref = row_ref(m[n], c);
+      if (__any(__builtin_fmaf(mx - ref.a, c, -ref.r) > 8.f)) {
+        m[n] = fmaxf(m[n], mx);
+        const RowRef up = row_ref(m[n], c);
+        const float f = ref_factor(ref, up, c);
+        ref = up;
+        l[n] *= f, e[n] *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[n][d] *= f;
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][i] - ref.a, c, -ref.r));
+      if constexpr (sizeof(T) == 2) {
+        const auto ones = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[n].v[j] = pack2_bf16(s[n][j / 2][2 * (j % 2)], s[n][j / 2][2 * (j % 2) + 1]);
+          l[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)p[n].v[j]), ones, l[n], false);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[n].v[j] = s[n][j / 4][j % 4];
+      }
+      const f32x4 t = s[n][0] + s[n][1];
+      e[n] += (t[0] + t[1]) + (t[2] + t[3]);
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      Frag<T> vf;
+      fr.template values<VOFF>(d, vf);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) o[n][d] = mma32(vf, p[n], o[n][d]);
+    }
+  }
+
+  __device__ __forceinline__ float sums(int n, float &f) {
+    const float ew = quarter_sum(e[n]);
+    f = 1.f;
+    if constexpr (sizeof(T) == 4) return ew;
+    const float lw = quarter_sum(l[n]);
+    if (lw > 0.f) f = ew / lw;
+    return lw > 0.f ? ew : lw;
+  }
+};
+
+// Few rows (16 NC per workgroup): the waves take different key tiles, each with its own buffer (no barrier in the loop; two
+// waves per SIMD, one multiplies while the other waits), and their running softmaxes are joined through LDS. Bound by the reading
+// of K and V where they are long (65520 keys, 8 key heads of 128: 46 us, 5.9 TB/s), by a launch and one chain of loads,
+// products and the join where they are short (32 keys 5.4 us, 260 keys of 64 channels 6.1). On 32 x 32 products, four waves with two
+// buffers each: 51, 7.7 and 8.3.
+template <class T, int DP, int NC>
+struct PastFew {
+  static constexpr int KT = 32, NW = sizeof(T) * DP == 512 ? 4 : 8;
+};
+
+template <class T, int DP, int NC>
+__global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>::NW / 4)) void past_few_kernel(const PastArgs a) {
+  using C = PastFew<T, DP, NC>;
+  constexpr int KT = C::KT, NW = C::NW, ND = DP / 16;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024;
-  static_assert(NW * NQ * ND * 4 * 64 * 16 <= 4 * TB * NW, "the waves' sums fit the buffers");
-  // one array, so that the readers' buffers start at multiples of 4 TB; (m, l) of [wave][n][query] behind them
-  __shared__ u32x4 smem[4 * TB * NW / 16 + NW * NQ * 16];
-  float2 (&ml)[NW][NQ][32] = *(float2 (*)[NW][NQ][32])(smem + 4 * TB * NW / 16);
+  static_assert(NC * ND * 64 * 16 <= 2 * TB, "a wave's sums fit its buffers");
+  // one array, (m, l) of [wave][n][query] behind them
+  __shared__ u32x4 smem[2 * TB * NW / 16 + NW * NC * 8];
+  float2 (&ml)[NW][NC][16] = *(float2 (*)[NW][NC][16])(smem + 2 * TB * NW / 16);
   const int wave = wave_id(), lane = threadIdx.x & 63;
-  MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 4 * TB;
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 2 * TB;
   Job job;
   job.init(a, blockIdx.x);
-  const int hk = job.hk, group = job.packed ? job.b : job.b / a.each;
+  const int hk = job.hk, r0 = job.rt * 16 * NC, group = job.packed ? job.b : job.b / a.each;
   Sample s{1, 0};
   KeyTiles<KT> tiles;
   WaveRows wr;
@@ -311,8 +490,9 @@ __global__ __launch_bounds__((64 * PastFew<T, DP>::NW), 1) void past_few_kernel(
     tiles.init(a, prefix_keys(a, group), 0, 0, 0);
   } else {
     s = uniform(sample_of(a, job.b));
-    tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start, 0), min(s.start + a.Lq - 1, s.n - 1));
-    wr.init(a, s, 0, a.rows);
+    tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start + r0 / a.G, 0),
+               min(s.start + min(r0 + 16 * NC - 1, a.rows - 1) / a.G, s.n - 1));
+    wr.init(a, s, r0, min(r0 + 16 * NC, a.rows));
   }
   const int t1 = job.share(tiles.count, job.sp + 1), t0 = min(job.share(tiles.count, job.sp) + wave, t1);
   const T *kp = static_cast<const T *>(a.k) + job.b * a.k_sb + hk * a.k_sh, *vp = static_cast<const T *>(a.v) + job.b * a.v_sb + hk * a.v_sh;
@@ -323,89 +503,83 @@ __global__ __launch_bounds__((64 * PastFew<T, DP>::NW), 1) void past_few_kernel(
     own = o;
     kl.init(lane, 0, 1, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, 0, 1, o ? a.v_sl : a.pv_sl, a.D);
   };
-  auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+  auto stage = [&](int t) __attribute__((always_inline)) {
     const bool o = tiles.own(t);
     if (o != own) aim(o);  // at the end of the prefix
     const int64_t k0 = tiles.key0(t);
-    const uint64_t bits = tiles.bits(t, t1);  // behind the last one nothing is read
-    kl.load(o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, bits, lds + buf * 2 * TB);
-    vl.load(o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl, bits, lds + buf * 2 * TB + TB);
+    const uint64_t bits = tiles.bits(t, t1);
+    const T *k = o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, *v = o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl;
+    if (bits == low_bits(KT)) {
+      kl.load_all(k, lds), vl.load_all(v, lds + TB);
+    } else {
+      kl.load(k, bits, lds), vl.load(v, bits, lds + TB);
+    }
   };
   aim(tiles.own(t0));
-  if (t0 < t1) stage(t0, 0);
-  FragReader<T, DP> fr;
+  if (t0 < t1) stage(t0);
+  FewReader<T, DP> fr;
   fr.init(lane, lds);
-  Softmax<T, DP, NQ, KT, true> sm;
+  FewSoftmax<T, DP, NC> sm;
   sm.init();
-  Row x[NQ];
-  bool there[NQ];
+  Row x[NC];
+  bool there[NC];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    x[n] = row_of(a, job.packed, job.b, hk, 32 * n + (lane & 31), job.rows, s);
-    there[n] = 32 * n + (lane & 31) < job.rows;
+  for (int n = 0; n < NC; ++n) {
+    x[n] = row_of(a, job.packed, job.b, hk, r0 + 16 * n + (lane & 15), job.rows, s);
+    there[n] = r0 + 16 * n + (lane & 15) < job.rows;
     const T *p = static_cast<const T *>(a.q) + row_place(a, x[n], hk, a.q_sb, a.q_sl, a.q_sh);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      const int d = 16 * ks + 8 * (lane >> 5);
+    for (int ks = 0; ks < DP / 32; ++ks) {
+      const int d = 32 * ks + 8 * (lane >> 4);
       load_frag(p, d, x[n].on && d < a.D, sm.q[n][ks]);
     }
   }
-  auto turn = [&](auto buf, int t) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
+  for (int t = t0; t < t1; t += NW) {
     wait_vmcnt<0>();  // tile t is in this wave's buffer
     asm volatile("" ::: "memory");
-    stage(t + NW, 1 - B);
     const int k0 = tiles.key0(t);
     const bool o = tiles.own(t);
-    const uint64_t all = tiles.bits(t, t1);
-    uint64_t bits[NQ];
-    bool masked = all != low_bits(KT);
+    const uint32_t all = (uint32_t)tiles.bits(t, t1);
+    uint32_t bits[NC];
+    bool masked = all != ~0u;
     const bool rows = o && !wr.everything(a, k0, KT);
     masked |= rows;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) bits[n] = rows ? x[n].bits(a, k0) : all;
-    sm.template step<2 * B * TB, 2 * B * TB + TB>(fr, masked, bits, a.c, lane);
-  };
-  for (int t = t0; t < t1; t += 2 * NW) {
-    turn(std::integral_constant<int, 0>{}, t);
-    if (t + NW < t1) turn(std::integral_constant<int, 1>{}, t + NW);
+    for (int n = 0; n < NC; ++n) bits[n] = rows ? (uint32_t)x[n].bits(a, k0) : all;
+    sm.template step<0, TB>(fr, masked, bits, a.c, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer is read
+    if (t + NW < t1) stage(t + NW);
   }
-  wait_vmcnt<0>();
-  // join the waves: every wave leaves its sums, then sums its share of the 32 x 32 tiles over the waves
-  float f[NQ];
+  // join the waves: every wave leaves its sums, then sums its share of the 16 x 16 tiles over the waves
+  float f[NC];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+  for (int n = 0; n < NC; ++n) {
     const float l = sm.sums(n, f[n]);
-    if (lane < 32) ml[wave][n][lane] = float2{sm.m[n], l};
+    if (lane < 16) ml[wave][n][lane] = float2{sm.m[n], l};
   }
-  __syncthreads();
-  f32x4 *sums = (f32x4 *)smem;
+  f32x4 *mine = (f32x4 *)smem + wave * 2 * TB / 16;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
+  for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sums[(((wave * NQ + n) * ND + d) * 4 + i) * 64 + lane] =
-            f32x4{sm.o[n][d][4 * i], sm.o[n][d][4 * i + 1], sm.o[n][d][4 * i + 2], sm.o[n][d][4 * i + 3]} * f[n];
+    for (int d = 0; d < ND; ++d) mine[(n * ND + d) * 64 + lane] = sm.o[n][d] * f[n];
   __syncthreads();
   const int64_t all = (int64_t)a.B * a.Hk * a.rows;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+  for (int n = 0; n < NC; ++n) {
     float m = kNoMax, lsum = 0.f, w[NW];
 #pragma unroll
-    for (int q = 0; q < NW; ++q) m = fmaxf(m, ml[q][n][lane & 31].x);
+    for (int q = 0; q < NW; ++q) m = fmaxf(m, ml[q][n][lane & 15].x);
     const RowRef top = row_ref(m, a.c);
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
-      const float2 v = ml[q][n][lane & 31];
+      const float2 v = ml[q][n][lane & 15];
       w[q] = ref_factor(row_ref(v.x, a.c), top, a.c);
       lsum += w[q] * v.y;
     }
     if (!x[n].on) lsum = 0.f;
     const bool some = lsum > 0.f || lsum != lsum;
     const float inv = a.slots > 1 ? 1.f : some ? 1.0f / lsum : 0.f;
-    if (wave == 0 && lane < 32 && there[n]) {
+    if (wave == 0 && lane < 16 && there[n]) {
       if (a.slots > 1) *(float2 *)(a.part_ml + 2 * (job.slot * all + x[n].at)) = float2{some ? m : kNoMax, lsum};
       else if (a.stats != nullptr) {
         a.stats[x[n].at] = lsum > 0.f ? top.r + __builtin_amdgcn_logf(lsum) : lsum != lsum ? lsum : INFINITY;
@@ -413,11 +587,11 @@ __global__ __launch_bounds__((64 * PastFew<T, DP>::NW), 1) void past_few_kernel(
       }
     }
     const int64_t at = row_place(a, x[n], hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
-    for (int u = wave; u < 4 * ND; u += NW) {  // 4 consecutive channels per lane
+    for (int d = wave; d < ND; d += NW) {  // 4 consecutive channels per lane
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < NW; ++q) o += w[q] * sums[((q * NQ + n) * 4 * ND + u) * 64 + lane];
-      const int ch = 32 * (u / 4) + 8 * (u % 4) + 4 * (lane >> 5);
+      for (int q = 0; q < NW; ++q) o += w[q] * ((const f32x4 *)smem + q * 2 * TB / 16)[(n * ND + d) * 64 + lane];
+      const int ch = 16 * d + 4 * (lane >> 4);
       if (!there[n] || ch >= a.D) continue;
       o *= inv;
       if (!some) o = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -441,7 +615,7 @@ __global__ __launch_bounds__(256) void past_join_kernel(const PastArgs a) {
   __shared__ f32x4 sums[8][32];
   __shared__ float ls[8];
   const int64_t all = (int64_t)a.B * a.Hk * a.rows, row = blockIdx.x;
-  const int at = threadIdx.x % 32, g = threadIdx.x / 32;
+  const int at = threadIdx.x % 32, g = threadIdx.x / 32, ch = min(4 * at, a.D - 4);
   float m = kNoMax;
   for (int s = at; s < a.slots; s += 32) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
 #pragma unroll
@@ -452,9 +626,10 @@ __global__ __launch_bounds__(256) void past_join_kernel(const PastArgs a) {
 #pragma unroll 4
   for (int s = g; s < a.slots; s += 8) {
     const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * all + row));
+    const f32x4 part = *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + ch);  // both loads before either is used
     const float w = ref_factor(row_ref(ml.x, a.c), top, a.c);
     l += w * ml.y;
-    if (4 * at < a.D && ml.y != 0.f) o += w * *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + 4 * at);
+    if (ml.y != 0.f) o += w * part;
   }
   sums[g][at] = o;
   if (at == 0) ls[g] = l;
@@ -945,6 +1120,7 @@ __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba
 #define MLORA_PAST(T, DP)                                             \
   template __global__ void past_fwd_kernel<T, DP>(const PastArgs);    \
   template __global__ void past_few_kernel<T, DP, 1>(const PastArgs); \
+  template __global__ void past_few_kernel<T, DP, 2>(const PastArgs); \
   template __global__ void past_dq_kernel<T, DP>(const PastBwdArgs);  \
   template __global__ void past_dkv_kernel<T, DP, 4>(const PastBwdArgs);
 MLORA_PAST(uint16_t, 64)
@@ -952,9 +1128,6 @@ MLORA_PAST(uint16_t, 128)
 MLORA_PAST(float, 64)
 MLORA_PAST(float, 128)
 #undef MLORA_PAST
-template __global__ void past_few_kernel<uint16_t, 64, 2>(const PastArgs);
-template __global__ void past_few_kernel<uint16_t, 128, 2>(const PastArgs);
-template __global__ void past_few_kernel<float, 64, 2>(const PastArgs);
 template __global__ void past_dkv_kernel<uint16_t, 128, 8>(const PastBwdArgs);
 
 // ------------------------------------------------------------------ host
@@ -1009,21 +1182,23 @@ struct PastPlan {
 
 static PastPlan past_plan(const PastSizes &z) {
   PastPlan p{};
-  const int64_t few_rows = z.f32 && z.D > 64 ? 32 : 64, waves = z.f32 && z.D > 64 ? 2 : 4, e = z.f32 ? 4 : 2;
+  const int64_t few_rows = 64, waves = z.f32 && z.D > 64 ? 4 : 8, e = z.f32 ? 4 : 2;
   p.few = z.rows <= few_rows;
   p.packed = p.few && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
-  p.row_tiles = p.few ? 1 : ceil_div(z.rows, 128);
+  p.row_tiles = ceil_div(z.rows, p.few ? 32 : 128);
   auto share = [&](int64_t items, int64_t tiles, bool few) {
-    const int64_t least = few ? (z.f32 ? waves : 4 * waves) : z.f32 ? 2 : 8;  // tiles that a share is worth its join for
-    return items > 0 ? between(between(256 / items, 1, 64), 1, between(tiles / least, 1, 64)) : 1;
+    // tiles that a share is worth its join for. Few rows: one tile per wave (1024 keys in 4 shares 10.1 us, in 2 11.8, in one 11.3),
+    // from four per wave on (576 keys in 2 shares 10.0 us, in one 7.2)
+    const int64_t least = few ? (tiles < 4 * waves ? tiles + 1 : waves) : z.f32 ? 2 : 8;
+    return items > 0 ? between(256 / items, 1, between(tiles / least, 1, 64)) : 1;
   };
   const int64_t kt = p.few || z.f32 ? 32 : 64;
   const int64_t prefix_tiles = p.packed ? 0 : ceil_div(z.Lp, kt);
-  p.splits = share(z.B * z.Hk * p.row_tiles, own_tiles(z, p.few ? z.rows : 128, kt) + prefix_tiles, p.few);
+  p.splits = share(z.B * z.Hk * p.row_tiles, own_tiles(z, p.few ? 32 : 128, kt) + prefix_tiles, p.few);
   if (p.packed) {
     const int64_t rows = z.each * z.rows;
     p.packed_few = rows <= few_rows;
-    p.packed_tiles = p.packed_few ? 1 : ceil_div(rows, 128);
+    p.packed_tiles = ceil_div(rows, p.packed_few ? 32 : 128);
     p.packed_splits = share(z.groups * z.Hk * p.packed_tiles, ceil_div(z.Lp, p.packed_few || z.f32 ? 32 : 64), p.packed_few);
   }
   p.slots = p.splits + p.packed_splits;
@@ -1160,7 +1335,7 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_head(z.f32, z.D, [&](auto t, auto dp) {
     using T = decltype(t);
-    constexpr int DP = decltype(dp)::value, NW = PastFew<T, DP>::NW;
+    constexpr int DP = decltype(dp)::value;
     if (!p.few) {
       hipLaunchKernelGGL((past_fwd_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a);
       return;
@@ -1171,11 +1346,13 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
     }
     a.packed_blocks = p.packed_few ? (int32_t)packed : 0;
     const dim3 grid((unsigned)(blocks + a.packed_blocks));
-    const bool two = (p.packed_few ? z.each * z.rows : z.rows) > 32;
-    if constexpr (sizeof(T) * DP < 512) {
-      if (two) hipLaunchKernelGGL((past_few_kernel<T, DP, 2>), grid, dim3(64 * NW), 0, s, a);
-    }
-    if (!two) hipLaunchKernelGGL((past_few_kernel<T, DP, 1>), grid, dim3(64 * NW), 0, s, a);
+    const int64_t rows = p.packed_few ? z.each * z.rows : z.rows;
+    auto go = [&](auto nc) {
+      constexpr int NC = decltype(nc)::value;
+      hipLaunchKernelGGL((past_few_kernel<T, DP, NC>), grid, dim3(64 * PastFew<T, DP, NC>::NW), 0, s, a);
+    };
+    if (rows <= 16) return go(std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 2>{});
   });
   st = launch_status();
   if (st || p.slots == 1) return st;
