@@ -1171,93 +1171,63 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return dq, dk, dv
 
 
-@functools.lru_cache(maxsize=512)
-def _past_shape(*values):
-    """A past-attention call's sizes as the entries take them, by value, with the bytes of its workspaces."""
-    dtype, from_end, sizes, strides, scale = values
-    shape = _lib.PastShape(dtype, from_end, *sizes, *[(ctypes.c_int64 * 3)(*s) for s in strides], scale)
+class PastPlan:
+    """A past-attention call's sizes, strides and options as the C entries take them, the bytes of its workspaces, and where
+    the backward's statistics lie; made once per combination of them by past_plan."""
+    __slots__ = ("shape", "ref", "forward", "backward", "stats", "saved", "g_strides", "empty", "pad")
+
+
+def past_plan(dtype: torch.dtype, sizes: Sequence[int], strides: Sequence[tuple], window: int, sinks: int, chunk: int, first: int,
+              from_end: bool, scale: float) -> PastPlan:
+    """sizes: B, Lq, Lk, H, Hk, D, groups, Lp; strides: the element strides {batch, token, head} of q, k, v[, prefix_k, prefix_v]
+    in layouts that attention_layout accepts (0 in a dimension of one)."""
+    plan = PastPlan()
+    pad = 5 - len(strides)
+    plan.shape = _lib.PastShape(_DT[dtype], from_end, *sizes, window, sinks, chunk, first,
+                                *[(ctypes.c_int64 * 3)(*s) for s in strides], *[(ctypes.c_int64 * 3)()] * pad, scale)
+    plan.ref = ctypes.byref(plan.shape)
     nbytes = []
     for name in ("mlora_past_attention_workspace_bytes", "mlora_past_attention_backward_workspace_bytes"):
-        nbytes.append(getattr(_lib.load(), name)(ctypes.byref(shape)))
+        nbytes.append(getattr(_lib.load(), name)(plan.ref))
         _lib.check(name, min(nbytes[-1], 0))
-    return ctypes.byref(shape), *nbytes
+    plan.forward, plan.backward = nbytes
+    B, Lq, _, H, _, D = sizes[:6]
+    plan.stats = (2 * B * H * Lq + 3) // 4 * 4  # floats; then, in bf16, what out's rounding left
+    plan.saved = plan.stats + (B * Lq * H * D // 2 if dtype is torch.bfloat16 else 0)
+    plan.g_strides = _i64s((Lq * H * D, H * D, D))
+    plan.empty = B == 0
+    plan.pad = (None,) * pad
+    return plan
 
 
-def _past_args(tensors, key_lengths, query_start, prefix_lengths, window, sinks, chunk, first, from_end, scale):
-    q, k = tensors[:2]
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1:3]
-    groups, Lp = tensors[3].shape[:2] if len(tensors) == 5 else (0, 0)
-    strides = tuple([_strides(t, 3) for t in tensors]) + ((0, 0, 0),) * (5 - len(tensors))
-    shape, forward, backward = _past_shape(_DT[q.dtype], from_end, (B, Lq, Lk, H, Hk, D, groups, Lp, window, sinks, chunk, first),
-                                           strides, scale)
-    pointers = [t.data_ptr() for t in tensors] + [None] * (5 - len(tensors))
-    return (shape, *pointers, _ptr(key_lengths), _ptr(query_start), _ptr(prefix_lengths)), forward, backward
-
-
-def _check_past(tensors, key_lengths, query_start, prefix_lengths) -> None:
-    _require(len(tensors) in (3, 5), "q, k and v, or these and a prefix's k and v")
-    q, k = tensors[:2]
-    _require(q.dim() == 4 and k.dim() == 4, "q, k and v must be [batch, tokens, heads, head_dim]")
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1:3]
-    shapes = [("q", (B, Lq, H, D)), ("k", (B, Lk, Hk, D)), ("v", (B, Lk, Hk, D))]
-    groups = 0
-    if len(tensors) == 5:
-        _require(tensors[3].dim() == 4, "prefix_k must be [groups, tokens, heads, head_dim]")
-        groups, Lp = tensors[3].shape[:2]
-        _require(groups > 0 and B % groups == 0, "the samples share the prefixes evenly")
-        shapes += [("prefix_k", (groups, Lp, Hk, D)), ("prefix_v", (groups, Lp, Hk, D))]
-    for (name, shape), t in zip(shapes, tensors):
-        _require(t.dtype == q.dtype and t.dtype in _DT and tuple(t.shape) == shape and attention_layout(t),
-                 f"{name} must be {list(shape)} of q's dtype with 16-byte aligned heads and a token stride below "
-                 f"{ATTENTION_MAX_STRIDE}")
-    for name, t, n in (("key_lengths", key_lengths, B), ("query_start", query_start, B), ("prefix_lengths", prefix_lengths, groups)):
-        _require(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()),
-                 f"{name} must be a contiguous int32 vector of {n}")
-    _check_device(q, *tensors, key_lengths, query_start, prefix_lengths)
-
-
-def past_attention(*tensors: torch.Tensor, key_lengths: torch.Tensor | None, query_start: torch.Tensor | None,
-                   prefix_lengths: torch.Tensor | None, window: int, sinks: int, chunk: int, first: int, from_end: bool,
-                   scale: float, for_backward: bool = False, checked: bool = False):
-    """(out, rest, stats) of q, k, v [, prefix_k, prefix_v]: softmax(scale q kᵀ) v over the keys that a token sees (window
-    0: all up to its chunk's end); rest (bf16 alone) and stats are the backward's, None without for_backward. checked: the
-    caller has made the checks."""
-    if not checked:
-        _check_past(tensors, key_lengths, query_start, prefix_lengths)
-    args, nbytes, _ = _past_args(tensors, key_lengths, query_start, prefix_lengths, window, sinks, chunk, first, from_end, scale)
+def past_attention(plan: PastPlan, tensors: Sequence[torch.Tensor], pointers: Sequence[int], key_lengths: torch.Tensor | None,
+                   query_start: torch.Tensor | None, prefix_lengths: torch.Tensor | None, for_backward: bool = False):
+    """(out, saved): softmax(scale q kᵀ) v over the keys that a token sees (window 0: all up to its chunk's end), of q, k, v [,
+    prefix_k, prefix_v] at these pointers, laid out as the plan has them; saved is the backward's, None without for_backward.
+    The vectors are contiguous int32."""
     q = tensors[0]
-    out, rest, stats = _new(q), None, None
+    out, saved, stats, rest = _new(q), None, None, None
     if for_backward:
-        stats = torch.empty(2 * q.shape[0] * q.shape[1] * q.shape[2], dtype=torch.float32, device=q.device)
-        rest = _new(q) if q.dtype is torch.bfloat16 else None
-    ws = _workspace(nbytes, q.device)
-    _call("mlora_past_attention", q, *args, out.data_ptr(), _ptr(rest), _ptr(stats), _ptr(ws), nbytes)
-    return out, rest, stats
+        saved = torch.empty(plan.saved, dtype=torch.float32, device=q.device)
+        stats = saved.data_ptr()
+        rest = stats + 4 * plan.stats
+    ws = _workspace(plan.forward, q.device)
+    _call("mlora_past_attention", q, plan.ref, *pointers, *plan.pad, _ptr(key_lengths), _ptr(query_start), _ptr(prefix_lengths),
+          out.data_ptr(), rest, stats, _ptr(ws), plan.forward)
+    return out, saved
 
 
-def past_attention_backward(out: torch.Tensor, rest: torch.Tensor | None, stats: torch.Tensor, g: torch.Tensor,
-                            *tensors: torch.Tensor, key_lengths: torch.Tensor | None, query_start: torch.Tensor | None,
-                            prefix_lengths: torch.Tensor | None, window: int, sinks: int, chunk: int, first: int,
-                            from_end: bool, scale: float, checked: bool = False) -> list[torch.Tensor]:
-    """The gradients of every tensor, contiguous, from the forward's results and the upstream gradient g of out."""
-    q = tensors[0]
-    if not checked:
-        _check_past(tensors, key_lengths, query_start, prefix_lengths)
-        for name, t in (("out", out), ("rest", rest), ("g", g)):
-            _require((t is None and name == "rest" and q.dtype is torch.float32) or
-                     (t is not None and t.dtype == q.dtype and t.shape == q.shape), f"{name} must have q's shape and dtype")
-        _require(out.is_contiguous() and (rest is None or rest.is_contiguous()) and attention_layout(g),
-                 "out and rest are contiguous, g's heads are 16-byte aligned")
-        _require(stats.dtype == torch.float32 and stats.is_contiguous() and
-                 stats.numel() == 2 * q.shape[0] * q.shape[1] * q.shape[2], "stats is the forward's")
-        _check_device(q, out, rest, stats, g)
-    args, _, nbytes = _past_args(tensors, key_lengths, query_start, prefix_lengths, window, sinks, chunk, first, from_end, scale)
-    if q.shape[0] == 0:
+def past_attention_backward(plan: PastPlan, out: torch.Tensor, saved: torch.Tensor, g: torch.Tensor, tensors: Sequence[torch.Tensor],
+                            key_lengths: torch.Tensor | None, query_start: torch.Tensor | None,
+                            prefix_lengths: torch.Tensor | None) -> list[torch.Tensor]:
+    """The gradients of every tensor, contiguous, from the forward's results and the upstream gradient g of out (attention_layout)."""
+    if plan.empty:
         return [torch.zeros_like(t, memory_format=torch.contiguous_format) for t in tensors]
     grads = [_new(t) for t in tensors]
-    ws = _workspace(nbytes, q.device)
-    _call("mlora_past_attention_backward", q, *args, out.data_ptr(), _ptr(rest), stats.data_ptr(), g.data_ptr(),
-          _i64s(_strides(g, 3)), *[d.data_ptr() for d in grads], *[None] * (5 - len(grads)), _ptr(ws), nbytes)
+    ws = _workspace(plan.backward, out.device)
+    stats = saved.data_ptr()
+    _call("mlora_past_attention_backward", out, plan.ref, *[t.data_ptr() for t in tensors], *plan.pad, _ptr(key_lengths),
+          _ptr(query_start), _ptr(prefix_lengths), out.data_ptr(), stats + 4 * plan.stats, stats, g.data_ptr(),
+          plan.g_strides if g.is_contiguous() else _i64s(_strides(g, 3)), *[d.data_ptr() for d in grads], *plan.pad,
+          _ptr(ws), plan.backward)
     return grads

@@ -55,51 +55,68 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if kernels.attention_layout(t) else t.clone()
 
 
+def _lay_out(call, tensors):
+    """(the kernels' plan, the tensors as they take them, their addresses): copies where a layout or an address is not theirs."""
+    plan, again = call
+    pointers = [t.data_ptr() for t in tensors]
+    if plan is None or any([p & 15 for p in pointers]):
+        tensors = [_aligned(t) for t in tensors]
+        plan, pointers = _plan(tuple([_meta(t) for t in tensors]), *again)[0], [t.data_ptr() for t in tensors]
+    return plan, tensors, pointers
+
+
 class PastAttentionFunction(torch.autograd.Function):
-    """``apply(cfg, key_lengths, query_start, prefix_lengths, q, k, v[, prefix_k, prefix_v])`` -> out; cfg as _plan
+    """``apply(call, key_lengths, query_start, prefix_lengths, q, k, v[, prefix_k, prefix_v])`` -> out; call as _plan
     gives it."""
 
     @staticmethod
-    def forward(ctx, cfg, key_lengths, query_start, prefix_lengths, *tensors):
-        tensors = [_aligned(t) for t in tensors]
-        out, rest, stats = kernels.past_attention(*tensors, key_lengths=key_lengths, query_start=query_start,
-                                                  prefix_lengths=prefix_lengths, for_backward=True, checked=True, **cfg)
-        ctx.save_for_backward(key_lengths, query_start, prefix_lengths, out, rest, stats, *tensors)
-        ctx.cfg = cfg
+    def forward(ctx, call, key_lengths, query_start, prefix_lengths, *tensors):
+        ctx.plan, tensors, pointers = _lay_out(call, tensors)
+        out, saved = kernels.past_attention(ctx.plan, tensors, pointers, key_lengths, query_start, prefix_lengths, True)
+        ctx.save_for_backward(key_lengths, query_start, prefix_lengths, out, saved, *tensors)
         return out
 
     @staticmethod
     @kernels.first_order
     def backward(ctx, g):
-        key_lengths, query_start, prefix_lengths, out, rest, stats, *tensors = ctx.saved_tensors
+        key_lengths, query_start, prefix_lengths, out, saved, *tensors = ctx.saved_tensors
         g = _aligned(g if g.dtype is out.dtype else g.to(out.dtype))
-        grads = kernels.past_attention_backward(out, rest, stats, g, *tensors, key_lengths=key_lengths, query_start=query_start,
-                                                prefix_lengths=prefix_lengths, checked=True, **ctx.cfg)
+        grads = kernels.past_attention_backward(ctx.plan, out, saved, g, tensors, key_lengths, query_start, prefix_lengths)
         return (None, None, None, None, *[d if want else None for d, want in zip(grads, ctx.needs_input_grad[4:])])
 
 
 def _meta(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.dtype, t.device)
+    return None if t is None else (t.shape, t.dtype, t.device, t.stride())
 
 
 def _check_vector(name: str, meta, n: int, device) -> None:
     if meta is not None:
-        shape, dtype, dev = meta
+        shape, dtype, dev, _ = meta
         if dev != device or dtype not in (torch.int32, torch.int64) or tuple(shape) != (n,):
             _fail(f"{name} must be int32 or int64 [{n}] on q's device")
 
 
-# What a call's shapes, types and options allow, checked once per combination of them.
+def _layout(shape, strides) -> bool:
+    """attention_layout but for the address, which is looked at on every call."""
+    return math.prod(shape) == 0 or (
+        (shape[3] < 2 or strides[3] == 1) and all([n < 2 or s % 8 == 0 for n, s in zip(shape[:3], strides)])
+        and (shape[1] < 2 or strides[1] < kernels.ATTENTION_MAX_STRIDE))
+
+
+# What a call's shapes, types, strides and options allow, checked once per combination of them: the kernels' plan (None where a
+# tensor's layout is not theirs) and what the same call with other tensors is planned from.
 @functools.lru_cache(maxsize=512)
-def _plan(q, k, v, pk, pv, key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale) -> dict:
-    for name, (shape, dtype, device) in (("q", q), ("k", k), ("v", v)):
+def _plan(metas, key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale):
+    again = (key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale)
+    q, k, v, pk, pv = metas if len(metas) == 5 else (*metas, None, None)
+    for name, (shape, dtype, device, _) in (("q", q), ("k", k), ("v", v)):
         if len(shape) != 4:
             _fail(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(shape)}")
         if dtype not in _DTYPES:
             _fail(f"{name} must be bfloat16 or float32, got {dtype}")
         if dtype != q[1] or device != q[2]:
             _fail("q, k and v share one dtype and device")
-    (B, Lq, H, D), dtype, device = q
+    (B, Lq, H, D), dtype, device, _ = q
     Lk, Hk = k[0][1:3]
     if k[0] != v[0] or k[0][0] != B or k[0][3] != D:
         _fail(f"k and v must be [{B}, tokens, heads, {D}], got {tuple(k[0])} and {tuple(v[0])}")
@@ -110,7 +127,7 @@ def _plan(q, k, v, pk, pv, key_lengths, query_start, prefix_lengths, window, sin
     if max(Lq, Lk) > _MOST:
         _fail(f"at most {_MOST} tokens")
     if pk is not None:
-        if pk[1:] != q[1:] or pv[1:] != q[1:]:
+        if pk[1:3] != q[1:3] or pv[1:3] != q[1:3]:
             _fail("prefix_k and prefix_v have q's dtype and device")
         if pk[0] != pv[0] or len(pk[0]) != 4 or tuple(pk[0][2:]) != (Hk, D):
             _fail(f"prefix_k and prefix_v must be [tokens, {Hk}, {D}] or [groups, tokens, {Hk}, {D}], got {tuple(pk[0])} and {tuple(pv[0])}")
@@ -138,8 +155,14 @@ def _plan(q, k, v, pk, pv, key_lengths, query_start, prefix_lengths, window, sin
     # past these nothing changes, and they fit the kernels' integers
     start = 0 if isinstance(query_start, tuple) else Lk - Lq if query_start is None else max(-Lq, min(query_start, Lk))
     chunk = min(chunk, max(Lk, 1))
-    return dict(window=0 if window is None else min(max(window, chunk), Lk + chunk), sinks=min(sinks, Lk), chunk=chunk, scale=scale,
-                first=start, from_end=query_start is None and key_lengths is not None and Lq < Lk)
+    groups, Lp = pk[0][:2] if pk is not None else (0, 0)
+    if not all(_layout(shape, strides) for shape, _, _, strides in metas):
+        return None, again
+    plan = kernels.past_plan(
+        dtype, (B, Lq, Lk, H, Hk, D, groups, Lp), [[s if n > 1 else 0 for s, n in zip(m[3][:3], m[0])] for m in metas],
+        0 if window is None else min(max(window, chunk), Lk + chunk), min(sinks, Lk), chunk, start,
+        query_start is None and key_lengths is not None and Lq < Lk, scale)
+    return plan, again
 
 
 def _int32(t: torch.Tensor | None, low: int, high: int) -> torch.Tensor | None:
@@ -158,18 +181,18 @@ def _attend(tensors, key_lengths, query_start, prefix_lengths, window, sinks, ch
         start = _meta(start)
     elif start is not None:
         start, query_start = _whole("query_start", start), None
-    metas = [_meta(t) for t in tensors]
-    cfg = _plan(*metas, *(() if len(tensors) == 5 else (None, None)), _meta(key_lengths), start, _meta(prefix_lengths),
-                None if window is None else _whole("window", window), _whole("sinks", sinks), _whole("chunk", chunk), scale)
-    Lq, Lk = tensors[0].shape[1], tensors[1].shape[1]
-    key_lengths = _int32(key_lengths, 0, Lk)
-    query_start = _int32(query_start, -Lq, Lk)
+    call = _plan(tuple([_meta(t) for t in tensors]), _meta(key_lengths), start, _meta(prefix_lengths),
+                 None if window is None else _whole("window", window), _whole("sinks", sinks), _whole("chunk", chunk), scale)
+    if key_lengths is not None:
+        key_lengths = _int32(key_lengths, 0, tensors[1].shape[1])
+    if query_start is not None:
+        query_start = _int32(query_start, -tensors[0].shape[1], tensors[1].shape[1])
     if prefix_lengths is not None:
         prefix_lengths = _int32(prefix_lengths, 0, tensors[3].shape[1])
     if kernels.wants_grad(tensors):
-        return PastAttentionFunction.apply(cfg, key_lengths, query_start, prefix_lengths, *tensors)
-    return kernels.past_attention(*[_aligned(t) for t in tensors], key_lengths=key_lengths, query_start=query_start,
-                                  prefix_lengths=prefix_lengths, checked=True, **cfg)[0]
+        return PastAttentionFunction.apply(call, key_lengths, query_start, prefix_lengths, *tensors)
+    plan, tensors, pointers = _lay_out(call, tensors)
+    return kernels.past_attention(plan, tensors, pointers, key_lengths, query_start, prefix_lengths)[0]
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
