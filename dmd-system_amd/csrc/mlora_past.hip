@@ -198,8 +198,9 @@ __device__ __forceinline__ void finish_rows(const PastArgs &a, const Row &x, boo
 
 // Four waves of 32 rows each against the same key tiles, two buffers of K and V in LDS: tile t + 1 loads while tile
 // t is multiplied; one barrier per tile.
-template <class T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_fwd_kernel(const PastArgs a) {
+template <int DP>
+__global__ __launch_bounds__(256, 2) void past_fwd_kernel(const PastArgs a) {
+  using T = uint16_t;
   constexpr int KT = AttnTile<T>::KT;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024 / 4;
@@ -291,11 +292,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_fwd_kernel(c
 __device__ __forceinline__ f32x4 mma32(const Frag<uint16_t> &a, const Frag<uint16_t> &b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a.v), as_bf16x8(b.v), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mma32(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
-  return c;
-}
+__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // over the four quarters of a column
 __device__ __forceinline__ float quarter_max(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -339,28 +336,93 @@ struct FewReader<uint16_t, DP> {
 template <int DP>
 struct FewReader<float, DP> {
   using Tile = HeadTile<float, DP>;
-  int32_t row, at, sw, r, g;
+  int32_t row[2], val[4], sw;
   __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
-    r = lane & 15, g = lane >> 4, sw = Tile::swz(r);
-    at = (int32_t)(uintptr_t)base, row = at + r * Tile::RB;
+    const int r = lane & 15, g = lane >> 4, at = (int32_t)(uintptr_t)base;
+    sw = Tile::swz(r) ^ (2 * g);
+    row[0] = at + r * Tile::RB, row[1] = row[0] + 16 * Tile::RB;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) val[j] = at + (4 * g + j) * Tile::RB + ((r ^ Tile::swz(4 * g + j)) << 4);
   }
-  template <int OFF, int R0>
+  template <int OFF, int R0>  // swz(r + 16) = swz(r)
   __device__ __forceinline__ void keys(int s, Frag<float> &f) const {
-    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)row + OFF + R0 * Tile::RB;
-    const f32x4 a = *(const lds_f4 *)(t + (((8 * s + 2 * g) ^ sw) << 4)), b = *(const lds_f4 *)(t + (((8 * s + 2 * g + 1) ^ sw) << 4));
+    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)row[R0 / 16] + OFF;
+    const f32x4 a = *(const lds_f4 *)(t + (((8 * s) ^ sw) << 4)), b = *(const lds_f4 *)(t + (((8 * s + 1) ^ sw) << 4));
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.v[j] = a[j], f.v[j + 4] = b[j];
   }
+  // channels 64h + 4·(lane % 16) .. + 3 of row 16·(j / 4) + 4·(lane / 16) + j % 4: element i is the operand of channels 64h + 4m + i, m the
+  // result's row
   template <int OFF>
-  __device__ __forceinline__ void values(int d, Frag<float> &f) const {
-    const MLORA_LDS char *t = (const MLORA_LDS char *)(uintptr_t)(uint32_t)at + OFF;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = 16 * (j / 4) + 4 * g + j % 4, chunk = 4 * d + (r >> 2);
-      f.v[j] = *(const MLORA_LDS float *)(t + key * Tile::RB + ((chunk ^ Tile::swz(key)) << 4) + 4 * (r & 3));
-    }
+  __device__ __forceinline__ f32x4 value4(int j, int h) const {
+    return *(const lds_f4 *)((const MLORA_LDS char *)(uintptr_t)(uint32_t)val[j % 4] + OFF + j / 4 * 16 * Tile::RB + 256 * h);
   }
 };
+
+// s[n][b] += rows 16b .. of the tile at OFF times the NC x 16 columns of x.
+template <int OFF, int DP, int NC>
+__device__ __forceinline__ void few_scores(const FewReader<uint16_t, DP> &fr, const Frag<uint16_t> (&x)[NC][DP / 32], f32x4 (&s)[NC][2]) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 32; ++ks)
+    static_for<2>([&](auto kb) __attribute__((always_inline)) {
+      Frag<uint16_t> kf;
+      fr.template keys<OFF, 16 * decltype(kb)::value>(ks, kf);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) s[n][kb] = mma32(kf, x[n][ks], s[n][kb]);
+      return true;
+    });
+}
+template <int OFF, int DP, int NC>
+__device__ __forceinline__ void few_scores(const FewReader<float, DP> &fr, const Frag<float> (&x)[NC][DP / 32], f32x4 (&s)[NC][2]) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 32; ++ks) {
+    Frag<float> kf[2];
+    fr.template keys<OFF, 0>(ks, kf[0]);
+    fr.template keys<OFF, 16>(ks, kf[1]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][kb] = mma4(kf[kb].v[j], x[n][ks].v[j], s[n][kb]);
+  }
+}
+
+// o[n] += the tile at OFF, transposed, times p[n].
+template <int OFF, int DP, int NC>
+__device__ __forceinline__ void few_weigh(const FewReader<uint16_t, DP> &fr, const Frag<uint16_t> (&p)[NC], f32x4 (&o)[NC][DP / 16]) {
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) {
+    Frag<uint16_t> vf;
+    fr.template values<OFF>(d, vf);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) o[n][d] = mma32(vf, p[n], o[n][d]);
+  }
+}
+template <int OFF, int DP, int NC>
+__device__ __forceinline__ void few_weigh(const FewReader<float, DP> &fr, const Frag<float> (&p)[NC], f32x4 (&o)[NC][DP / 16]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h) {
+      const f32x4 v = fr.template value4<OFF>(j, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) o[n][4 * h + i] = mma4(v[i], p[n].v[j], o[n][4 * h + i]);
+    }
+}
+
+// Four channels that follow each other, few_channel(d) .. + 3, of a lane's column of such sums, d < DP / 16.
+template <class T, int ND>
+__device__ __forceinline__ f32x4 few_vector(const f32x4 (&o)[ND], int d) {
+  if constexpr (sizeof(T) == 2) return o[d];
+  else return f32x4{o[d & ~3][d & 3], o[(d & ~3) + 1][d & 3], o[(d & ~3) + 2][d & 3], o[(d & ~3) + 3][d & 3]};
+}
+template <class T>
+__device__ __forceinline__ int few_channel(int d, int lane) {
+  return sizeof(T) == 2 ? 16 * d + 4 * (lane >> 4) : 64 * (d >> 2) + 16 * (lane >> 4) + 4 * (d & 3);
+}
 
 // The running softmax of NC x 16 rows against 32 keys per step, as Softmax does it (two sums: e of the weights before their
 // rounding to bf16, l of what the product with V sees).
@@ -385,15 +447,7 @@ struct FewSoftmax {
     f32x4 s[NC][2];
 #pragma unroll
     for (int n = 0; n < NC; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < NS; ++ks)
-      static_for<2>([&](auto kb) __attribute__((always_inline)) {
-        Frag<T> kf;
-        fr.template keys<KOFF, 16 * decltype(kb)::value>(ks, kf);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) s[n][kb] = mma32(kf, q[n][ks], s[n][kb]);
-        return true;
-      });
+    few_scores<KOFF, DP, NC>(fr, q, s);
     if (masked) {
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
@@ -438,13 +492,7 @@ struct FewSoftmax {
       const f32x4 t = s[n][0] + s[n][1];
       e[n] += (t[0] + t[1]) + (t[2] + t[3]);
     }
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      Frag<T> vf;
-      fr.template values<VOFF>(d, vf);
-#pragma unroll
-      for (int n = 0; n < NC; ++n) o[n][d] = mma32(vf, p[n], o[n][d]);
-    }
+    few_weigh<VOFF, DP, NC>(fr, p, o);
   }
 
   __device__ __forceinline__ float sums(int n, float &f) {
@@ -457,20 +505,61 @@ struct FewSoftmax {
   }
 };
 
+// A workgroup's key tiles of K and V on their way into LDS, N blocks of 1024 bytes of either by the calling wave.
+template <class T, int DP, int KT, int N>
+struct TileStream {
+  const T *kp, *vp, *pkp, *pvp;
+  TileLoader<T, DP, N> kl, vl;
+  int end;
+  bool own;
+  __device__ __forceinline__ void aim(const PastArgs &a, int wave, int waves, int lane, bool o) {
+    own = o;
+    kl.init(lane, wave, waves, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, wave, waves, o ? a.v_sl : a.pv_sl, a.D);
+  }
+  __device__ __forceinline__ void init(const PastArgs &a, int b, int group, int hk, int wave, int waves, int lane, const KeyTiles<KT> &tiles, int t0, int t1) {
+    kp = static_cast<const T *>(a.k) + b * a.k_sb + hk * a.k_sh, vp = static_cast<const T *>(a.v) + b * a.v_sb + hk * a.v_sh;
+    pkp = static_cast<const T *>(a.pk) + group * a.pk_sb + hk * a.pk_sh, pvp = static_cast<const T *>(a.pv) + group * a.pv_sb + hk * a.pv_sh;
+    end = t1;
+    aim(a, wave, waves, lane, tiles.own(t0));
+  }
+  __device__ __forceinline__ void stage(const PastArgs &a, const KeyTiles<KT> &tiles, int t, MLORA_LDS char *to) {
+    constexpr int TB = KT * HeadTile<T, DP>::RB;
+    const bool o = tiles.own(t);
+    if (o != own) aim(a, kl.first, kl.step, threadIdx.x & 63, o);  // at the end of the prefix
+    const int64_t k0 = tiles.key0(t);
+    const uint64_t bits = tiles.bits(t, end);
+    const T *k = o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, *v = o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl;
+    if (bits == low_bits(KT)) kl.load_all(k, to), vl.load_all(v, to + TB);
+    else kl.load(k, bits, to), vl.load(v, bits, to + TB);
+  }
+};
+
+// A row as a column operand of 16 x 16 products.
+template <class T, int DP>
+__device__ __forceinline__ void load_row(const T *p, bool on, int D, int lane, Frag<T> (&f)[DP / 32]) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 32; ++ks) {
+    const int d = 32 * ks + 8 * (lane >> 4);
+    load_frag(p, d, on && d < D, f[ks]);
+  }
+}
+
 // Few rows (16 NC per workgroup): the waves take different key tiles, each with its own buffer (no barrier in the loop; two
 // waves per SIMD, one multiplies while the other waits), and their running softmaxes are joined through LDS. Bound by the reading
 // of K and V where they are long (65520 keys, 8 key heads of 128: 46 us, 5.9 TB/s), by a launch and one chain of loads,
 // products and the join where they are short (32 keys 5.4 us, 260 keys of 64 channels 6.1). On 32 x 32 products, four waves with two
 // buffers each: 51, 7.7 and 8.3.
-template <class T, int DP, int NC>
-struct PastFew {
-  static constexpr int KT = 32, NW = sizeof(T) * DP == 512 ? 4 : 8;
-};
+// float32 takes any number of rows this way (waves of 32 rows that share tiles behind a barrier: 1573 tokens, window 257, 12 heads of
+// 64: 46 us, here 37; 524 rows on 646 keys 32 and 21): the matrix core takes 2048 cycles for 32 rows by 32 keys by 64 channels, so
+// that reading the tiles again costs less than waiting. Half the waves where there is more than a workgroup per
+// compute unit, so that two share one (8 heads, 4096 tokens, window 1024, 64 channels: 102 -> 89 us; 352 workgroups of 700 tokens
+// 22 -> 27).
+template <class T, int DP, bool MANY>
+constexpr int kFewWaves = (sizeof(T) * DP == 512 ? 4 : 8) / (MANY ? 2 : 1);
 
-template <class T, int DP, int NC>
-__global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>::NW / 4)) void past_few_kernel(const PastArgs a) {
-  using C = PastFew<T, DP, NC>;
-  constexpr int KT = C::KT, NW = C::NW, ND = DP / 16;
+template <class T, int DP, int NC, bool MANY>
+__global__ __launch_bounds__((64 * kFewWaves<T, DP, MANY>), (kFewWaves<T, DP, false> / 4)) void past_few_kernel(const PastArgs a) {
+  constexpr int KT = 32, NW = kFewWaves<T, DP, MANY>, ND = DP / 16;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024;
   static_assert(NC * ND * 64 * 16 <= 2 * TB, "a wave's sums fit its buffers");
@@ -495,28 +584,9 @@ __global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>:
     wr.init(a, s, r0, min(r0 + 16 * NC, a.rows));
   }
   const int t1 = job.share(tiles.count, job.sp + 1), t0 = min(job.share(tiles.count, job.sp) + wave, t1);
-  const T *kp = static_cast<const T *>(a.k) + job.b * a.k_sb + hk * a.k_sh, *vp = static_cast<const T *>(a.v) + job.b * a.v_sb + hk * a.v_sh;
-  const T *pkp = static_cast<const T *>(a.pk) + group * a.pk_sb + hk * a.pk_sh, *pvp = static_cast<const T *>(a.pv) + group * a.pv_sb + hk * a.pv_sh;
-  TileLoader<T, DP, N> kl, vl;
-  bool own = false;
-  auto aim = [&](bool o) __attribute__((always_inline)) {
-    own = o;
-    kl.init(lane, 0, 1, o ? a.k_sl : a.pk_sl, a.D), vl.init(lane, 0, 1, o ? a.v_sl : a.pv_sl, a.D);
-  };
-  auto stage = [&](int t) __attribute__((always_inline)) {
-    const bool o = tiles.own(t);
-    if (o != own) aim(o);  // at the end of the prefix
-    const int64_t k0 = tiles.key0(t);
-    const uint64_t bits = tiles.bits(t, t1);
-    const T *k = o ? kp + k0 * a.k_sl : pkp + k0 * a.pk_sl, *v = o ? vp + k0 * a.v_sl : pvp + k0 * a.pv_sl;
-    if (bits == low_bits(KT)) {
-      kl.load_all(k, lds), vl.load_all(v, lds + TB);
-    } else {
-      kl.load(k, bits, lds), vl.load(v, bits, lds + TB);
-    }
-  };
-  aim(tiles.own(t0));
-  if (t0 < t1) stage(t0);
+  TileStream<T, DP, KT, N> in;
+  in.init(a, job.b, group, hk, 0, 1, lane, tiles, t0, t1);
+  if (t0 < t1) in.stage(a, tiles, t0, lds);
   FewReader<T, DP> fr;
   fr.init(lane, lds);
   FewSoftmax<T, DP, NC> sm;
@@ -527,12 +597,7 @@ __global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>:
   for (int n = 0; n < NC; ++n) {
     x[n] = row_of(a, job.packed, job.b, hk, r0 + 16 * n + (lane & 15), job.rows, s);
     there[n] = r0 + 16 * n + (lane & 15) < job.rows;
-    const T *p = static_cast<const T *>(a.q) + row_place(a, x[n], hk, a.q_sb, a.q_sl, a.q_sh);
-#pragma unroll
-    for (int ks = 0; ks < DP / 32; ++ks) {
-      const int d = 32 * ks + 8 * (lane >> 4);
-      load_frag(p, d, x[n].on && d < a.D, sm.q[n][ks]);
-    }
+    load_row<T, DP>(static_cast<const T *>(a.q) + row_place(a, x[n], hk, a.q_sb, a.q_sl, a.q_sh), x[n].on, a.D, lane, sm.q[n]);
   }
   for (int t = t0; t < t1; t += NW) {
     wait_vmcnt<0>();  // tile t is in this wave's buffer
@@ -548,7 +613,7 @@ __global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>:
     for (int n = 0; n < NC; ++n) bits[n] = rows ? (uint32_t)x[n].bits(a, k0) : all;
     sm.template step<0, TB>(fr, masked, bits, a.c, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer is read
-    if (t + NW < t1) stage(t + NW);
+    if (t + NW < t1) in.stage(a, tiles, t + NW, lds);
   }
   // join the waves: every wave leaves its sums, then sums its share of the 16 x 16 tiles over the waves
   float f[NC];
@@ -561,7 +626,7 @@ __global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>:
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int d = 0; d < ND; ++d) mine[(n * ND + d) * 64 + lane] = sm.o[n][d] * f[n];
+    for (int d = 0; d < ND; ++d) mine[(n * ND + d) * 64 + lane] = few_vector<T, ND>(sm.o[n], d) * f[n];
   __syncthreads();
   const int64_t all = (int64_t)a.B * a.Hk * a.rows;
 #pragma unroll
@@ -591,7 +656,7 @@ __global__ __launch_bounds__((64 * PastFew<T, DP, NC>::NW), (PastFew<T, DP, NC>:
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < NW; ++q) o += w[q] * ((const f32x4 *)smem + q * 2 * TB / 16)[(n * ND + d) * 64 + lane];
-      const int ch = 16 * d + 4 * (lane >> 4);
+      const int ch = few_channel<T>(d, lane);
       if (!there[n] || ch >= a.D) continue;
       o *= inv;
       if (!some) o = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -680,8 +745,9 @@ struct PastBwdArgs {
   int64_t sink_part, own_part;  // where a class's shares begin, in 16-byte vectors
 };
 
-template <class T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_dq_kernel(const PastBwdArgs ba) {
+template <int DP>
+__global__ __launch_bounds__(256, 2) void past_dq_kernel(const PastBwdArgs ba) {
+  using T = uint16_t;
   const PastArgs &a = ba.f;
   constexpr int KT = AttnTile<T>::KT, ND = DP / 32;
   using Tile = HeadTile<T, DP>;
@@ -736,17 +802,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_dq_kernel(co
       load_frag(qp, d, on, q[ks]);
       load_frag(gp_, d, on, g[ks]);
       load_frag(static_cast<const T *>(a.out) + oat, d, on, of);
-      if constexpr (sizeof(T) == 2) {
-        Frag<T> rf;
-        load_frag(a.rest + oat, d, on, rf);
+      Frag<T> rf;
+      load_frag(a.rest + oat, d, on, rf);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          delta += __uint_as_float(g[ks].v[j] << 16) * (__uint_as_float(of.v[j] << 16) + __uint_as_float(rf.v[j] << 16));
-          delta += __uint_as_float(g[ks].v[j] & 0xffff0000u) * (__uint_as_float(of.v[j] & 0xffff0000u) + __uint_as_float(rf.v[j] & 0xffff0000u));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) delta += g[ks].v[j] * of.v[j];
+      for (int j = 0; j < 4; ++j) {
+        delta += __uint_as_float(g[ks].v[j] << 16) * (__uint_as_float(of.v[j] << 16) + __uint_as_float(rf.v[j] << 16));
+        delta += __uint_as_float(g[ks].v[j] & 0xffff0000u) * (__uint_as_float(of.v[j] & 0xffff0000u) + __uint_as_float(rf.v[j] & 0xffff0000u));
       }
     }
   }
@@ -831,20 +892,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void past_dq_kernel(co
   store_row<T, DP>(static_cast<T *>(ba.dq), oat, there, dq, ba.scale, a.D, lane);
 }
 
-// Adds the shares of dq in order and writes them out.
+// Adds the shares of dq in order and writes them out. bf16: in the order of its kernel's registers; float32: rows in order.
 template <class T, int DP>
 __global__ __launch_bounds__(256) void past_dq_join_kernel(const PastBwdArgs ba) {
   const PastArgs &a = ba.f;
   constexpr int ND = DP / 32;
-  const int64_t per = (int64_t)a.B * a.row_tiles * a.Hk * 4 * ND * 4 * 64;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
-  int64_t u = e / 64;
-  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % 4);
-  u /= 4 * ND * 4;  // (b, row tile, hk)
-  const int hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * 128 + wave * 32 + (lane & 31);
-  const int64_t b = u / a.Hk / a.row_tiles;
-  const int ch = 32 * d + 8 * i + 4 * (lane >> 5);
-  if (r >= a.rows || ch >= a.D) return;
+  const int64_t per = sizeof(T) == 2 ? (int64_t)a.B * a.row_tiles * a.Hk * 4 * ND * 4 * 64 : (int64_t)a.B * a.Hk * a.rows * (a.D / 4);
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int hk, r, ch;
+  int64_t b;
+  if constexpr (sizeof(T) == 2) {  // per is a multiple of 256
+    int64_t u = e / 64;
+    const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), wave = (int)(u / 4 / ND % 4);
+    u /= 4 * ND * 4;  // (b, row tile, hk)
+    hk = (int)(u % a.Hk), r = (int)(u / a.Hk % a.row_tiles) * 128 + wave * 32 + (lane & 31);
+    b = u / a.Hk / a.row_tiles, ch = 32 * d + 8 * i + 4 * (lane >> 5);
+    if (r >= a.rows || ch >= a.D) return;
+  } else {
+    if (e >= per) return;
+    const int64_t u = e / (a.D / 4);
+    ch = (int)(e % (a.D / 4)) * 4, r = (int)(u % a.rows), hk = (int)(u / a.rows % a.Hk), b = u / a.rows / a.Hk;
+  }
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(ba.part + s * per + e);
@@ -854,13 +922,14 @@ __global__ __launch_bounds__(256) void past_dq_join_kernel(const PastBwdArgs ba)
   else *(MLORA_GLOBAL f32x4 *)p = x;
 }
 
-// NW waves own 32 keys each (K fragments in registers; V in LDS for bf16, whose two waves per SIMD leave no room
-// for them) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient and the rows'
+// bf16: NW waves own 32 keys each (K fragments in registers; V in LDS, two waves per SIMD leave no room for it) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient and the rows'
 // x, delta and a.
-template <class T, int DP, int NW>
+template <int DP, int NW>
 struct PastDkv {
-  static constexpr int QT = sizeof(T) == 2 && !(DP == 128 && NW == 4) ? 64 : 32;
+  static constexpr int QT = DP == 128 && NW == 4 ? 32 : 64;
 };
+
+constexpr int kF32Keys = 32;  // of a workgroup in float32
 
 // A workgroup of dk / dv: which keys, and which share of the rows that see them. Blocks of the prefix come first, then those
 // that hold a sink (both meet many rows and are shared out), then the other own ones.
@@ -888,13 +957,13 @@ struct KeyJob {
   int64_t items, item;
 };
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void past_dkv_kernel(const PastBwdArgs ba) {
+template <int DP, int NW>
+__global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArgs ba) {
+  using T = uint16_t;
   const PastArgs &a = ba.f;
-  constexpr int QT = PastDkv<T, DP, NW>::QT, ND = DP / 32, NS = DP / 16;
-  constexpr bool VLDS = sizeof(T) == 2;
+  constexpr int QT = PastDkv<DP, NW>::QT, ND = DP / 32, NS = DP / 16;
   using Tile = HeadTile<T, DP>;
-  constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = VLDS ? 32 * Tile::RB : 0;
+  constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = 32 * Tile::RB;
   static_assert(64 * NW >= 3 * QT, "a thread loads one of a row's three values");
   // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then x, delta and a per buffer
   __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + 3 * QT / 2];
@@ -913,15 +982,14 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void past_dkv_
   const T *kp = static_cast<const T *>(job.prefix ? a.pk : a.k) + job.o * (job.prefix ? a.pk_sb : a.k_sb) + hk * (job.prefix ? a.pk_sh : a.k_sh);
   const T *vp = static_cast<const T *>(job.prefix ? a.pv : a.v) + job.o * (job.prefix ? a.pv_sb : a.v_sb) + hk * (job.prefix ? a.pv_sh : a.v_sh);
   const int64_t k_sl = job.prefix ? a.pk_sl : a.k_sl, v_sl = job.prefix ? a.pv_sl : a.v_sl;
-  Frag<T> k[NS], v[VLDS ? 1 : NS];
+  Frag<T> k[NS];
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks) {
     const int d = 16 * ks + 8 * (lane >> 5);
     load_frag(kp, key * k_sl + d, live && d < a.D, k[ks]);
-    if constexpr (!VLDS) load_frag(vp, key * v_sl + d, live && d < a.D, v[ks]);
   }
   MLORA_LDS char *vt = lds + 4 * TB + wave * VB;
-  if constexpr (VLDS) {
+  {
     TileLoader<T, DP, VB / 1024> vl;
     vl.init(lane, 0, 1, v_sl, a.D);
     vl.load(vp + (int64_t)key0 * v_sl, live_bits, vt);
@@ -1002,8 +1070,7 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void past_dkv_
         fr.template rows<0, 32 * qb>(ks, qf);
         sc = mma16(qf, k[ks], sc);
         fr.template rows<TB, 32 * qb>(ks, gf);
-        if constexpr (VLDS) vr.template rows<0, 0>(ks, vf);
-        else vf = v[ks];
+        vr.template rows<0, 0>(ks, vf);
         dp = mma16(gf, vf, dp);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -1088,25 +1155,42 @@ __global__ __launch_bounds__((64 * NW), (sizeof(T) == 2 ? 2 : 1)) void past_dkv_
   store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpv : ba.dv) + at, dv, fv, key0, L, key_at, a.D, lane);
 }
 
-// Adds the shares of a class of key blocks in order and writes them out: 0 the prefix's, 1 those with a sink, 2 the others.
+// Adds the shares of the key blocks of all classes that have several (the prefix's, those with a sink, the others) in order and
+// writes them out; which: its workgroups of each class. bf16: a share is in the order of its kernel's registers, [wave][dk, dv][..];
+// float32: [key][dk, dv][D].
+struct JoinBlocks {
+  int64_t upto[3];  // workgroups up to the end of each class
+};
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba, int which_class) {
+__global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba, const JoinBlocks which) {
   const PastArgs &a = ba.f;
-  constexpr int ND = DP / 32;
-  const bool prefix = which_class == 0;
-  const int blocks = prefix ? ba.prefix_blocks : which_class == 1 ? ba.sink_blocks : ba.key_blocks - ba.sink_blocks;
-  const int splits = prefix ? ba.prefix_splits : which_class == 1 ? ba.sink_splits : ba.own_splits;
-  const f32x4 *part = ba.part + (prefix ? 0 : which_class == 1 ? ba.sink_part : ba.own_part);
-  const int64_t per = (int64_t)(prefix ? a.B / a.each : a.B) * a.Hk * blocks * NW * 2 * ND * 4 * 64;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;  // per is a multiple of 256
+  constexpr int ND = DP / 32, KEYS = sizeof(T) == 2 ? 32 * NW : kF32Keys;
+  const int64_t id = blockIdx.x;
+  const int cls = id < which.upto[0] ? 0 : id < which.upto[1] ? 1 : 2;
+  const bool prefix = cls == 0;
+  const int blocks = prefix ? ba.prefix_blocks : cls == 1 ? ba.sink_blocks : ba.key_blocks - ba.sink_blocks;
+  const int splits = prefix ? ba.prefix_splits : cls == 1 ? ba.sink_splits : ba.own_splits;
+  const f32x4 *part = ba.part + (prefix ? 0 : cls == 1 ? ba.sink_part : ba.own_part);
+  const int64_t items = (int64_t)(prefix ? a.B / a.each : a.B) * a.Hk * blocks;
+  const int64_t per = items * (sizeof(T) == 2 ? NW * 2 * ND * 4 * 64 : KEYS * (a.D / 2));
+  const int64_t e = (id - (cls == 0 ? 0 : which.upto[cls - 1])) * 256 + threadIdx.x;
+  if (e >= per) return;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) x += *(const MLORA_GLOBAL f32x4 *)(part + s * per + e);
-  int64_t u = e / 64;
-  const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND), value = (int)(u / 4 / ND % 2);
-  u /= 4 * ND * 2;  // (sample or group, hk, block, wave)
-  const int64_t key = (u % (NW * blocks) + (which_class == 2 ? NW * ba.sink_blocks : 0)) * 32 + (lane & 31), bh = u / (NW * blocks);
-  const int ch = 32 * d + 8 * i + 4 * (lane >> 5), L = prefix ? a.Lp : a.Lk;
+  int64_t u;
+  int in, ch, value;  // key within the block
+  if constexpr (sizeof(T) == 2) {
+    u = e / 64;
+    const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND);
+    value = (int)(u / 4 / ND % 2), u /= 4 * ND * 2;
+    in = (int)(u % NW) * 32 + (lane & 31), ch = 32 * d + 8 * i + 4 * (lane >> 5), u /= NW;
+  } else {
+    u = e / (a.D / 4), ch = (int)(e % (a.D / 4)) * 4;
+    value = (int)(u % 2), u /= 2, in = (int)(u % KEYS), u /= KEYS;
+  }
+  const int64_t key = (u % blocks + (cls == 2 ? ba.sink_blocks : 0)) * KEYS + in, bh = u / blocks;
+  const int L = prefix ? a.Lp : a.Lk;
   if (key >= L || ch >= a.D) return;
   void *base = value ? (prefix ? ba.dpv : ba.dv) : prefix ? ba.dpk : ba.dk;
   T *p = static_cast<T *>(base) + ((bh / a.Hk * L + key) * a.Hk + bh % a.Hk) * a.D + ch;
@@ -1115,24 +1199,264 @@ __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba
   else *(MLORA_GLOBAL f32x4 *)p = x;
 }
 
+// ---------------------------------------------------------------- backward, float32
+//
+// As the forward of few rows: 32 rows (or keys) per workgroup, the waves take different tiles and their sums are joined through LDS.
+// A product of 32 x 32 x 64 channels holds the matrix core for 2048 cycles, so that reading the tiles again for every 32 rows
+// costs less than it would in bf16.
+template <int DP, bool MANY>
+__global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float, DP, false> / 4)) void past_dq_f32_kernel(const PastBwdArgs ba) {
+  const PastArgs &a = ba.f;
+  using Tile = HeadTile<float, DP>;
+  constexpr int KT = 32, NW = kFewWaves<float, DP, MANY>, ND = DP / 16, NS = DP / 32, TB = KT * Tile::RB;
+  static_assert(2 * ND * 64 * 16 <= 2 * TB, "a wave's sums fit its buffer");
+  __shared__ u32x4 smem[2 * TB * NW / 16];
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 2 * TB;
+  Job job;
+  job.init(a, blockIdx.x);
+  const int hk = job.hk, r0 = job.rt * 32, group = job.b / a.each;
+  const Sample s = uniform(sample_of(a, job.b));
+  KeyTiles<KT> tiles;
+  WaveRows wr;
+  tiles.init(a, a.with_prefix ? prefix_keys(a, group) : 0, s.n, max(s.start + r0 / a.G, 0), min(s.start + min(r0 + 31, a.rows - 1) / a.G, s.n - 1));
+  wr.init(a, s, r0, min(r0 + 32, a.rows));
+  const int t1 = job.share(tiles.count, job.sp + 1), t0 = min(job.share(tiles.count, job.sp) + wave, t1);
+  TileStream<float, DP, KT, TB / 1024> in;
+  in.init(a, job.b, group, hk, 0, 1, lane, tiles, t0, t1);
+  if (t0 < t1) in.stage(a, tiles, t0, lds);
+  FewReader<float, DP> fr;
+  fr.init(lane, lds);
+  Row x[2];
+  Frag<float> q[2][NS], g[2][NS];
+  float delta[2], ref[2], shift[2];
+  f32x4 dq[2][ND];
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    x[n] = row_of(a, false, job.b, hk, r0 + 16 * n + (lane & 15), a.rows, s);
+    const bool on = x[n].on;
+    Frag<float> o[NS];
+    load_row<float, DP>(static_cast<const float *>(a.q) + row_place(a, x[n], hk, a.q_sb, a.q_sl, a.q_sh), on, a.D, lane, q[n]);
+    load_row<float, DP>(static_cast<const float *>(ba.g) + row_place(a, x[n], hk, ba.g_sb, ba.g_sl, ba.g_sh), on, a.D, lane, g[n]);
+    load_row<float, DP>(static_cast<const float *>(a.out) + row_place(a, x[n], hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D), on, a.D, lane, o);
+    ref[n] = on ? a.stats[x[n].at] : INFINITY, shift[n] = on ? a.stats[all + x[n].at] : 0.f;
+    delta[n] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta[n] += g[n][ks].v[j] * o[ks].v[j];
+    delta[n] = quarter_sum(delta[n]);
+    if (job.sp == 0 && wave == 0 && lane < 16 && r0 + 16 * n + lane < a.rows) ba.delta[x[n].at] = delta[n];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int t = t0; t < t1; t += NW) {
+    wait_vmcnt<0>();  // tile t is in this wave's buffer
+    asm volatile("" ::: "memory");
+    const int k0 = tiles.key0(t);
+    const bool o = tiles.own(t), rows = o && !wr.everything(a, k0, KT);
+    const uint32_t bits = (uint32_t)tiles.bits(t, t1);
+    f32x4 sc[2][2], dp[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = dp[n][0] = dp[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    few_scores<0, DP, 2>(fr, q, sc);
+    few_scores<TB, DP, 2>(fr, g, dp);
+    Frag<float> ds[2];
+    const bool masked = rows || bits != ~0u;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const uint32_t mine = (rows ? (uint32_t)x[n].bits(a, k0) : bits) >> (4 * (lane >> 4));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float y = sc[n][j / 4][j % 4], z = dp[n][j / 4][j % 4];
+        if (masked && !((mine >> (16 * (j / 4) + j % 4)) & 1)) y = -INFINITY, z = 0.f;
+        ds[n].v[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y - shift[n], a.c, -ref[n])) * (z - delta[n]);
+      }
+    }
+    few_weigh<0, DP, 2>(fr, ds, dq);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and read
+    if (t + NW < t1) in.stage(a, tiles, t + NW, lds);
+  }
+  f32x4 *mine = (f32x4 *)smem + wave * (2 * TB / 16);
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) mine[(n * ND + d) * 64 + lane] = few_vector<float, ND>(dq[n], d);
+  __syncthreads();
+  for (int u = wave; u < 2 * ND; u += NW) {
+    const int n = u / ND, d = u % ND, ch = few_channel<float>(d, lane), r = r0 + 16 * n + (lane & 15);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) y += ((const f32x4 *)smem + w * (2 * TB / 16))[u * 64 + lane];
+    if (r >= a.rows || ch >= a.D) continue;
+    const Row &xr = n == 0 ? x[0] : x[1];
+    if (!xr.on) y = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.splits > 1) ba.part[(job.sp * all + xr.at) * (a.D / 4) + ch / 4] = y;
+    else *(MLORA_GLOBAL f32x4 *)(static_cast<float *>(ba.dq) + row_place(a, xr, hk, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D) + ch) = y * ba.scale;
+  }
+}
+
+template <int DP, bool MANY>
+__global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float, DP, false> / 4)) void past_dkv_f32_kernel(const PastBwdArgs ba) {
+  const PastArgs &a = ba.f;
+  using Tile = HeadTile<float, DP>;
+  constexpr int QT = 32, NW = kFewWaves<float, DP, MANY>, ND = DP / 16, NS = DP / 32, TB = QT * Tile::RB, N = TB / 1024;
+  static_assert(2 * ND * 64 * 16 <= 2 * TB, "half of a wave's sums fit its buffer");
+  __shared__ u32x4 smem[2 * TB * NW / 16 + NW * 24];  // q and the output's gradient of every wave; x, delta and a of its rows
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  MLORA_LDS char *lds = (MLORA_LDS char *)smem + wave * 2 * TB;
+  float *stats = (float *)(smem + 2 * TB * NW / 16 + wave * 24);  // [3][32]
+  KeyJob job;
+  job.init(ba, blockIdx.x);
+  const int hk = job.hk;
+  Sample s{0, 0};
+  if (!job.prefix) s = uniform(sample_of(a, job.o));
+  const int len = job.prefix ? prefix_keys(a, job.o) : s.n, key0 = job.block * kF32Keys;
+  const float *kp = static_cast<const float *>(job.prefix ? a.pk : a.k) + job.o * (job.prefix ? a.pk_sb : a.k_sb) + hk * (job.prefix ? a.pk_sh : a.k_sh);
+  const float *vp = static_cast<const float *>(job.prefix ? a.pv : a.v) + job.o * (job.prefix ? a.pv_sb : a.v_sb) + hk * (job.prefix ? a.pv_sh : a.v_sh);
+  const int64_t k_sl = job.prefix ? a.pk_sl : a.k_sl, v_sl = job.prefix ? a.pv_sl : a.v_sl;
+  // the tokens whose rows see a key, as in the bf16 kernel
+  auto from = [&](int j) __attribute__((always_inline)) { return (int)((uint32_t)j / (uint32_t)a.chunk) * a.chunk; };
+  auto to = [&](int j) __attribute__((always_inline)) {
+    return job.prefix || j < a.sinks ? kEver : (int)((uint32_t)(j + a.window) / (uint32_t)a.chunk) * a.chunk;
+  };
+  const int last_key = min(key0 + kF32Keys, len) - 1;
+  int i0 = 0, i1 = key0 < len ? a.Lq : 0, full_a = 0, full_b = kEver;
+  if (!job.prefix && key0 < len) {
+    const int last = key0 < a.sinks ? kEver : to(last_key);
+    i0 = max(from(key0) - s.start, 0), i1 = max(min(min(last, s.n) - s.start, a.Lq), i0);
+    full_a = from(last_key), full_b = to(max(key0, min(a.sinks, last_key)));
+  }
+  const int tile0 = i0 / QT, head_tiles = max((i1 + QT - 1) / QT - tile0, 0), tiles = head_tiles * a.G * (job.prefix ? a.each : 1);
+  const int t1 = (int)((int64_t)tiles * (job.sp + 1) / job.splits), t0 = min((int)((int64_t)tiles * job.sp / job.splits) + wave, t1);
+  TileLoader<float, DP, N> ql, gl;
+  ql.init(lane, 0, 1, a.q_sl, a.D), gl.init(lane, 0, 1, ba.g_sl, a.D);
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows;
+  uint32_t rows = 0;  // the rows on their way that are tokens
+  int p0 = 0;         // the position of the first
+  float x = 0.f, y = 0.f, z = 0.f;  // of lane's row: x, delta, a
+  auto stage = [&](int t) __attribute__((always_inline)) {
+    const int h = t / head_tiles, m = h / a.G, b = job.prefix ? job.o * a.each + m : job.o, i = (tile0 + t - h * head_tiles) * QT;
+    const Sample ks = job.prefix ? uniform(sample_of(a, b)) : s;
+    const int head = h - m * a.G;
+    const uint64_t live = low_bits(min(min(a.Lq, ks.n - ks.start) - i, QT)) & ~low_bits(-ks.start - i);
+    rows = (uint32_t)live, p0 = ks.start + i;
+    const float *q = static_cast<const float *>(a.q) + b * a.q_sb + (hk * a.G + head) * a.q_sh + i * a.q_sl;
+    const float *g = static_cast<const float *>(ba.g) + b * ba.g_sb + (hk * a.G + head) * ba.g_sh + i * ba.g_sl;
+    if (live == low_bits(QT)) ql.load_all(q, lds), gl.load_all(g, lds + TB);
+    else ql.load(q, live, lds), gl.load(g, live, lds + TB);
+    const int64_t at = ((int64_t)b * a.Hk + hk) * a.rows + (int64_t)(i + (lane & 31)) * a.G + head;
+    const bool on = (rows >> (lane & 31)) & 1;
+    x = on ? a.stats[at] : INFINITY, y = on ? ba.delta[at] : 0.f, z = on ? a.stats[all + at] : 0.f;  // rows without a token: P = 0
+  };
+  if (t0 < t1) stage(t0);
+  Frag<float> k[2][NS], v[2][NS];
+  f32x4 dk[2][ND], dv[2][ND];
+  int mine_a[2], mine_b[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int64_t key = key0 + 16 * n + (lane & 15);
+    const bool live = key < len;
+    load_row<float, DP>(kp + (live ? key * k_sl : 0), live, a.D, lane, k[n]);
+    load_row<float, DP>(vp + (live ? key * v_sl : 0), live, a.D, lane, v[n]);
+    mine_a[n] = job.prefix ? 0 : from((int)key), mine_b[n] = to((int)key);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[n][d] = dv[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  FewReader<float, DP> fr;
+  fr.init(lane, lds);
+  for (int t = t0; t < t1; t += NW) {
+    wait_vmcnt<0>();  // tile t is in this wave's buffer
+    if (lane < 32) stats[lane] = x, stats[32 + lane] = y, stats[64 + lane] = z;
+    asm volatile("" ::: "memory");
+    // rows that are no tokens too: a key that none of the tokens sees may hold anything
+    const bool part = !job.prefix && (p0 < full_a || p0 + QT > full_b), masked = part || rows != ~0u;
+    f32x4 sc[2][2], dp[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = dp[n][0] = dp[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    few_scores<0, DP, 2>(fr, k, sc);
+    few_scores<TB, DP, 2>(fr, v, dp);
+    Frag<float> pf[2], df[2];
+    uint32_t mine[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      mine[n] = rows;
+      if (part) mine[n] &= (uint32_t)(low_bits(mine_b[n] - p0) & ~low_bits(mine_a[n] - p0));
+      mine[n] >>= 4 * (lane >> 4);
+    }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const int r = 16 * qb + 4 * (lane >> 4);
+      const f32x4 ref = *(const f32x4 *)(stats + r), delta = *(const f32x4 *)(stats + 32 + r), shift = *(const f32x4 *)(stats + 64 + r);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float u = sc[n][qb][i], w = dp[n][qb][i];
+          if (masked && !((mine[n] >> (16 * qb + i)) & 1)) u = -INFINITY, w = 0.f;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(u - shift[i], a.c, -ref[i]));
+          pf[n].v[4 * qb + i] = p, df[n].v[4 * qb + i] = p * (w - delta[i]);
+        }
+    }
+    few_weigh<TB, DP, 2>(fr, pf, dv);
+    few_weigh<0, DP, 2>(fr, df, dk);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and read
+    if (t + NW < t1) stage(t + NW);
+  }
+  // the waves' sums, dk and then dv, through the buffers
+  const int L = job.prefix ? a.Lp : a.Lk;
+#pragma unroll
+  for (int value = 0; value < 2; ++value) {
+    __syncthreads();
+    f32x4 *to_sum = (f32x4 *)smem + wave * (2 * TB / 16);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) to_sum[(n * ND + d) * 64 + lane] = few_vector<float, ND>(value ? dv[n] : dk[n], d);
+    __syncthreads();
+    for (int u = wave; u < 2 * ND; u += NW) {
+      const int in = 16 * (u / ND) + (lane & 15), ch = few_channel<float>(u % ND, lane);
+      const int64_t key = key0 + in;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sum += ((const f32x4 *)smem + w * (2 * TB / 16))[u * 64 + lane];
+      if (ch >= a.D) continue;
+      if (key >= len) sum = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever its zeroed fragments gave
+      if (job.splits > 1) {
+        ba.part[job.part + (((job.sp * job.items + job.item) * kF32Keys + in) * 2 + value) * (a.D / 4) + ch / 4] = sum;
+      } else if (key < L) {
+        float *p = static_cast<float *>(value ? (job.prefix ? ba.dpv : ba.dv) : job.prefix ? ba.dpk : ba.dk);
+        *(MLORA_GLOBAL f32x4 *)(p + ((job.o * (int64_t)L + key) * a.Hk + hk) * a.D + ch) = value ? sum : sum * ba.scale;
+      }
+    }
+  }
+}
+
 // The kernels are named here because hipcc's host pass does not instantiate a kernel that holds generic lambdas
 // from a launch inside one.
-#define MLORA_PAST(T, DP)                                             \
-  template __global__ void past_fwd_kernel<T, DP>(const PastArgs);    \
-  template __global__ void past_few_kernel<T, DP, 1>(const PastArgs); \
-  template __global__ void past_few_kernel<T, DP, 2>(const PastArgs); \
-  template __global__ void past_dq_kernel<T, DP>(const PastBwdArgs);  \
-  template __global__ void past_dkv_kernel<T, DP, 4>(const PastBwdArgs);
-MLORA_PAST(uint16_t, 64)
-MLORA_PAST(uint16_t, 128)
-MLORA_PAST(float, 64)
-MLORA_PAST(float, 128)
+#define MLORA_PAST(DP)                                                             \
+  template __global__ void past_fwd_kernel<DP>(const PastArgs);                    \
+  template __global__ void past_few_kernel<uint16_t, DP, 1, false>(const PastArgs); \
+  template __global__ void past_few_kernel<uint16_t, DP, 2, false>(const PastArgs); \
+  template __global__ void past_few_kernel<float, DP, 1, false>(const PastArgs);   \
+  template __global__ void past_few_kernel<float, DP, 2, false>(const PastArgs);   \
+  template __global__ void past_few_kernel<float, DP, 2, true>(const PastArgs);    \
+  template __global__ void past_dq_kernel<DP>(const PastBwdArgs);                  \
+  template __global__ void past_dq_f32_kernel<DP, false>(const PastBwdArgs);       \
+  template __global__ void past_dq_f32_kernel<DP, true>(const PastBwdArgs);        \
+  template __global__ void past_dkv_kernel<DP, 4>(const PastBwdArgs);              \
+  template __global__ void past_dkv_f32_kernel<DP, false>(const PastBwdArgs);      \
+  template __global__ void past_dkv_f32_kernel<DP, true>(const PastBwdArgs);
+MLORA_PAST(64)
+MLORA_PAST(128)
 #undef MLORA_PAST
-template __global__ void past_dkv_kernel<uint16_t, 128, 8>(const PastBwdArgs);
+template __global__ void past_dkv_kernel<128, 8>(const PastBwdArgs);
 
 // ------------------------------------------------------------------ host
 
-constexpr int64_t kPastMostTokens = 1 << 28;
+constexpr int64_t kPastMostTokens = 1 << 28, kPastMostBlocks = INT32_MAX - 65536;
+constexpr int64_t kFewMany = 256;  // float32 workgroups from which on they have half the waves
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -1156,8 +1480,8 @@ static int past_sizes(PastSizes &z, const mlora_past_shape *s) {
   if (z.Lq > kPastMostTokens || z.Lk > kPastMostTokens || z.Lp > kPastMostTokens || z.H > 65536) return MLORA_ERR_LIMIT;
   z.groups = s->groups > 0 ? s->groups : z.B, z.each = z.groups > 0 ? z.B / z.groups : 1;
   z.rows = z.G * z.Lq;
-  // workgroups: one per (sample, key head, 128 rows or keys), a few thousand shares beside them; rows of a group
-  const int64_t most = INT32_MAX - 65536, blocks = ceil_div(z.rows, 128) + ceil_div(z.Lk, 128) + ceil_div(z.Lp, 128) + 1;
+  // workgroups: one per (sample, key head, 32 rows or keys at least), a few thousand shares beside them; rows of a group
+  const int64_t most = kPastMostBlocks, blocks = ceil_div(z.rows, 32) + ceil_div(z.Lk, 32) + ceil_div(z.Lp, 32) + 1;
   if (z.rows > most || (z.B > 0 && (z.Hk > most / z.B || blocks + 4096 > most / (z.B * z.Hk) || z.rows > most / z.B))) return MLORA_ERR_LIMIT;
   z.chunk = between(s->chunk, 1, z.Lk > 1 ? z.Lk : 1);  // from there on all keys are one chunk
   z.window = s->window > 0 ? between(s->window, z.chunk, z.Lk + z.chunk) : z.Lk + z.chunk;
@@ -1172,9 +1496,9 @@ static int64_t own_tiles(const PastSizes &z, int64_t rows, int64_t kt) {
   return some < all ? some : all;
 }
 
-// How a forward is cut. Few rows per key head run waves over different keys, more rows 128 per workgroup. Few rows
-// of samples that share a prefix take it together, in workgroups of its own: then all shares are joined. Keys are shared
-// out where there is less than a workgroup for every compute unit.
+// How a forward is cut. Up to 64 rows per key head, and all of them in float32, run waves over different keys, 32 rows per workgroup;
+// more rows 128 per workgroup. Up to 64 rows of samples that share a prefix take it together, in workgroups of its own: then
+// all shares are joined. Keys are shared out where there is less than a workgroup for every compute unit.
 struct PastPlan {
   bool few, packed, packed_few;
   int64_t packed_tiles, packed_splits, row_tiles, splits, slots;
@@ -1182,15 +1506,15 @@ struct PastPlan {
 
 static PastPlan past_plan(const PastSizes &z) {
   PastPlan p{};
-  const int64_t few_rows = 64, waves = z.f32 && z.D > 64 ? 4 : 8, e = z.f32 ? 4 : 2;
+  const int64_t few_rows = z.f32 ? INT64_MAX : 64, waves = z.f32 && z.D > 64 ? 4 : 8, e = z.f32 ? 4 : 2;
   p.few = z.rows <= few_rows;
-  p.packed = p.few && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
+  p.packed = z.rows <= 64 && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
   p.row_tiles = ceil_div(z.rows, p.few ? 32 : 128);
   auto share = [&](int64_t items, int64_t tiles, bool few) {
     // tiles that a share is worth its join for. Few rows: one tile per wave (1024 keys in 4 shares 10.1 us, in 2 11.8, in one 11.3),
     // from four per wave on (576 keys in 2 shares 10.0 us, in one 7.2)
     const int64_t least = few ? (tiles < 4 * waves ? tiles + 1 : waves) : z.f32 ? 2 : 8;
-    return items > 0 ? between(256 / items, 1, between(tiles / least, 1, 64)) : 1;
+    return items > 0 ? between((few || !z.f32 ? 256 : 256) / items, 1, between(tiles / least, 1, 64)) : 1;
   };
   const int64_t kt = p.few || z.f32 ? 32 : 64;
   const int64_t prefix_tiles = p.packed ? 0 : ceil_div(z.Lp, kt);
@@ -1209,6 +1533,11 @@ static int64_t past_floats(const PastPlan &p, const PastSizes &z) {
   return p.slots > 1 ? p.slots * ceil_div(z.B * z.Hk * z.rows * (z.D + 2), 4) * 4 : 0;
 }
 
+// Shares are joined by a workgroup per row.
+static int past_join_limit(const PastPlan &p, const PastSizes &z) {
+  return p.slots > 1 && z.B * z.Hk > kPastMostBlocks / z.rows ? MLORA_ERR_LIMIT : MLORA_OK;
+}
+
 struct PastBwdPlan {
   int nw;  // waves of dk / dv, 32 keys each
   int64_t row_tiles, splits;
@@ -1220,13 +1549,14 @@ struct PastBwdPlan {
 static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   PastBwdPlan p{};
   const int64_t kt = z.f32 ? 32 : 64, dp = z.D > 64 ? 128 : 64;
-  p.row_tiles = ceil_div(z.rows, 128);
-  const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, 128, kt) + ceil_div(z.Lp, kt), places = z.f32 ? 256 : 512;
-  p.splits = items > 0 ? between(places / items, 1, between(tiles / (z.f32 ? 1 : 4), 1, 64)) : 1;
-  p.dq_vectors = items * 4 * (dp / 32) * 4 * 64;
+  const int64_t row_tile = z.f32 ? 32 : 128;
+  p.row_tiles = ceil_div(z.rows, row_tile);
+  const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, row_tile, kt) + ceil_div(z.Lp, kt), places = z.f32 ? 256 : 512;
+  p.splits = items > 0 ? between(places / items, 1, between(tiles / (z.f32 ? 8 : 4), 1, 64)) : 1;
+  p.dq_vectors = z.f32 ? z.B * z.Hk * z.rows * (z.D / 4) : items * 4 * (dp / 32) * 4 * 64;
   const int64_t longest = z.Lk > z.Lp ? z.Lk : z.Lp;
   p.nw = !z.f32 && z.D > 64 && longest > 128 ? 8 : 4;
-  const int64_t qt = z.f32 || (z.D > 64 && p.nw == 4) ? 32 : 64, keys = 32 * p.nw;
+  const int64_t qt = z.f32 || (z.D > 64 && p.nw == 4) ? 32 : 64, keys = z.f32 ? kF32Keys : 32 * p.nw;
   p.key_blocks = ceil_div(z.Lk, keys), p.prefix_blocks = ceil_div(z.Lp, keys);
   const bool bounded = z.window < z.Lk;
   p.sink_blocks = bounded ? between(ceil_div(z.sinks, keys), 0, p.key_blocks) : 0;  // without a window all blocks are alike
@@ -1236,13 +1566,13 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   const int64_t prefix_items = z.groups * z.Hk * p.prefix_blocks, sink_items = z.B * z.Hk * p.sink_blocks,
                 own_items = z.B * z.Hk * (p.key_blocks - p.sink_blocks);
   const int64_t total = prefix_items * prefix_work + sink_items * sink_work + own_items * own_work;
-  const int64_t slots = p.nw == 8 || z.f32 ? 256 : 512;
+  const int64_t slots = p.nw == 8 ? 256 : 1024;
   int64_t target = ceil_div(total, slots);
-  const int64_t least = z.f32 ? 2 : 4;
+  const int64_t least = z.f32 ? 8 : 4;
   if (target < least) target = least;
   auto cut = [&](int64_t work, int64_t n) { return n > 0 ? between(work / target, 1, 64) : 1; };
   p.prefix_splits = cut(prefix_work, prefix_items), p.sink_splits = cut(sink_work, sink_items), p.own_splits = cut(own_work, own_items);
-  const int64_t per = p.nw * 2 * (dp / 32) * 4 * 64;
+  const int64_t per = z.f32 ? keys * (z.D / 2) : p.nw * 2 * (dp / 32) * 4 * 64;
   p.prefix_vectors = p.prefix_splits > 1 ? prefix_items * p.prefix_splits * per : 0;
   p.sink_vectors = p.sink_splits > 1 ? sink_items * p.sink_splits * per : 0;
   p.own_vectors = p.own_splits > 1 ? own_items * p.own_splits * per : 0;
@@ -1303,8 +1633,11 @@ using namespace mlora;
 
 extern "C" int64_t mlora_past_attention_workspace_bytes(const mlora_past_shape *shape) {
   PastSizes z;
-  const int st = past_sizes(z, shape);
-  return st ? st : past_floats(past_plan(z), z) * (int64_t)sizeof(float);
+  int st = past_sizes(z, shape);
+  if (st) return st;
+  const PastPlan p = past_plan(z);
+  st = past_join_limit(p, z);
+  return st ? st : past_floats(p, z) * (int64_t)sizeof(float);
 }
 
 extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q, const void *k, const void *v, const void *pk,
@@ -1320,6 +1653,8 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   if (out == nullptr || (stats != nullptr && !z.f32 && rest == nullptr)) return MLORA_ERR_INVALID;
   if (!aligned16(out) || !aligned16(rest) || (reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return MLORA_ERR_UNSUPPORTED;
   const PastPlan p = past_plan(z);
+  st = past_join_limit(p, z);
+  if (st) return st;
   const int64_t floats = past_floats(p, z);
   if (floats > 0) {
     if (workspace == nullptr || workspace_bytes < floats * (int64_t)sizeof(float)) return MLORA_ERR_WORKSPACE;
@@ -1336,23 +1671,31 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   with_head(z.f32, z.D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
-    if (!p.few) {
-      hipLaunchKernelGGL((past_fwd_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-      return;
-    }
-    if (p.packed && !p.packed_few) {  // the prefix's workgroups are of the other kernel
-      a.packed_blocks = (int32_t)packed;
-      hipLaunchKernelGGL((past_fwd_kernel<T, DP>), dim3((unsigned)packed), dim3(256), 0, s, a);
+    if constexpr (sizeof(T) == 2) {
+      if (!p.few) {
+        hipLaunchKernelGGL(past_fwd_kernel<DP>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        return;
+      }
+      if (p.packed && !p.packed_few) {  // the prefix's workgroups are of the other kernel
+        a.packed_blocks = (int32_t)packed;
+        hipLaunchKernelGGL(past_fwd_kernel<DP>, dim3((unsigned)packed), dim3(256), 0, s, a);
+      }
     }
     a.packed_blocks = p.packed_few ? (int32_t)packed : 0;
     const dim3 grid((unsigned)(blocks + a.packed_blocks));
     const int64_t rows = p.packed_few ? z.each * z.rows : z.rows;
-    auto go = [&](auto nc) {
-      constexpr int NC = decltype(nc)::value;
-      hipLaunchKernelGGL((past_few_kernel<T, DP, NC>), grid, dim3(64 * PastFew<T, DP, NC>::NW), 0, s, a);
-    };
-    if (rows <= 16) return go(std::integral_constant<int, 1>{});
-    go(std::integral_constant<int, 2>{});
+    constexpr int threads = 64 * kFewWaves<T, DP, false>;
+    if (rows <= 16) {
+      hipLaunchKernelGGL((past_few_kernel<T, DP, 1, false>), grid, dim3(threads), 0, s, a);
+      return;
+    }
+    if constexpr (sizeof(T) == 4) {
+      if (blocks + a.packed_blocks > kFewMany) {
+        hipLaunchKernelGGL((past_few_kernel<T, DP, 2, true>), grid, dim3(threads / 2), 0, s, a);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((past_few_kernel<T, DP, 2, false>), grid, dim3(threads), 0, s, a);
   });
   st = launch_status();
   if (st || p.slots == 1) return st;
@@ -1405,8 +1748,11 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
     with_head(z.f32, z.D, [&](auto t, auto dp) {
       using T = decltype(t);
       constexpr int DP = decltype(dp)::value;
-      hipLaunchKernelGGL((past_dq_kernel<T, DP>), dim3((unsigned)(z.B * z.Hk * p.row_tiles * p.splits)), dim3(256), 0, s, ba);
-      if (p.splits > 1) hipLaunchKernelGGL((past_dq_join_kernel<T, DP>), dim3((unsigned)(p.dq_vectors / 256)), dim3(256), 0, s, ba);
+      const dim3 grid((unsigned)(z.B * z.Hk * p.row_tiles * p.splits));
+      if constexpr (sizeof(T) == 2) hipLaunchKernelGGL(past_dq_kernel<DP>, grid, dim3(256), 0, s, ba);
+      else if (grid.x > kFewMany) hipLaunchKernelGGL((past_dq_f32_kernel<DP, true>), grid, dim3(64 * kFewWaves<float, DP, true>), 0, s, ba);
+      else hipLaunchKernelGGL((past_dq_f32_kernel<DP, false>), grid, dim3(64 * kFewWaves<float, DP, false>), 0, s, ba);
+      if (p.splits > 1) hipLaunchKernelGGL((past_dq_join_kernel<T, DP>), dim3((unsigned)ceil_div(p.dq_vectors, 256)), dim3(256), 0, s, ba);
     });
     st = launch_status();
     if (st) return st;
@@ -1415,15 +1761,19 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
   const int64_t splits[3] = {p.prefix_splits, p.sink_splits, p.own_splits};
   const int64_t blocks = items[0] * splits[0] + items[1] * splits[1] + items[2] * splits[2];
   if (blocks == 0) return MLORA_OK;
+  const int64_t vectors[3] = {p.prefix_vectors, p.sink_vectors, p.own_vectors};
+  JoinBlocks joins;
+  int64_t join_blocks = 0;
+  for (int c = 0; c < 3; ++c) joins.upto[c] = join_blocks += splits[c] > 1 ? ceil_div(vectors[c] / splits[c], 256) : 0;
   with_head(z.f32, z.D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     auto go = [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
-      hipLaunchKernelGGL((past_dkv_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, ba);
-      for (int c = 0; c < 3; ++c)
-        if (splits[c] > 1)
-          hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, NW>), dim3((unsigned)(items[c] * NW * 2 * (DP / 32))), dim3(256), 0, s, ba, c);
+      if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((past_dkv_kernel<DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, ba);
+      else if (blocks > kFewMany) hipLaunchKernelGGL((past_dkv_f32_kernel<DP, true>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, true>), 0, s, ba);
+      else hipLaunchKernelGGL((past_dkv_f32_kernel<DP, false>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, false>), 0, s, ba);
+      if (join_blocks > 0) hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, NW>), dim3((unsigned)join_blocks), dim3(256), 0, s, ba, joins);
     };
     if constexpr (sizeof(T) == 2 && DP == 128) {
       if (p.nw == 8) return go(std::integral_constant<int, 8>{});
