@@ -1504,17 +1504,36 @@ struct PastPlan {
   int64_t packed_tiles, packed_splits, row_tiles, splits, slots;
 };
 
+// Into how many shares the key tiles of `items` workgroups of 128 rows are cut, two of which share a compute unit: what takes least
+// time, in microseconds. A tile of 64 keys takes 1.5 where a workgroup has the unit for itself and 2.0 where two share it (128
+// channels; the ratio is what counts), a share one and a half tiles more for its start; its sums are written, read and joined by
+// another launch (the forward's, row by row, at 4 TB/s, dq's, as they lie in registers, at 8). A frame of 1560 tokens on nine
+// others, 12 heads (156 workgroups of 244 tiles): 381 us in one share, 203 in three; on 14040 keys that two samples share (312) 478
+// and 386; by itself (156 of 25) 46 and 50: under 7 % it is not worth the launch.
+static int64_t wide_shares(int64_t items, int64_t tiles, int64_t floats, double bytes_per_us) {
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t n = 1; n <= 16 && (n == 1 || tiles >= 8 * n); ++n) {
+    const int64_t blocks = items * n, left = blocks % 512;
+    double t = (2.0 * (double)(blocks / 512) + (left == 0 ? 0.0 : left <= 256 ? 1.5 : 2.0)) * ((double)ceil_div(tiles, n) + 1.5);
+    if (n > 1) t += 5.0 + (double)blocks * (double)floats * 8 / bytes_per_us;
+    if (n == 1 || t < 0.93 * least) least = t, best = n;
+  }
+  return best;
+}
+
 static PastPlan past_plan(const PastSizes &z) {
   PastPlan p{};
   const int64_t few_rows = z.f32 ? INT64_MAX : 64, waves = z.f32 && z.D > 64 ? 4 : 8, e = z.f32 ? 4 : 2;
   p.few = z.rows <= few_rows;
   p.packed = z.rows <= 64 && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
   p.row_tiles = ceil_div(z.rows, p.few ? 32 : 128);
-  auto share = [&](int64_t items, int64_t tiles, bool few) {
-    // tiles that a share is worth its join for. Few rows: one tile per wave (1024 keys in 4 shares 10.1 us, in 2 11.8, in one 11.3),
-    // from four per wave on (576 keys in 2 shares 10.0 us, in one 7.2)
-    const int64_t least = few ? (tiles < 4 * waves ? tiles + 1 : waves) : z.f32 ? 2 : 8;
-    return items > 0 ? between((few || !z.f32 ? 256 : 256) / items, 1, between(tiles / least, 1, 64)) : 1;
+  auto share = [&](int64_t items, int64_t tiles, bool few) -> int64_t {
+    if (items <= 0) return 1;
+    if (!few) return wide_shares(items, tiles, 128 * z.D, 4e6);
+    // tiles that a share is worth its join for: one per wave (1024 keys in 4 shares 10.1 us, in 2 11.8, in one 11.3), from four per
+    // wave on (576 keys in 2 shares 10.0 us, in one 7.2)
+    return between(256 / items, 1, between(tiles < 4 * waves ? 1 : tiles / waves, 1, 64));
   };
   const int64_t kt = p.few || z.f32 ? 32 : 64;
   const int64_t prefix_tiles = p.packed ? 0 : ceil_div(z.Lp, kt);
@@ -1535,7 +1554,7 @@ static int64_t past_floats(const PastPlan &p, const PastSizes &z) {
 
 // Shares are joined by a workgroup per row.
 static int past_join_limit(const PastPlan &p, const PastSizes &z) {
-  return p.slots > 1 && z.B * z.Hk > kPastMostBlocks / z.rows ? MLORA_ERR_LIMIT : MLORA_OK;
+  return p.slots > 1 && z.rows > 0 && z.B * z.Hk > kPastMostBlocks / z.rows ? MLORA_ERR_LIMIT : MLORA_OK;
 }
 
 struct PastBwdPlan {
@@ -1551,8 +1570,8 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   const int64_t kt = z.f32 ? 32 : 64, dp = z.D > 64 ? 128 : 64;
   const int64_t row_tile = z.f32 ? 32 : 128;
   p.row_tiles = ceil_div(z.rows, row_tile);
-  const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, row_tile, kt) + ceil_div(z.Lp, kt), places = z.f32 ? 256 : 512;
-  p.splits = items > 0 ? between(places / items, 1, between(tiles / (z.f32 ? 8 : 4), 1, 64)) : 1;
+  const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, row_tile, kt) + ceil_div(z.Lp, kt);
+  p.splits = items <= 0 ? 1 : !z.f32 ? wide_shares(items, tiles, 128 * dp, 8e6) : between(256 / items, 1, between(tiles / 8, 1, 64));
   p.dq_vectors = z.f32 ? z.B * z.Hk * z.rows * (z.D / 4) : items * 4 * (dp / 32) * 4 * 64;
   const int64_t longest = z.Lk > z.Lp ? z.Lk : z.Lp;
   p.nw = !z.f32 && z.D > 64 && longest > 128 ? 8 : 4;
