@@ -13,6 +13,8 @@
 // so that 32 rows are 32 / G neighbouring tokens and see almost the same keys.
 #include "mlora_attention.h"
 
+#include <algorithm>
+
 namespace mlora {
 
 struct PastArgs {
@@ -194,6 +196,106 @@ __device__ __forceinline__ void finish_rows(const PastArgs &a, const Row &x, boo
       }
     store_row<uint16_t, DP>(a.rest, at, there, o, 1.f, a.D, lane);
   }
+}
+
+// Tiles of bf16 rows padded to 128 channels, laid out so that a lane's fragment addresses are one register and constants: 1024 bytes
+// hold four rows, 64 bytes of each after the other, and blocks of four rows lie 1040 bytes apart: 16 rows read at one chunk, and
+// the 4 rows x 64 bytes of a transposing read, meet every bank once. HeadTile's swizzle takes 24 address registers in dk / dv, which
+// then has none left to read an operand ahead of its product.
+template <int DP>
+struct PastTile {
+  static constexpr int BLOCK = 1024, ROWS = 8, ROW = 128;
+  template <int RT>
+  static constexpr int bytes() { return RT * ROW; }
+};
+template <>
+struct PastTile<128> {
+  static constexpr int BLOCK = 1040, ROWS = 4;
+  template <int RT>
+  static constexpr int bytes() { return RT / 4 * 1040; }
+};
+
+template <int DP>
+struct PastReader {
+  FragReader<uint16_t, DP> fr;
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) { fr.init(lane, base); }
+  __device__ __forceinline__ void move(int by) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) fr.row[s] += by;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) fr.col[d][0] += by, fr.col[d][1] += by;
+  }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void rows(int s, Frag<uint16_t> &f) const { fr.template rows<OFF, R0>(s, f); }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void cols(int d, Frag<uint16_t> &f) const { fr.template cols<OFF, R0>(d, f); }
+};
+template <>
+struct PastReader<128> {
+  int32_t row, col;
+  __device__ __forceinline__ void init(int lane, const MLORA_LDS char *base) {
+    const int at = (int)(uintptr_t)base, r = lane & 31, g = lane >> 4, m = lane & 15;
+    row = at + (r >> 2) * 1040 + (r & 3) * 64 + (lane >> 5) * 16;
+    col = at + (g >> 1) * 1040 + (m >> 2) * 64 + (2 * (g & 1) + ((m & 3) >> 1)) * 16 + 8 * (m & 1);
+  }
+  __device__ __forceinline__ void move(int by) { row += by, col += by; }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void rows(int s, Frag<uint16_t> &f) const {
+    f.v = *(const lds_u4 *)((const MLORA_LDS char *)(uintptr_t)(uint32_t)row + OFF + R0 / 4 * 1040 + s / 2 * 256 + s % 2 * 32);
+  }
+  template <int OFF, int R0>
+  __device__ __forceinline__ void cols(int d, Frag<uint16_t> &f) const {
+    typedef MLORA_LDS bf16x4 lds_b4;
+    const MLORA_LDS char *p = (const MLORA_LDS char *)(uintptr_t)(uint32_t)col + OFF + R0 / 4 * 1040 + d * 256;
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)p));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4 *)(p + 2 * 1040)));
+    f.v = u32x4{x[0], x[1], y[0], y[1]};
+  }
+};
+
+// TileLoader for them: N of a tile's blocks by the calling wave.
+template <int DP, int N>
+struct PastLoader {
+  static constexpr int ROWS = PastTile<DP>::ROWS;
+  int32_t off[N], first, step, r0;
+  __device__ __forceinline__ void init(int lane, int first_block, int block_step, int64_t stride, int head_dim) {
+    first = first_block, step = block_step, r0 = DP == 128 ? (lane >> 2) & 3 : lane / 8;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (first + i * step) * ROWS + r0;
+      const int c = DP == 128 ? (lane >> 4) * 4 + (lane & 3) : (lane % 8) ^ HeadTile<uint16_t, 64>::swz(r);
+      off[i] = c * 8 < head_dim ? (int32_t)(r * stride * 2) + c * 16 : kOOB;
+    }
+  }
+  __device__ __forceinline__ void load(const void *base, uint64_t live, MLORA_LDS char *lds) const {
+    const auto rsrc = make_rsrc(base, (int64_t)kOOB);
+    const bool all = live == ~0ull;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int blk = first + i * step;
+      const bool on = all || ((live >> (blk * ROWS + r0)) & 1);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (MLORA_LDS void *)(lds + blk * PastTile<DP>::BLOCK), 16, on ? off[i] : kOOB, 0, 0, 0);
+    }
+  }
+};
+
+// use(i, f) for i = 0 .. N - 1 with f as read(i) gave it, each read AHEAD uses before. The compiler alone reads an operand right before
+// its product and waits for it.
+template <int N, int AHEAD, class Read, class Use>
+__device__ __forceinline__ void read_ahead(Read &&read, Use &&use) {
+  using F = decltype(read(std::integral_constant<int, 0>{}));
+  F ring[AHEAD + 1];
+  static_for<(AHEAD < N ? AHEAD : N)>([&](auto i) __attribute__((always_inline)) {
+    ring[decltype(i)::value] = read(i);
+    return true;
+  });
+  static_for<N>([&](auto i) __attribute__((always_inline)) {
+    constexpr int I = decltype(i)::value;
+    if constexpr (I + AHEAD < N) ring[(I + AHEAD) % (AHEAD + 1)] = read(std::integral_constant<int, I + AHEAD>{});
+    use(i, ring[I % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+    return true;
+  });
 }
 
 // Four waves of 32 rows each against the same key tiles, two buffers of K and V in LDS: tile t + 1 loads while tile
@@ -922,13 +1024,6 @@ __global__ __launch_bounds__(256) void past_dq_join_kernel(const PastBwdArgs ba)
   else *(MLORA_GLOBAL f32x4 *)p = x;
 }
 
-// bf16: NW waves own 32 keys each (K fragments in registers; V in LDS, two waves per SIMD leave no room for it) and share tiles of QT query rows of one head in LDS, double-buffered: q, the output's gradient and the rows'
-// x, delta and a.
-template <int DP, int NW>
-struct PastDkv {
-  static constexpr int QT = DP == 128 && NW == 4 ? 32 : 64;
-};
-
 constexpr int kF32Keys = 32;  // of a workgroup in float32
 
 // A workgroup of dk / dv: which keys, and which share of the rows that see them. Blocks of the prefix come first, then those
@@ -957,26 +1052,33 @@ struct KeyJob {
   int64_t items, item;
 };
 
-template <int DP, int NW>
-__global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArgs ba) {
+// bf16: KW waves own 32 keys each (K fragments in registers; V in LDS, two waves per SIMD leave no room for it) and share tiles of query
+// rows of one head in LDS: q, the output's gradient and the rows' x, delta and a, NB buffers, so that a tile has NB - 1 others' time to
+// arrive in. RG 2: two such groups take half of every tile's rows each and add their sums at the end, so that half the keys
+// fill a compute unit.
+template <int DP, int RG>
+constexpr int kDkvBuffers = DP == 128 && RG == 1 ? 2 : 3;
+
+template <int DP, int KW, int RG>
+__global__ __launch_bounds__((64 * KW * RG), 2) void past_dkv_kernel(const PastBwdArgs ba) {
   using T = uint16_t;
   const PastArgs &a = ba.f;
-  constexpr int QT = PastDkv<DP, NW>::QT, ND = DP / 32, NS = DP / 16;
-  using Tile = HeadTile<T, DP>;
-  constexpr int TB = QT * Tile::RB, N = TB / 1024 / NW, VB = 32 * Tile::RB;
-  static_assert(64 * NW >= 3 * QT, "a thread loads one of a row's three values");
-  // one array, so that the readers' buffers start at a multiple of 4 TB; then V, then x, delta and a per buffer
-  __shared__ u32x4 smem[(4 * TB + NW * VB) / 16 + 3 * QT / 2];
-  f32x4 (&stats)[2][3][QT / 4] = *(f32x4 (*)[2][3][QT / 4])(smem + (4 * TB + NW * VB) / 16);
+  constexpr int NW = KW * RG, QT = 64, NB = kDkvBuffers<DP, RG>, ND = DP / 32, NS = DP / 16;
+  using Tile = PastTile<DP>;
+  constexpr int TB = Tile::template bytes<QT>(), N = QT / Tile::ROWS / NW, VB = Tile::template bytes<32>();
+  static_assert(NW >= 4 && (NB - 2) * (2 * N + 1) < 64, "a wave for each of a row's values; the loads on their way");
+  // q and the output's gradient of every buffer; V; x, delta and a (and nothing) of every buffer's rows
+  constexpr int ST = 4 * 256;
+  __shared__ u32x4 smem[(NB * (2 * TB + ST) + KW * VB) / 16];
   MLORA_LDS char *lds = (MLORA_LDS char *)smem;
-  const int wave = wave_id(), lane = threadIdx.x & 63;
+  const int wave = wave_id(), kw = wave % KW, rg = wave / KW, lane = threadIdx.x & 63;
   KeyJob job;
   job.init(ba, blockIdx.x);
   const int hk = job.hk;
   Sample s{0, 0};
   if (!job.prefix) s = uniform(sample_of(a, job.o));
   const int len = job.prefix ? prefix_keys(a, job.o) : s.n;
-  const int key0 = (job.block * NW + wave) * 32, key = key0 + (lane & 31);
+  const int key0 = (job.block * KW + kw) * 32, key = key0 + (lane & 31);
   const bool live = key < len;
   const uint64_t live_bits = low_bits(min(len - key0, 32));
   const T *kp = static_cast<const T *>(job.prefix ? a.pk : a.k) + job.o * (job.prefix ? a.pk_sb : a.k_sb) + hk * (job.prefix ? a.pk_sh : a.k_sh);
@@ -988,9 +1090,9 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
     const int d = 16 * ks + 8 * (lane >> 5);
     load_frag(kp, key * k_sl + d, live && d < a.D, k[ks]);
   }
-  MLORA_LDS char *vt = lds + 4 * TB + wave * VB;
-  {
-    TileLoader<T, DP, VB / 1024> vl;
+  MLORA_LDS char *vt = lds + NB * 2 * TB + kw * VB, *values = lds + NB * 2 * TB + KW * VB;
+  if (rg == 0) {
+    PastLoader<DP, 32 / Tile::ROWS> vl;
     vl.init(lane, 0, 1, v_sl, a.D);
     vl.load(vp + (int64_t)key0 * v_sl, live_bits, vt);
   }
@@ -1004,7 +1106,7 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
   auto to = [&](int j) __attribute__((always_inline)) {
     return job.prefix || j < a.sinks ? kEver : (int)((uint32_t)(j + a.window) / (uint32_t)a.chunk) * a.chunk;
   };
-  const int bk0 = job.block * NW * 32, bk1 = min(bk0 + NW * 32, len) - 1;  // the block's keys
+  const int bk0 = job.block * KW * 32, bk1 = min(bk0 + KW * 32, len) - 1;  // the block's keys
   int i0 = 0, i1 = bk0 < len ? a.Lq : 0;  // the block's tokens, of an own block
   if (!job.prefix && bk0 < len) {
     const int last = bk0 < a.sinks ? kEver : to(bk1);
@@ -1019,61 +1121,72 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
     some_a = from(key0), full_a = from(k1), full_b = to(k2), some_b = key0 < a.sinks ? kEver : to(k1);
     mine_a = from(key), mine_b = to(key);
   }
-  TileLoader<T, DP, N> ql, gl;
+  PastLoader<DP, N> ql, gl;
   ql.init(lane, wave, NW, a.q_sl, a.D), gl.init(lane, wave, NW, ba.g_sl, a.D);
   const int64_t all = (int64_t)a.B * a.Hk * a.rows;
-  FragReader<T, DP> fr, vr;
-  fr.init(lane, lds), vr.init(lane, vt);
-  struct Tokens {
-    int b, g, i;  // sample, head, first token
-  };
-  auto tokens = [&](int t) __attribute__((always_inline)) {
-    const int h = t / head_tiles, m = h / a.G;
-    return Tokens{job.prefix ? job.o * a.each + m : job.o, h - m * a.G, (tile0 + t - h * head_tiles) * QT};
-  };
-  // a tile's rows into LDS, those that are tokens as bits in `rows`; returns x (threads 0 .. QT - 1), delta (QT .. 2 QT - 1) or
-  // a (.. 3 QT - 1) of the thread's row
-  uint64_t rows = 0, next = 0;
-  auto stage = [&](int t, int buf) __attribute__((always_inline)) -> float {
-    const int i = threadIdx.x % QT, which = threadIdx.x / QT;
-    float x = which == 0 ? INFINITY : 0.f;  // rows without a token: P = 0
-    if (t >= t1) return x;
-    const Tokens k = tokens(t);
-    const Sample ks = job.prefix ? uniform(sample_of(a, k.b)) : s;
-    next = low_bits(min(min(a.Lq, ks.n - ks.start) - k.i, QT)) & ~low_bits(-ks.start - k.i);
-    const int h = hk * a.G + k.g;
-    ql.load(static_cast<const T *>(a.q) + k.b * a.q_sb + h * a.q_sh + k.i * a.q_sl, next, lds + buf * 2 * TB);
-    gl.load(static_cast<const T *>(ba.g) + k.b * ba.g_sb + h * ba.g_sh + k.i * ba.g_sl, next, lds + buf * 2 * TB + TB);
-    const int64_t at = ((int64_t)k.b * a.Hk + hk) * a.rows + (int64_t)(k.i + i) * a.G + k.g;
-    if (which < 3 && ((next >> i) & 1)) x = which == 1 ? ba.delta[at] : a.stats[(which / 2) * all + at];
-    return x;
-  };
-  auto keep = [&](int buf, float x) __attribute__((always_inline)) {
-    if (threadIdx.x < 3 * QT) ((float *)stats[buf][threadIdx.x / QT])[threadIdx.x % QT] = x;
+  PastReader<DP> fr, vr;
+  fr.init(lane, lds + rg * Tile::template bytes<32>()), vr.init(lane, vt);
+  // the tile to load next: its place in its head, the head and the sample (of a prefix's group)
+  int tile = head_tiles > 0 ? t0 % head_tiles : 0, head = head_tiles > 0 ? t0 / head_tiles % a.G : 0;
+  int member = job.prefix && head_tiles > 0 ? t0 / head_tiles / a.G : 0, loaded = t0;
+  uint64_t rows[NB];  // of the tiles from the one at work on: those that are tokens
+  int place[NB];      // and the position of the first
+#pragma unroll
+  for (int i = 0; i < NB; ++i) rows[i] = 0, place[i] = 0;
+  auto stage = [&](int buf) __attribute__((always_inline)) {
+    const int b = job.prefix ? job.o * a.each + member : job.o, i = (tile0 + tile) * QT, h = hk * a.G + head;
+    uint64_t live = 0;
+    if (loaded < t1) {
+      const Sample ks = job.prefix ? uniform(sample_of(a, b)) : s;
+      live = low_bits(min(min(a.Lq, ks.n - ks.start) - i, QT)) & ~low_bits(-ks.start - i);
+      place[NB - 1] = ks.start + i;
+    }
+    rows[NB - 1] = live;
+    // behind the last tile nothing is read; every stage has the same number of loads
+    const int at = loaded < t1 ? i : 0, from_b = loaded < t1 ? b : job.prefix ? job.o * a.each : job.o;
+    ql.load(static_cast<const T *>(a.q) + from_b * a.q_sb + h * a.q_sh + at * a.q_sl, live, lds + buf * 2 * TB);
+    gl.load(static_cast<const T *>(ba.g) + from_b * ba.g_sb + h * ba.g_sh + at * ba.g_sl, live, lds + buf * 2 * TB + TB);
+    const int which = min(wave, 3);
+    const float *x = (which == 1 ? ba.delta : a.stats + (which == 2 ? all : 0)) + ((int64_t)from_b * a.Hk + hk) * a.rows + (int64_t)at * a.G + head;
+    const bool on = which < 3 && ((live >> lane) & 1);  // the others read as zero: they are masked
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(x, (int64_t)kOOB), (MLORA_LDS void *)(values + buf * ST + which * 256), 4,
+                                             on ? lane * a.G * 4 : kOOB, 0, 0, 0);
+    ++loaded;
+    if (++tile == head_tiles) {
+      tile = 0;
+      if (++head == a.G) head = 0, ++member;
+    }
   };
   auto step = [&](int buf, int p0) __attribute__((always_inline)) {  // p0: the position of the tile's first token
     if (!job.prefix && (p0 + QT <= some_a || p0 >= some_b)) return;
     // rows that are no tokens too: a key that none of the tokens sees may hold anything
-    const bool masked = rows != low_bits(QT) || (!job.prefix && (p0 < full_a || p0 + QT > full_b));
-    uint64_t mine = rows;
+    const bool masked = rows[0] != low_bits(QT) || (!job.prefix && (p0 < full_a || p0 + QT > full_b));
+    uint64_t mine = rows[0];
+    const MLORA_LDS char *val = values + buf * ST;
     if (masked && !job.prefix) mine &= low_bits(mine_b - p0) & ~low_bits(mine_a - p0);
-    mine >>= 4 * (lane >> 5);
-    static_for<QT / 32>([&](auto block) __attribute__((always_inline)) {
+    mine >>= 4 * (lane >> 5) + 32 * rg;
+    static_for<QT / 32 / RG>([&](auto block) __attribute__((always_inline)) {
       constexpr int qb = decltype(block)::value;
+      const int at = 8 * (qb + rg) + (lane >> 5);  // of the rows' x, delta and a
       __builtin_amdgcn_sched_barrier(0);  // between the phases too: interleaved, they spill
       f32x16 sc, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {  // the two sums in turn: a sum waits for its last product
-        Frag<T> qf, gf, vf;
-        fr.template rows<0, 32 * qb>(ks, qf);
-        sc = mma16(qf, k[ks], sc);
-        fr.template rows<TB, 32 * qb>(ks, gf);
-        vr.template rows<0, 0>(ks, vf);
-        dp = mma16(gf, vf, dp);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      struct Three {
+        Frag<T> q, g, v;
+      };
+      read_ahead<NS, 2>(
+          [&](auto ks) __attribute__((always_inline)) {
+            Three f;
+            fr.template rows<0, 32 * qb>(ks, f.q);
+            fr.template rows<TB, 32 * qb>(ks, f.g);
+            vr.template rows<0, 0>(ks, f.v);
+            return f;
+          },
+          [&](auto ks, const Three &f) __attribute__((always_inline)) {  // the two sums in turn: a sum waits for its last product
+            sc = mma16(f.q, k[ks], sc);
+            dp = mma16(f.g, f.v, dp);
+          });
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1083,8 +1196,8 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
       }
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 x = stats[buf][0][8 * qb + 2 * i4 + (lane >> 5)], delta = stats[buf][1][8 * qb + 2 * i4 + (lane >> 5)];
-        const f32x4 shift = stats[buf][2][8 * qb + 2 * i4 + (lane >> 5)];
+        const f32x4 x = *(const lds_f4 *)(val + 0 + 16 * (at + 2 * i4)), delta = *(const lds_f4 *)(val + 256 + 16 * (at + 2 * i4));
+        const f32x4 shift = *(const lds_f4 *)(val + 512 + 16 * (at + 2 * i4));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * i4 + j] - shift[j], a.c, -x[j]));
@@ -1092,42 +1205,43 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
           dp[4 * i4 + j] = p * (dp[4 * i4 + j] - delta[j]);
         }
       }
+      Frag<T> pf[2], df[2];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) to_frag(sc, ks, pf[ks]), to_frag(dp, ks, df[ks]);
       __builtin_amdgcn_sched_barrier(0);
-      static_for<2>([&](auto ks) __attribute__((always_inline)) {
-        Frag<T> pf;
-        to_frag(sc, ks, pf);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          Frag<T> f;
-          fr.template cols<TB, 32 * qb + 16 * decltype(ks)::value>(d, f);
-          dv[0][d] = mma16(f, pf, dv[0][d]);
-        }
-        return true;
-      });
-      static_for<2>([&](auto ks) __attribute__((always_inline)) {
-        Frag<T> df;
-        to_frag(dp, ks, df);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          Frag<T> f;
-          fr.template cols<0, 32 * qb + 16 * decltype(ks)::value>(d, f);
-          dk[0][d] = mma16(f, df, dk[0][d]);
-        }
-        return true;
-      });
+      read_ahead<4 * ND, 3>(
+          [&](auto u) __attribute__((always_inline)) {
+            constexpr int U = decltype(u)::value, VALUE = U / (2 * ND), KS = U / ND % 2;
+            Frag<T> f;
+            fr.template cols<VALUE ? 0 : TB, 32 * qb + 16 * KS>(U % ND, f);
+            return f;
+          },
+          [&](auto u, const Frag<T> &f) __attribute__((always_inline)) {
+            constexpr int U = decltype(u)::value, KS = U / ND % 2;
+            if constexpr (U / (2 * ND) == 0) dv[0][U % ND] = mma16(f, pf[KS], dv[0][U % ND]);
+            else dk[0][U % ND] = mma16(f, df[KS], dk[0][U % ND]);
+          });
       return true;
     });
   };
-  if (t0 < t1) keep(0, stage(t0, 0)), rows = next;
+  auto shift = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i + 1 < NB; ++i) rows[i] = rows[i + 1], place[i] = place[i + 1];
+  };
+  if (t0 < t1) {
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i) shift(), stage(i);
+    shift();
+  }
+  int buf = 0;
   for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    wait_vmcnt<0>();
+    wait_vmcnt<(NB - 2) * (2 * N + 1)>();
     lds_pipeline_barrier();  // tile t is in LDS, and every wave has read tile t - 1
-    const float x = stage(t + 1, buf ^ 1);
-    if (key0 < len) step(buf, s.start + tokens(t).i);
-    keep(buf ^ 1, x);
-    rows = next;
-    fr.flip(2 * TB);
+    stage(buf == 0 ? NB - 1 : buf - 1);
+    if (key0 < len) step(buf, place[0]);
+    shift();
+    fr.move(buf == NB - 1 ? -(NB - 1) * 2 * TB : 2 * TB);
+    buf = buf == NB - 1 ? 0 : buf + 1;
   }
   wait_vmcnt<0>();
   if (!live) {  // a column of keys that are none holds whatever its zeroed fragments gave
@@ -1136,14 +1250,43 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) dk[0][d][i] = 0.f, dv[0][d][i] = 0.f;
   }
+  if constexpr (RG == 2) {  // the first group has dk, the second dv
+    static_assert(KW * ND * 4 * 64 <= NB * 2 * TB / 16, "the sums fit the buffers");
+    f32x4 *to = (f32x4 *)smem + kw * (ND * 4 * 64) + lane;
+    auto hand = [&](const f32x16 (&x)[1][ND]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(d * 4 + i) * 64] = f32x4{x[0][d][4 * i], x[0][d][4 * i + 1], x[0][d][4 * i + 2], x[0][d][4 * i + 3]};
+    };
+    auto take = [&](f32x16 (&x)[1][ND]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 y = to[(d * 4 + i) * 64];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[0][d][4 * i + j] += y[j];
+        }
+    };
+    __syncthreads();
+    if (rg == 1) hand(dk);
+    __syncthreads();
+    if (rg == 0) take(dk);
+    __syncthreads();
+    if (rg == 0) hand(dv);
+    __syncthreads();
+    if (rg == 1) take(dv);
+  }
+  const bool has_dk = RG == 1 || rg == 0, has_dv = RG == 1 || rg == 1;
   if (job.splits > 1) {
-    f32x4 *p = ba.part + job.part + ((job.sp * job.items + job.item) * NW + wave) * (2 * ND * 4 * 64) + lane;
+    f32x4 *p = ba.part + job.part + ((job.sp * job.items + job.item) * KW + kw) * (2 * ND * 4 * 64) + lane;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dk[0][d][4 * i], dk[0][d][4 * i + 1], dk[0][d][4 * i + 2], dk[0][d][4 * i + 3]};
-        *(MLORA_GLOBAL f32x4 *)(p + ((ND + d) * 4 + i) * 64) = f32x4{dv[0][d][4 * i], dv[0][d][4 * i + 1], dv[0][d][4 * i + 2], dv[0][d][4 * i + 3]};
+        if (has_dk) *(MLORA_GLOBAL f32x4 *)(p + (d * 4 + i) * 64) = f32x4{dk[0][d][4 * i], dk[0][d][4 * i + 1], dk[0][d][4 * i + 2], dk[0][d][4 * i + 3]};
+        if (has_dv) *(MLORA_GLOBAL f32x4 *)(p + ((ND + d) * 4 + i) * 64) = f32x4{dv[0][d][4 * i], dv[0][d][4 * i + 1], dv[0][d][4 * i + 2], dv[0][d][4 * i + 3]};
       }
     return;
   }
@@ -1151,8 +1294,8 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
   const int64_t at = ((int64_t)job.o * L * a.Hk + hk) * a.D;
   const float fk[1] = {ba.scale}, fv[1] = {1.f};
   auto key_at = [&](int key) { return (int64_t)key * a.Hk * a.D; };
-  store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpk : ba.dk) + at, dk, fk, key0, L, key_at, a.D, lane);
-  store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpv : ba.dv) + at, dv, fv, key0, L, key_at, a.D, lane);
+  if (has_dk) store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpk : ba.dk) + at, dk, fk, key0, L, key_at, a.D, lane);
+  if (has_dv) store_rows<T, DP, 1>(static_cast<T *>(job.prefix ? ba.dpv : ba.dv) + at, dv, fv, key0, L, key_at, a.D, lane);
 }
 
 // Adds the shares of the key blocks of all classes that have several (the prefix's, those with a sink, the others) in order and
@@ -1161,10 +1304,10 @@ __global__ __launch_bounds__((64 * NW), 2) void past_dkv_kernel(const PastBwdArg
 struct JoinBlocks {
   int64_t upto[3];  // workgroups up to the end of each class
 };
-template <class T, int DP, int NW>
+template <class T, int DP, int KW>
 __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba, const JoinBlocks which) {
   const PastArgs &a = ba.f;
-  constexpr int ND = DP / 32, KEYS = sizeof(T) == 2 ? 32 * NW : kF32Keys;
+  constexpr int ND = DP / 32, KEYS = sizeof(T) == 2 ? 32 * KW : kF32Keys;
   const int64_t id = blockIdx.x;
   const int cls = id < which.upto[0] ? 0 : id < which.upto[1] ? 1 : 2;
   const bool prefix = cls == 0;
@@ -1172,7 +1315,7 @@ __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba
   const int splits = prefix ? ba.prefix_splits : cls == 1 ? ba.sink_splits : ba.own_splits;
   const f32x4 *part = ba.part + (prefix ? 0 : cls == 1 ? ba.sink_part : ba.own_part);
   const int64_t items = (int64_t)(prefix ? a.B / a.each : a.B) * a.Hk * blocks;
-  const int64_t per = items * (sizeof(T) == 2 ? NW * 2 * ND * 4 * 64 : KEYS * (a.D / 2));
+  const int64_t per = items * (sizeof(T) == 2 ? KW * 2 * ND * 4 * 64 : KEYS * (a.D / 2));
   const int64_t e = (id - (cls == 0 ? 0 : which.upto[cls - 1])) * 256 + threadIdx.x;
   if (e >= per) return;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -1184,7 +1327,7 @@ __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba
     u = e / 64;
     const int lane = (int)(e % 64), i = (int)(u % 4), d = (int)(u / 4 % ND);
     value = (int)(u / 4 / ND % 2), u /= 4 * ND * 2;
-    in = (int)(u % NW) * 32 + (lane & 31), ch = 32 * d + 8 * i + 4 * (lane >> 5), u /= NW;
+    in = (int)(u % KW) * 32 + (lane & 31), ch = 32 * d + 8 * i + 4 * (lane >> 5), u /= KW;
   } else {
     u = e / (a.D / 4), ch = (int)(e % (a.D / 4)) * 4;
     value = (int)(u % 2), u /= 2, in = (int)(u % KEYS), u /= KEYS;
@@ -1445,13 +1588,13 @@ __global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float
   template __global__ void past_dq_kernel<DP>(const PastBwdArgs);                  \
   template __global__ void past_dq_f32_kernel<DP, false>(const PastBwdArgs);       \
   template __global__ void past_dq_f32_kernel<DP, true>(const PastBwdArgs);        \
-  template __global__ void past_dkv_kernel<DP, 4>(const PastBwdArgs);              \
+template __global__ void past_dkv_kernel<DP, 4, DP / 64>(const PastBwdArgs);      \
   template __global__ void past_dkv_f32_kernel<DP, false>(const PastBwdArgs);      \
   template __global__ void past_dkv_f32_kernel<DP, true>(const PastBwdArgs);
 MLORA_PAST(64)
 MLORA_PAST(128)
 #undef MLORA_PAST
-template __global__ void past_dkv_kernel<128, 8>(const PastBwdArgs);
+template __global__ void past_dkv_kernel<128, 8, 1>(const PastBwdArgs);
 
 // ------------------------------------------------------------------ host
 
@@ -1558,11 +1701,12 @@ static int past_join_limit(const PastPlan &p, const PastSizes &z) {
 }
 
 struct PastBwdPlan {
-  int nw;  // waves of dk / dv, 32 keys each
+  int kw;       // waves of dk / dv over different keys, 32 each
   int64_t row_tiles, splits;
   int64_t key_blocks, prefix_blocks, sink_blocks, prefix_splits, sink_splits, own_splits;
   int64_t prefix_vectors, sink_vectors, own_vectors;  // 16-byte vectors of all shares of a class, 0 where it has one
   int64_t dq_vectors;                                 // of one share of dq
+  double cost;  // of dk / dv, to choose by
 };
 
 static PastBwdPlan past_bwd_plan(const PastSizes &z) {
@@ -1573,29 +1717,44 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, row_tile, kt) + ceil_div(z.Lp, kt);
   p.splits = items <= 0 ? 1 : !z.f32 ? wide_shares(items, tiles, 128 * dp, 8e6) : between(256 / items, 1, between(tiles / 8, 1, 64));
   p.dq_vectors = z.f32 ? z.B * z.Hk * z.rows * (z.D / 4) : items * 4 * (dp / 32) * 4 * 64;
-  const int64_t longest = z.Lk > z.Lp ? z.Lk : z.Lp;
-  p.nw = !z.f32 && z.D > 64 && longest > 128 ? 8 : 4;
-  const int64_t qt = z.f32 || (z.D > 64 && p.nw == 4) ? 32 : 64, keys = z.f32 ? kF32Keys : 32 * p.nw;
-  p.key_blocks = ceil_div(z.Lk, keys), p.prefix_blocks = ceil_div(z.Lp, keys);
   const bool bounded = z.window < z.Lk;
-  p.sink_blocks = bounded ? between(ceil_div(z.sinks, keys), 0, p.key_blocks) : 0;  // without a window all blocks are alike
-  const int64_t head_tiles = ceil_div(z.Lq, qt), seen = z.window + z.chunk + keys;
-  const int64_t prefix_work = z.each * z.G * head_tiles, sink_work = z.G * head_tiles;
-  const int64_t own_work = z.G * (bounded && seen < z.Lq ? ceil_div(seen, qt) + 1 : head_tiles);
-  const int64_t prefix_items = z.groups * z.Hk * p.prefix_blocks, sink_items = z.B * z.Hk * p.sink_blocks,
-                own_items = z.B * z.Hk * (p.key_blocks - p.sink_blocks);
-  const int64_t total = prefix_items * prefix_work + sink_items * sink_work + own_items * own_work;
-  const int64_t slots = p.nw == 8 ? 256 : 1024;
-  int64_t target = ceil_div(total, slots);
-  const int64_t least = z.f32 ? 8 : 4;
-  if (target < least) target = least;
-  auto cut = [&](int64_t work, int64_t n) { return n > 0 ? between(work / target, 1, 64) : 1; };
-  p.prefix_splits = cut(prefix_work, prefix_items), p.sink_splits = cut(sink_work, sink_items), p.own_splits = cut(own_work, own_items);
-  const int64_t per = z.f32 ? keys * (z.D / 2) : p.nw * 2 * (dp / 32) * 4 * 64;
-  p.prefix_vectors = p.prefix_splits > 1 ? prefix_items * p.prefix_splits * per : 0;
-  p.sink_vectors = p.sink_splits > 1 ? sink_items * p.sink_splits * per : 0;
-  p.own_vectors = p.own_splits > 1 ? own_items * p.own_splits * per : 0;
-  return p;
+  auto plan = [&](int kw) {
+    PastBwdPlan c = p;
+    c.kw = kw;
+    const int64_t qt = z.f32 ? 32 : 64, keys = z.f32 ? kF32Keys : 32 * kw;
+    c.key_blocks = ceil_div(z.Lk, keys), c.prefix_blocks = ceil_div(z.Lp, keys);
+    c.sink_blocks = bounded ? between(ceil_div(z.sinks, keys), 0, c.key_blocks) : 0;  // without a window all blocks are alike
+    const int64_t head_tiles = ceil_div(z.Lq, qt), seen = z.window + z.chunk + keys;
+    const int64_t work[3] = {z.each * z.G * head_tiles, z.G * head_tiles, z.G * (bounded && seen < z.Lq ? ceil_div(seen, qt) + 1 : head_tiles)};
+    const int64_t items[3] = {z.groups * z.Hk * c.prefix_blocks, z.B * z.Hk * c.sink_blocks, z.B * z.Hk * (c.key_blocks - c.sink_blocks)};
+    const int64_t total = items[0] * work[0] + items[1] * work[1] + items[2] * work[2];
+    const int64_t slots = z.f32 ? 1024 : z.D > 64 ? 256 : 512, least = z.f32 ? 8 : 4;
+    const int64_t target = std::max(ceil_div(total, slots), least);
+    int64_t splits[3], blocks = 0, longest = 0;
+    for (int i = 0; i < 3; ++i) {
+      splits[i] = items[i] > 0 ? between(work[i] / target, 1, 64) : 1;
+      blocks += items[i] * splits[i];
+      if (items[i] > 0) longest = std::max(longest, ceil_div(work[i], splits[i]));
+    }
+    c.prefix_splits = splits[0], c.sink_splits = splits[1], c.own_splits = splits[2];
+    const int64_t per = z.f32 ? keys * (z.D / 2) : kw * 2 * (dp / 32) * 4 * 64;
+    c.prefix_vectors = splits[0] > 1 ? items[0] * splits[0] * per : 0;
+    c.sink_vectors = splits[1] > 1 ? items[1] * splits[1] * per : 0;
+    c.own_vectors = splits[2] > 1 ? items[2] * splits[2] * per : 0;
+    // in tiles of 256 keys by 64 rows, 2.4 us each: as long as the longest share, or full rounds of 256 workgroups and half of it; three
+    // tiles for a workgroup's start and end, the shares' sums at 6 TB/s. Of whole sequences the later keys are seen by fewer tokens.
+    const double shares = (double)(c.prefix_vectors + c.sink_vectors + c.own_vectors) * 32 / 6e6 / 2.4;
+    const double part = z.Lq == z.Lk && z.Lk > 0 ? 1.0 - 0.5 * (double)std::max<int64_t>(std::min(seen, z.Lk) - z.chunk, 0) / (double)z.Lk : 1.0;
+    const double all = (double)(items[0] * work[0] + items[1] * work[1]) + part * (double)(items[2] * work[2]) + 3.0 * (double)blocks;
+    c.cost = (blocks <= slots ? (double)longest + 3.0 : std::max((double)longest + 3.0, all / (double)slots + 0.5 * (double)longest)) *
+                 (kw == 8 ? 1.0 : 0.66) + shares + (shares > 0 ? 2.0 : 0.0);
+    return c;
+  };
+  if (z.f32 || z.D <= 64) return plan(4);
+  // 256 keys per workgroup, or 128 whose tiles take 0.66 of the time (a barrier per 32 rows of a wave): 32760 keys, 12 heads, in one 4.7 ms,
+  // in the other 5.4; 4096 keys without a window, 12 heads, 240 us and 165
+  const PastBwdPlan wide = plan(8), narrow = plan(4);
+  return wide.cost <= narrow.cost ? wide : narrow;
 }
 
 // The rows' deltas, then the shares of dq, and after they are joined those of dk and dv in the same place.
@@ -1787,15 +1946,15 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
   with_head(z.f32, z.D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
-    auto go = [&](auto nw) {
-      constexpr int NW = decltype(nw)::value;
-      if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((past_dkv_kernel<DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, ba);
+    auto go = [&](auto kw) {
+      constexpr int KW = decltype(kw)::value, RG = KW == 4 ? DP / 64 : 1;
+      if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((past_dkv_kernel<DP, KW, RG>), dim3((unsigned)blocks), dim3(64 * KW * RG), 0, s, ba);
       else if (blocks > kFewMany) hipLaunchKernelGGL((past_dkv_f32_kernel<DP, true>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, true>), 0, s, ba);
       else hipLaunchKernelGGL((past_dkv_f32_kernel<DP, false>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, false>), 0, s, ba);
-      if (join_blocks > 0) hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, NW>), dim3((unsigned)join_blocks), dim3(256), 0, s, ba, joins);
+      if (join_blocks > 0) hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, KW>), dim3((unsigned)join_blocks), dim3(256), 0, s, ba, joins);
     };
     if constexpr (sizeof(T) == 2 && DP == 128) {
-      if (p.nw == 8) return go(std::integral_constant<int, 8>{});
+      if (p.kw == 8) return go(std::integral_constant<int, 8>{});
     }
     go(std::integral_constant<int, 4>{});
   });
