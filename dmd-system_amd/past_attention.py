@@ -86,7 +86,11 @@ class PastAttentionFunction(torch.autograd.Function):
 
 
 def _meta(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.dtype, t.device, t.stride())
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        _fail(f"q, k, v, prefixes and lengths must be a tensor each, got a {type(t).__name__}")
+    return t.shape, t.dtype, t.device, t.stride()
 
 
 def _check_vector(name: str, meta, n: int, device) -> None:

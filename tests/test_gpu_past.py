@@ -330,3 +330,97 @@ def test_offsets_past_32_bits(pkg, dev):
     whole = base.view(1, 2 * Lk, 2, H, D)  # token offsets of 4.5e9 elements
     got = run(pkg, [tail[0], whole[:, :, 0], whole[:, :, 1]], window=500)
     ref.check(got, *tail, window=500)
+
+
+def some_heads(pkg, tensors, g, heads, **kw):
+    """As `both`, for many heads (each with its own key head): those of `heads` against the definition."""
+    got = run(pkg, tensors, g, **kw)
+    ref.check({n: t[:, :, heads].contiguous() for n, t in got.items()}, *[t[:, :, heads] for t in tensors], do=g[:, :, heads], **kw)
+    return got
+
+
+MANY_BLOCKS = [  # groups, each, L, Lp, H, D, options: more blocks of 256 keys than compute units
+    (0, 1, 1100, 0, 64, 128, dict(window=600, sinks=300, chunk=275)),   # sinks in blocks of their own
+    (0, 1, 520, 0, 256, 72, dict(chunk=520)),
+    (2, 3, 200, 900, 64, 128, dict(window=100)),                        # a prefix that three samples add to
+    (0, 2, 1024, 0, 48, 64, dict(window=130, sinks=5)),
+]
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", MANY_BLOCKS, ids=str)
+def test_many_blocks(pkg, dev, case, ragged):
+    groups, each, L, Lp, H, D, kw = case
+    B = max(groups, 1) * each
+    tensors, g = make(BF, dev, L, B, L, L, H, H, D, groups, Lp)
+    gen = torch.Generator().manual_seed(H)
+    lengths = torch.randint(0, L + 1, (B,), generator=gen) if ragged else None
+    plens = i32(Lp, Lp // 3) if ragged and groups else None
+    more = dict(kw, plens=plens) if groups else kw
+    some_heads(pkg, tensors, g, [0, H // 2, H - 1], lengths=lengths, **more)
+
+
+SHARED_OUT = [  # dtype, B, Lq, Lk, H, Hk, D, groups, Lp, options: few rows or heads, so that keys and rows are shared out and joined
+    (BF, 1, 2600, 2600, 2, 1, 128, 0, 0, dict(chunk=100)),
+    (BF, 3, 700, 700, 4, 2, 128, 1, 900, dict()),
+    (BF, 1, 1300, 1300, 4, 2, 96, 0, 0, dict(window=300, sinks=200, chunk=7)),
+    (BF, 2, 600, 2000, 2, 2, 64, 0, 0, dict()),
+    (F, 1, 40, 3000, 2, 1, 128, 1, 2000, dict()),
+    (F, 1, 700, 700, 3, 1, 128, 0, 0, dict(window=90, sinks=130)),
+    (F, 2, 260, 1100, 2, 2, 64, 0, 0, dict(chunk=260)),
+]
+
+
+@pytest.mark.parametrize("case", SHARED_OUT, ids=str)
+def test_shared_out(pkg, dev, case):
+    dtype, B, Lq, Lk, H, Hk, D, groups, Lp, kw = case
+    tensors, g = make(dtype, dev, Lq + Lp, B, Lq, Lk, H, Hk, D, groups, Lp)
+    got = both(pkg, tensors, g, **kw)
+    again = run(pkg, tensors, g, **kw)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_float32_with_many_workgroups(pkg, dev, D):
+    """More workgroups of 32 rows than compute units, whose waves are halved."""
+    tensors, g = make(F, dev, D, 2, 420, 420, 24, 24, D)
+    some_heads(pkg, tensors, g, [0, 11, 23], window=77, sinks=40, lengths=i32(420, 333))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_backward_of_gradients_in_any_layout(pkg, dev, dtype):
+    """An upstream gradient that is expanded, strided by token, misaligned or of another type."""
+    tensors, _ = make(dtype, dev, 41, 2, 70, 70, 4, 2, 64)
+    gen = torch.Generator().manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev).to(dtype)  # noqa: E731
+    for g in (r(1, 1, 1, 64).expand(2, 70, 4, 64), r(2, 70, 3, 4, 64)[:, :, 1], r(2 * 70 * 4 * 64 + 1)[1:].view(2, 70, 4, 64)):
+        got = run(pkg, tensors, g, window=9)
+        same = run(pkg, tensors, g.contiguous().clone(), window=9)
+        ref.check(got, *tensors, do=g, window=9)
+        assert all(torch.equal(got[n], same[n]) for n in got)
+
+
+def test_calls_that_follow_each_other(pkg, dev):
+    """A streaming sampler and its training pass as they are used together: chunks generated one after the other against a growing
+    cache give what the whole sequence gives in one pass, forward, and the gradients of that pass are the definition's."""
+    C, n, H, D = 40, 6, 4, 64
+    (q, k, v), g = make(BF, dev, 51, 2, C * n, C * n, H, H, D)
+    kw = dict(window=2 * C, sinks=C, chunk=C)
+    whole = both(pkg, [q, k, v], g, **kw)["out"]
+    cache_k, cache_v = torch.full_like(k, math.nan), torch.full_like(v, math.nan)
+    u = ref.half_step(BF)
+    with torch.no_grad():
+        for i in range(n):
+            at = slice(i * C, (i + 1) * C)
+            cache_k[:, at], cache_v[:, at] = k[:, at], v[:, at]
+            filled = torch.full((2,), (i + 1) * C, dtype=torch.int32, device=dev)
+            step = pkg.window_attention(q[:, at], cache_k, cache_v, key_lengths=filled, **kw)
+            # each within u |out| + 1.3 u (sum p |v| + |out|) of the exact value (past_reference.check), u for the rounding of out and
+            # of the weights, 0.3 u for the scores' and sums'; sum p |v| <= max |v|
+            room = 6 * u * whole[:, at].float().abs() + 3 * u * v.float().abs().max()
+            assert ((step.float() - whole[:, at].float()).abs() <= room).all()
+        # both samples' third chunk as continuations of the first one's past
+        past = k[:1, :2 * C], v[:1, :2 * C]
+        own = slice(2 * C, 3 * C)
+        shared = pkg.prefix_attention(q[:, own], k[:, own], v[:, own], past[0][0], past[1][0], chunk=C)
+    ref.check({"out": shared}, q[:, own], k[:, own], v[:, own], *past, chunk=C)

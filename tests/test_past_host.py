@@ -1,0 +1,189 @@
+"""What window_attention and prefix_attention refuse, and their C entries' checks before any launch (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+BF, F = torch.bfloat16, torch.float32
+
+
+def heads(B=2, L=5, H=4, D=64, dtype=F):
+    return torch.zeros(B, L, H, D, dtype=dtype)
+
+
+def test_window_refusals(pkg):
+    q, k = heads(), heads(L=7, H=2)
+
+    def bad(match, q=q, k=k, v=None, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            pkg.window_attention(q, k, k if v is None else v, **kw)
+
+    bad("batch, tokens", q=q[0])
+    bad("batch, tokens", k=k[0])
+    bad("bfloat16 or float32", q=q.half())
+    bad("one dtype", k=k.to(BF))
+    bad("k and v must be", v=k[:, :6])
+    bad("k and v must be", k=k[:1])
+    bad("k and v must be", k=heads(L=7, H=2, D=32))
+    bad("share", k=heads(L=7, H=3))
+    bad("share", k=heads(L=7, H=0))
+    bad("share", q=heads(H=0), k=heads(L=7, H=0))
+    bad("multiple of 8", q=heads(D=60), k=heads(L=7, H=2, D=60))
+    bad("multiple of 8", q=heads(D=136), k=heads(L=7, H=2, D=136))
+    bad("chunk", chunk=0)
+    bad("window", window=0)
+    bad("window", window=3, chunk=4)
+    bad("sinks", sinks=-1)
+    for name in ("window", "sinks", "chunk", "query_start"):
+        bad(name, **{name: 2.5})
+        bad(name, **{name: "many"})
+        bad(name, **{name: float("nan")})
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        bad("scale", scale=scale)
+    bad("no gradient", scale=torch.tensor(0.5, requires_grad=True))
+    bad("give query_start", q=heads(L=9))
+    for name in ("key_lengths", "query_start"):
+        bad(name, **{name: torch.zeros(2)})
+        bad(name, **{name: torch.zeros(3, dtype=torch.int32)})
+        bad(name, **{name: torch.zeros(2, 1, dtype=torch.int32)})
+    bad("must be a tensor", key_lengths=[5, 5])
+    bad("must be a tensor", v=[1.0])
+    bad("at most", q=heads(B=1, L=1), k=torch.zeros(1, 1, 2, 64).expand(1, (1 << 28) + 1, 2, 64))
+    bad("ROCm device", window=2, sinks=3, chunk=2, key_lengths=torch.zeros(2, dtype=torch.int64), query_start=-1)
+
+
+def test_prefix_refusals(pkg):
+    q, k, p = heads(B=4), heads(B=4, L=7, H=2), heads(L=9, H=2)
+
+    def bad(match, pk=p, pv=None, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            pkg.prefix_attention(q, k, k, pk, pk if pv is None else pv, **kw)
+
+    bad("share 3 prefixes", pk=heads(B=3, L=9, H=2))
+    bad("share 0 prefixes", pk=heads(B=0, L=9, H=2))
+    bad("prefix_k and prefix_v must be", pv=p[:, :8])
+    bad("prefix_k and prefix_v must be", pv=p[0])
+    bad("prefix_k and prefix_v must be", pk=heads(L=9, H=4))
+    bad("prefix_k and prefix_v must be", pk=heads(L=9, H=2, D=32))
+    bad("prefix_k and prefix_v must be", pk=p[0, 0], pv=p[0, 0])
+    bad("dtype and device", pk=p.to(BF))
+    bad("dtype and device", pv=p.to(BF))
+    bad("prefix_lengths", prefix_lengths=torch.zeros(4, dtype=torch.int32))
+    bad("prefix_lengths", prefix_lengths=torch.zeros(2))
+    bad("ROCm device", prefix_lengths=torch.zeros(2, dtype=torch.int64), window=3)
+    bad("ROCm device", pk=p[0])
+
+
+def test_forward_mode_is_refused(pkg, monkeypatch):
+    """A tangent is never dropped without a word; without one the same call reaches the kernel."""
+    from torch.autograd import forward_ad
+
+    reached = []
+    monkeypatch.setattr(pkg.past_attention, "_plan", lambda *a: (None, a[1:]))
+    monkeypatch.setattr(pkg.past_attention, "_lay_out", lambda call, tensors: (None, tensors, []))
+    monkeypatch.setattr(pkg.kernels, "past_attention", lambda *a: (reached.append(a), (None, None))[1])
+    q = heads()
+    for at in range(3):
+        with forward_ad.dual_level(), torch.no_grad():
+            tensors = [forward_ad.make_dual(q, torch.ones_like(q)) if i == at else q for i in range(3)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                pkg.window_attention(*tensors)
+    pkg.window_attention(q, q, q)
+    assert len(reached) == 1
+
+
+def shape(L, **kw):
+    d = dict(dtype=L.BF16, from_end=0, B=2, Lq=5, Lk=7, H=4, Hk=4, D=64, groups=0, Lp=0, window=0, sinks=0, chunk=1, first=2,
+             q=(1280, 256, 64), k=(1792, 256, 64), v=(1792, 256, 64), pk=(0, 0, 0), pv=(0, 0, 0), scale=0.125)
+    d.update(kw)
+    strides = [(ctypes.c_int64 * 3)(*d.pop(n)) for n in ("q", "k", "v", "pk", "pv")]
+    scale = d.pop("scale")
+    return ctypes.byref(L.PastShape(*d.values(), *strides, scale))
+
+
+BAD_SHAPES = [
+    (dict(dtype=2), "ERR_UNSUPPORTED"), (dict(B=-1), "ERR_INVALID"), (dict(Lq=-1), "ERR_INVALID"), (dict(Lk=-1), "ERR_INVALID"),
+    (dict(H=0), "ERR_INVALID"), (dict(Hk=0), "ERR_INVALID"), (dict(Hk=3), "ERR_INVALID"), (dict(D=60), "ERR_UNSUPPORTED"),
+    (dict(D=0), "ERR_UNSUPPORTED"), (dict(D=136), "ERR_UNSUPPORTED"), (dict(window=-1), "ERR_INVALID"), (dict(sinks=-1), "ERR_INVALID"),
+    (dict(chunk=0), "ERR_INVALID"), (dict(window=3, chunk=4), "ERR_INVALID"), (dict(groups=-1), "ERR_INVALID"),
+    (dict(groups=3), "ERR_INVALID"), (dict(Lp=4), "ERR_INVALID"), (dict(groups=1, Lp=-1), "ERR_INVALID"), (dict(scale=0.0), "ERR_INVALID"),
+    (dict(scale=float("inf")), "ERR_INVALID"), (dict(scale=3e38), "ERR_INVALID"), (dict(Lk=(1 << 28) + 1), "ERR_LIMIT"),
+    (dict(Lq=(1 << 28) + 1), "ERR_LIMIT"), (dict(groups=1, Lp=(1 << 28) + 1), "ERR_LIMIT"), (dict(H=1 << 17), "ERR_LIMIT"),
+    (dict(Lq=1 << 28, H=16, Hk=1), "ERR_LIMIT"), (dict(B=1 << 24, Lk=1 << 20), "ERR_LIMIT"), (dict(B=1 << 40), "ERR_LIMIT"),
+]
+
+
+@pytest.mark.parametrize("case", BAD_SHAPES, ids=str)
+def test_entries_refuse_sizes(pkg, case):
+    L, lib = pkg._lib, pkg._lib.load()
+    kw, code = case
+    s, code = shape(L, **kw), getattr(L, code)
+    assert lib.mlora_past_attention_workspace_bytes(s) == code and lib.mlora_past_attention_backward_workspace_bytes(s) == code
+    ptr = [0x1000] * 5
+    assert lib.mlora_past_attention(s, *ptr, None, None, None, 0x2000, 0x3000, 0x4000, 0x5000, 1 << 40, None) == code
+    assert lib.mlora_past_attention_backward(s, *ptr, None, None, None, 0x2000, 0x3000, 0x4000, 0x6000,
+                                             (ctypes.c_int64 * 3)(1280, 256, 64), *[0x7000] * 5, 0x5000, 1 << 40, None) == code
+
+
+def test_entries_validate_before_launch(pkg):
+    L, lib = pkg._lib, pkg._lib.load()
+
+    def fwd(q=0x1000, k=0x2000, v=0x3000, pk=None, pv=None, out=0x4000, rest=0x5000, stats=0x6000, work=0x7000, nbytes=1 << 40, **kw):
+        return lib.mlora_past_attention(shape(L, **kw), q, k, v, pk, pv, None, None, None, out, rest, stats, work, nbytes, None)
+
+    assert lib.mlora_past_attention_workspace_bytes(None) == L.ERR_INVALID
+    assert fwd(B=0) == L.OK and fwd(Lq=0, q=None, out=None, rest=None, stats=None) == L.OK
+    group = dict(groups=1, Lp=4, pk=0x8000, pv=0x9000)
+    for kw, code in ((dict(q=None), L.ERR_INVALID), (dict(q=0x1008), L.ERR_UNSUPPORTED), (dict(k=None), L.ERR_INVALID),
+                     (dict(v=0x3004), L.ERR_UNSUPPORTED), (dict(out=None), L.ERR_INVALID), (dict(out=0x4008), L.ERR_UNSUPPORTED),
+                     (dict(rest=None), L.ERR_INVALID), (dict(rest=0x5002), L.ERR_UNSUPPORTED), (dict(stats=0x6002), L.ERR_UNSUPPORTED),
+                     (dict(group, pk=None), L.ERR_INVALID), (dict(group, pv=0x9008), L.ERR_UNSUPPORTED)):
+        kw = dict(kw)
+        pk, pv = kw.pop("pk", None), kw.pop("pv", None)
+        strides = {}
+        if "groups" in kw:
+            strides = dict(groups=kw.pop("groups"), Lp=kw.pop("Lp"))
+            s = shape(L, **strides, pk=(1024, 256, 64), pv=(1024, 256, 64))
+            assert lib.mlora_past_attention(s, 0x1000, 0x2000, 0x3000, pk, pv, None, None, None, 0x4000, 0x5000, 0x6000, 0x7000, 1 << 40,
+                                            None) == code, kw
+        else:
+            assert fwd(**kw) == code, kw
+    for name, index in (("q", 0), ("k", 0), ("v", 0)):
+        for strides, code in (((1280, 252, 64), L.ERR_UNSUPPORTED), ((1280, -256, 64), L.ERR_UNSUPPORTED), ((1280, 256, 60), L.ERR_UNSUPPORTED),
+                              ((1284, 256, 64), L.ERR_UNSUPPORTED), ((1280, 1 << 22, 64), L.ERR_LIMIT)):
+            s = shape(L, **{name: strides})
+            assert lib.mlora_past_attention(s, 0x1000, 0x2000, 0x3000, None, None, None, None, None, 0x4000, 0x5000, 0x6000, 0x7000, 1 << 40,
+                                            None) == code, (name, strides)
+
+
+def test_workspaces(pkg):
+    """Shares of the keys need a workspace, the backward its deltas; one byte less is refused."""
+    L, lib = pkg._lib, pkg._lib.load()
+    token = dict(B=1, Lq=1, Lk=4096, first=4095)
+    need = lib.mlora_past_attention_workspace_bytes(shape(L, **token))
+    assert need > 0 and need % ((64 + 2) * 4 * 4) == 0
+    assert lib.mlora_past_attention_workspace_bytes(shape(L, B=1, Lq=4096, Lk=64)) == 0
+    for empty in (dict(B=0), dict(Lq=0), dict(Lk=0), dict(B=0, Lq=0, Lk=0), dict(Lq=0, groups=1, Lp=1 << 20, Lk=1 << 20)):
+        assert lib.mlora_past_attention_workspace_bytes(shape(L, **empty)) >= 0
+        assert lib.mlora_past_attention_backward_workspace_bytes(shape(L, **empty)) >= 0
+
+    def fwd(work=0x7000, nbytes=need):
+        return lib.mlora_past_attention(shape(L, **token), 0x1000, 0x2000, 0x3000, None, None, None, None, None, 0x4000, None, None, work,
+                                        nbytes, None)
+
+    assert fwd(nbytes=need - 1) == L.ERR_WORKSPACE and fwd(work=None) == L.ERR_WORKSPACE and fwd(work=0x7008) == L.ERR_UNSUPPORTED
+    # windows, sinks and chunks of any size mean what they mean at the number of keys
+    for kw in (dict(window=1 << 62), dict(sinks=1 << 62), dict(window=1 << 62, chunk=1 << 62)):
+        assert lib.mlora_past_attention_workspace_bytes(shape(L, **token, **kw)) == need
+    back = lib.mlora_past_attention_backward_workspace_bytes(shape(L))
+    assert back >= 2 * 4 * 5 * 4
+
+    def bwd(g=0x8000, gs=(1280, 256, 64), out=0x4000, rest=0x5000, stats=0x6000, dq=0x9000, dk=0xa000, dv=0xb000, work=0x7000, nbytes=back):
+        return lib.mlora_past_attention_backward(shape(L), 0x1000, 0x2000, 0x3000, None, None, None, None, None, out, rest, stats, g,
+                                                 gs if gs is None else (ctypes.c_int64 * 3)(*gs), dq, dk, dv, None, None, work, nbytes, None)
+
+    for kw, code in ((dict(g=None), L.ERR_INVALID), (dict(gs=None), L.ERR_INVALID), (dict(gs=(1280, 252, 64)), L.ERR_UNSUPPORTED),
+                     (dict(out=None), L.ERR_INVALID), (dict(rest=None), L.ERR_INVALID), (dict(stats=None), L.ERR_INVALID),
+                     (dict(dq=None), L.ERR_INVALID), (dict(dk=None), L.ERR_INVALID), (dict(dv=0xb008), L.ERR_UNSUPPORTED),
+                     (dict(work=None), L.ERR_WORKSPACE), (dict(nbytes=back - 1), L.ERR_WORKSPACE), (dict(work=0x7004), L.ERR_UNSUPPORTED)):
+        assert bwd(**kw) == code, kw
