@@ -652,16 +652,14 @@ __device__ __forceinline__ void load_row(const T *p, bool on, int D, int lane, F
 // products and the join where they are short (32 keys 5.4 us, 260 keys of 64 channels 6.1). On 32 x 32 products, four waves with two
 // buffers each: 51, 7.7 and 8.3.
 // float32 takes any number of rows this way (waves of 32 rows that share tiles behind a barrier: 1573 tokens, window 257, 12 heads of
-// 64: 46 us, here 37; 524 rows on 646 keys 32 and 21): the matrix core takes 2048 cycles for 32 rows by 32 keys by 64 channels, so
-// that reading the tiles again costs less than waiting. Half the waves where there is more than a workgroup per
-// compute unit, so that two share one (8 heads, 4096 tokens, window 1024, 64 channels: 102 -> 89 us; 352 workgroups of 700 tokens
-// 22 -> 27).
-template <class T, int DP, bool MANY>
-constexpr int kFewWaves = (sizeof(T) * DP == 512 ? 4 : 8) / (MANY ? 2 : 1);
+// 64: 46 us, here 30; 524 rows on 646 keys 32 and 21): the matrix core takes 2048 cycles for 32 rows by 32 keys by 64 channels, so
+// that reading the tiles again costs less than waiting. f32_waves chooses between NW and half or a quarter of it.
+template <class T, int DP>
+constexpr int kFewWaves = sizeof(T) * DP == 512 ? 4 : 8;
 
-template <class T, int DP, int NC, bool MANY>
-__global__ __launch_bounds__((64 * kFewWaves<T, DP, MANY>), (kFewWaves<T, DP, false> / 4)) void past_few_kernel(const PastArgs a) {
-  constexpr int KT = 32, NW = kFewWaves<T, DP, MANY>, ND = DP / 16;
+template <class T, int DP, int NC, int NW>
+__global__ __launch_bounds__((64 * NW), (kFewWaves<T, DP> / 4)) void past_few_kernel(const PastArgs a) {
+  constexpr int KT = 32, ND = DP / 16;
   using Tile = HeadTile<T, DP>;
   constexpr int TB = KT * Tile::RB, N = TB / 1024;
   static_assert(NC * ND * 64 * 16 <= 2 * TB, "a wave's sums fit its buffers");
@@ -1347,11 +1345,11 @@ __global__ __launch_bounds__(256) void past_dkv_join_kernel(const PastBwdArgs ba
 // As the forward of few rows: 32 rows (or keys) per workgroup, the waves take different tiles and their sums are joined through LDS.
 // A product of 32 x 32 x 64 channels holds the matrix core for 2048 cycles, so that reading the tiles again for every 32 rows
 // costs less than it would in bf16.
-template <int DP, bool MANY>
-__global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float, DP, false> / 4)) void past_dq_f32_kernel(const PastBwdArgs ba) {
+template <int DP, int NW>
+__global__ __launch_bounds__((64 * NW), (kFewWaves<float, DP> / 4)) void past_dq_f32_kernel(const PastBwdArgs ba) {
   const PastArgs &a = ba.f;
   using Tile = HeadTile<float, DP>;
-  constexpr int KT = 32, NW = kFewWaves<float, DP, MANY>, ND = DP / 16, NS = DP / 32, TB = KT * Tile::RB;
+  constexpr int KT = 32, ND = DP / 16, NS = DP / 32, TB = KT * Tile::RB;
   static_assert(2 * ND * 64 * 16 <= 2 * TB, "a wave's sums fit its buffer");
   __shared__ u32x4 smem[2 * TB * NW / 16];
   const int wave = wave_id(), lane = threadIdx.x & 63;
@@ -1440,11 +1438,11 @@ __global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float
   }
 }
 
-template <int DP, bool MANY>
-__global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float, DP, false> / 4)) void past_dkv_f32_kernel(const PastBwdArgs ba) {
+template <int DP, int NW>
+__global__ __launch_bounds__((64 * NW), (kFewWaves<float, DP> / 4)) void past_dkv_f32_kernel(const PastBwdArgs ba) {
   const PastArgs &a = ba.f;
   using Tile = HeadTile<float, DP>;
-  constexpr int QT = 32, NW = kFewWaves<float, DP, MANY>, ND = DP / 16, NS = DP / 32, TB = QT * Tile::RB, N = TB / 1024;
+  constexpr int QT = 32, ND = DP / 16, NS = DP / 32, TB = QT * Tile::RB, N = TB / 1024;
   static_assert(2 * ND * 64 * 16 <= 2 * TB, "half of a wave's sums fit its buffer");
   __shared__ u32x4 smem[2 * TB * NW / 16 + NW * 24];  // q and the output's gradient of every wave; x, delta and a of its rows
   const int wave = wave_id(), lane = threadIdx.x & 63;
@@ -1578,28 +1576,34 @@ __global__ __launch_bounds__((64 * kFewWaves<float, DP, MANY>), (kFewWaves<float
 
 // The kernels are named here because hipcc's host pass does not instantiate a kernel that holds generic lambdas
 // from a launch inside one.
-#define MLORA_PAST(DP)                                                             \
-  template __global__ void past_fwd_kernel<DP>(const PastArgs);                    \
-  template __global__ void past_few_kernel<uint16_t, DP, 1, false>(const PastArgs); \
-  template __global__ void past_few_kernel<uint16_t, DP, 2, false>(const PastArgs); \
-  template __global__ void past_few_kernel<float, DP, 1, false>(const PastArgs);   \
-  template __global__ void past_few_kernel<float, DP, 2, false>(const PastArgs);   \
-  template __global__ void past_few_kernel<float, DP, 2, true>(const PastArgs);    \
-  template __global__ void past_dq_kernel<DP>(const PastBwdArgs);                  \
-  template __global__ void past_dq_f32_kernel<DP, false>(const PastBwdArgs);       \
-  template __global__ void past_dq_f32_kernel<DP, true>(const PastBwdArgs);        \
-template __global__ void past_dkv_kernel<DP, 4, DP / 64>(const PastBwdArgs);      \
-  template __global__ void past_dkv_f32_kernel<DP, false>(const PastBwdArgs);      \
-  template __global__ void past_dkv_f32_kernel<DP, true>(const PastBwdArgs);
+#define MLORA_PAST(DP)                                                                           \
+  template __global__ void past_fwd_kernel<DP>(const PastArgs);                                  \
+  template __global__ void past_few_kernel<uint16_t, DP, 1, 8>(const PastArgs);                  \
+  template __global__ void past_few_kernel<uint16_t, DP, 2, 8>(const PastArgs);                  \
+  template __global__ void past_few_kernel<float, DP, 1, kFewWaves<float, DP>>(const PastArgs); \
+  template __global__ void past_dq_kernel<DP>(const PastBwdArgs);                                \
+  template __global__ void past_dkv_kernel<DP, 4, DP / 64>(const PastBwdArgs);
+#define MLORA_PAST_F32(DP, NW)                                             \
+  template __global__ void past_few_kernel<float, DP, 2, NW>(const PastArgs); \
+  template __global__ void past_dq_f32_kernel<DP, NW>(const PastBwdArgs);
 MLORA_PAST(64)
 MLORA_PAST(128)
+MLORA_PAST_F32(64, 8)
+MLORA_PAST_F32(64, 4)
+MLORA_PAST_F32(64, 2)
+MLORA_PAST_F32(128, 4)
+MLORA_PAST_F32(128, 2)
 #undef MLORA_PAST
+#undef MLORA_PAST_F32
+template __global__ void past_dkv_f32_kernel<64, 8>(const PastBwdArgs);
+template __global__ void past_dkv_f32_kernel<64, 4>(const PastBwdArgs);
+template __global__ void past_dkv_f32_kernel<128, 4>(const PastBwdArgs);
+template __global__ void past_dkv_f32_kernel<128, 2>(const PastBwdArgs);
 template __global__ void past_dkv_kernel<128, 8, 1>(const PastBwdArgs);
 
 // ------------------------------------------------------------------ host
 
 constexpr int64_t kPastMostTokens = 1 << 28, kPastMostBlocks = INT32_MAX - 65536;
-constexpr int64_t kFewMany = 256;  // float32 workgroups from which on they have half the waves
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -1644,8 +1648,20 @@ static int64_t own_tiles(const PastSizes &z, int64_t rows, int64_t kt) {
 // all shares are joined. Keys are shared out where there is less than a workgroup for every compute unit.
 struct PastPlan {
   bool few, packed, packed_few;
+  int waves;  // of few rows
   int64_t packed_tiles, packed_splits, row_tiles, splits, slots;
 };
+
+// How many waves a float32 workgroup has: `items` workgroups whose waves share `tiles` tiles. A tile waits for its loads, so that it
+// takes a SIMD's one wave as long as two; fewer waves leave room for more workgroups on a compute unit. Half where there is more than one
+// per unit (8 heads of 64, 4096 tokens, window 1024: 102 -> 88 us; 156 workgroups 50 -> 59, so not below); a quarter
+// where halves would be a second, mostly empty round and tiles are few (1573 tokens, window 257, 12 heads of 64, 600 workgroups of
+// ten tiles: 39, 37 and 30 us; not with many: 1024 workgroups of up to 22 27 -> 44).
+static int f32_waves(int64_t D, int64_t items, int64_t tiles) {
+  const int most = D > 64 ? 4 : 8;
+  if (items <= 256) return most;
+  return D <= 64 && items > 512 && items <= 1024 && tiles <= 16 ? most / 4 : most / 2;
+}
 
 // Into how many shares the key tiles of `items` workgroups of 128 rows are cut, two of which share a compute unit: what takes least
 // time, in microseconds. A tile of 64 keys takes 1.5 where a workgroup has the unit for itself and 2.0 where two share it (128
@@ -1667,7 +1683,8 @@ static int64_t wide_shares(int64_t items, int64_t tiles, int64_t floats, double 
 
 static PastPlan past_plan(const PastSizes &z) {
   PastPlan p{};
-  const int64_t few_rows = z.f32 ? INT64_MAX : 64, waves = z.f32 && z.D > 64 ? 4 : 8, e = z.f32 ? 4 : 2;
+  const int waves = z.f32 && z.D > 64 ? 4 : 8;
+  const int64_t few_rows = z.f32 ? INT64_MAX : 64, e = z.f32 ? 4 : 2;
   p.few = z.rows <= few_rows;
   p.packed = z.rows <= 64 && z.each > 1 && z.groups * (z.each - 1) * z.Lp * z.Hk * z.D * 2 * e > (16 << 20);
   p.row_tiles = ceil_div(z.rows, p.few ? 32 : 128);
@@ -1688,6 +1705,11 @@ static PastPlan past_plan(const PastSizes &z) {
     p.packed_splits = share(z.groups * z.Hk * p.packed_tiles, ceil_div(z.Lp, p.packed_few || z.f32 ? 32 : 64), p.packed_few);
   }
   p.slots = p.splits + p.packed_splits;
+  p.waves = waves;
+  if (z.f32) {
+    const int64_t own = z.B * z.Hk * p.row_tiles * p.splits, packed = z.groups * z.Hk * p.packed_tiles * p.packed_splits;
+    p.waves = f32_waves(z.D, own + packed, ceil_div(own_tiles(z, 32, kt) + prefix_tiles, p.splits));
+  }
   return p;
 }
 
@@ -1707,6 +1729,7 @@ struct PastBwdPlan {
   int64_t prefix_vectors, sink_vectors, own_vectors;  // 16-byte vectors of all shares of a class, 0 where it has one
   int64_t dq_vectors;                                 // of one share of dq
   double cost;  // of dk / dv, to choose by
+  int dq_waves;  // float32
 };
 
 static PastBwdPlan past_bwd_plan(const PastSizes &z) {
@@ -1717,6 +1740,7 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   const int64_t items = z.B * z.Hk * p.row_tiles, tiles = own_tiles(z, row_tile, kt) + ceil_div(z.Lp, kt);
   p.splits = items <= 0 ? 1 : !z.f32 ? wide_shares(items, tiles, 128 * dp, 8e6) : between(256 / items, 1, between(tiles / 8, 1, 64));
   p.dq_vectors = z.f32 ? z.B * z.Hk * z.rows * (z.D / 4) : items * 4 * (dp / 32) * 4 * 64;
+  p.dq_waves = f32_waves(z.D, items * p.splits, ceil_div(tiles, p.splits));
   const bool bounded = z.window < z.Lk;
   auto plan = [&](int kw) {
     PastBwdPlan c = p;
@@ -1805,6 +1829,19 @@ static void with_head(bool f32, int64_t D, F &&f) {
   else f(uint16_t{}, large);
 }
 
+// f with a workgroup's waves: bf16 has one number.
+template <class T, int DP, class F>
+static void with_waves(int waves, F &&f) {
+  constexpr int most = kFewWaves<T, DP>;
+  if constexpr (sizeof(T) == 4) {
+    if (waves == most / 2) return f(std::integral_constant<int, most / 2>{});
+    if constexpr (most == 8) {
+      if (waves == 2) return f(std::integral_constant<int, 2>{});
+    }
+  }
+  f(std::integral_constant<int, most>{});
+}
+
 }  // namespace mlora
 
 using namespace mlora;
@@ -1862,18 +1899,14 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
     a.packed_blocks = p.packed_few ? (int32_t)packed : 0;
     const dim3 grid((unsigned)(blocks + a.packed_blocks));
     const int64_t rows = p.packed_few ? z.each * z.rows : z.rows;
-    constexpr int threads = 64 * kFewWaves<T, DP, false>;
+    constexpr int most = kFewWaves<T, DP>;
     if (rows <= 16) {
-      hipLaunchKernelGGL((past_few_kernel<T, DP, 1, false>), grid, dim3(threads), 0, s, a);
+      hipLaunchKernelGGL((past_few_kernel<T, DP, 1, most>), grid, dim3(64 * most), 0, s, a);
       return;
     }
-    if constexpr (sizeof(T) == 4) {
-      if (blocks + a.packed_blocks > kFewMany) {
-        hipLaunchKernelGGL((past_few_kernel<T, DP, 2, true>), grid, dim3(threads / 2), 0, s, a);
-        return;
-      }
-    }
-    hipLaunchKernelGGL((past_few_kernel<T, DP, 2, false>), grid, dim3(threads), 0, s, a);
+    with_waves<T, DP>(p.waves, [&](auto nw) {
+      hipLaunchKernelGGL((past_few_kernel<T, DP, 2, decltype(nw)::value>), grid, dim3(64 * decltype(nw)::value), 0, s, a);
+    });
   });
   st = launch_status();
   if (st || p.slots == 1) return st;
@@ -1928,8 +1961,9 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
       constexpr int DP = decltype(dp)::value;
       const dim3 grid((unsigned)(z.B * z.Hk * p.row_tiles * p.splits));
       if constexpr (sizeof(T) == 2) hipLaunchKernelGGL(past_dq_kernel<DP>, grid, dim3(256), 0, s, ba);
-      else if (grid.x > kFewMany) hipLaunchKernelGGL((past_dq_f32_kernel<DP, true>), grid, dim3(64 * kFewWaves<float, DP, true>), 0, s, ba);
-      else hipLaunchKernelGGL((past_dq_f32_kernel<DP, false>), grid, dim3(64 * kFewWaves<float, DP, false>), 0, s, ba);
+      else with_waves<T, DP>(p.dq_waves, [&](auto nw) {
+        hipLaunchKernelGGL((past_dq_f32_kernel<DP, decltype(nw)::value>), grid, dim3(64 * decltype(nw)::value), 0, s, ba);
+      });
       if (p.splits > 1) hipLaunchKernelGGL((past_dq_join_kernel<T, DP>), dim3((unsigned)ceil_div(p.dq_vectors, 256)), dim3(256), 0, s, ba);
     });
     st = launch_status();
@@ -1949,8 +1983,8 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
     auto go = [&](auto kw) {
       constexpr int KW = decltype(kw)::value, RG = KW == 4 ? DP / 64 : 1;
       if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((past_dkv_kernel<DP, KW, RG>), dim3((unsigned)blocks), dim3(64 * KW * RG), 0, s, ba);
-      else if (blocks > kFewMany) hipLaunchKernelGGL((past_dkv_f32_kernel<DP, true>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, true>), 0, s, ba);
-      else hipLaunchKernelGGL((past_dkv_f32_kernel<DP, false>), dim3((unsigned)blocks), dim3(64 * kFewWaves<float, DP, false>), 0, s, ba);
+      else if (blocks > 256) hipLaunchKernelGGL((past_dkv_f32_kernel<DP, kFewWaves<T, DP> / 2>), dim3((unsigned)blocks), dim3(32 * kFewWaves<T, DP>), 0, s, ba);
+      else hipLaunchKernelGGL((past_dkv_f32_kernel<DP, kFewWaves<T, DP>>), dim3((unsigned)blocks), dim3(64 * kFewWaves<T, DP>), 0, s, ba);
       if (join_blocks > 0) hipLaunchKernelGGL((past_dkv_join_kernel<T, DP, KW>), dim3((unsigned)join_blocks), dim3(256), 0, s, ba, joins);
     };
     if constexpr (sizeof(T) == 2 && DP == 128) {

@@ -424,3 +424,9 @@ def test_calls_that_follow_each_other(pkg, dev):
         own = slice(2 * C, 3 * C)
         shared = pkg.prefix_attention(q[:, own], k[:, own], v[:, own], past[0][0], past[1][0], chunk=C)
     ref.check({"out": shared}, q[:, own], k[:, own], v[:, own], *past, chunk=C)
+
+
+def test_float32_between_one_and_two_rounds(pkg, dev):
+    """512 to 1024 workgroups of few tiles: a quarter of the waves."""
+    tensors, g = make(F, dev, 61, 2, 600, 600, 18, 18, 64)
+    some_heads(pkg, tensors, g, [0, 9, 17], window=60, sinks=3, lengths=i32(555, 600))
