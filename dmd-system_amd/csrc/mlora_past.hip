@@ -1742,7 +1742,7 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
   p.dq_vectors = z.f32 ? z.B * z.Hk * z.rows * (z.D / 4) : items * 4 * (dp / 32) * 4 * 64;
   p.dq_waves = f32_waves(z.D, items * p.splits, ceil_div(tiles, p.splits));
   const bool bounded = z.window < z.Lk;
-  auto plan = [&](int kw) {
+  auto plan = [&](int kw, double finer) {
     PastBwdPlan c = p;
     c.kw = kw;
     const int64_t qt = z.f32 ? 32 : 64, keys = z.f32 ? kF32Keys : 32 * kw;
@@ -1753,7 +1753,7 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
     const int64_t items[3] = {z.groups * z.Hk * c.prefix_blocks, z.B * z.Hk * c.sink_blocks, z.B * z.Hk * (c.key_blocks - c.sink_blocks)};
     const int64_t total = items[0] * work[0] + items[1] * work[1] + items[2] * work[2];
     const int64_t slots = z.f32 ? 1024 : z.D > 64 ? 256 : 512, least = z.f32 ? 8 : 4;
-    const int64_t target = std::max(ceil_div(total, slots), least);
+    const int64_t target = std::max((int64_t)(finer * (double)ceil_div(total, slots)), least);
     int64_t splits[3], blocks = 0, longest = 0;
     for (int i = 0; i < 3; ++i) {
       splits[i] = items[i] > 0 ? between(work[i] / target, 1, 64) : 1;
@@ -1774,11 +1774,17 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
                  (kw == 8 ? 1.0 : 0.66) + shares + (shares > 0 ? 2.0 : 0.0);
     return c;
   };
-  if (z.f32 || z.D <= 64) return plan(4);
+  if (z.f32 || z.D <= 64) return plan(4, 1.0);
   // 256 keys per workgroup, or 128 whose tiles take 0.66 of the time (a barrier per 32 rows of a wave): 32760 keys, 12 heads, in one 4.7 ms,
-  // in the other 5.4; 4096 keys without a window, 12 heads, 240 us and 165
-  const PastBwdPlan wide = plan(8), narrow = plan(4);
-  return wide.cost <= narrow.cost ? wide : narrow;
+  // in the other 5.4; 4096 keys without a window, 12 heads, 240 us and 165. Shares of an even part of the work,
+  // or finer ones (two samples of 4096 and 2777 tokens, window 1024, 16 / 4 heads: 160 workgroups 270 us, in finer shares 165).
+  PastBwdPlan best = plan(8, 1.0);
+  for (int kw : {8, 4})
+    for (double finer : {1.0, 0.8, 0.6}) {
+      const PastBwdPlan c = plan(kw, finer);
+      if (c.cost < 0.97 * best.cost) best = c;
+    }
+  return best;
 }
 
 // The rows' deltas, then the shares of dq, and after they are joined those of dk and dv in the same place.
