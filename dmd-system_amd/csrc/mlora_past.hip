@@ -773,7 +773,61 @@ __global__ __launch_bounds__((64 * NW), (kFewWaves<T, DP> / 4)) void past_few_ke
   }
 }
 
-// Joins the shares of a row, one workgroup per row: weights 2^((m_s − max m)·c). Eight groups of 32 lanes (4 channels
+// Writes a joined row, four channels per lane `at` of 32: its sums o and l relative to top.
+template <class T>
+__device__ __forceinline__ void write_joined(const PastArgs &a, int64_t all, int64_t row, int at, f32x4 o, float l, const RowRef &top) {
+  if (at == 0 && a.stats != nullptr) {
+    a.stats[row] = l > 0.f ? top.r + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
+    a.stats[all + row] = l > 0.f ? top.a : 0.f;
+  }
+  if (4 * at >= a.D) return;
+  const int r = (int)(row % a.rows), hk = (int)(row / a.rows % a.Hk);
+  const int64_t b = row / a.rows / a.Hk;
+  const int64_t place = (b * a.Lq + r / a.G) * a.H * a.D + (int64_t)(hk * a.G + r % a.G) * a.D + 4 * at;
+  o *= l > 0.f || l != l ? 1.0f / l : 0.f;
+  T *p = static_cast<T *>(a.out) + place;
+  if constexpr (sizeof(T) == 2) {
+    *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+    if (a.stats == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] -= bf16_to_f32(f32_to_bf16_rne(o[j]));
+    *(MLORA_GLOBAL u32x2 *)(a.rest + place) = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
+  } else *(MLORA_GLOBAL f32x4 *)p = o;
+}
+
+// Joins up to eight shares of a row, weights 2^((m_s − max m)·c): 32 lanes per row, every share's sums asked for before any is used
+// (18720 rows of three shares 7.6 us; with a workgroup per row 18.8).
+template <class T>
+__global__ __launch_bounds__(256) void past_join_rows_kernel(const PastArgs a) {
+  constexpr int MOST = 8;
+  const int64_t all = (int64_t)a.B * a.Hk * a.rows, row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int at = threadIdx.x % 32, ch = min(4 * at, a.D - 4);
+  if (row >= all) return;
+  float2 ml[MOST];
+  f32x4 part[MOST];
+#pragma unroll
+  for (int s = 0; s < MOST; ++s) {
+    if (s >= a.slots) break;
+    ml[s] = *(const float2 *)(a.part_ml + 2 * (s * all + row));
+    part[s] = *(const MLORA_GLOBAL f32x4 *)(a.part_o + (s * all + row) * a.D + ch);
+  }
+  float m = kNoMax, l = 0.f;
+#pragma unroll
+  for (int s = 0; s < MOST; ++s)
+    if (s < a.slots) m = fmaxf(m, ml[s].x);
+  const RowRef top = row_ref(m, a.c);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < MOST; ++s) {
+    if (s >= a.slots) break;
+    const float w = ref_factor(row_ref(ml[s].x, a.c), top, a.c);
+    l += w * ml[s].y;
+    if (ml[s].y != 0.f) o += w * part[s];
+  }
+  write_joined<T>(a, all, row, at, o, l, top);
+}
+
+// Joins more shares of a row, one workgroup per row: weights 2^((m_s − max m)·c). Eight groups of 32 lanes (4 channels
 // each) take every eighth share, and their sums are added in order through LDS.
 template <class T>
 __global__ __launch_bounds__(256) void past_join_kernel(const PastArgs a) {
@@ -803,23 +857,7 @@ __global__ __launch_bounds__(256) void past_join_kernel(const PastArgs a) {
   l = ls[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) o += sums[i][at], l += ls[i];
-  if (at == 0 && a.stats != nullptr) {
-    a.stats[row] = l > 0.f ? top.r + __builtin_amdgcn_logf(l) : l != l ? l : INFINITY;
-    a.stats[all + row] = l > 0.f ? top.a : 0.f;
-  }
-  if (4 * at >= a.D) return;
-  const int r = (int)(row % a.rows), hk = (int)(row / a.rows % a.Hk);
-  const int64_t b = row / a.rows / a.Hk;
-  const int64_t place = (b * a.Lq + r / a.G) * a.H * a.D + (int64_t)(hk * a.G + r % a.G) * a.D + 4 * at;
-  o *= l > 0.f || l != l ? 1.0f / l : 0.f;
-  T *p = static_cast<T *>(a.out) + place;
-  if constexpr (sizeof(T) == 2) {
-    *(MLORA_GLOBAL u32x2 *)p = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
-    if (a.stats == nullptr) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] -= bf16_to_f32(f32_to_bf16_rne(o[j]));
-    *(MLORA_GLOBAL u32x2 *)(a.rest + place) = u32x2{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3])};
-  } else *(MLORA_GLOBAL f32x4 *)p = o;
+  write_joined<T>(a, all, row, at, o, l, top);
 }
 
 // ------------------------------------------------------------------ backward
@@ -1667,8 +1705,8 @@ static int f32_waves(int64_t D, int64_t items, int64_t tiles) {
 // time, in microseconds. A tile of 64 keys takes 1.5 where a workgroup has the unit for itself and 2.0 where two share it (128
 // channels; the ratio is what counts), a share one and a half tiles more for its start; its sums are written, read and joined by
 // another launch (the forward's, row by row, at 4 TB/s, dq's, as they lie in registers, at 8). A frame of 1560 tokens on nine
-// others, 12 heads (156 workgroups of 244 tiles): 381 us in one share, 203 in three; on 14040 keys that two samples share (312) 478
-// and 386; by itself (156 of 25) 46 and 50: under 7 % it is not worth the launch.
+// others, 12 heads (156 workgroups of 244 tiles): 381 us in one share, 188 in three; on 14040 keys that two samples share (312) 478
+// and 362; by itself (156 of 25) 46 and 50: under 7 % it is not worth the launch.
 static int64_t wide_shares(int64_t items, int64_t tiles, int64_t floats, double bytes_per_us) {
   int64_t best = 1;
   double least = 0;
@@ -1916,9 +1954,16 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   });
   st = launch_status();
   if (st || p.slots == 1) return st;
-  const dim3 joins((unsigned)(z.B * z.Hk * z.rows));
-  if (z.f32) hipLaunchKernelGGL(past_join_kernel<float>, joins, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(past_join_kernel<uint16_t>, joins, dim3(256), 0, s, a);
+  const int64_t rows = z.B * z.Hk * z.rows;
+  if (p.slots <= (rows < 1024 ? 4 : 8)) {  // 64 rows of 8 shares 16.7 us with the forward, by a workgroup per row 16.2
+    const dim3 joins((unsigned)ceil_div(rows, 8));
+    if (z.f32) hipLaunchKernelGGL(past_join_rows_kernel<float>, joins, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(past_join_rows_kernel<uint16_t>, joins, dim3(256), 0, s, a);
+  } else {
+    const dim3 joins((unsigned)rows);
+    if (z.f32) hipLaunchKernelGGL(past_join_kernel<float>, joins, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(past_join_kernel<uint16_t>, joins, dim3(256), 0, s, a);
+  }
   return launch_status();
 }
 
