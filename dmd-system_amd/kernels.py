@@ -1173,8 +1173,9 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 
 class PastPlan:
     """A past-attention call's sizes, strides and options as the C entries take them, the bytes of its workspaces, and where
-    the backward's statistics lie; made once per combination of them by past_plan."""
-    __slots__ = ("shape", "ref", "forward", "backward", "stats", "saved", "g_strides", "empty", "pad")
+    the backward's statistics lie; made once per combination of them by past_plan. metas: shape, type, device and strides of what
+    the backward reads, for who calls it."""
+    __slots__ = ("shape", "ref", "forward", "backward", "stats", "saved", "g_strides", "empty", "pad", "metas")
 
 
 def past_plan(dtype: torch.dtype, sizes: Sequence[int], strides: Sequence[tuple], window: int, sinks: int, chunk: int, first: int,

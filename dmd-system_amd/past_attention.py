@@ -61,8 +61,28 @@ def _lay_out(call, tensors):
     pointers = [t.data_ptr() for t in tensors]
     if plan is None or any([p & 15 for p in pointers]):
         tensors = [_aligned(t) for t in tensors]
-        plan, pointers = _plan(tuple([_meta(t) for t in tensors]), *again)[0], [t.data_ptr() for t in tensors]
+        plan, pointers = _planned(tuple([_meta(t) for t in tensors]), again), [t.data_ptr() for t in tensors]
     return plan, tensors, pointers
+
+
+def _planned(metas, again):
+    return _plan(metas, *again)[0]
+
+
+def _unpack(ctx):
+    """(the kernels' plan, what the forward saved, as the plan has it). A saved-tensor hook may return a copy in another layout,
+    which is planned again; anything but the tensor it was given is refused."""
+    plan, saved = ctx.plan, ctx.saved_tensors
+    metas = tuple([_meta(t) for t in saved])
+    if metas == plan.metas and not any([t.data_ptr() & 15 for t in saved[3:]]):
+        return plan, saved
+    for was, now in zip(plan.metas, metas):
+        if (was and was[:3]) != (now and now[:3]):
+            _fail(f"a saved-tensor hook returned {now and now[:3]} in place of {was and was[:3]}")
+    flat = [t if t is None else t.contiguous() for t in saved[:5]]  # the vectors, out and the statistics
+    flat = [t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in flat]
+    tensors = [_aligned(t) for t in saved[5:]]
+    return _planned(tuple([_meta(t) for t in tensors]), ctx.again), (*flat, *tensors)
 
 
 class PastAttentionFunction(torch.autograd.Function):
@@ -71,6 +91,7 @@ class PastAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, call, key_lengths, query_start, prefix_lengths, *tensors):
+        ctx.again = call[1]
         ctx.plan, tensors, pointers = _lay_out(call, tensors)
         out, saved = kernels.past_attention(ctx.plan, tensors, pointers, key_lengths, query_start, prefix_lengths, True)
         ctx.save_for_backward(key_lengths, query_start, prefix_lengths, out, saved, *tensors)
@@ -79,9 +100,9 @@ class PastAttentionFunction(torch.autograd.Function):
     @staticmethod
     @kernels.first_order
     def backward(ctx, g):
-        key_lengths, query_start, prefix_lengths, out, saved, *tensors = ctx.saved_tensors
+        plan, (key_lengths, query_start, prefix_lengths, out, saved, *tensors) = _unpack(ctx)
         g = _aligned(g if g.dtype is out.dtype else g.to(out.dtype))
-        grads = kernels.past_attention_backward(ctx.plan, out, saved, g, tensors, key_lengths, query_start, prefix_lengths)
+        grads = kernels.past_attention_backward(plan, out, saved, g, tensors, key_lengths, query_start, prefix_lengths)
         return (None, None, None, None, *[d if want else None for d, want in zip(grads, ctx.needs_input_grad[4:])])
 
 
@@ -166,7 +187,13 @@ def _plan(metas, key_lengths, query_start, prefix_lengths, window, sinks, chunk,
         dtype, (B, Lq, Lk, H, Hk, D, groups, Lp), [[s if n > 1 else 0 for s, n in zip(m[3][:3], m[0])] for m in metas],
         0 if window is None else min(max(window, chunk), Lk + chunk), min(sinks, Lk), chunk, start,
         query_start is None and key_lengths is not None and Lq < Lk, scale)
+    plan.metas = (_vector(key_lengths), _vector(query_start if isinstance(query_start, tuple) else None), _vector(prefix_lengths),
+                  (q[0], dtype, device, (Lq * H * D, H * D, D, 1)), (torch.Size((plan.saved,)), torch.float32, device, (1,)), *metas)
     return plan, again
+
+
+def _vector(meta):
+    return meta and (meta[0], torch.int32, meta[2], (1,))
 
 
 def _int32(t: torch.Tensor | None, low: int, high: int) -> torch.Tensor | None:

@@ -430,3 +430,26 @@ def test_float32_between_one_and_two_rounds(pkg, dev):
     """512 to 1024 workgroups of few tiles: a quarter of the waves."""
     tensors, g = make(F, dev, 61, 2, 600, 600, 18, 18, 64)
     some_heads(pkg, tensors, g, [0, 9, 17], window=60, sinks=3, lengths=i32(555, 600))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_gradients_under_saved_tensor_hooks(pkg, dev, prefix, dtype):
+    """Tensors that are offloaded, copied or laid out anew between forward and backward give the gradients that they give as they lie."""
+    gen = torch.Generator().manual_seed(71)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev).to(dtype)  # noqa: E731
+    packed = r(2, 150, 3, 4, 64)
+    tensors, g = [packed[:, :, 0], r(2, 4, 150, 64).transpose(1, 2), r(1, 150, 4, 64).expand(2, 150, 4, 64)], r(2, 150, 4, 64)
+    kw = dict(window=40, lengths=i32(150, 97))
+    if prefix:
+        past = r(1, 70, 2, 4, 64)
+        tensors += [past[:, :, 0], past[:, :, 1]]
+    want = both(pkg, tensors, g, **kw)
+    lay = lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))  # noqa: E731
+    graph = torch.autograd.graph
+    for hooks in (graph.save_on_cpu(), graph.save_on_cpu(pin_memory=True), graph.saved_tensors_hooks(torch.clone, torch.clone),
+                  graph.saved_tensors_hooks(lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format)),
+                  graph.saved_tensors_hooks(lambda t: t, lay)):
+        with hooks:
+            got = run(pkg, tensors, g, **kw)
+        assert all(torch.equal(got[n], want[n]) for n in want)

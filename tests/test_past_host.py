@@ -187,3 +187,92 @@ def test_workspaces(pkg):
                      (dict(dq=None), L.ERR_INVALID), (dict(dk=None), L.ERR_INVALID), (dict(dv=0xb008), L.ERR_UNSUPPORTED),
                      (dict(work=None), L.ERR_WORKSPACE), (dict(nbytes=back - 1), L.ERR_WORKSPACE), (dict(work=0x7004), L.ERR_UNSUPPORTED)):
         assert bwd(**kw) == code, kw
+
+
+@pytest.fixture
+def told(pkg, monkeypatch):
+    """The operators up to their launches, on host tensors: what kernels.past_attention_backward is called with, call by call."""
+    past, calls = pkg.past_attention, []
+    meta = past._meta
+
+    def on_device(*a):
+        m = meta(*a)
+        return m and (*m[:2], torch.device("cuda", 0), *m[3:])
+
+    def forward(plan, tensors, pointers, *rest):
+        return torch.zeros(tensors[0].shape, dtype=tensors[0].dtype), torch.zeros(plan.saved)
+
+    def backward(plan, out, saved, g, tensors, *vectors):
+        calls.append((plan, out, saved, g, tensors, vectors))
+        return [torch.zeros(t.shape, dtype=t.dtype) for t in tensors]
+
+    monkeypatch.setattr(past, "_meta", on_device)
+    monkeypatch.setattr(pkg.kernels, "past_attention", forward)
+    monkeypatch.setattr(pkg.kernels, "past_attention_backward", backward)
+    return calls
+
+
+def strided_last(t):
+    return torch.stack((t, t), dim=-1).flatten(-2)[..., ::2]
+
+
+def misaligned(t):
+    return torch.cat((t.new_zeros(1), t.reshape(-1)))[1:].view(t.shape)
+
+
+HOOKS = {
+    "contiguous": lambda t: t.clone(memory_format=torch.contiguous_format),
+    "clone": torch.clone,
+    "reversed": lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim()))),
+    "strided last": strided_last,
+    "misaligned": misaligned,
+    "as it was": lambda t: t,
+}
+
+
+def operands(dtype, prefix):
+    """q, k and v of packed projections, head-major and expanded storage."""
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(len(s) + s[1])).to(dtype)  # noqa: E731
+    t = [r(2, 50, 3, 4, 64)[:, :, 0], r(2, 4, 50, 64).transpose(1, 2), r(1, 50, 4, 64).expand(2, 50, 4, 64)]
+    return t + ([r(2, 9, 2, 4, 64)[:, :, 1], r(2, 9, 4, 64)] if prefix else [])
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("hook", [*HOOKS, "save_on_cpu"])
+def test_backward_reads_what_saved_tensor_hooks_return(pkg, told, hook, dtype, prefix):
+    """Hooks may return a saved tensor in another layout: the kernels are told the strides of what they are given."""
+    tensors = operands(dtype, prefix)
+    leaves = [t.detach().requires_grad_(True) for t in tensors]
+    lengths, start = torch.tensor([50, 31]), torch.tensor([0, 3], dtype=torch.int32)
+    kw = dict(key_lengths=lengths, query_start=start, window=9)
+    if prefix:
+        kw["prefix_lengths"] = torch.tensor([9, 4], dtype=torch.int32)
+    context = torch.autograd.graph.save_on_cpu() if hook == "save_on_cpu" else \
+        torch.autograd.graph.saved_tensors_hooks(lambda t: t, HOOKS[hook])
+    with context:
+        out = (pkg.prefix_attention if prefix else pkg.window_attention)(*leaves, **kw)
+    torch.autograd.grad(out, leaves, [torch.ones_like(out)])
+    (plan, out, saved, g, given, vectors), = told
+    for name, t, want in zip("q k v pk pv".split(), given, tensors):
+        assert torch.equal(t, want) and t.dtype == want.dtype and t.data_ptr() % 16 == 0 and t.stride(3) == 1, name
+        have = getattr(plan.shape, name + "_strides")
+        assert all(n < 2 or a == b for n, a, b in zip(t.shape, have, t.stride())), name
+    assert (plan.shape.window, plan.shape.Lq, plan.shape.Lk, plan.shape.groups) == (9, 50, 50, 2 if prefix else 0)
+    assert all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (out, saved, g))
+    assert vectors[0].tolist() == [50, 31] and vectors[1].tolist() == [0, 3] and (not prefix or vectors[2].tolist() == [9, 4])
+    assert all(v is None or (v.is_contiguous() and v.dtype is torch.int32) for v in vectors)
+
+
+@pytest.mark.parametrize("at", range(5))
+@pytest.mark.parametrize("hook", [lambda t: t.double(), lambda t: t[..., :-1]], ids=["type", "shape"])
+def test_backward_refuses_what_is_no_saved_tensor(pkg, told, hook, at):
+    """A hook that returns something else than it was given: not read as if it were it. at: of the tensors in the order they are
+    unpacked (the vector of lengths, out, the statistics, q, k)."""
+    count = iter(range(100))
+    leaves = [t.detach().requires_grad_(True) for t in operands(BF, False)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: hook(t) if next(count) == at else t):
+        out = pkg.window_attention(*leaves, key_lengths=torch.tensor([50, 31]))
+    with pytest.raises(RuntimeError, match="saved-tensor hook"):
+        torch.autograd.grad(out, leaves, [torch.ones_like(out)])
+    assert not told
