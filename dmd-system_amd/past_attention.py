@@ -30,6 +30,7 @@ from . import kernels
 
 _DTYPES = (torch.bfloat16, torch.float32)
 _MOST = 1 << 28  # tokens
+_NAMES = ("q", "k", "v", "prefix_k", "prefix_v")
 
 
 def _fail(message: str) -> None:
@@ -107,11 +108,13 @@ class PastAttentionFunction(torch.autograd.Function):
 
 
 def _meta(t: torch.Tensor | None):
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor):
-        _fail(f"q, k, v, prefixes and lengths must be a tensor each, got a {type(t).__name__}")
-    return t.shape, t.dtype, t.device, t.stride()
+    return None if t is None else (t.shape, t.dtype, t.device, t.stride())
+
+
+def _check_tensors(**tensors) -> None:
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            _fail(f"{name} must be a tensor, got a {type(t).__name__}")
 
 
 def _check_vector(name: str, meta, n: int, device) -> None:
@@ -205,6 +208,12 @@ def _int32(t: torch.Tensor | None, low: int, high: int) -> torch.Tensor | None:
 
 
 def _attend(tensors, key_lengths, query_start, prefix_lengths, window, sinks, chunk, scale):
+    if not all([isinstance(t, torch.Tensor) for t in tensors]):
+        _check_tensors(**dict(zip(_NAMES, tensors)))
+    if key_lengths is not None and not isinstance(key_lengths, torch.Tensor):
+        _check_tensors(key_lengths=key_lengths)
+    if prefix_lengths is not None and not isinstance(prefix_lengths, torch.Tensor):
+        _check_tensors(prefix_lengths=prefix_lengths)
     if scale is not None:
         scale = kernels.number("scale", scale, _fail)
     start = query_start
@@ -249,6 +258,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     prefix_k and prefix_v: [Lp, Hk, D] for all samples, or [groups, Lp, Hk, D], each for B / groups samples in a row.
     prefix_lengths: int32 or int64 [groups] on q's device, the leading keys a prefix has (clamped to [0, Lp]). k and v hold the
     samples' own keys; positions, window, chunk and key_lengths count these alone."""
+    _check_tensors(prefix_k=prefix_k, prefix_v=prefix_v)
     if prefix_k.dim() == 3 and prefix_v.dim() == 3:
         prefix_k, prefix_v = prefix_k.unsqueeze(0), prefix_v.unsqueeze(0)
     return _attend((q, k, v, prefix_k, prefix_v), key_lengths, query_start, prefix_lengths, window, 0, chunk, scale)

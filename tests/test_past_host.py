@@ -276,3 +276,19 @@ def test_backward_refuses_what_is_no_saved_tensor(pkg, told, hook, at):
     with pytest.raises(RuntimeError, match="saved-tensor hook"):
         torch.autograd.grad(out, leaves, [torch.ones_like(out)])
     assert not told
+
+
+@pytest.mark.parametrize("what", [None, [1.0], 3], ids=["None", "list", "number"])
+def test_what_is_no_tensor_is_refused_by_name(pkg, what):
+    t = dict(q=heads(), k=heads(), v=heads(), prefix_k=heads(L=9), prefix_v=heads(L=9))
+    for fn, names in ((pkg.window_attention, "q k v"), (pkg.prefix_attention, "q k v prefix_k prefix_v")):
+        for bad in ([n] for n in names.split()):
+            with pytest.raises(RuntimeError, match=f"{bad[0]} must be a tensor, got a {type(what).__name__}"):
+                fn(*[what if n in bad else t[n] for n in names.split()])
+    for prefix in ((what, what), (t["prefix_k"][0], what)):
+        with pytest.raises(RuntimeError, match="prefix_[kv] must be a tensor"):
+            pkg.prefix_attention(*list(t.values())[:3], *prefix)
+    if what is not None:
+        for name in ("key_lengths", "prefix_lengths"):
+            with pytest.raises(RuntimeError, match=f"{name} must be a tensor"):
+                pkg.prefix_attention(*t.values(), **{name: what})
