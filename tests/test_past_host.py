@@ -292,3 +292,15 @@ def test_what_is_no_tensor_is_refused_by_name(pkg, what):
         for name in ("key_lengths", "prefix_lengths"):
             with pytest.raises(RuntimeError, match=f"{name} must be a tensor"):
                 pkg.prefix_attention(*t.values(), **{name: what})
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "prefix_k", "prefix_v"])
+def test_rows_wider_than_the_kernels_take_are_refused(pkg, told, name):
+    """A contiguous copy does not help where a token's heads alone are past the limit of token strides."""
+    wide, narrow = (torch.zeros(1).expand(1, 2, h, 128) for h in (1 << 15, 1))
+    t = dict(q=wide, k=narrow, v=narrow, prefix_k=narrow, prefix_v=narrow)
+    if name != "q":
+        t = dict(q=wide[:, :1], k=wide[:, :1], v=wide[:, :1], prefix_k=wide[:, :1], prefix_v=wide[:, :1])
+        t.update({n: wide for n in (("k", "v") if name in "kv" else ("prefix_k", "prefix_v"))})
+    with pytest.raises(RuntimeError, match="heads of a token"):
+        pkg.prefix_attention(*t.values())
