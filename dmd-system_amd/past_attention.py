@@ -184,7 +184,11 @@ def _plan(metas, key_lengths, query_start, prefix_lengths, window, sinks, chunk,
     start = 0 if isinstance(query_start, tuple) else Lk - Lq if query_start is None else max(-Lq, min(query_start, Lk))
     chunk = min(chunk, max(Lk, 1))
     groups, Lp = pk[0][:2] if pk is not None else (0, 0)
-    if not all(_layout(shape, strides) for shape, _, _, strides in metas):
+    copied = [(name, shape) for name, (shape, _, _, strides) in zip(_NAMES, metas) if not _layout(shape, strides)]
+    for name, shape in copied:
+        if shape[1] > 1 and shape[2] * shape[3] >= kernels.ATTENTION_MAX_STRIDE:  # not theirs after a copy either
+            _fail(f"the heads of a token of {name} have {shape[2] * shape[3]} elements, they must be fewer than {kernels.ATTENTION_MAX_STRIDE}")
+    if copied:
         return None, again
     plan = kernels.past_plan(
         dtype, (B, Lq, Lk, H, Hk, D, groups, Lp), [[s if n > 1 else 0 for s, n in zip(m[3][:3], m[0])] for m in metas],
