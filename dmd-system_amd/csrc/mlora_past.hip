@@ -1665,9 +1665,10 @@ static int past_sizes(PastSizes &z, const mlora_past_shape *s) {
   if (z.Lq > kPastMostTokens || z.Lk > kPastMostTokens || z.Lp > kPastMostTokens || z.H > 65536) return MLORA_ERR_LIMIT;
   z.groups = s->groups > 0 ? s->groups : z.B, z.each = z.groups > 0 ? z.B / z.groups : 1;
   z.rows = z.G * z.Lq;
-  // workgroups: one per (sample, key head, 32 rows or keys at least), a few thousand shares beside them; rows of a group
+  // workgroups: one per (sample, key head, 32 rows or keys at least), a few thousand shares beside them; rows of a group. What a launch
+  // takes is checked of each (launch_fits)
   const int64_t most = kPastMostBlocks, blocks = ceil_div(z.rows, 32) + ceil_div(z.Lk, 32) + ceil_div(z.Lp, 32) + 1;
-  if (z.rows > most || (z.B > 0 && (z.Hk > most / z.B || blocks + 4096 > most / (z.B * z.Hk) || z.rows > most / z.B))) return MLORA_ERR_LIMIT;
+  if (z.rows > most || (z.B > 0 && (z.Hk > most / z.B || blocks > most / (z.B * z.Hk) || z.rows > most / z.B))) return MLORA_ERR_LIMIT;
   z.chunk = between(s->chunk, 1, z.Lk > 1 ? z.Lk : 1);  // from there on all keys are one chunk
   z.window = s->window > 0 ? between(s->window, z.chunk, z.Lk + z.chunk) : z.Lk + z.chunk;
   z.sinks = between(s->sinks, 0, z.Lk);
@@ -1755,9 +1756,27 @@ static int64_t past_floats(const PastPlan &p, const PastSizes &z) {
   return p.slots > 1 ? p.slots * ceil_div(z.B * z.Hk * z.rows * (z.D + 2), 4) * 4 : 0;
 }
 
-// Shares are joined by a workgroup per row.
-static int past_join_limit(const PastPlan &p, const PastSizes &z) {
-  return p.slots > 1 && z.rows > 0 && z.B * z.Hk > kPastMostBlocks / z.rows ? MLORA_ERR_LIMIT : MLORA_OK;
+// HIP launches fewer than 2^32 work items (threads: a power of two).
+static bool launch_fits(int64_t blocks, int64_t threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
+static int64_t packed_blocks(const PastPlan &p, const PastSizes &z) { return z.groups * z.Hk * p.packed_tiles * p.packed_splits; }
+static int64_t own_blocks(const PastPlan &p, const PastSizes &z) { return z.B * z.Hk * p.row_tiles * p.splits; }
+
+// Whether the rows of a few-row launch fit one block of 16.
+static bool one_block(const PastPlan &p, const PastSizes &z) { return (p.packed_few ? z.each * z.rows : z.rows) <= 16; }
+
+// A row's shares are joined by 32 lanes, or by a workgroup where they are many or rows are few.
+static bool join_by_lanes(const PastPlan &p, const PastSizes &z) {  // 64 rows of 8 shares 16.7 us with the forward, by a workgroup per row 16.2
+  return p.slots <= (z.B * z.Hk * z.rows < 1024 ? 4 : 8);
+}
+
+static int past_limit(const PastPlan &p, const PastSizes &z) {
+  const int64_t rows = z.B * z.Hk * z.rows, most = z.f32 && z.D > 64 ? 4 : 8;
+  bool fits = p.few ? launch_fits(own_blocks(p, z) + (p.packed_few ? packed_blocks(p, z) : 0), 64 * (one_block(p, z) ? most : p.waves))
+                    : launch_fits(own_blocks(p, z), 256);
+  if (p.packed && !p.packed_few) fits = fits && launch_fits(packed_blocks(p, z), 256);
+  if (p.slots > 1) fits = fits && launch_fits(join_by_lanes(p, z) ? ceil_div(rows, 8) : rows, 256);
+  return fits ? MLORA_OK : MLORA_ERR_LIMIT;
 }
 
 struct PastBwdPlan {
@@ -1831,6 +1850,28 @@ static int64_t past_bwd_bytes(const PastBwdPlan &p, const PastSizes &z) {
   return (ceil_div(z.B * z.Hk * z.rows, 4) + (dq > dkv ? dq : dkv)) * 16;
 }
 
+// The workgroups of dk / dv, over all classes, and the work items of one; the vectors of a class's share, 0 where it has one.
+static int64_t dkv_blocks(const PastBwdPlan &p, const PastSizes &z) {
+  return z.groups * z.Hk * p.prefix_blocks * p.prefix_splits + z.B * z.Hk * (p.sink_blocks * p.sink_splits + (p.key_blocks - p.sink_blocks) * p.own_splits);
+}
+static int64_t dkv_threads(const PastBwdPlan &p, const PastSizes &z) {
+  if (z.f32) return (z.D > 64 ? 256 : 512) / (dkv_blocks(p, z) > 256 ? 2 : 1);
+  return p.kw == 8 || z.D > 64 ? 512 : 256;
+}
+static int64_t dkv_join_blocks(const PastBwdPlan &p, int64_t (&upto)[3]) {
+  const int64_t vectors[3] = {p.prefix_vectors, p.sink_vectors, p.own_vectors}, splits[3] = {p.prefix_splits, p.sink_splits, p.own_splits};
+  int64_t blocks = 0;
+  for (int c = 0; c < 3; ++c) upto[c] = blocks += splits[c] > 1 ? ceil_div(vectors[c] / splits[c], 256) : 0;
+  return blocks;
+}
+static int past_bwd_limit(const PastBwdPlan &p, const PastSizes &z) {
+  int64_t upto[3];
+  const bool fits = launch_fits(z.B * z.Hk * p.row_tiles * p.splits, z.f32 ? 64 * p.dq_waves : 256) &&
+                    (p.splits == 1 || launch_fits(ceil_div(p.dq_vectors, 256), 256)) && launch_fits(dkv_blocks(p, z), dkv_threads(p, z)) &&
+                    launch_fits(dkv_join_blocks(p, upto), 256);
+  return fits ? MLORA_OK : MLORA_ERR_LIMIT;
+}
+
 // A [B, L, heads, D] operand: 16-byte aligned heads, token strides whose tiles stay within 32-bit offsets.
 static int past_operand(const void *p, const int64_t *st, bool empty) {
   if (empty) return MLORA_OK;
@@ -1895,7 +1936,7 @@ extern "C" int64_t mlora_past_attention_workspace_bytes(const mlora_past_shape *
   int st = past_sizes(z, shape);
   if (st) return st;
   const PastPlan p = past_plan(z);
-  st = past_join_limit(p, z);
+  st = past_limit(p, z);
   return st ? st : past_floats(p, z) * (int64_t)sizeof(float);
 }
 
@@ -1912,7 +1953,7 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   if (out == nullptr || (stats != nullptr && !z.f32 && rest == nullptr)) return MLORA_ERR_INVALID;
   if (!aligned16(out) || !aligned16(rest) || (reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return MLORA_ERR_UNSUPPORTED;
   const PastPlan p = past_plan(z);
-  st = past_join_limit(p, z);
+  st = past_limit(p, z);
   if (st) return st;
   const int64_t floats = past_floats(p, z);
   if (floats > 0) {
@@ -1924,7 +1965,7 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   a.part_ml = a.part_o + p.slots * z.B * z.Hk * z.rows * z.D;
   a.row_tiles = (int32_t)p.row_tiles, a.splits = (int32_t)p.splits, a.slots = (int32_t)p.slots;
   a.packed_tiles = (int32_t)p.packed_tiles, a.packed_splits = (int32_t)p.packed_splits;
-  const int64_t packed = z.groups * z.Hk * p.packed_tiles * p.packed_splits, blocks = z.B * z.Hk * p.row_tiles * p.splits;
+  const int64_t packed = packed_blocks(p, z), blocks = own_blocks(p, z);
   if (p.packed) a.with_prefix = 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_head(z.f32, z.D, [&](auto t, auto dp) {
@@ -1942,9 +1983,8 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
     }
     a.packed_blocks = p.packed_few ? (int32_t)packed : 0;
     const dim3 grid((unsigned)(blocks + a.packed_blocks));
-    const int64_t rows = p.packed_few ? z.each * z.rows : z.rows;
     constexpr int most = kFewWaves<T, DP>;
-    if (rows <= 16) {
+    if (one_block(p, z)) {
       hipLaunchKernelGGL((past_few_kernel<T, DP, 1, most>), grid, dim3(64 * most), 0, s, a);
       return;
     }
@@ -1955,7 +1995,7 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
   st = launch_status();
   if (st || p.slots == 1) return st;
   const int64_t rows = z.B * z.Hk * z.rows;
-  if (p.slots <= (rows < 1024 ? 4 : 8)) {  // 64 rows of 8 shares 16.7 us with the forward, by a workgroup per row 16.2
+  if (join_by_lanes(p, z)) {
     const dim3 joins((unsigned)ceil_div(rows, 8));
     if (z.f32) hipLaunchKernelGGL(past_join_rows_kernel<float>, joins, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(past_join_rows_kernel<uint16_t>, joins, dim3(256), 0, s, a);
@@ -1969,8 +2009,11 @@ extern "C" int mlora_past_attention(const mlora_past_shape *shape, const void *q
 
 extern "C" int64_t mlora_past_attention_backward_workspace_bytes(const mlora_past_shape *shape) {
   PastSizes z;
-  const int st = past_sizes(z, shape);
-  return st ? st : past_bwd_bytes(past_bwd_plan(z), z);
+  int st = past_sizes(z, shape);
+  if (st) return st;
+  const PastBwdPlan p = past_bwd_plan(z);
+  st = past_bwd_limit(p, z);
+  return st ? st : past_bwd_bytes(p, z);
 }
 
 extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, const void *q, const void *k, const void *v,
@@ -1995,6 +2038,8 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
   for (const void *p : {out, rest, (const void *)dq, (const void *)dk, (const void *)dv, (const void *)dpk, (const void *)dpv})
     if (!aligned16(p)) return MLORA_ERR_UNSUPPORTED;
   const PastBwdPlan p = past_bwd_plan(z);
+  st = past_bwd_limit(p, z);
+  if (st) return st;
   if (workspace_bytes < past_bwd_bytes(p, z) || (workspace == nullptr && workspace_bytes > 0)) return MLORA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MLORA_ERR_UNSUPPORTED;
   a.out = const_cast<void *>(out), a.rest = static_cast<uint16_t *>(const_cast<void *>(rest)), a.stats = const_cast<float *>(stats);
@@ -2020,14 +2065,10 @@ extern "C" int mlora_past_attention_backward(const mlora_past_shape *shape, cons
     st = launch_status();
     if (st) return st;
   }
-  const int64_t items[3] = {z.groups * z.Hk * p.prefix_blocks, z.B * z.Hk * p.sink_blocks, z.B * z.Hk * (p.key_blocks - p.sink_blocks)};
-  const int64_t splits[3] = {p.prefix_splits, p.sink_splits, p.own_splits};
-  const int64_t blocks = items[0] * splits[0] + items[1] * splits[1] + items[2] * splits[2];
+  const int64_t blocks = dkv_blocks(p, z);
   if (blocks == 0) return MLORA_OK;
-  const int64_t vectors[3] = {p.prefix_vectors, p.sink_vectors, p.own_vectors};
   JoinBlocks joins;
-  int64_t join_blocks = 0;
-  for (int c = 0; c < 3; ++c) joins.upto[c] = join_blocks += splits[c] > 1 ? ceil_div(vectors[c] / splits[c], 256) : 0;
+  const int64_t join_blocks = dkv_join_blocks(p, joins.upto);
   with_head(z.f32, z.D, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;

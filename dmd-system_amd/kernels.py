@@ -1178,6 +1178,9 @@ class PastPlan:
     __slots__ = ("shape", "ref", "forward", "backward", "stats", "saved", "g_strides", "empty", "pad", "metas")
 
 
+_PAST_BACKWARD_BYTES = "mlora_past_attention_backward_workspace_bytes"
+
+
 def past_plan(dtype: torch.dtype, sizes: Sequence[int], strides: Sequence[tuple], window: int, sinks: int, chunk: int, first: int,
               from_end: bool, scale: float) -> PastPlan:
     """sizes: B, Lq, Lk, H, Hk, D, groups, Lp; strides: the element strides {batch, token, head} of q, k, v[, prefix_k, prefix_v]
@@ -1188,10 +1191,10 @@ def past_plan(dtype: torch.dtype, sizes: Sequence[int], strides: Sequence[tuple]
                                 *[(ctypes.c_int64 * 3)(*s) for s in strides], *[(ctypes.c_int64 * 3)()] * pad, scale)
     plan.ref = ctypes.byref(plan.shape)
     nbytes = []
-    for name in ("mlora_past_attention_workspace_bytes", "mlora_past_attention_backward_workspace_bytes"):
+    for name in ("mlora_past_attention_workspace_bytes", _PAST_BACKWARD_BYTES):
         nbytes.append(getattr(_lib.load(), name)(plan.ref))
-        _lib.check(name, min(nbytes[-1], 0))
-    plan.forward, plan.backward = nbytes
+    plan.forward, plan.backward = nbytes  # a negative one of the backward's is a refusal of training alone
+    _lib.check("mlora_past_attention_workspace_bytes", min(plan.forward, 0))
     B, Lq, _, H, _, D = sizes[:6]
     plan.stats = (2 * B * H * Lq + 3) // 4 * 4  # floats; then, in bf16, what out's rounding left
     plan.saved = plan.stats + (B * Lq * H * D // 2 if dtype is torch.bfloat16 else 0)
@@ -1209,6 +1212,7 @@ def past_attention(plan: PastPlan, tensors: Sequence[torch.Tensor], pointers: Se
     q = tensors[0]
     out, saved, stats, rest = _new(q), None, None, None
     if for_backward:
+        _lib.check(_PAST_BACKWARD_BYTES, min(plan.backward, 0))
         saved = torch.empty(plan.saved, dtype=torch.float32, device=q.device)
         stats = saved.data_ptr()
         rest = stats + 4 * plan.stats

@@ -609,7 +609,8 @@ int mlora_cross_attention_backward(const void *q, const int64_t *q_strides, cons
  *   with groups > 0 its prefix: the first prefix_lengths[g] (NULL: Lp; clamped) keys of pk / pv [groups, Lp, Hk, D],
  *   g = b / (B / groups), shared by the group's samples.
  * out = softmax(scale * q kT) v over these keys. Queries with p < 0 or p >= n belong to no token: zeros. Keys that no query
- * of a sample sees may hold anything. window is 0 or at least chunk; D a multiple of 8 up to 128; Lq, Lk and Lp up to 2^28;
+ * of a sample sees may hold anything. window is 0 or at least chunk; D a multiple of 8 up to 128; Lq, Lk and Lp up to 2^28,
+ * launches of fewer than 2^32 work items (512 for up to 32 rows of a sample's key head where it has few);
  * scale > 0 and scale * log2 e finite in float32.
  *   out    [B, Lq, H, D] contiguous
  *   stats  NULL, or float [2 * B * H * Lq] for the backward; rest then takes what out's rounding to bf16 left ([B, Lq, H, D]

@@ -453,3 +453,22 @@ def test_gradients_under_saved_tensor_hooks(pkg, dev, prefix, dtype):
         with hooks:
             got = run(pkg, tensors, g, **kw)
         assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq, Lk", [(1, 2), (3, 3)])
+def test_many_samples(pkg, dev, Lq, Lk, dtype):
+    """A million samples' heads of a few tokens, as the pixels of a clip over its frames: some of them against the definition, all of
+    them finite and the same as in a batch of their own."""
+    B, H, D = 1 << 16, 16, 8
+    tensors, g = make(dtype, dev, 83, B, Lq, Lk, H, H, D)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(5))
+    got = run(pkg, tensors, g, lengths=lengths, window=2)
+    assert all(t.isfinite().all() for t in got.values())
+    for at in (0, 31111, B - 3):
+        s = slice(at, at + 3)
+        part, pg, n = [t[s] for t in tensors], g[s], lengths[s]
+        mine = {k: t[s] for k, t in got.items()}
+        ref.check(mine, *part, do=pg, lengths=n, window=2)
+        alone = run(pkg, part, pg, lengths=n, window=2)
+        assert all(torch.equal(mine[k], alone[k]) for k in mine)

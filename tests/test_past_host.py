@@ -190,14 +190,21 @@ def test_workspaces(pkg):
 
 
 @pytest.fixture
-def told(pkg, monkeypatch):
-    """The operators up to their launches, on host tensors: what kernels.past_attention_backward is called with, call by call."""
-    past, calls = pkg.past_attention, []
-    meta = past._meta
+def on_device(pkg, monkeypatch):
+    """Host tensors pass for device tensors."""
+    meta = pkg.past_attention._meta
 
-    def on_device(*a):
+    def moved(*a):
         m = meta(*a)
         return m and (*m[:2], torch.device("cuda", 0), *m[3:])
+
+    monkeypatch.setattr(pkg.past_attention, "_meta", moved)
+
+
+@pytest.fixture
+def told(pkg, on_device, monkeypatch):
+    """The operators up to their launches, on host tensors: what kernels.past_attention_backward is called with, call by call."""
+    calls = []
 
     def forward(plan, tensors, pointers, *rest):
         return torch.zeros(tensors[0].shape, dtype=tensors[0].dtype), torch.zeros(plan.saved)
@@ -206,7 +213,6 @@ def told(pkg, monkeypatch):
         calls.append((plan, out, saved, g, tensors, vectors))
         return [torch.zeros(t.shape, dtype=t.dtype) for t in tensors]
 
-    monkeypatch.setattr(past, "_meta", on_device)
     monkeypatch.setattr(pkg.kernels, "past_attention", forward)
     monkeypatch.setattr(pkg.kernels, "past_attention_backward", backward)
     return calls
@@ -304,3 +310,43 @@ def test_rows_wider_than_the_kernels_take_are_refused(pkg, told, name):
         t.update({n: wide for n in (("k", "v") if name in "kv" else ("prefix_k", "prefix_v"))})
     with pytest.raises(RuntimeError, match="heads of a token"):
         pkg.prefix_attention(*t.values())
+
+
+LAUNCHES = [  # sizes, the forward's and the backward's refusal: fewer than 2^32 work items a launch, whatever the tensors' sizes
+    (dict(B=1 << 16, Lq=1, Lk=2, H=12, Hk=12), False, False),      # many samples of one token
+    (dict(B=(1 << 20) - 1, Lq=1, Lk=2, H=8, Hk=8), False, False),  # 512 work items for up to 32 rows
+    (dict(B=1 << 20, Lq=1, Lk=2, H=8, Hk=8), True, False),
+    (dict(B=1, Lq=1 << 28, Lk=1 << 28, H=1, Hk=1, D=8, dtype=0), False, False),
+    (dict(B=2, Lq=1 << 28, Lk=1 << 28, H=1, Hk=1, D=8, dtype=0), True, True),
+    (dict(B=1 << 13, Lq=1, Lk=1 << 16, H=1, Hk=1, D=8, dtype=0), False, True),  # a backward of many keys, a forward of few rows
+]
+
+
+@pytest.mark.parametrize("case", LAUNCHES, ids=str)
+def test_limits_of_a_launch(pkg, case):
+    L, lib = pkg._lib, pkg._lib.load()
+    kw, fwd, bwd = dict(case[0]), *case[1:]
+    if "dtype" in kw:
+        kw["dtype"] = L.F32
+    D, H = kw.get("D", 64), kw["H"]
+    for n, length in (("q", "Lq"), ("k", "Lk"), ("v", "Lk")):
+        kw[n] = (kw[length] * H * D, H * D, D)
+    s = shape(L, window=16, first=0, **kw)
+    need = [lib.mlora_past_attention_workspace_bytes(s), lib.mlora_past_attention_backward_workspace_bytes(s)]
+    assert [n == L.ERR_LIMIT for n in need] == [fwd, bwd] and all(n >= 0 or n == L.ERR_LIMIT for n in need)
+    ptr = [0x1000] * 3 + [None] * 5
+    if fwd:
+        assert lib.mlora_past_attention(s, *ptr, 0x2000, 0x3000, 0x4000, 0x5000, 1 << 40, None) == L.ERR_LIMIT
+    if bwd:
+        assert lib.mlora_past_attention_backward(s, *ptr, 0x2000, 0x3000, 0x4000, 0x6000, (ctypes.c_int64 * 3)(*kw["q"]),
+                                                 *[0x7000] * 3, None, None, 0x5000, 1 << 50, None) == L.ERR_LIMIT
+
+
+def test_a_backward_past_its_limit_does_not_refuse_the_forward(pkg, on_device, monkeypatch):
+    monkeypatch.setattr(pkg.kernels, "_call", lambda *a: None)
+    q = torch.zeros(1, 1, 1, 8)
+    k = torch.zeros(1, 1, 1, 8).expand(1 << 13, 1 << 16, 1, 8)
+    q = q.expand(1 << 13, 1, 1, 8)
+    assert pkg.window_attention(q, k, k, window=16).shape == q.shape
+    with pytest.raises(RuntimeError, match="limit"):
+        pkg.window_attention(q.detach().requires_grad_(True), k, k, window=16)
