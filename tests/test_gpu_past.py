@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import past_plans
 import past_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -472,3 +473,45 @@ def test_many_samples(pkg, dev, Lq, Lk, dtype):
         ref.check(mine, *part, do=pg, lengths=n, window=2)
         alone = run(pkg, part, pg, lengths=n, window=2)
         assert all(torch.equal(mine[k], alone[k]) for k in mine)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", past_plans.PLANS, ids=str)
+def test_how_dk_and_dv_are_cut(pkg, dev, case, ragged):
+    """Every way to cut the keys' blocks and their rows, the first and the last key head with all its query heads."""
+    groups, each, L, Lp, H, Hk, window, sinks, chunk = case[:9]
+    B, G = max(groups, 1) * each, H // Hk
+    tensors, g = make(BF, dev, L + H, B, L, L, H, Hk, 128, groups, Lp)
+    gen = torch.Generator().manual_seed(H)
+    lengths = torch.randint(L // 2, L + 1, (B,), generator=gen) if ragged else None
+    kw = dict(window=window, chunk=chunk, lengths=lengths)
+    kw.update(dict(plens=i32(Lp - 1, Lp // 3)[:groups] if ragged else None) if groups else dict(sinks=sinks))
+    got = run(pkg, tensors, g, **kw)
+    for hk in {0, Hk - 1}:
+        pick = lambda t: t[:, :, hk * G:hk * G + G] if t.shape[2] == H and G > 1 else t[:, :, hk:hk + 1]  # noqa: E731, B023
+        ref.check({n: pick(t).contiguous() for n, t in got.items()}, *map(pick, tensors), do=pick(g), **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Lq", [3, 600])
+def test_every_operand_past_32_bits(pkg, dev, Lq, dtype):
+    """Tokens of q, k, v and a prefix that lie 2^22 - 8 elements apart, the last ones behind 2^31 elements; a second prefix
+    behind as many. Forward and every gradient."""
+    H, D, n, far = 2, 64, 600, (1 << 22) - 8
+    tensors, g = make(dtype, dev, 91, 2, Lq, n, H, H, D, 2, n)
+    base = torch.empty(n * far + 8 * H * D * 2, dtype=dtype, device=dev)
+    views, at = [], 0
+    for t in tensors:
+        v = base.as_strided(t.shape, (H * D, far, D, 1), at)
+        v.copy_(t)
+        views.append(v)
+        at += 2 * H * D
+    kw = dict(window=70, chunk=3, lengths=i32(n, 555), plens=i32(n, 599))
+    got = run(pkg, views, g, **kw)
+    ref.check(got, *tensors, do=g, **kw)
+    same = run(pkg, tensors, g, **kw)
+    assert all(torch.equal(got[k], same[k]) for k in got)
+    apart = base.as_strided((2, n, 2, H, D), (n * far - n * 2 * H * D, 2 * H * D, H * D, D, 1))
+    apart[:, :, 0], apart[:, :, 1] = tensors[3], tensors[4]
+    got = run(pkg, [*tensors[:3], apart[:, :, 0], apart[:, :, 1]], g, **kw)
+    assert all(torch.equal(got[k], same[k]) for k in got)

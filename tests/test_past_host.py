@@ -4,6 +4,8 @@ import ctypes
 import pytest
 import torch
 
+import past_plans
+
 BF, F = torch.bfloat16, torch.float32
 
 
@@ -350,3 +352,21 @@ def test_a_backward_past_its_limit_does_not_refuse_the_forward(pkg, on_device, m
     assert pkg.window_attention(q, k, k, window=16).shape == q.shape
     with pytest.raises(RuntimeError, match="limit"):
         pkg.window_attention(q.detach().requires_grad_(True), k, k, window=16)
+
+
+@pytest.mark.parametrize("case", past_plans.PLANS, ids=str)
+def test_how_dk_and_dv_are_cut(pkg, case):
+    """The calls of the GPU test of the same name are cut as the table says: the shares' sums are what the workspace holds."""
+    L, lib = pkg._lib, pkg._lib.load()
+    groups, each, n, Lp, H, Hk, window, sinks, chunk = case[:9]
+    s = shape(L, B=max(groups, 1) * each, Lq=n, Lk=n, H=H, Hk=Hk, D=128, groups=groups, Lp=Lp, window=window or 0, sinks=sinks, chunk=chunk,
+              first=0)
+    dq, dkv = past_plans.workspace_bytes(case)
+    assert lib.mlora_past_attention_backward_workspace_bytes(s) == max(dq, dkv) and (dq < dkv or max(case[9:]) == case[9])
+
+
+def test_every_cut_is_in_the_table():
+    for waves in (8, 4):
+        rows = [c for c in past_plans.PLANS if c[9] == waves]
+        assert {(c[11] > 1, c[12] > 1, c[13] > 1) for c in rows} >= {(a, b, c) for a in (0, 1) for b in (0, 1) for c in (0, 1) if a + b < 2} - (
+            {(0, 0, 0)} if waves == 4 else set())
