@@ -648,7 +648,7 @@ __device__ __forceinline__ void load_row(const T *p, bool on, int D, int lane, F
 
 // Few rows (16 NC per workgroup): the waves take different key tiles, each with its own buffer (no barrier in the loop; two
 // waves per SIMD, one multiplies while the other waits), and their running softmaxes are joined through LDS. Bound by the reading
-// of K and V where they are long (65520 keys, 8 key heads of 128: 46 us, 5.9 TB/s), by a launch and one chain of loads,
+// of K and V where they are long (65520 keys, 8 key heads of 128: 46 us, 5.9 TB/s, much of it out of the 256 MB cache), by a launch and one chain of loads,
 // products and the join where they are short (32 keys 5.4 us, 260 keys of 64 channels 6.1). On 32 x 32 products, four waves with two
 // buffers each: 51, 7.7 and 8.3.
 // float32 takes any number of rows this way (waves of 32 rows that share tiles behind a barrier: 1573 tokens, window 257, 12 heads of
@@ -1692,10 +1692,14 @@ struct PastPlan {
 };
 
 // How many waves a float32 workgroup has: `items` workgroups whose waves share `tiles` tiles. A tile waits for its loads, so that it
-// takes a SIMD's one wave as long as two; fewer waves leave room for more workgroups on a compute unit. Half where there is more than one
-// per unit (8 heads of 64, 4096 tokens, window 1024: 102 -> 88 us; 156 workgroups 50 -> 59, so not below); a quarter
-// where halves would be a second, mostly empty round and tiles are few (1573 tokens, window 257, 12 heads of 64, 600 workgroups of
-// ten tiles: 39, 37 and 30 us; not with many: 1024 workgroups of up to 22 27 -> 44).
+// takes a SIMD's one wave as long as two; fewer waves leave room for more workgroups on a compute unit. Measured as all / half / a quarter
+// of the waves, us of the forward of 64 channels (the backward's dq goes the same way):
+//   half above 256 workgroups: 200 of 12 tiles 14.0 / 14.3 / 19.3, 296 of 12 23.9 / 18.4 / 23.8, 448 of 26 40.8 / 35.5 / 59.0;
+//   a quarter from 513 to 1024, which halves take in two rounds and quarters in one, where tiles are few: 600 of 8 31.9 / 24.2 / 22.0, 896 of
+//   12 50.7 / 40.3 / 31.9, 1024 of 12 50.6 / 40.3 / 32.3 (544 of 12 loses: 32.0 / 26.8 / 30.5). Not where they are many: 600 of 18 44.3 / 36.6 / 43.1,
+//   696 of 26 59.7 / 53.3 / 60.1, though a full second round would gain there too (1024 of 26 79.0 / 67.4 / 62.1).
+// 128 channels, all / half of four: 296 of 5 25.0 / 19.8, 448 of 26 77.0 / 69.9, 2048 of 12 183.9 / 143.3. Where a half's second workgroup per unit
+// is missing on most units and tiles are many, all would be faster: 296 of 26 41.6 / 67.1.
 static int f32_waves(int64_t D, int64_t items, int64_t tiles) {
   const int most = D > 64 ? 4 : 8;
   if (items <= 256) return most;
@@ -1831,6 +1835,10 @@ static PastBwdPlan past_bwd_plan(const PastSizes &z) {
                  (kw == 8 ? 1.0 : 0.66) + shares + (shares > 0 ? 2.0 : 0.0);
     return c;
   };
+  // float32 and up to 64 channels: even parts. Finer ones (0.8 and 0.6 of an even part), us of the backward: 2 x 4096 tokens, window 1024,
+  // 16 / 4 heads of 64 233, 205 and 217, 4096 tokens without a window, 12 heads 224, 225 and 190; but 2 x 1024, 16 / 4 heads 66, 77 and 75, a frame of
+  // 1560, 12 heads 72, 80 and 81; float32, the same frame of 128 channels 840, 756 and 756, 2 x 2048, 8 / 2 heads 288, 310 and 308. The cost
+  // below is of tiles of 128 channels in bf16 and does not tell these apart.
   if (z.f32 || z.D <= 64) return plan(4, 1.0);
   // 256 keys per workgroup, or 128 whose tiles take 0.66 of the time (a barrier per 32 rows of a wave): 32760 keys, 12 heads, in one 4.7 ms,
   // in the other 5.4; 4096 keys without a window, 12 heads, 240 us and 165. Shares of an even part of the work,

@@ -5,15 +5,21 @@ to its own chunk and to what was generated before it, mostly to the last chunks 
 (sinks), and several samples may continue one past (conditional and unconditional passes, rollouts of one history).
 
 ``window_attention(q, k, v, window=..., sinks=..., chunk=...)`` covers whole sequences (training, prompts) and the newest
-tokens of a cache; ``prefix_attention(q, k, v, prefix_k, prefix_v, ...)`` adds a prefix that the samples of a group share,
-read once for all of them where they have few tokens each. Both with gradients of every tensor, the prefix's summed over its
-samples, all in a fixed order. Query heads may share key heads (H a multiple of Hk).
+tokens of a cache; ``prefix_attention(q, k, v, prefix_k, prefix_v, ...)`` adds a prefix that the samples of a group share.
+Where they have few tokens each it is read for the rows of all of them together, once per 32 rows (128 where a key head has more
+than 64 of them in bf16). Both with gradients of every tensor, the prefix's summed over its samples, all in a fixed order. Query heads may share key heads (H a multiple of Hk).
 
 A token at position p of a sample with n keys sees the own keys j < min(e, n) with j >= e - window or j < sinks, where
 e = (p // chunk + 1) * chunk is the end of its chunk, and all keys of its prefix. Queries that are no token of the sample
 (p < 0 or p >= n: padding) get zeros, and so do their gradients, whatever they hold; so do keys behind n. What lies in
-k and v where no token of the sample sees it is not used. A NaN or infinity in v where only some tokens see it may reach
-others among the 128 rows computed with them, as a product with weight zero does.
+k and v where no token of the sample sees it is not used. What is not finite in a token, or in a key that some tokens see, may
+reach others in the tiles that hold it, as a product with weight zero does: from v the outputs and from k the dq of rows that do not see
+the key (tiles of up to 32 rows and 64 keys), from q and the upstream gradient the dk and dv of keys that the token does not see (tiles
+of up to 64 tokens and 32 keys).
+
+The gradients of q, k, v and the prefix are all computed where one is wanted. Saved-tensor hooks may return copies in any layout.
+What a call's shapes and strides allow is looked up by them: a cache that grows by slices is planned anew for every length, one of a
+fixed size with key_lengths once.
 
 bf16: scores, softmax and sums in float32; the weights are rounded to bf16 for their products (dS too); out is rounded
 once, and what that rounding left is kept for the backward (bf16, the size of out). float32: float32 throughout, on
