@@ -80,10 +80,12 @@ def _unpack(ctx):
     """(the kernels' plan, what the forward saved, as the plan has it). A saved-tensor hook may return a copy in another layout,
     which is planned again; anything but the tensor it was given is refused."""
     plan, saved = ctx.plan, ctx.saved_tensors
-    metas = tuple([_meta(t) for t in saved])
-    if metas == plan.metas and not any([t.data_ptr() & 15 for t in saved[3:]]):
+    given = [t for t in saved if t is not None]
+    # strides, size and device are what the kernels could go astray by; three short lists cost a third of _meta's tuples
+    if (([t.stride() for t in given], [t.nbytes for t in given], [t.get_device() for t in given]) == plan.given
+            and not any([t.data_ptr() & 15 for t in saved[3:]])):
         return plan, saved
-    for was, now in zip(plan.metas, metas):
+    for was, now in zip(plan.metas, [_meta(t) for t in saved]):
         if (was and was[:3]) != (now and now[:3]):
             _fail(f"a saved-tensor hook returned {now and now[:3]} in place of {was and was[:3]}")
     flat = [t if t is None else t.contiguous() for t in saved[:5]]  # the vectors, out and the statistics
@@ -202,6 +204,8 @@ def _plan(metas, key_lengths, query_start, prefix_lengths, window, sinks, chunk,
         query_start is None and key_lengths is not None and Lq < Lk, scale)
     plan.metas = (_vector(key_lengths), _vector(query_start if isinstance(query_start, tuple) else None), _vector(prefix_lengths),
                   (q[0], dtype, device, (Lq * H * D, H * D, D, 1)), (torch.Size((plan.saved,)), torch.float32, device, (1,)), *metas)
+    given = [m for m in plan.metas if m]
+    plan.given = ([m[3] for m in given], [math.prod(m[0]) * m[1].itemsize for m in given], [device.index] * len(given))
     return plan, again
 
 
