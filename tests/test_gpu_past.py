@@ -515,3 +515,40 @@ def test_every_operand_past_32_bits(pkg, dev, Lq, dtype):
     apart[:, :, 0], apart[:, :, 1] = tensors[3], tensors[4]
     got = run(pkg, [*tensors[:3], apart[:, :, 0], apart[:, :, 1]], g, **kw)
     assert all(torch.equal(got[k], same[k]) for k in got)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_checkpointed(pkg, dev, dtype):
+    """Non-reentrant checkpointing forms the saved tensors again in the backward: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    x = make(dtype, dev, 87, 2, 90, 270, 2, 2, 64)[0][1].reshape(2, 90, 3, 128)
+    past = make(dtype, dev, 88, 1, 33, 33, 2, 2, 64)[0][1:]
+
+    def block(x, pk, pv):
+        q, k, v = (x[:, :, i].view(2, 90, 2, 64) for i in range(3))
+        return pkg.prefix_attention(q, k, v, pk, pv, window=25) + pkg.window_attention(q, k, v, window=25, sinks=2)
+
+    leaves = [t.detach().requires_grad_(True) for t in (x, *past)]
+    g = torch.randn(2, 90, 2, 64, generator=torch.Generator().manual_seed(2)).to(dev).to(dtype)
+    want = torch.autograd.grad(block(*leaves), leaves, [g])
+    got = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, [g])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_smallest_and_largest_scales(pkg, dev, dtype):
+    """Scales at the ends of float32 with scores that stay in its range: the mean of what a token sees, or the key of the largest product."""
+    # u |out| for out's rounding and u max |v| for the weights', max |v| < 4, 2^-18 for the sums
+    (q, k, v), _ = make(dtype, dev, 89, 1, 70, 70, 2, 2, 32)
+    assert v.abs().max() < 4
+    vis = ref.seen(70, 70, 70, 0, 20, 2, 1).double()
+    for scale in (2.0 ** -140, 2.0 ** -126, 2.0 ** -60):
+        got = run(pkg, [q, k, v], window=20, sinks=2, scale=scale)["out"]
+        want = torch.einsum("ij,jhd->ihd", vis / vis.sum(1, keepdim=True), ref.f64(v)[0])
+        assert ((ref.f64(got)[0] - want).abs() <= 2 * ref.half_step(dtype) * 4 + 2 ** -18).all()
+    whole = torch.randint(-3, 4, q.shape, generator=torch.Generator().manual_seed(1)).to(dev).to(dtype)
+    s = torch.einsum("ihd,jhd->hij", ref.f64(whole)[0], ref.f64(k.sign())[0]).masked_fill(vis == 0, -math.inf)  # whole numbers
+    best = (s == s.amax(-1, keepdim=True)).double()
+    want = torch.einsum("hij,jhd->ihd", best / best.sum(-1, keepdim=True), ref.f64(v)[0])
+    got = run(pkg, [whole, k.sign(), v], window=20, sinks=2, scale=2.0 ** 100)["out"]
+    assert ((ref.f64(got)[0] - want).abs() <= 2 * ref.half_step(dtype) * 4 + 2 ** -18).all()
