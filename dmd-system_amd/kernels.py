@@ -1174,7 +1174,7 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 class PastPlan:
     """A past-attention call's sizes, strides and options as the C entries take them, the bytes of its workspaces, and where
     the backward's statistics lie; made once per combination of them by past_plan. metas: shape, type, device and strides of what
-    the backward reads, given: the strides, bytes and devices alone, for who calls it."""
+    the backward reads, given: the same of those that are there, as lists, for who calls it."""
     __slots__ = ("shape", "ref", "forward", "backward", "stats", "saved", "g_strides", "empty", "pad", "metas", "given")
 
 

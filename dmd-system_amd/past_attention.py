@@ -7,7 +7,8 @@ to its own chunk and to what was generated before it, mostly to the last chunks 
 ``window_attention(q, k, v, window=..., sinks=..., chunk=...)`` covers whole sequences (training, prompts) and the newest
 tokens of a cache; ``prefix_attention(q, k, v, prefix_k, prefix_v, ...)`` adds a prefix that the samples of a group share.
 Where they have few tokens each it is read for the rows of all of them together, once per 32 rows (128 where a key head has more
-than 64 of them in bf16). Both with gradients of every tensor, the prefix's summed over its samples, all in a fixed order. Query heads may share key heads (H a multiple of Hk).
+than 64 of them in bf16). Both with gradients of every tensor, the prefix's summed over its samples, all in a fixed order. Query
+heads may share key heads (H a multiple of Hk).
 
 A token at position p of a sample with n keys sees the own keys j < min(e, n) with j >= e - window or j < sinks, where
 e = (p // chunk + 1) * chunk is the end of its chunk, and all keys of its prefix. Queries that are no token of the sample
@@ -81,8 +82,8 @@ def _unpack(ctx):
     which is planned again; anything but the tensor it was given is refused."""
     plan, saved = ctx.plan, ctx.saved_tensors
     given = [t for t in saved if t is not None]
-    # strides, size and device are what the kernels could go astray by; three short lists cost a third of _meta's tuples
-    if (([t.stride() for t in given], [t.nbytes for t in given], [t.get_device() for t in given]) == plan.given
+    # four short lists: _meta's tuples cost a small backward 3 us more
+    if (([t.shape for t in given], [t.dtype for t in given], [t.get_device() for t in given], [t.stride() for t in given]) == plan.given
             and not any([t.data_ptr() & 15 for t in saved[3:]])):
         return plan, saved
     for was, now in zip(plan.metas, [_meta(t) for t in saved]):
@@ -205,7 +206,7 @@ def _plan(metas, key_lengths, query_start, prefix_lengths, window, sinks, chunk,
     plan.metas = (_vector(key_lengths), _vector(query_start if isinstance(query_start, tuple) else None), _vector(prefix_lengths),
                   (q[0], dtype, device, (Lq * H * D, H * D, D, 1)), (torch.Size((plan.saved,)), torch.float32, device, (1,)), *metas)
     given = [m for m in plan.metas if m]
-    plan.given = ([m[3] for m in given], [math.prod(m[0]) * m[1].itemsize for m in given], [device.index] * len(given))
+    plan.given = ([m[0] for m in given], [m[1] for m in given], [device.index] * len(given), [m[3] for m in given])
     return plan, again
 
 

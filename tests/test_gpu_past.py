@@ -552,3 +552,16 @@ def test_smallest_and_largest_scales(pkg, dev, dtype):
     want = torch.einsum("hij,jhd->ihd", best / best.sum(-1, keepdim=True), ref.f64(v)[0])
     got = run(pkg, [whole, k.sign(), v], window=20, sinks=2, scale=2.0 ** 100)["out"]
     assert ((ref.f64(got)[0] - want).abs() <= 2 * ref.half_step(dtype) * 4 + 2 ** -18).all()
+
+
+def test_a_hook_that_returns_another_type_or_shape_is_refused(pkg, dev):
+    """Of the same strides, bytes and device too: fp16 in place of bf16, fewer samples of more tokens over the same rows."""
+    wide = lambda t: t.new_empty(t.numel()).as_strided((t.shape[0] // 2, t.shape[1] * 2, *t.shape[2:]), t.stride())  # noqa: E731
+    half = lambda t: t.to(torch.float16)  # noqa: E731
+    for at, hook in ((0, half), (2, half), (4, half), (2, wide)):  # of out, the statistics, q, k, v
+        count = iter(range(100))
+        q, k, v = (torch.zeros(4, 50, 2, 64, dtype=BF, device=dev).requires_grad_(True) for _ in range(3))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: hook(t) if next(count) == at else t):  # noqa: B023
+            out = pkg.window_attention(q, k, v)
+        with pytest.raises(RuntimeError, match="saved-tensor hook"):
+            torch.autograd.grad(out, [q, k, v], [torch.ones_like(out)])
